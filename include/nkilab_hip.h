@@ -394,6 +394,115 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
              long y_sh, long y_ss, int pos0, float base, int dtype,
              void* stream);
 
+/*
+ * ---- The paged cache.  No counterpart in the reference, whose block has no
+ * cache (nkilab/model.py:59-67 attends over one prompt).
+ *
+ * K and V rows of many sequences live in pages of page_size rows: k and v are
+ * [pages, kv_heads, page_size, d] with any strides that keep a row's d elements
+ * together.  Row j of sequence b is row j % page_size of page
+ * table[b table_row + j / page_size]; an entry outside [0, pages) names no
+ * page: its rows are not visible, and nothing is written to them.
+ *
+ * A call brings `rows` new rows, those of sequence b at rows
+ * q_start[b] .. q_start[b + 1] - 1 of its packed tensors (q_start null: max_new
+ * each).  max_new is the most that a sequence brings: rows past it, and rows
+ * behind the last sequence's, are left as they are.  lens[b] counts the
+ * sequence's rows with its new ones, which are its last: new row i of n is at
+ * position lens[b] - n + i.  (A position below 0 has no row.)
+ *
+ * table, lens and q_start are device arrays, read by the kernels only, so a
+ * captured graph can be replayed with other contents.  A table addresses at
+ * most 2^30 rows.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  long k_page, k_head, k_row;
+  long v_page, v_head, v_row;
+  const int* table;
+  long table_row;
+  const int* lens;
+  const int* q_start;
+  int pages, kv_heads, page_size, d;
+  int table_cols, batch, rows, max_new;
+  int dtype;
+} nkl_paged_cache;
+
+/*
+ * Writes new K and V rows to the cache and, with rope_base != 0, rotates K on
+ * the way and q into q_out (which may be q): rotate-half layout as nkl_rope,
+ * but each row by its own position and with the angle in 64 bits.  With a tree
+ * (mask words as nkl_tree_mask makes them) a node's position is lens[b] - n - 1
+ * + the nodes it sees.  k, v: [rows, kv_heads, d], q, q_out: [rows, H, d], with
+ * element strides; H = 0 and null pointers for no q.  d even (and at most 1024)
+ * with a rotary base.  Two sequences of a call must not share a page that either
+ * writes.
+ */
+int nkl_cache_append(const nkl_paged_cache* cache, const void* k, const void* v,
+                     long k_row, long k_head, long v_row, long v_head,
+                     const void* q, void* q_out, int H, long q_row, long q_head,
+                     long qo_row, long qo_head, const void* tree,
+                     int tree_words, float rope_base, void* stream);
+
+/*
+ * Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, K and V, in each of
+ * `layers` layers (k_layer and v_layer elements apart).  pairs is a HOST array,
+ * read before the call returns.  A page written twice, or both read and
+ * written, is refused.  Of the cache only k, v, strides, pages, kv_heads,
+ * page_size, d and dtype are used.
+ */
+int nkl_cache_copy_pages(const nkl_paged_cache* cache, const int* pairs, int n,
+                         int layers, long k_layer, long v_layer, void* stream);
+
+/*
+ * Keeps the accepted path of each sequence's new rows: with ctx = lens[b] - n,
+ * row ctx + paths[b path_row + i] moves to row ctx + i, as if every row were
+ * read before any is written, in each layer, and new_lens[b] = ctx + the path's
+ * length.  A path is a strictly ascending list of nodes in [0, n): it ends
+ * at its first entry that is not one (-1 by custom), or after path_cols.
+ * A sequence's pages from ctx on must be its own.
+ */
+int nkl_cache_accept(const nkl_paged_cache* cache, const int* paths,
+                     long path_row, int path_cols, int* new_lens, int layers,
+                     long k_layer, long v_layer, void* stream);
+
+/*
+ * words[t] (tree_words 64-bit words a row) = node t of its tree and its
+ * ancestors, bit i for node i of the sequence.  parents[t] is a node's parent
+ * within its sequence's rows, below it; anything else (-1 by custom) makes it a
+ * root.  q_start as in nkl_paged_cache (null: n_each nodes a sequence).
+ */
+int nkl_tree_mask(const int* parents, const int* q_start, int batch, int rows,
+                  int n_each, void* words, int tree_words, void* stream);
+
+/*
+ * Attention of the new rows over the cache (which holds their K and V already):
+ * q, o: [rows, H, d], H a multiple of kv_heads; query head h reads K/V head
+ * h / (H / kv_heads).  Row i of n, at position pos, sees the keys j <= pos with
+ * j > pos - window or j < sinks (window 0: every key).  With a tree it sees the
+ * new rows whose bits are set in its mask words, and of the rows before them
+ * those within the window of position lens[b] - n - 1 + (nodes it sees), and the
+ * sinks.  A row that sees nothing gets zeros; keys that a row does not see take
+ * no part, whatever they hold, and pages that no row of a call sees are not
+ * read.  Arithmetic as nkl_flash_attn_causal's: P rounded to the 16-bit types,
+ * statistics and O in fp32.
+ * d <= 128; d, strides multiples of 8 (F32: 4), pointers 16-byte aligned;
+ * scale > 0.  table may be null for one sequence whose rows are page 0's
+ * (lens then too): a prompt's own K and V.
+ * The workspace (nkl_paged_attention_workspace_bytes(), 16-byte aligned, no
+ * initialisation; 0 where the tiles of rows fill the card) holds the states of
+ * keys split over workgroups.  The size depends on the call's sizes alone, not
+ * on what its device arrays hold.  One or two kernel launches.
+ */
+size_t nkl_paged_attention_workspace_bytes(const nkl_paged_cache* cache, int H,
+                                           int window, int sinks, int tree);
+int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, void* o,
+                        int H, long q_row, long q_head, long o_row, long o_head,
+                        int window, int sinks, const void* tree, int tree_words,
+                        float scale, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

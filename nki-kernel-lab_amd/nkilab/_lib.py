@@ -19,6 +19,17 @@ ABI_VERSION = 1
 _c_int, _c_long, _c_float, _c_size = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_size_t
 _vp = ctypes.c_void_p
 
+
+class PagedCacheDesc(ctypes.Structure):
+    """nkl_paged_cache of include/nkilab_hip.h, field for field."""
+    _fields_ = ([("k", _vp), ("v", _vp)] + [(n, _c_long) for n in ("k_page", "k_head", "k_row", "v_page", "v_head", "v_row")]
+                + [("table", _vp), ("table_row", _c_long), ("lens", _vp), ("q_start", _vp)]
+                + [(n, _c_int) for n in ("pages", "kv_heads", "page_size", "d", "table_cols", "batch", "rows", "max_new",
+                                         "dtype")])
+
+
+_cache_p = ctypes.POINTER(PagedCacheDesc)
+
 # name -> (restype, argtypes); mirrors include/nkilab_hip.h one for one.
 SIGNATURES = {
     "nkl_abi_version": (_c_int, []),
@@ -65,6 +76,14 @@ SIGNATURES = {
     "nkl_attention_naive_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "nkl_attention_naive": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_int, _c_long, _c_long,
                                      _c_long, _c_long, _c_long, _c_long, _c_long, _c_long, _c_float, _c_int, _vp]),
+    "nkl_cache_append": (_c_int, [_cache_p, _vp, _vp, _c_long, _c_long, _c_long, _c_long, _vp, _vp, _c_int, _c_long,
+                                  _c_long, _c_long, _c_long, _vp, _c_int, _c_float, _vp]),
+    "nkl_cache_copy_pages": (_c_int, [_cache_p, _vp, _c_int, _c_int, _c_long, _c_long, _vp]),
+    "nkl_cache_accept": (_c_int, [_cache_p, _vp, _c_long, _c_int, _vp, _c_int, _c_long, _c_long, _vp]),
+    "nkl_tree_mask": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
+    "nkl_paged_attention_workspace_bytes": (_c_size, [_cache_p, _c_int, _c_int, _c_int, _c_int]),
+    "nkl_paged_attention": (_c_int, [_cache_p, _vp, _vp, _c_int, _c_long, _c_long, _c_long, _c_long, _c_int, _c_int, _vp,
+                                     _c_int, _c_float, _vp, _c_size, _vp]),
 }
 
 _lib = None

@@ -84,6 +84,7 @@ def _stream_handle_raw() -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _get_device = getattr(torch._C, "_cuda_getDevice", None)
 stream_handle = _stream_handle_raw if _raw_stream and _get_device else _stream_handle_slow
+current_device = _get_device or torch.cuda.current_device
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

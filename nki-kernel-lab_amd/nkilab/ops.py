@@ -16,6 +16,7 @@ what nkilab.model uses.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 
@@ -23,7 +24,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._tensors import dtype_code, from_device, ptr, stream_handle, to_device, workspace
+from ._tensors import current_device, dtype_code, from_device, ptr, stream_handle, to_device, workspace
 
 # Reference tile sizes (nkilab/kernels/matmul.py:19-21, attention.py:24).  They
 # define choose_blocks' grid and _pad_to's semantics; the HIP kernels handle
@@ -442,11 +443,13 @@ def _attn_operand(t: torch.Tensor, E: int) -> torch.Tensor:
 
 
 def attention_into(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
-                   variant: str = "flash_pipelined", scale: float | None = None) -> torch.Tensor:
+                   variant: str = "flash_pipelined", scale: float | None = None, window: int | None = None,
+                   sinks: int = 0) -> torch.Tensor:
     """Causal attention into o; q, o: [H, S, d] and k, v: [Hkv, S, d] GPU tensors
     (Hkv = H, or a divisor of H for grouped-query attention: query head h reads
     K/V head h // (H / Hkv)), any strides along heads and S (d contiguous).
-    d must be a multiple of 8 (bf16) / 4 (fp32)."""
+    d must be a multiple of 8 (bf16) / 4 (fp32).  window and sinks as in
+    ``attention``."""
     spec = ATTENTION_VARIANTS[variant]
     H, S, d = q.shape
     Hkv = k.shape[0]
@@ -456,12 +459,15 @@ def attention_into(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.T
     if o.shape != q.shape or o.dtype != q.dtype or not (q.dtype == k.dtype == v.dtype):
         raise ValueError(f"attention_into: o {tuple(o.shape)} {o.dtype} must match q {tuple(q.shape)} {q.dtype}, "
                          "and k, v share q's dtype")
-    return _attention(q, k, v, o, spec, H, Hkv, S, d, 1.0 / math.sqrt(d) if scale is None else float(scale))
+    return _attention(q, k, v, o, spec, H, Hkv, S, d, 1.0 / math.sqrt(d) if scale is None else float(scale), window,
+                      sinks)
 
 
 def _attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, spec: AttentionVariant, H: int,
-               Hkv: int, S: int, d: int, scale: float) -> torch.Tensor:
+               Hkv: int, S: int, d: int, scale: float, window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """attention_into on shapes and dtypes already checked."""
+    if window is not None or sinks:
+        return _window_attention(q, k, v, o, spec, H, Hkv, S, d, scale, window, sinks)
     E = 8 if q.element_size() == 2 else 4
     q, k, v = (_attn_operand(t, E) for t in (q, k, v))
     o_ok = _attn_strides_ok(o, E)
@@ -494,12 +500,50 @@ def _attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tenso
     return o
 
 
-def attention(q, k, v, variant: str = "flash_pipelined", scale: float | None = None):
+def _window_sinks(fn: str, window: int | None, sinks: int) -> tuple[int, int]:
+    """The C ABI's (window, sinks): 0 for no window."""
+    if window is None:
+        if sinks:
+            raise ValueError(f"{fn}: sinks={sinks} without a window (every key is visible)")
+        return 0, 0
+    if int(window) < 1 or int(sinks) < 0:
+        raise ValueError(f"{fn}: window={window} must be at least 1 and sinks={sinks} at least 0")
+    return min(int(window), MAX_ROWS), min(int(sinks), MAX_ROWS)
+
+
+def _window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, spec: AttentionVariant, H: int,
+                      Hkv: int, S: int, d: int, scale: float, window: int | None, sinks: int) -> torch.Tensor:
+    """_attention under a window: the paged kernel over one sequence, k and v as its one page."""
+    if spec.path != "flash":
+        raise ValueError(f"attention: variant {spec.name!r} has no window; one of the flash variants expected")
+    w, sinks = _window_sinks("attention", window, sinks)
+    if S == 0 or H == 0:
+        return o
+    if d == 0:
+        raise ValueError("attention: head dim 0")
+    if S > MAX_ROWS:
+        raise ValueError(f"attention: {S} positions, at most {MAX_ROWS} under a window")
+    E = 16 // q.element_size()
+    q, k, v = (_rows_operand(t, E) for t in (q, k, v))
+    out = o if _rows_ok(o, E) else torch.empty((H, S, d), dtype=o.dtype, device=o.device)
+    desc = _lib.PagedCacheDesc(k.data_ptr(), v.data_ptr(), 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), None, 0,
+                               None, None, 1, Hkv, S, d, 1, 1, S, S, dtype_code(q.dtype))
+    _paged_attention(desc, q, (q.stride(1), q.stride(0)), out, (out.stride(1), out.stride(0)), H, w, sinks, None, 0, scale)
+    if out is not o:
+        o.copy_(out)
+    return o
+
+
+def attention(q, k, v, variant: str = "flash_pipelined", scale: float | None = None, window: int | None = None,
+              sinks: int = 0):
     """Causal attention. q, k, v: [H, S, d] (ops.py:77-91); scale 1/sqrt(d)
     unless given (the kernel-level entry points of nkilab.kernels.attention
     pass theirs).
     k and v may also have fewer heads Hkv dividing H (grouped-query attention:
     query head h uses K/V head h // (H / Hkv)), which the reference lacks.
+    With a window, query i sees the keys j <= i with j > i - window or
+    j < sinks (the paged cache's attention over one sequence; the flash
+    variants only, scale > 0), which the reference lacks too.
 
     The reference pads S to a multiple of 128 and transposes q and k on the
     host; the HIP kernels take [H, S, d] as is and bound-check ragged S, so
@@ -523,7 +567,305 @@ def attention(q, k, v, variant: str = "flash_pipelined", scale: float | None = N
     if dp != d:
         tq, tk, tv = (torch.nn.functional.pad(t, (0, dp - d)) for t in (tq, tk, tv))
     o = tq.new_empty((H, S, dp))
-    _attention(tq, tk, tv, o, spec, H, tk.shape[0], S, dp, 1.0 / math.sqrt(d) if scale is None else float(scale))
+    _attention(tq, tk, tv, o, spec, H, tk.shape[0], S, dp, 1.0 / math.sqrt(d) if scale is None else float(scale),
+               window, sinks)
     if dp != d:
         o = o[:, :, :d].contiguous()
     return from_device(o, kind)
+
+
+# ---------------------------------------------------------- paged cache --
+
+MAX_ROWS = 1 << 30  # rows a page table addresses at most, and new rows of a call
+
+
+def _rows_ok(t: torch.Tensor, E: int) -> bool:
+    """Whether the paged kernels take t [., ., d] as it lies: a row's elements together, rows on 16 bytes."""
+    a, b, c = t.stride()
+    return c == 1 and a % E == 0 and b % E == 0 and a >= 0 and b >= 0 and t.data_ptr() % 16 == 0
+
+
+def _rows_operand(t: torch.Tensor, E: int) -> torch.Tensor:
+    return t if _rows_ok(t, E) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _on_current_device(fn: str, *tensors: torch.Tensor | None) -> None:
+    """The kernels run on the current device's current stream: every tensor has to be there."""
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.get_device() == current_device()):
+            raise ValueError(f"{fn}: a tensor is on {t.device}, which is not the current device")
+
+
+def _int32(fn: str, name: str, t: torch.Tensor, shape: tuple) -> None:
+    if t.dtype is not torch.int32 or t.shape != shape or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{fn}: {name} must be int32 {list(shape)} with unit stride, got {t.dtype} {list(t.shape)}")
+
+
+def _cache_tensors(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, layers: bool = False) -> None:
+    dims = (4, 5) if layers else (4,)
+    if k_cache.dim() not in dims or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError(f"{fn}: k_cache {tuple(k_cache.shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} "
+                         f"{v_cache.dtype} must be equal {'[layers,] ' if layers else ''}[pages, kv_heads, page_size, d]")
+    for t in (k_cache, v_cache):
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{fn}: the caches' head dim must be contiguous")
+
+
+def _cache_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                q_start: torch.Tensor | None, rows: int, max_q: int | None) -> _lib.PagedCacheDesc:
+    """The C ABI's description of a cache and a call's new rows, checked."""
+    _cache_tensors(fn, k_cache, v_cache)
+    pages, Hkv, page_size, d = k_cache.shape
+    if page_table.dim() != 2:
+        raise ValueError(f"{fn}: page_table must be [batch, pages of a sequence], got {tuple(page_table.shape)}")
+    B = page_table.shape[0]
+    _int32(fn, "page_table", page_table, page_table.shape)
+    _int32(fn, "lens", lens, (B,))
+    if q_start is not None:
+        _int32(fn, "q_start", q_start, (B + 1,))
+        if max_q is None:
+            raise ValueError(f"{fn}: q_start needs max_q, the most new rows of a sequence")
+    else:
+        each = rows // B if B else 0
+        if each * B != rows:
+            raise ValueError(f"{fn}: {rows} rows are not a number for each of {B} sequences; q_start expected")
+        if max_q is not None and int(max_q) != each:
+            raise ValueError(f"{fn}: max_q={max_q}, and {each} rows for each sequence")
+        max_q = each
+    if int(max_q) < 0:
+        raise ValueError(f"{fn}: max_q={max_q} is negative")
+    sk, sv = k_cache.stride(), v_cache.stride()
+    return _lib.PagedCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
+                               page_table.data_ptr(), page_table.stride(0), lens.data_ptr(),
+                               None if q_start is None else q_start.data_ptr(), pages, Hkv, page_size, d,
+                               page_table.shape[1], B, rows, min(int(max_q), rows), dtype_code(k_cache.dtype))
+
+
+def _tree_words(fn: str, tree: torch.Tensor | None, rows: int, max_q: int) -> tuple[int | None, int]:
+    if tree is None:
+        return None, 0
+    if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] != rows or 64 * tree.shape[1] < max_q:
+        raise ValueError(f"{fn}: tree must be int64 [{rows}, words of 64 nodes for up to {max_q}], got {tree.dtype} "
+                         f"{list(tree.shape)}")
+    if not tree.is_contiguous():
+        raise ValueError(f"{fn}: tree must be contiguous")
+    return tree.data_ptr(), tree.shape[1]
+
+
+def tree_mask(parents: torch.Tensor, q_start: torch.Tensor | None = None, max_q: int | None = None,
+              batch: int = 1) -> torch.Tensor:
+    """Mask words [rows, words] (int64, bit i % 64 of word i // 64 for node i) of
+    drafted trees: node t sees itself and its ancestors.  parents: int32 [rows],
+    each node's parent as an index within its own sequence's nodes, below the
+    node's (-1: a root, which hangs off the context).  q_start: int32
+    [batch + 1], the sequences' first rows, with max_q their most nodes;
+    without it, rows / batch nodes each."""
+    fn = "tree_mask"
+    rows = parents.shape[0] if parents.dim() == 1 else -1
+    _int32(fn, "parents", parents, (rows,))
+    each = 0
+    if q_start is not None:
+        batch = q_start.shape[0] - 1 if q_start.dim() == 1 else -1
+        _int32(fn, "q_start", q_start, (batch + 1,))
+        if batch < 0 or max_q is None or int(max_q) < 0:
+            raise ValueError(f"{fn}: q_start [batch + 1] and max_q, the most nodes of a sequence, expected")
+    else:
+        each = rows // batch if batch > 0 else 0
+        if each * batch != rows or (max_q is not None and int(max_q) != each):
+            raise ValueError(f"{fn}: {rows} nodes are not a number (max_q={max_q}) for each of {batch} sequences")
+        max_q = each
+    _on_current_device(fn, parents, q_start)
+    # (rows that belong to no sequence see nothing)
+    words = (torch.empty if q_start is None else torch.zeros)((rows, max(1, -(-int(max_q) // 64))), dtype=torch.int64,
+                                                              device=parents.device)
+    _lib.call("nkl_tree_mask", ptr(parents), ptr(q_start), batch, rows, each, ptr(words), words.shape[1], stream_handle())
+    return words
+
+
+def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      page_table: torch.Tensor, lens: torch.Tensor, q_start: torch.Tensor | None = None,
+                      max_q: int | None = None, tree: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                      q_out: torch.Tensor | None = None, rope_base: float | None = None) -> None:
+    """Writes new K and V rows (k, v: [rows, kv_heads, d]) to a paged cache
+    (k_cache, v_cache: [pages, kv_heads, page_size, d], any strides, d
+    contiguous), in one launch with their rotary embedding.
+
+    page_table: int32 [batch, columns], the pages of each sequence in order;
+    entries outside [0, pages) name none.  lens: int32 [batch], each sequence's
+    rows with the new ones, which are its last.  q_start: int32 [batch + 1],
+    the sequences' first new rows, with max_q the most of one (None:
+    rows / batch each).  A row that has no place is not written.
+
+    With rope_base, K rows are rotated by their positions on the way (and q
+    [rows, H, d] into q_out, which may be q): rotate-half layout, angles in 64
+    bits.  tree (``tree_mask``'s words): a node's position is the context's
+    length and its depth.  Sequences of one call must not share a page that
+    either writes."""
+    fn = "cache_append_into"
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
+        raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} must be [rows, kv_heads, d] of the caches "
+                         f"{tuple(k_cache.shape)}")
+    if not (k.dtype == v.dtype == k_cache.dtype):
+        raise TypeError(f"{fn}: k {k.dtype}, v {v.dtype} and the caches {k_cache.dtype} must share a dtype")
+    desc = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, k.shape[0], max_q)
+    words, nwords = _tree_words(fn, tree, k.shape[0], desc.max_new)
+    base = 0.0
+    if rope_base is not None:
+        base = float(rope_base)
+        if not base > 1.0:
+            raise ValueError(f"{fn}: rope_base {rope_base} must be above 1")
+    H, sq, so = 0, (0, 0), (0, 0)
+    if q is not None or q_out is not None:
+        if rope_base is None or q is None or q_out is None:
+            raise ValueError(f"{fn}: q, q_out and rope_base go together")
+        if q.dim() != 3 or q.shape != q_out.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+            raise ValueError(f"{fn}: q {tuple(q.shape)} and q_out {tuple(q_out.shape)} must be [{k.shape[0]}, H, "
+                             f"{k.shape[2]}]")
+        if not (q.dtype == q_out.dtype == k.dtype):
+            raise TypeError(f"{fn}: q {q.dtype} and q_out {q_out.dtype} must have k's dtype {k.dtype}")
+        H, sq, so = q.shape[1], q.stride()[:2], q_out.stride()[:2]
+        if H == 0:
+            q = q_out = None
+    for t in (k, v, q, q_out):
+        if t is not None and t.stride(2) != 1 and t.shape[2] > 1:
+            raise ValueError(f"{fn}: the head dim must be contiguous")
+    _on_current_device(fn, k, v, k_cache, v_cache, page_table, lens, q_start, tree, q, q_out)
+    _lib.call("nkl_cache_append", ctypes.byref(desc), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
+              v.stride(1), ptr(q), ptr(q_out), H, *sq, *so, words, nwords, base, stream_handle())
+
+
+def _layer_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, tuple, tuple, tuple]:
+    """(layers, layer strides, [pages, kv_heads, page_size, d], its strides in both) of caches with or without layers."""
+    _cache_tensors(fn, k_cache, v_cache, layers=True)
+    if k_cache.dim() == 5:
+        return (k_cache.shape[0], k_cache.stride(0), v_cache.stride(0), k_cache.shape[1:], k_cache.stride()[1:4],
+                v_cache.stride()[1:4])
+    return 1, 0, 0, k_cache.shape, k_cache.stride()[:3], v_cache.stride()[:3]
+
+
+def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs) -> None:
+    """Copies pages of a cache ([pages, kv_heads, page_size, d], or with a
+    leading axis of layers, in each): pairs is a list of (from, to) page ids on
+    the host (or an integer array [n, 2]).  A page that is written twice, or
+    both read and written, is refused."""
+    fn = "cache_copy_pages"
+    layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
+    if isinstance(pairs, torch.Tensor) and pairs.is_cuda:
+        raise ValueError(f"{fn}: pairs are read on the host: a list, an array or a CPU tensor expected")
+    p = np.asarray(pairs)
+    if p.size == 0:
+        return
+    if p.ndim != 2 or p.shape[1] != 2 or p.dtype.kind not in "iu":
+        raise ValueError(f"{fn}: pairs must be whole numbers [n, 2], got {p.dtype} {list(p.shape)}")
+    if int(p.min()) < 0 or int(p.max()) >= shape[0]:
+        raise ValueError(f"{fn}: pages {int(p.min())} .. {int(p.max())} outside [0, {shape[0]})")
+    p = np.ascontiguousarray(p, dtype=np.int32)
+    _on_current_device(fn, k_cache, v_cache)
+    desc = _lib.PagedCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), *sk, *sv, None, 0, None, None, *shape, 0, 0, 0, 0,
+                               dtype_code(k_cache.dtype))
+    _lib.call("nkl_cache_copy_pages", ctypes.byref(desc), p.ctypes.data, p.shape[0], layers, kl, vl, stream_handle())
+
+
+def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                 paths: torch.Tensor, q_start: torch.Tensor | None = None, n_nodes: int | None = None) -> torch.Tensor:
+    """Keeps the accepted path of each sequence's newest rows (the nodes of a
+    drafted tree): row paths[b, i] of them moves to row i, in every layer of
+    the caches ([layers,] pages, kv_heads, page_size, d), and the sequence's
+    new length is returned (int32 [batch], lens unchanged).
+
+    lens: int32 [batch], rows with the nodes.  paths: int32 [batch, columns],
+    strictly ascending nodes, ended by the first entry that is not (-1 by
+    custom).  The nodes of each sequence: q_start (int32 [batch + 1]), or
+    n_nodes for every one.  A sequence's pages from its first node on must be
+    its own."""
+    fn = "cache_accept"
+    layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
+    if page_table.dim() != 2 or paths.dim() != 2:
+        raise ValueError(f"{fn}: page_table {tuple(page_table.shape)} and paths {tuple(paths.shape)} must have two axes")
+    B = page_table.shape[0]
+    _int32(fn, "page_table", page_table, page_table.shape)
+    _int32(fn, "lens", lens, (B,))
+    _int32(fn, "paths", paths, (B, paths.shape[1]))
+    if (q_start is None) == (n_nodes is None):
+        raise ValueError(f"{fn}: either q_start or n_nodes expected")
+    if q_start is not None:
+        _int32(fn, "q_start", q_start, (B + 1,))
+        rows = most = MAX_ROWS
+    else:
+        most = int(n_nodes)
+        rows = most * B
+        if most < 0 or rows > MAX_ROWS:
+            raise ValueError(f"{fn}: n_nodes={n_nodes} for {B} sequences")
+    _on_current_device(fn, k_cache, v_cache, page_table, lens, paths, q_start)
+    out = torch.empty_like(lens, memory_format=torch.contiguous_format)
+    desc = _lib.PagedCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), *sk, *sv, page_table.data_ptr(), page_table.stride(0),
+                               lens.data_ptr(), ptr(q_start), *shape, page_table.shape[1], B, rows, most,
+                               dtype_code(k_cache.dtype))
+    _lib.call("nkl_cache_accept", ctypes.byref(desc), paths.data_ptr(), paths.stride(0), paths.shape[1], out.data_ptr(),
+              layers, kl, vl, stream_handle())
+    return out
+
+
+def _paged_attention(desc, q, sq, o, so, H: int, window: int, sinks: int, words: int | None, nwords: int,
+                     scale: float) -> None:
+    """nkl_paged_attention on operands already checked."""
+    L, ref = _lib.lib(), ctypes.byref(desc)
+    nbytes = L.nkl_paged_attention_workspace_bytes(ref, H, window, sinks, int(words is not None))
+    ws = workspace(nbytes, q.device) if nbytes else None
+    rc = L.nkl_paged_attention(ref, q.data_ptr(), o.data_ptr(), H, *sq, *so, window, sinks, words, nwords, scale, ptr(ws),
+                               nbytes, stream_handle())
+    if rc:
+        _lib.check("nkl_paged_attention", rc)
+
+
+def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         page_table: torch.Tensor, lens: torch.Tensor, q_start: torch.Tensor | None = None,
+                         max_q: int | None = None, window: int | None = None, sinks: int = 0,
+                         tree: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Attention of new tokens over a paged cache that holds their K and V rows
+    already (``cache_append_into``), into o; q, o: [rows, H, d], H a multiple of
+    the caches' kv_heads (query head h reads K/V head h // (H / kv_heads)).
+    The cache arguments are those of ``cache_append_into``.
+
+    New row i of n, at position p = lens[b] - n + i, sees the keys j <= p: all
+    of them, or with a window those with j > p - window or j < sinks.  With a
+    tree (``tree_mask``'s words, or any bits: bit i lets it see new row i) it
+    sees those new rows, and of the rows before them those in the window of
+    position lens[b] - n - 1 + (new rows it sees), and the sinks.  A row that
+    sees nothing gets zeros.  Keys a row does not see take no part, whatever
+    they hold; pages that no row of the call sees are not read, and may have
+    been freed.  Rows of o that belong to no sequence are left as they are.
+    d a multiple of 8 (fp32: 4), at most 128; scale above 0."""
+    fn = "paged_attention_into"
+    if q.dim() != 3 or o.shape != q.shape or o.dtype != q.dtype:
+        raise ValueError(f"{fn}: q {tuple(q.shape)} {q.dtype} and o {tuple(o.shape)} {o.dtype} must be equal [rows, H, d]")
+    if q.dtype != k_cache.dtype:
+        raise TypeError(f"{fn}: q {q.dtype} and the caches {k_cache.dtype} must share a dtype")
+    desc = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, q.shape[0], max_q)
+    rows, H, d = q.shape
+    if d != desc.d or H < 1 or H % max(desc.kv_heads, 1):
+        raise ValueError(f"{fn}: q {tuple(q.shape)} does not match caches {tuple(k_cache.shape)}")
+    window, sinks = _window_sinks(fn, window, sinks)
+    words, nwords = _tree_words(fn, tree, rows, desc.max_new)
+    if scale is None:
+        scale = 1.0 / math.sqrt(d) if d else 1.0
+    _on_current_device(fn, q, o, k_cache, v_cache, page_table, lens, q_start, tree)
+    if rows == 0 or desc.max_new == 0:
+        return o
+    E = 16 // q.element_size()
+    q = _rows_operand(q, E)
+    out = o if _rows_ok(o, E) else o.clone(memory_format=torch.contiguous_format)
+    _paged_attention(desc, q, q.stride()[:2], out, out.stride()[:2], H, window, sinks, words, nwords, float(scale))
+    if out is not o:
+        o.copy_(out)
+    return o
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    lens: torch.Tensor, q_start: torch.Tensor | None = None, max_q: int | None = None,
+                    window: int | None = None, sinks: int = 0, tree: torch.Tensor | None = None,
+                    scale: float | None = None) -> torch.Tensor:
+    """``paged_attention_into`` a new tensor (whose rows that belong to no
+    sequence, if there are any, hold nothing of meaning)."""
+    return paged_attention_into(q, torch.empty(q.shape, dtype=q.dtype, device=q.device), k_cache, v_cache, page_table,
+                                lens, q_start, max_q, window, sinks, tree, scale)
