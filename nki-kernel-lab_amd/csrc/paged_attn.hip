@@ -36,6 +36,8 @@
 // captured graph can be replayed with other lengths.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.h"
 
 namespace nkl {
@@ -48,6 +50,11 @@ using fsched::kRescaleSlack;
 
 constexpr int BN = 32;  // keys per tile
 
+// A row tile whose keys are split: it begins in a range, and has `parts` parts.
+struct Join {
+  int b, kvh, r0, parts;
+};
+
 struct PagedArgs {
   CacheArgs c;
   const unsigned char* q;
@@ -58,9 +65,10 @@ struct PagedArgs {
   int H, group, window, sinks;  // window 0: none
   float scale_log2e;
   Div32 dv_group;
-  // Split over keys (part != nullptr): workgroups to aim for, the fewest key
-  // tiles of a share.
+  // Split over keys (part != nullptr): workgroups, and the fewest key tiles of
+  // a range.  joins: one for each range.
   float* part;
+  Join* joins;
   int target, min_tiles;
   int tiles_max;  // row tiles of the longest sequence
   int per_xcd;    // not split: items per XCD
@@ -95,61 +103,55 @@ __device__ __forceinline__ Span span_of(const PagedArgs& p, const Seq& s, int r0
   return x;
 }
 
-// Split schedule.  Shares hold C key tiles at most: C is the total over every
-// (sequence, K/V head, row tile) divided by the target, and an item of nt
-// tiles has ceil(nt / C) shares of equal length.  Numbered by sequence, then
-// row tile, share and K/V head.  Every lane of a wavefront takes a sequence.
+// Split schedule.  A row tile of a K/V head holds as many units as it has key
+// tiles (one where it sees nothing: its zeros are to be written), numbered by
+// sequence, row tile and K/V head.  The units are cut into ranges of equal
+// length, one a workgroup, so that ragged lengths leave no workgroup behind;
+// only a range's first and last segment can be part of a row tile.
 template <int MR>
-__device__ __forceinline__ int seq_tiles(const PagedArgs& p, const Seq& s, int share) {
+__device__ __forceinline__ int seq_units(const PagedArgs& p, const Seq& s) {
   int sum = 0;
   const int rows = s.use * p.group;
-  for (int r0 = 0; r0 < rows; r0 += MR) {
-    const int nt = span_of(p, s, r0, MR).nt;
-    // (a tile of rows that sees nothing still has its zeros to write)
-    sum += share ? (max(nt, 1) + share - 1) / share : nt;
-  }
-  return sum;
+  for (int r0 = 0; r0 < rows; r0 += MR) sum += max(span_of(p, s, r0, MR).nt, 1);
+  return sum * p.c.kv_heads;
 }
 
+// Where workgroup w's range lies: its units [u, u1), the sequence that u is of
+// and that sequence's first unit.  Every lane of a wavefront takes a sequence
+// (64 at a time); the results are the same in all of them.  The plan refuses
+// calls of 2^31 units.
 template <int MR>
-__device__ int share_tiles(const PagedArgs& p) {
-  const int lane = threadIdx.x & 63;
-  long total = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += 64)
-    if (b0 + lane < p.c.batch) total += seq_tiles<MR>(p, seq_of(p.c, b0 + lane), 0);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, kWave);
-  total *= p.c.kv_heads;
-  const long c = (total + p.target - 1) / p.target;
-  return (int)max(c, (long)p.min_tiles);
-}
-
-// Shares of the sequences before b, over every K/V head: wavefront-wide.
-// Finds, for workgroup w, its sequence and the number of its first share
-// (b = batch when w lies past the last).
-template <int MR>
-__device__ void find_seq(const PagedArgs& p, int share, int w, int& b, int& first) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += 64) {
-    const int n = b0 + lane < p.c.batch ? seq_tiles<MR>(p, seq_of(p.c, b0 + lane), share) * p.c.kv_heads : 0;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(incl, o, kWave);
-      if (lane >= o) incl += x;
+__device__ __forceinline__ void find_range(const PagedArgs& p, int w, int& len, int& u, int& u1, int& b, int& first) {
+  const int lane = threadIdx.x & 63, batch = p.c.batch;
+  auto scan = [&](int b0) __attribute__((always_inline)) {  // units of sequences b0 .. b0 + lane
+    int x = b0 + lane < batch ? seq_units<MR>(p, seq_of(p.c, b0 + lane)) : 0;
+    for (int o = 1; o < 64 && o < batch; o <<= 1) {
+      const int y = __shfl_up(x, o, kWave);
+      if (lane >= o) x += y;
     }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(w < base + incl);
+    return x;
+  };
+  int incl = scan(0);
+  int total = __builtin_amdgcn_readlane(incl, 63 < batch ? 63 : batch - 1);
+  for (int b0 = 64; b0 < batch; b0 += 64)
+    total += __builtin_amdgcn_readlane(scan(b0), batch - b0 > 64 ? 63 : batch - b0 - 1);
+  len = max((int)(((long)total + p.target - 1) / p.target), p.min_tiles);
+  u = (int)min((long)w * len, (long)total);
+  u1 = (int)min((long)u + len, (long)total);
+  first = 0;
+  b = batch;
+  if (u >= u1) return;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    if (b0 > 0) incl = scan(b0);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(b0 + lane < batch && u < first + incl);
     if (past) {
       const int l = __builtin_ctzll(past);
       b = b0 + l;
-      first = base + __shfl(incl - n, l, kWave);
+      if (l > 0) first += __builtin_amdgcn_readlane(incl, l - 1);
       return;
     }
-    base += __shfl(incl, 63, kWave);
+    first += __builtin_amdgcn_readlane(incl, 63);
   }
-  b = p.c.batch;
-  first = 0;
 }
 
 __device__ __forceinline__ unsigned low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
@@ -200,182 +202,124 @@ struct Lay {
   static_assert(BYTES <= 160 * 1024, "LDS");
 };
 
+// All ones in the elements of w (one of 32 bits or two of 16) that are
+// infinite or NaN: an exponent of ones carries into the sign's place.
+template <typename T>
+__device__ __forceinline__ unsigned not_finite(unsigned w) {
+  if constexpr (El<T>::W32) {
+    return (unsigned)((int)((w & 0x7f800000u) + 0x00800000u) >> 31);
+  } else {
+    constexpr unsigned kExp = El<T>::H ? 0x7c007c00u : 0x7f807f80u, kLow = El<T>::H ? 0x04000400u : 0x00800080u;
+    const unsigned x = ((w & kExp) + kLow) & 0x80008000u;
+    return x | (x - (x >> 15));
+  }
+}
+
 // State of a share in the workspace: MR rows of DP floats, then MR (m, l).
 template <int DP, int MR>
 constexpr long part_floats() {
   return (long)MR * (DP + 2);
 }
 
-template <typename T, int DP, int WPT, int NT>
-__global__ __launch_bounds__(64 * WPT * NT) __attribute__((amdgpu_waves_per_eu(1, 2)))
+template <typename T, int DP, int WPT, int NT, bool TP, bool SPLIT>
+__global__ __launch_bounds__(64 * WPT * NT) __attribute__((amdgpu_waves_per_eu(El<T>::W32 && WPT == 1 && DP == 128 ? 1 : 2)))
 void paged_attn_kernel(PagedArgs p) {
   using L = Lay<T, DP, WPT, NT>;
   constexpr bool W32 = L::W32, H16 = El<T>::H;
   constexpr int MR = L::MR, TT = L::TT, CPR = L::CPR, CH = L::CH, NDB = L::NDB, E = L::E;
   __shared__ __align__(16) unsigned char smem[L::BYTES];
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int team = wid / WPT, wq = wid % WPT, ttid = tid % TT;
-  const int h32 = lane >> 5, l32 = lane & 31;
   const CacheArgs& c = p.c;
 
-  // ---- which rows, and which of their key tiles
-  int b, kvh, r0, c0, c1;
-  bool whole = true;
+  // ---- this workgroup's units: a range of them, or one row tile's
+  int b, kvh, r0;
+  int len = 1, u = 0, u1 = 1;
+  int skip = 0;  // key tiles of the row tile before the range
   Seq s;
-  Span sp;
-  if (p.part) {
-    const int share = share_tiles<MR>(p);
+  if constexpr (SPLIT) {
     int first;
-    find_seq<MR>(p, share, blockIdx.x, b, first);
-    b = __builtin_amdgcn_readfirstlane(b);
-    if (b >= c.batch) return;
-    s = seq_of(c, b);
-    const int x = (int)blockIdx.x - __builtin_amdgcn_readfirstlane(first);
-    kvh = x % c.kv_heads;
-    int k = x / c.kv_heads, n = 0;
-    for (r0 = 0;; r0 += MR) {
-      sp = span_of(p, s, r0, MR);
-      n = (max(sp.nt, 1) + share - 1) / share;
-      if (k < n) break;
-      k -= n;
+    find_range<MR>(p, blockIdx.x, len, u, u1, b, first);
+    if (u >= u1) {
+      if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
+      return;
     }
-    whole = n == 1;
-    c0 = (int)((long)sp.nt * k / n);
-    c1 = (int)((long)sp.nt * (k + 1) / n);
+    s = seq_of(c, b);
+    int x = u - first;
+    for (r0 = 0;; r0 += MR) {
+      const int nt = max(span_of(p, s, r0, MR).nt, 1);
+      if (x < nt * c.kv_heads) {
+        kvh = x / nt;
+        skip = x - kvh * nt;
+        break;
+      }
+      x -= nt * c.kv_heads;
+    }
   } else {
     // Workgroups are dealt to the 8 XCDs in turn: item (id % 8) per_xcd + id / 8
     // keeps the row tiles of a K/V head, which read the same keys, on one L2.
     const int id = blockIdx.x, item = (id & 7) * p.per_xcd + (id >> 3);
-    const int heads = c.batch * c.kv_heads;
     const int hb = item / p.tiles_max;
-    if (hb >= heads) return;
+    if (hb >= c.batch * c.kv_heads) return;
     b = hb / c.kv_heads;
     kvh = hb - b * c.kv_heads;
     r0 = (item - hb * p.tiles_max) * MR;
     s = seq_of(c, b);
     if (r0 >= s.use * p.group) return;
-    sp = span_of(p, s, r0, MR);
-    c0 = 0;
-    c1 = sp.nt;
   }
 
-  // ---- this lane's row
-  const int row = r0 + 32 * wq + l32;
-  const bool row_ok = row < s.use * p.group;
-  const int ri = row_ok ? (int)div32(p.dv_group, (unsigned)row) : 0;  // its token
-  const int head = kvh * p.group + (row_ok ? row - ri * p.group : 0);
-  const unsigned* words = p.tree ? p.tree + (long)(s.t0 + ri) * p.tree_words32 : nullptr;
-  int pos = s.pos0 + ri;
-  if (p.tree) {
-    int seen = 0;
-    if (p.window)
-      for (int w = 0; 32 * w < s.n && w < p.tree_words32; ++w) seen += __popc(words[w] & low_bits(s.n - 32 * w));
-    pos = s.pos0 - 1 + seen;
-  }
-  // Keys of a tile that every row of the wavefront sees need no mask: those
-  // below `below`, from `from` on (or below the sinks).
-  int below, from = 0;
-  {
-    const int first_i = (int)div32(p.dv_group, (unsigned)min(r0 + 32 * wq, s.use * p.group - 1));
-    const int last_i = (int)div32(p.dv_group, (unsigned)min(r0 + 32 * wq + 31, s.use * p.group - 1));
-    below = p.tree ? s.pos0 : s.pos0 + first_i + 1;
-    if (p.window) from = (p.tree ? s.pos0 + s.n - 1 : s.pos0 + last_i) - p.window + 1;
-  }
-
-  typedef typename std::conditional<W32, float, bf16x8>::type qfrag;
-  qfrag qf[L::NQ];
-  {
-    const T* qr = reinterpret_cast<const T*>(p.q) + (long)(s.t0 + ri) * p.q_t + (long)head * p.q_h;
-    if constexpr (W32) {
-#pragma unroll
-      for (int f = 0; f < L::NQ / 4; ++f) {
-        const int dd = 8 * f + 4 * h32;
-        const float4 t = __builtin_bit_cast(float4, ld16_or_zero(qr, dd, row_ok && dd < c.d));
-        qf[4 * f] = t.x; qf[4 * f + 1] = t.y; qf[4 * f + 2] = t.z; qf[4 * f + 3] = t.w;
-      }
-    } else {
-#pragma unroll
-      for (int f = 0; f < L::NQ; ++f) {
-        const int dd = 16 * f + 8 * h32;
-        qf[f] = __builtin_bit_cast(bf16x8, ld16_or_zero(qr, dd, row_ok && dd < c.d));
-      }
+  for (;;) {
+    // (The thread's place is read anew for each segment: the addresses made of
+    // it would else be held in registers across segments.)
+    int tid = threadIdx.x;
+    if constexpr (SPLIT) asm volatile("" : "+v"(tid));
+    const int lane = tid & 63;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int team = wid / WPT, wq = wid % WPT, ttid = tid % TT;
+    const int h32 = lane >> 5, l32 = lane & 31;
+    T* const stage0 = reinterpret_cast<T*>(smem) + team * L::TEAM;
+    // This thread's chunks of a tile in one page: byte offsets from the tile's
+    // first row, columns past d out of range.
+    int voff_k, voff_v;
+    {
+      const int ci = min(ttid, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
+      voff_k = col < c.d ? (int)sizeof(T) * (r * (int)c.k_row + col) : 0x40000000;
+      voff_v = col < c.d ? (int)sizeof(T) * (r * (int)c.v_row + col) : 0x40000000;
     }
-  }
 
-  // ---- staging
-  T* const stage0 = reinterpret_cast<T*>(smem) + team * L::TEAM;
-  const T* const Kb = reinterpret_cast<const T*>(c.k) + (long)kvh * c.k_head;
-  const T* const Vb = reinterpret_cast<const T*>(c.v) + (long)kvh * c.v_head;
-  const int nit = (c1 - c0 - team + NT - 1) / NT;       // this team's tiles
-  const int nsteps = (c1 - c0 + NT - 1) / NT;           // the workgroup's steps
-  auto tile_key = [&](int it) __attribute__((always_inline)) {
-    const int x = c0 + team + NT * it;
-    return BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
-  };
-  // The page of key l32 of the team's tile `it`, -1 where it is no key that a
-  // row of this workgroup may see.
-  auto look_up = [&](int it, int& within) __attribute__((always_inline)) {
-    within = 0;
-    if (it >= nit) return -1;
-    const int j = tile_key(it) + l32;
-    const bool in = j < sp.hi && (j >= sp.lo || j < p.sinks);
-    return in ? page_of(c, b, j, within) : -1;
-  };
-  uint4 rk[CH], rv[CH];
-  auto gload = [&](int pid, int within) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int ci = min(ttid + TT * i, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
-      const int pg = __shfl(pid, r, kWave), wi = __shfl(within, r, kWave);
-      const bool ok = pg >= 0 && col < c.d;
-      rk[i] = ld16_or_zero(Kb, (long)pg * c.k_page + (long)wi * c.k_row + col, ok);
-      rv[i] = ld16_or_zero(Vb, (long)pg * c.v_page + (long)wi * c.v_row + col, ok);
-    }
-  };
-  auto lstore = [&](T* st) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int ci = min(ttid + TT * i, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
-      *reinterpret_cast<uint4*>(st + r * L::LDK + col) = rk[i];
-      *reinterpret_cast<uint4*>(st + BN * L::LDK + r * L::LDV + col) = rv[i];
-    }
-  };
+    // ---- the segment: key tiles c0 .. c1 - 1 of row tile r0, K/V head kvh
+    const Span sp = span_of(p, s, r0, MR);
+    const int c0 = skip;
+    const int c1 = SPLIT ? min(sp.nt, skip + (u1 - u)) : sp.nt;
+    const bool whole = !SPLIT || (c0 == 0 && c1 == sp.nt);
 
-  const float cs = p.scale_log2e;
-  float m_run = -INFINITY, l_run = 0.f;
-  floatx16 oacc[NDB];
-#pragma unroll
-  for (int db = 0; db < NDB; ++db)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
-
-  // One tile from LDS: kvalid has a bit for each of its keys that was read.
-  auto compute = [&](const T* st, int k0, unsigned kvalid) __attribute__((always_inline)) {
-    floatx16 sc;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
-    if constexpr (W32) {
-#pragma unroll
-      for (int f = 0; f < L::NQ / 4; ++f) {
-        const float4 kf = *reinterpret_cast<const float4*>(st + l32 * L::LDK + 8 * f + 4 * h32);
-        sc = Mfma32<float>::mma(kf.x, qf[4 * f], sc);
-        sc = Mfma32<float>::mma(kf.y, qf[4 * f + 1], sc);
-        sc = Mfma32<float>::mma(kf.z, qf[4 * f + 2], sc);
-        sc = Mfma32<float>::mma(kf.w, qf[4 * f + 3], sc);
-      }
-    } else {
-      bf16x8 kf[L::NQ];
-#pragma unroll
-      for (int f = 0; f < L::NQ; ++f)
-        kf[f] = *reinterpret_cast<const bf16x8*>(st + l32 * L::LDK + 16 * f + 8 * h32);
-#pragma unroll
-      for (int f = 0; f < L::NQ; ++f) sc = mma32_16b<H16>(kf[f], qf[f], sc);
+    // ---- this lane's row
+    const int nrows = s.use * p.group;
+    const int row = r0 + 32 * wq + l32;
+    const bool row_ok = row < nrows;
+    const int ri = row_ok ? (int)div32(p.dv_group, (unsigned)row) : 0;  // its token
+    const int head = kvh * p.group + (row_ok ? row - ri * p.group : 0);
+    const unsigned* words = p.tree ? p.tree + (long)(s.t0 + ri) * p.tree_words32 : nullptr;
+    int pos = s.pos0 + ri;
+    if (p.tree) {
+      int seen = 0;
+      if (p.window)
+        for (int w = 0; 32 * w < s.n && w < p.tree_words32; ++w) seen += __popc(words[w] & low_bits(s.n - 32 * w));
+      pos = s.pos0 - 1 + seen;
     }
-    const bool masked = kvalid != ~0u || k0 + BN > below || (p.window && k0 < from && k0 + BN > p.sinks);
-    unsigned seen = ~0u;  // bit 8 (e / 4) + e % 4: score e's key is visible
-    if (masked) {
+    // Keys that every row of the row tile sees need no mask: those below
+    // `below`, from `from` on (or below the sinks).
+    int below, from = 0;
+    {
+      const int first_i = (int)div32(p.dv_group, (unsigned)r0);
+      const int last_i = (int)div32(p.dv_group, (unsigned)(min(r0 + MR, nrows) - 1));
+      below = p.tree ? s.pos0 : s.pos0 + first_i + 1;
+      if (p.window) from = (p.tree ? s.pos0 + s.n - 1 : s.pos0 + last_i) - p.window + 1;
+    }
+    auto is_masked = [&](int k0, unsigned kvalid) __attribute__((always_inline)) {
+      return kvalid != ~0u || k0 + BN > below || (p.window && k0 < from && k0 + BN > p.sinks);
+    };
+    // The keys k0 .. k0 + 31 that this lane's row may see, a bit each.
+    auto row_bits = [&](int k0) __attribute__((always_inline)) {
       unsigned vis = ~0u;
       if (p.window) vis = ~low_bits(pos - p.window + 1 - k0) | low_bits(p.sinks - k0);
       if (p.tree) {
@@ -384,320 +328,468 @@ void paged_attn_kernel(PagedArgs p) {
       } else {
         vis &= low_bits(pos + 1 - k0);
       }
-      seen = (vis & kvalid) >> (4 * h32);
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (!((seen >> (8 * (e >> 2) + (e & 3))) & 1)) sc[e] = -INFINITY;
-    }
-    float mx = sc[0];
-#pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
-    mx = max_xor32(mx) * cs;
-    // The running max is raised lazily: see kRescaleSlack.
-    if (__builtin_amdgcn_ballot_w64(mx > m_run + kRescaleSlack)) {
-      const float m_new = fmaxf(m_run, mx);
-      const float corr = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
-      m_run = m_new;
-      l_run *= corr;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[db][e] *= corr;
-    }
-    const float mneg = m_run == -INFINITY ? 0.f : -m_run;  // a row that has seen nothing keeps exp2(-inf) = 0
-    float rs = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      sc[e] = fast_exp2(fmaf(sc[e], cs, mneg));
-      rs += sc[e];
-    }
-    l_run += rs;
+      return vis;
+    };
 
-    const T* vt = st + BN * L::LDK;
-    if constexpr (W32) {
-      bool bad = false;
+    typedef typename std::conditional<W32, float, bf16x8>::type qfrag;
+    qfrag qf[L::NQ];
+    {
+      const T* qr = reinterpret_cast<const T*>(p.q) + (long)(s.t0 + ri) * p.q_t + (long)head * p.q_h;
+      if constexpr (W32) {
+#pragma unroll
+        for (int f = 0; f < L::NQ / 4; ++f) {
+          const int dd = 8 * f + 4 * h32;
+          const float4 t = __builtin_bit_cast(float4, ld16_or_zero(qr, dd, row_ok && dd < c.d));
+          qf[4 * f] = t.x; qf[4 * f + 1] = t.y; qf[4 * f + 2] = t.z; qf[4 * f + 3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int f = 0; f < L::NQ; ++f) {
+          const int dd = 16 * f + 8 * h32;
+          qf[f] = __builtin_bit_cast(bf16x8, ld16_or_zero(qr, dd, row_ok && dd < c.d));
+        }
+      }
+    }
+
+    // ---- staging
+    const T* const Kb = reinterpret_cast<const T*>(c.k) + (long)kvh * c.k_head;
+    const T* const Vb = reinterpret_cast<const T*>(c.v) + (long)kvh * c.v_head;
+    const int nit = (c1 - c0 - team + NT - 1) / NT;  // this team's tiles
+    const int nsteps = (c1 - c0 + NT - 1) / NT;      // the workgroup's steps
+    auto tile_key = [&](int it) __attribute__((always_inline)) {
+      const int x = c0 + team + NT * it;
+      return BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
+    };
+    // Where a tile's rows are.  In one page (TP): the page, the same for every
+    // lane, and the tile's first row in it; keys behind the first unseen one
+    // are out of range of the loads.  Otherwise: key l32's page, -1 where no
+    // row of this workgroup may see it, and its row there.
+    struct Place {
+      int pid, within;
+    };
+    auto look_up = [&](int it) __attribute__((always_inline)) {
+      Place x = {-1, 0};
+      if (it >= nit) return x;
+      if constexpr (TP) {
+        x.pid = page_of(c, b, tile_key(it), x.within);
+      } else {
+        const int j = tile_key(it) + l32;
+        if (j < sp.hi && (j >= sp.lo || j < p.sinks)) x.pid = page_of(c, b, j, x.within);
+      }
+      return x;
+    };
+    uint4 rk[CH], rv[CH];
+    // Loads tile `it` and returns a bit for each of its keys that is read.
+    auto gload = [&](int it, Place x) __attribute__((always_inline)) -> unsigned {
+      if constexpr (TP) {
+        const int n = x.pid >= 0 ? min(BN, sp.hi - tile_key(it)) : 0;
+        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(Kb + (n > 0 ? x.pid * c.k_page + x.within * c.k_row : 0)), (short)0,
+            n > 0 ? (int)sizeof(T) * ((n - 1) * (int)c.k_row + c.d) : 0, fsched::kBufferFlags);
+        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(Vb + (n > 0 ? x.pid * c.v_page + x.within * c.v_row : 0)), (short)0,
+            n > 0 ? (int)sizeof(T) * ((n - 1) * (int)c.v_row + c.d) : 0, fsched::kBufferFlags);
+        // (left opaque, so that no register holds an offset for each of the loads)
+        int step_k = (TT / CPR) * (int)sizeof(T) * (int)c.k_row, step_v = (TT / CPR) * (int)sizeof(T) * (int)c.v_row;
+        asm volatile("" : "+s"(step_k), "+s"(step_v));
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, 0));
+          rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, 0));
+        }
+        return low_bits(n);
+      } else {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int ci = min(ttid + TT * i, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
+          const int pg = __shfl(x.pid, r, kWave), wi = __shfl(x.within, r, kWave);
+          const bool ok = pg >= 0 && col < c.d;
+          rk[i] = ld16_or_zero(Kb, (long)pg * c.k_page + (long)wi * c.k_row + col, ok);
+          rv[i] = ld16_or_zero(Vb, (long)pg * c.v_page + (long)wi * c.v_row + col, ok);
+        }
+        return (unsigned)__builtin_amdgcn_ballot_w64(x.pid >= 0);
+      }
+    };
+    // Stages the loaded tile.  Where the tile is masked its infinities and NaN
+    // of V are left out (0 * inf would reach the rows that do not see them) and
+    // counted, to be given to the rows that see them after the loop.
+    unsigned odd_v = 0;
+    auto lstore = [&](T* st, bool masked) __attribute__((always_inline)) {
       if (masked) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          unsigned w[4] = {rv[i].x, rv[i].y, rv[i].z, rv[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned odd = not_finite<T>(w[k]);
+            w[k] &= ~odd;
+            odd_v |= odd;
+          }
+          rv[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int ci = min(ttid + TT * i, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
+        *reinterpret_cast<uint4*>(st + r * L::LDK + col) = rk[i];
+        *reinterpret_cast<uint4*>(st + BN * L::LDK + r * L::LDV + col) = rv[i];
+      }
+    };
+
+    const float cs = p.scale_log2e;
+    float m_run = -INFINITY, l_run = 0.f;
+    floatx16 oacc[NDB];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
+
+    auto qk = [&](const T* st, floatx16& sc) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+      if constexpr (W32) {
+#pragma unroll
+        for (int f = 0; f < L::NQ / 4; ++f) {
+          const float4 kf = *reinterpret_cast<const float4*>(st + l32 * L::LDK + 8 * f + 4 * h32);
+          sc = Mfma32<float>::mma(kf.x, qf[4 * f], sc);
+          sc = Mfma32<float>::mma(kf.y, qf[4 * f + 1], sc);
+          sc = Mfma32<float>::mma(kf.z, qf[4 * f + 2], sc);
+          sc = Mfma32<float>::mma(kf.w, qf[4 * f + 3], sc);
+        }
+      } else {
+        // Every fragment read is in flight before the first MFMA waits for one.
+        bf16x8 kf[L::NQ];
+#pragma unroll
+        for (int f = 0; f < L::NQ; ++f)
+          kf[f] = *reinterpret_cast<const bf16x8*>(st + l32 * L::LDK + 16 * f + 8 * h32);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < L::NQ; ++f) sc = mma32_16b<H16>(kf[f], qf[f], sc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // Masks the scores of keys k0 .., raises the running max and turns S into P.
+    auto softmax = [&](floatx16& sc, int k0, unsigned kvalid) __attribute__((always_inline)) {
+      if (is_masked(k0, kvalid)) {
+        const unsigned seen = (row_bits(k0) & kvalid) >> (4 * h32);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const unsigned m = (unsigned)((int)(seen << (31 - (8 * (e >> 2) + (e & 3)))) >> 31);
+          sc[e] = __uint_as_float((__float_as_uint(sc[e]) & m) | (0xff800000u & ~m));
+        }
+      }
+      float mx = sc[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+      mx = max_xor32(mx) * cs;
+      // The running max is raised lazily: see kRescaleSlack.
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + kRescaleSlack)) {
+        const float m_new = fmaxf(m_run, mx);
+        const float corr = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            bad |= (__float_as_uint(vt[(8 * (e >> 2) + 4 * h32 + (e & 3)) * L::LDV + 32 * db + l32]) & 0x7f800000u) ==
-                   0x7f800000u;
+          for (int e = 0; e < 16; ++e) oacc[db][e] *= corr;
       }
-      if (__builtin_amdgcn_ballot_w64(bad)) {
-#pragma unroll 1
-        for (int db = 0; db < NDB; ++db) {
-          floatx16 fin, pos_inf, neg_inf;
+      const float mneg = m_run == -INFINITY ? 0.f : -m_run;  // a row that has seen nothing keeps exp2(-inf) = 0
+      float rs = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) fin[e] = pos_inf[e] = neg_inf[e] = 0.f;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float v = vt[(8 * (e >> 2) + 4 * h32 + (e & 3)) * L::LDV + 32 * db + l32];
-            const float ind = (seen >> (8 * (e >> 2) + (e & 3))) & 1 ? 1.f : 0.f;
-            fin = Mfma32<float>::mma(fabsf(v) < INFINITY ? v : 0.f, sc[e], fin);
-            pos_inf = Mfma32<float>::mma(!(v < INFINITY) ? 1.f : 0.f, ind, pos_inf);
-            neg_inf = Mfma32<float>::mma(!(v > -INFINITY) ? 1.f : 0.f, ind, neg_inf);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float x = fin[e] + (pos_inf[e] > 0.f ? INFINITY : 0.f) + (neg_inf[e] > 0.f ? -INFINITY : 0.f);
-#pragma unroll
-            for (int d2 = 0; d2 < NDB; ++d2) oacc[d2][e] += d2 == db ? x : 0.f;
-          }
-        }
-      } else {
+      for (int e = 0; e < 16; ++e) {
+        sc[e] = fast_exp2(fmaf(sc[e], cs, mneg));
+        rs += sc[e];
+      }
+      l_run += rs;
+    };
+    auto pv = [&](const T* st, const floatx16& sc) __attribute__((always_inline)) {
+      const T* vt = st + BN * L::LDK;
+      if constexpr (W32) {
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             oacc[db] = Mfma32<float>::mma(vt[(8 * (e >> 2) + 4 * h32 + (e & 3)) * L::LDV + 32 * db + l32], sc[e], oacc[db]);
+      } else {
+        // P is rounded to the operands' type for the MFMA; the row sums are of
+        // the unrounded values.
+        bf16x8 pf[2];
+#pragma unroll
+        for (int u2 = 0; u2 < 2; ++u2)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pf[u2][j] = round16<H16>(sc[8 * u2 + j]);
+        const int i16 = lane & 15, g2 = (lane >> 4) & 1;
+        const T* va = vt + (4 * h32 + (i16 >> 2)) * L::LDV + 16 * g2 + 4 * (i16 & 3);
+        // Two d-blocks' fragments are read together before their MFMAs.
+        constexpr int G = NDB >= 2 ? 2 : 1;
+#pragma unroll
+        for (int d0 = 0; d0 < NDB; d0 += G) {
+          bf16x8 vf[G][2];
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int u2 = 0; u2 < 2; ++u2) {
+              const T* a = va + 16 * u2 * L::LDV + 32 * (d0 + g);
+              const shortx4 x = ds_read_tr16_b64_tracked(a), y = ds_read_tr16_b64_tracked(a + 8 * L::LDV);
+              vf[g][u2] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int u2 = 0; u2 < 2; ++u2) oacc[d0 + g] = mma32_16b<H16>(vf[g][u2], pf[u2], oacc[d0 + g]);
+        }
+      }
+    };
+
+    Place at = look_up(0);
+    unsigned kvalid = gload(0, at), kv_next;
+    at = look_up(1);
+    if constexpr (WPT > 1) {
+      // A team's wavefronts share its tiles: two stages, tile it + 1 written to
+      // the other stage between a step's first MFMAs and its softmax, one
+      // barrier a step.
+      auto lds_barrier = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wavefront's LDS accesses
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_barrier();
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      };
+      lstore(stage0, is_masked(tile_key(0), kvalid));
+      lds_barrier();
+      kv_next = gload(1, at);
+      at = look_up(2);
+#pragma unroll 1
+      for (int it = 0; it < nsteps; ++it) {
+        const T* st = stage0 + (it & 1) * L::STAGE;
+        const int k0 = tile_key(it);
+        floatx16 sc;
+        if (it < nit) qk(st, sc);
+        lstore(stage0 + ((it + 1) & 1) * L::STAGE, is_masked(tile_key(it + 1), kv_next));
+        const unsigned kv = kvalid;
+        kvalid = kv_next;
+        kv_next = gload(it + 2, at);
+        at = look_up(it + 3);
+        if (it < nit) {
+          softmax(sc, k0, kv);
+          __builtin_amdgcn_sched_barrier(0);
+          pv(st, sc);
+        }
+        lds_barrier();
       }
     } else {
-      // P is rounded to the operands' type for the MFMA; the sum above is of
-      // the unrounded values.
-      bf16x8 pf[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pf[u][j] = round16<H16>(sc[8 * u + j]);
-      const int i16 = lane & 15, g2 = (lane >> 4) & 1;
-      const T* va = vt + (4 * h32 + (i16 >> 2)) * L::LDV + 16 * g2 + 4 * (i16 & 3);
-      auto vfrag = [&](int db, int u) __attribute__((always_inline)) {
-        const T* a = va + 16 * u * L::LDV + 32 * db;
-        const shortx4 x = ds_read_tr16_b64_tracked(a), y = ds_read_tr16_b64_tracked(a + 8 * L::LDV);
-        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-      };
-      bf16x8 vf[NDB][2];
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) vf[db][u] = vfrag(db, u);
-      constexpr unsigned kExp = H16 ? 0x7c00u : 0x7f80u, kOne = H16 ? 0x3c00u : 0x3f80u;
-      bool bad = false;
-      if (masked) {
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint4 x = __builtin_bit_cast(uint4, vf[db][u]);
-            const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              bad |= (w[k] & kExp) == kExp || ((w[k] >> 16) & kExp) == kExp;
-          }
-      }
-      if (__builtin_amdgcn_ballot_w64(bad)) {
-        // Some V of this tile is not finite: its finite values are multiplied
-        // as ever, and what its infinities and NaN do to the rows that see
-        // them is found with 0/1 operands (a NaN counts as both infinities).
-        typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-        u16x8 ind[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int e = 8 * u + j;
-            ind[u][j] = (seen >> (8 * (e >> 2) + (e & 3))) & 1 ? kOne : 0;
-          }
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          floatx16 pos_inf, neg_inf;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pos_inf[e] = neg_inf[e] = 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const u16x8 v = __builtin_bit_cast(u16x8, vf[db][u]);
-            u16x8 f, pi, ni;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const bool fin = (v[j] & kExp) != kExp, nan = !fin && (v[j] & (0x7fffu & ~kExp)) != 0;
-              f[j] = fin ? v[j] : 0;
-              pi[j] = !fin && (nan || !(v[j] & 0x8000u)) ? kOne : 0;
-              ni[j] = !fin && (nan || (v[j] & 0x8000u)) ? kOne : 0;
-            }
-            oacc[db] = mma32_16b<H16>(__builtin_bit_cast(bf16x8, f), pf[u], oacc[db]);
-            pos_inf = mma32_16b<H16>(__builtin_bit_cast(bf16x8, pi), __builtin_bit_cast(bf16x8, ind[u]), pos_inf);
-            neg_inf = mma32_16b<H16>(__builtin_bit_cast(bf16x8, ni), __builtin_bit_cast(bf16x8, ind[u]), neg_inf);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            oacc[db][e] += (pos_inf[e] > 0.f ? INFINITY : 0.f) + (neg_inf[e] > 0.f ? -INFINITY : 0.f);
-        }
-      } else {
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) oacc[db] = mma32_16b<H16>(vf[db][u], pf[u], oacc[db]);
-      }
-    }
-  };
-  auto valid_bits = [&](int pid) __attribute__((always_inline)) {
-    return (unsigned)__builtin_amdgcn_ballot_w64(pid >= 0);
-  };
-
-  int within, pid = look_up(0, within);
-  unsigned kvalid = valid_bits(pid);
-  gload(pid, within);
-  pid = look_up(1, within);
-  const int steps = WPT > 1 ? nsteps : nit;
 #pragma unroll 1
-  for (int it = 0; it < steps; ++it) {
-    T* st = stage0 + (L::STAGES > 1 ? (it & 1) * L::STAGE : 0);
-    lstore(st);
-    if constexpr (WPT > 1) {
-      // A stage is written again two steps on, past the next step's barrier,
-      // which every wavefront reaches with this step's reads behind it.
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wavefront's LDS writes
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      __builtin_amdgcn_s_barrier();
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      for (int it = 0; it < nit; ++it) {
+        const int k0 = tile_key(it);
+        lstore(stage0, is_masked(k0, kvalid));
+        const unsigned kv = kvalid;
+        kvalid = gload(it + 1, at);
+        at = look_up(it + 2);
+        floatx16 sc;
+        qk(stage0, sc);
+        softmax(sc, k0, kv);
+        pv(stage0, sc);
+      }
     }
-    const unsigned kv = kvalid;
-    kvalid = valid_bits(pid);
-    gload(pid, within);
-    pid = look_up(it + 2, within);
-    if (it < nit) compute(st, tile_key(it), kv);
-  }
 
-  // ---- the teams' states joined: team t finishes d-blocks db % NT == t
-  float l_tot = sum_xor32(l_run);  // lanes l and l ^ 32 hold the same row
-  if constexpr (NT > 1) {
-    __syncthreads();
-    float2* ml = reinterpret_cast<float2*>(smem);
-    float4* xo = reinterpret_cast<float4*>(smem + L::ML);
-    ml[wid * 64 + lane] = make_float2(m_run, l_tot);
+    // ---- what was left out of masked tiles' V, key by key
+    if (__syncthreads_or(odd_v)) {
+#pragma unroll 1
+      for (int it = 0; it < nit; ++it) {
+        const int k0 = tile_key(it);
+        const unsigned vis = row_bits(k0);
+#pragma unroll 1
+        for (int kk = 0; kk < BN; ++kk) {
+          const int j = k0 + kk;
+          if (j >= sp.hi || (j < sp.lo && j >= p.sinks)) continue;
+          int within;
+          const int pid = page_of(c, b, j, within);
+          // (only where the loop left it out: a tile that it took as masked)
+          if (pid < 0 || !is_masked(k0, TP && sp.hi - k0 >= BN ? ~0u : 0u)) continue;
+          const T* vr = Vb + (long)pid * c.v_page + (long)within * c.v_row + 4 * h32;
+          const unsigned sees = (unsigned)((int)(vis << (31 - kk)) >> 31);
+          // (left opaque, so that no register holds a bound for each of the loads)
+          int left = c.d;
+          asm volatile("" : "+s"(left));
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
-      if (db % NT != team)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          xo[((wid * NDB + db) * 4 + k) * 64 + lane] =
-              make_float4(oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]);
-    __syncthreads();
-    float mt[NT], lt[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const float2 x = ml[(t * WPT + wq) * 64 + lane];
-      mt[t] = x.x;
-      lt[t] = x.y;
-    }
-    m_run = mt[0];
-#pragma unroll
-    for (int t = 1; t < NT; ++t) m_run = fmaxf(m_run, mt[t]);
-    l_tot = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      mt[t] = mt[t] == -INFINITY ? 0.f : fast_exp2(mt[t] - m_run);  // now the team's weight
-      l_tot += lt[t] * mt[t];
-    }
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-      if (db % NT == team) {
-        floatx16 acc;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (t == db % NT) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = fmaf(oacc[db][e], mt[t], acc[e]);
-          } else {
+          for (int db = 0; db < NDB; ++db)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const float4 x = xo[(((t * WPT + wq) * NDB + db) * 4 + k) * 64 + lane];
-              acc[4 * k] = fmaf(x.x, mt[t], acc[4 * k]);
-              acc[4 * k + 1] = fmaf(x.y, mt[t], acc[4 * k + 1]);
-              acc[4 * k + 2] = fmaf(x.z, mt[t], acc[4 * k + 2]);
-              acc[4 * k + 3] = fmaf(x.w, mt[t], acc[4 * k + 3]);
+              if (32 * db + 8 * k + 4 * h32 < left) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const unsigned v = __float_as_uint(to_f32(vr[32 * db + 8 * k + e]));
+                  oacc[db][4 * k + e] += __uint_as_float(v & not_finite<float>(v) & sees);
+                }
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+      }
+    }
+
+    // ---- the teams' states joined: team t finishes d-blocks db % NT == t
+    float l_tot = sum_xor32(l_run);  // lanes l and l ^ 32 hold the same row
+    if constexpr (NT > 1) {
+      __syncthreads();
+      float2* ml = reinterpret_cast<float2*>(smem);
+      float4* xo = reinterpret_cast<float4*>(smem + L::ML);
+      ml[wid * 64 + lane] = make_float2(m_run, l_tot);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        if (db % NT != team)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            xo[((wid * NDB + db) * 4 + k) * 64 + lane] =
+                make_float4(oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]);
+      __syncthreads();
+      float mt[NT], lt[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 x = ml[(t * WPT + wq) * 64 + lane];
+        mt[t] = x.x;
+        lt[t] = x.y;
+      }
+      m_run = mt[0];
+#pragma unroll
+      for (int t = 1; t < NT; ++t) m_run = fmaxf(m_run, mt[t]);
+      l_tot = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        mt[t] = mt[t] == -INFINITY ? 0.f : fast_exp2(mt[t] - m_run);  // now the team's weight
+        l_tot += lt[t] * mt[t];
+      }
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        if (db % NT == team) {
+          floatx16 acc;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (t == db % NT) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[e] = fmaf(oacc[db][e], mt[t], acc[e]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float4 x = xo[(((t * WPT + wq) * NDB + db) * 4 + k) * 64 + lane];
+                acc[4 * k] = fmaf(x.x, mt[t], acc[4 * k]);
+                acc[4 * k + 1] = fmaf(x.y, mt[t], acc[4 * k + 1]);
+                acc[4 * k + 2] = fmaf(x.z, mt[t], acc[4 * k + 2]);
+                acc[4 * k + 3] = fmaf(x.w, mt[t], acc[4 * k + 3]);
+              }
             }
           }
+          oacc[db] = acc;
         }
-        oacc[db] = acc;
-      }
-  }
+    }
 
-  if (whole) {
-    if (row_ok) {
-      const float linv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // a row that sees nothing: zeros
-      T* orow = reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h;
+    if (whole) {
+      if (row_ok) {
+        const float linv = l_tot == 0.f ? 0.f : 1.f / l_tot;  // a row that sees nothing: zeros
+        T* orow = reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+          if (NT == 1 || db % NT == team)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int dd = 32 * db + 8 * k + 4 * h32;
+              if (dd < c.d) {
+                const float x[4] = {oacc[db][4 * k] * linv, oacc[db][4 * k + 1] * linv, oacc[db][4 * k + 2] * linv,
+                                    oacc[db][4 * k + 3] * linv};
+                store_vec<4>(orow + dd, x);
+              }
+            }
+      }
+    } else {
+      // A range's first segment, if its row tile began before: slot 0.  Else the
+      // row tile begins here and goes on in the next ranges: slot 1, and the
+      // entry by which the second kernel finds its parts.
+      if (c0 == 0 && threadIdx.x == 0)
+        p.joins[blockIdx.x] = {b, kvh, r0, (u + sp.nt - 1) / len - (int)blockIdx.x + 1};
+      float* part = p.part + (2L * blockIdx.x + (c0 > 0 ? 0 : 1)) * part_floats<DP, MR>();
+      const int r = 32 * wq + l32;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
         if (NT == 1 || db % NT == team)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int dd = 32 * db + 8 * k + 4 * h32;
-            if (dd < c.d) {
-              const float x[4] = {oacc[db][4 * k] * linv, oacc[db][4 * k + 1] * linv, oacc[db][4 * k + 2] * linv,
-                                  oacc[db][4 * k + 3] * linv};
-              store_vec<4>(orow + dd, x);
-            }
-          }
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(part + r * DP + 32 * db + 8 * k + 4 * h32) =
+                make_float4(oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]);
+      if (team == 0 && h32 == 0)
+        *reinterpret_cast<float2*>(part + MR * DP + 2 * r) = make_float2(m_run, l_tot);
     }
-  } else {
-    float* part = p.part + (long)blockIdx.x * part_floats<DP, MR>();
-    const int r = 32 * wq + l32;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-      if (NT == 1 || db % NT == team)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<float4*>(part + r * DP + 32 * db + 8 * k + 4 * h32) =
-              make_float4(oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]);
-    if (team == 0 && h32 == 0)
-      *reinterpret_cast<float2*>(part + MR * DP + 2 * r) = make_float2(m_run, l_tot);
+
+    if constexpr (!SPLIT) break;
+    // ---- the range's next segment: the next K/V head, row tile or sequence
+    u += max(c1 - c0, 1);
+    if (u >= u1) {
+      if ((whole || c0 > 0) && threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
+      break;
+    }
+    skip = 0;
+    if (++kvh == c.kv_heads) {
+      kvh = 0;
+      r0 += MR;
+      while (r0 >= s.use * p.group) {  // (u < the units in all: a later sequence has rows)
+        s = seq_of(c, ++b);
+        r0 = 0;
+      }
+    }
+    __syncthreads();  // the hand-over area is read before the next segment's tiles land there
   }
 }
 
-// Joins the shares' states: a wavefront for each row of each item that was
-// split, its lanes over the head dim.
+// Joins the parts of the row tile that begins in range blockIdx.x and ends in
+// another: a wavefront for each of its rows, its lanes over the head dim.
 template <typename T, int DP, int MR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   const CacheArgs& c = p.c;
+  const Join jn = p.joins[blockIdx.x];
+  const int n = jn.parts;
+  if (n == 0) return;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  // Row (of the longest sequence's), K/V head, sequence.
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wid);
-  const Seq s = seq_of(c, b);
+  const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + wid), row = jn.r0 + r;
+  const Seq s = seq_of(c, jn.b);
   if (row >= s.use * p.group) return;
-  const int share = share_tiles<MR>(p);
-  // The number of the sequence's first share.
-  int first = 0;
-  for (int b0 = 0; b0 < b; b0 += 64)
-    if (b0 + lane < b) first += seq_tiles<MR>(p, seq_of(c, b0 + lane), share);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, kWave);
-  const int r0 = row / MR * MR, r = row - r0;
-  for (int x = 0; x < r0; x += MR) first += (max(span_of(p, s, x, MR).nt, 1) + share - 1) / share;
-  const int n = (max(span_of(p, s, r0, MR).nt, 1) + share - 1) / share;
-  if (n == 1) return;
-  const float* part = p.part + ((long)first * c.kv_heads + kvh) * part_floats<DP, MR>();
-  const long step = (long)c.kv_heads * part_floats<DP, MR>();
-  // A lane's share(s): the max, then the weights.
+  // Part i is slot 0 of range blockIdx.x + i, the first slot 1.
+  auto part_of = [&](int i) __attribute__((always_inline)) {
+    return p.part + (2L * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0)) * part_floats<DP, MR>();
+  };
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, part[i * step + MR * DP + 2 * r]);
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, part_of(i)[MR * DP + 2 * r]);
   m = wave_max(m);
-  float l = 0.f, acc[DP / 64 > 0 ? DP / 64 : 1] = {};
   constexpr int PL = DP >= 64 ? DP / 64 : 1;
+  float l = 0.f, acc[PL] = {};
   for (int i0 = 0; i0 < n; i0 += 64) {
     float w = 0.f;
     if (i0 + lane < n) {
-      const float2 x = *reinterpret_cast<const float2*>(part + (i0 + lane) * step + MR * DP + 2 * r);
+      const float2 x = *reinterpret_cast<const float2*>(part_of(i0 + lane) + MR * DP + 2 * r);
       w = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m);
       l += x.y * w;
     }
     const int cnt = min(64, n - i0);
-#pragma unroll 4
-    for (int i = 0; i < cnt; ++i) {
-      const float wi = __shfl(w, i, kWave);
-      const float* pr = part + (i0 + i) * step + (long)r * DP;
+    for (int i1 = 0; i1 < cnt; i1 += 4) {  // four parts' loads in flight (past the last: again, weight 0)
+      float x[4][PL], wi[4];
 #pragma unroll
-      for (int k = 0; k < PL; ++k)
-        if (PL * lane + k < DP) acc[k] = fmaf(pr[PL * lane + k], wi, acc[k]);
+      for (int i = 0; i < 4; ++i) {
+        const int j = min(i1 + i, cnt - 1);
+        wi[i] = i1 + i < cnt ? __shfl(w, j, kWave) : 0.f;
+        const float* pr = part_of(i0 + j) + (long)r * DP;
+#pragma unroll
+        for (int k = 0; k < PL; ++k) x[i][k] = PL * lane + k < DP ? pr[PL * lane + k] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (wi[i] > 0.f)
+#pragma unroll
+          for (int k = 0; k < PL; ++k) acc[k] = fmaf(x[i][k], wi[i], acc[k]);
     }
   }
   l = wave_sum(l);
   const float linv = l == 0.f ? 0.f : 1.f / l;
-  const int ri = (int)div32(p.dv_group, (unsigned)row), head = kvh * p.group + row - ri * p.group;
+  const int ri = (int)div32(p.dv_group, (unsigned)row), head = jn.kvh * p.group + row - ri * p.group;
   T* orow = reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h;
 #pragma unroll
   for (int k = 0; k < PL; ++k)
@@ -712,6 +804,7 @@ struct Plan {
   bool split;
   int tiles_max; // row tiles of the longest sequence
   long items;    // row tiles at most
+  bool one_page; // a key tile lies in one page
   int target, min_tiles;
   long grid;
   size_t bytes;  // workspace
@@ -735,12 +828,19 @@ int plan_paged(const char* fn, const CacheArgs& c, int H, int window, int sinks,
   }
   const long key_tiles = (keys + BN - 1) / BN + 1;
   const int cus = cu_count();
-  pl.target = pl.wide ? cus : 4 * cus;
-  pl.min_tiles = pl.wide ? 8 : 8;
-  pl.split = pl.items < pl.target && key_tiles > 2 * pl.min_tiles;
+  pl.target = pl.wide ? cus : 2 * cus;
+  pl.min_tiles = pl.wide ? 4 : 8;
+  // Split where the row tiles leave workgroups idle, or may be of lengths so
+  // different that the longest outlasts the rest (several sequences, or a
+  // causal prompt with no window): up to four rounds of them.
+  const long rounds = c.batch == 1 && window ? 1 : 4;
+  pl.split = pl.items < rounds * pl.target && key_tiles > 2 * pl.min_tiles;
+  if (pl.split && pl.items * (key_tiles + 1) >= 1L << 31) pl.split = false;
+  // (32-bit byte offsets within a tile)
+  pl.one_page = (!c.table || c.page_size % BN == 0) && c.k_row <= (1L << 21) && c.v_row <= (1L << 21);
   if (pl.split) {
-    pl.grid = pl.target + pl.items;
-    pl.bytes = (size_t)pl.grid * mr * (pl.dp + 2) * 4;
+    pl.grid = pl.target;
+    pl.bytes = (size_t)pl.grid * (sizeof(Join) + 2 * (size_t)mr * (pl.dp + 2) * 4);
   } else {
     pl.grid = (pl.items + 7) / 8 * 8;
     pl.bytes = 0;
@@ -748,25 +848,39 @@ int plan_paged(const char* fn, const CacheArgs& c, int H, int window, int sinks,
   return NKL_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int WPT, int NT>
 int paged_launch(PagedArgs& p, const Plan& pl, hipStream_t st) {
-  const unsigned grid = (unsigned)pl.grid;
-  const dim3 jgrid((unsigned)(((long)p.c.max_new * p.group + 3) / 4), (unsigned)p.c.kv_heads, (unsigned)p.c.batch);
-  if (pl.wide) {
-    paged_attn_kernel<T, DP, 4, 2><<<dim3(grid), dim3(512), 0, st>>>(p);
-    if (pl.split) paged_join_kernel<T, DP, 128><<<jgrid, dim3(256), 0, st>>>(p);
+  const dim3 grid((unsigned)pl.grid), block(64 * WPT * NT);
+  constexpr bool TP = !El<T>::W32;
+  if (TP && pl.one_page) {
+    if (pl.split)
+      paged_attn_kernel<T, DP, WPT, NT, TP, true><<<grid, block, 0, st>>>(p);
+    else
+      paged_attn_kernel<T, DP, WPT, NT, TP, false><<<grid, block, 0, st>>>(p);
   } else {
-    paged_attn_kernel<T, DP, 1, 4><<<dim3(grid), dim3(256), 0, st>>>(p);
-    if (pl.split) paged_join_kernel<T, DP, 32><<<jgrid, dim3(256), 0, st>>>(p);
+    if (pl.split)
+      paged_attn_kernel<T, DP, WPT, NT, false, true><<<grid, block, 0, st>>>(p);
+    else
+      paged_attn_kernel<T, DP, WPT, NT, false, false><<<grid, block, 0, st>>>(p);
+  }
+  if (pl.split) {
+    const long rows = (long)p.c.max_new * p.group;
+    const dim3 jgrid((unsigned)pl.grid, (unsigned)(((rows < 32 * WPT ? rows : 32 * WPT) + 3) / 4));
+    paged_join_kernel<T, DP, 32 * WPT><<<jgrid, dim3(256), 0, st>>>(p);
   }
   return check_launch("nkl_paged_attention");
 }
 
 template <typename T>
 int paged_launch_d(PagedArgs& p, const Plan& pl, hipStream_t st) {
-  if (pl.dp == 32) return paged_launch<T, 32>(p, pl, st);
-  if (pl.dp == 64) return paged_launch<T, 64>(p, pl, st);
-  return paged_launch<T, 128>(p, pl, st);
+  if (pl.wide) {
+    if (pl.dp == 32) return paged_launch<T, 32, 4, 2>(p, pl, st);
+    if (pl.dp == 64) return paged_launch<T, 64, 4, 2>(p, pl, st);
+    return paged_launch<T, 128, 4, 2>(p, pl, st);
+  }
+  if (pl.dp == 32) return paged_launch<T, 32, 1, 4>(p, pl, st);
+  if (pl.dp == 64) return paged_launch<T, 64, 1, 4>(p, pl, st);
+  return paged_launch<T, 128, 1, 4>(p, pl, st);
 }
 
 int paged_check(const char* fn, const nkl_paged_cache* cache, int H, int window, int sinks, CacheArgs& c) {
@@ -834,7 +948,10 @@ extern "C" int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, 
   p.sinks = sinks < kMaxRows ? sinks : kMaxRows;
   p.scale_log2e = scale * kLog2e;
   p.dv_group = fsched::make_div32((unsigned)p.group);
-  p.part = pl.split ? static_cast<float*>(workspace) : nullptr;
+  if (pl.split) {
+    p.joins = static_cast<Join*>(workspace);
+    p.part = reinterpret_cast<float*>(p.joins + pl.grid);
+  }
   p.target = pl.target;
   p.min_tiles = pl.min_tiles;
   p.tiles_max = pl.tiles_max;
