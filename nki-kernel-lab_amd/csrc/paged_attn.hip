@@ -65,6 +65,7 @@ struct PagedArgs {
   int H, group, window, sinks;  // window 0: none
   float scale_log2e;
   Div32 dv_group;
+  unsigned k_page32, k_row32, v_page32, v_row32;  // byte strides, where a tile lies in one page
   // Split over keys (part != nullptr): workgroups, and the fewest key tiles of
   // a range.  joins: one for each range.
   float* part;
@@ -189,7 +190,7 @@ struct Lay {
   static constexpr int LDK = W32 ? DP + 4 : DP + 8;       // rows 4 banks apart
   static constexpr int LDV = W32 ? DP + 4 : DP + 32;      // 16-bit: rows 16 banks apart (transposed reads)
   static constexpr int STAGE = BN * (LDK + LDV);          // elements
-  static constexpr int STAGES = WPT > 1 ? 2 : 1;
+  static constexpr int STAGES = WPT == 1 ? 1 : W32 ? 2 : 3;
   static constexpr int TEAM = STAGES * STAGE;
   static constexpr int NDB = DP / 32;
   static constexpr int NQ = W32 ? DP / 2 : DP / 16;       // Q values (32-bit) or fragments a lane
@@ -282,8 +283,8 @@ void paged_attn_kernel(PagedArgs p) {
     int voff_k, voff_v;
     {
       const int ci = min(ttid, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
-      voff_k = col < c.d ? (int)sizeof(T) * (r * (int)c.k_row + col) : 0x40000000;
-      voff_v = col < c.d ? (int)sizeof(T) * (r * (int)c.v_row + col) : 0x40000000;
+      voff_k = col < c.d ? r * (int)p.k_row32 + col * (int)sizeof(T) : 0x40000000;
+      voff_v = col < c.d ? r * (int)p.v_row32 + col * (int)sizeof(T) : 0x40000000;
     }
 
     // ---- the segment: key tiles c0 .. c1 - 1 of row tile r0, K/V head kvh
@@ -306,18 +307,18 @@ void paged_attn_kernel(PagedArgs p) {
         for (int w = 0; 32 * w < s.n && w < p.tree_words32; ++w) seen += __popc(words[w] & low_bits(s.n - 32 * w));
       pos = s.pos0 - 1 + seen;
     }
-    // Keys that every row of the row tile sees need no mask: those below
-    // `below`, from `from` on (or below the sinks).
-    int below, from = 0;
+    // Tiles whose keys every row of the row tile sees need no mask: tiles
+    // f0 .. f0 + fn - 1 of the row tile (sinks' tiles are masked as others are).
+    int f0;
+    unsigned fn;
     {
       const int first_i = (int)div32(p.dv_group, (unsigned)r0);
       const int last_i = (int)div32(p.dv_group, (unsigned)(min(r0 + MR, nrows) - 1));
-      below = p.tree ? s.pos0 : s.pos0 + first_i + 1;
-      if (p.window) from = (p.tree ? s.pos0 + s.n - 1 : s.pos0 + last_i) - p.window + 1;
+      const int below = max(0, min(p.tree ? s.pos0 : s.pos0 + first_i + 1, sp.hi));
+      const int from = p.window ? (p.tree ? s.pos0 + s.n - 1 : s.pos0 + last_i) - p.window + 1 : 0;
+      f0 = sp.ns + max(0, (max(from, 0) + BN - 1) / BN - sp.m0);
+      fn = (unsigned)max(0, sp.ns + below / BN - sp.m0 - f0);
     }
-    auto is_masked = [&](int k0, unsigned kvalid) __attribute__((always_inline)) {
-      return kvalid != ~0u || k0 + BN > below || (p.window && k0 < from && k0 + BN > p.sinks);
-    };
     // The keys k0 .. k0 + 31 that this lane's row may see, a bit each.
     auto row_bits = [&](int k0) __attribute__((always_inline)) {
       unsigned vis = ~0u;
@@ -352,62 +353,83 @@ void paged_attn_kernel(PagedArgs p) {
     }
 
     // ---- staging
-    const T* const Kb = reinterpret_cast<const T*>(c.k) + (long)kvh * c.k_head;
-    const T* const Vb = reinterpret_cast<const T*>(c.v) + (long)kvh * c.v_head;
+    const unsigned char* const Kb = c.k + (long)kvh * c.k_head * (long)sizeof(T);
+    const unsigned char* const Vb = c.v + (long)kvh * c.v_head * (long)sizeof(T);
+    const int* const trow = c.table + (c.table ? (long)b * c.table_row : 0);
+    const int row_bytes = c.d * (int)sizeof(T);
     const int nit = (c1 - c0 - team + NT - 1) / NT;  // this team's tiles
     const int nsteps = (c1 - c0 + NT - 1) / NT;      // the workgroup's steps
-    auto tile_key = [&](int it) __attribute__((always_inline)) {
-      const int x = c0 + team + NT * it;
-      return BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
-    };
-    // Where a tile's rows are.  In one page (TP): the page, the same for every
-    // lane, and the tile's first row in it; keys behind the first unseen one
-    // are out of range of the loads.  Otherwise: key l32's page, -1 where no
-    // row of this workgroup may see it, and its row there.
-    struct Place {
-      int pid, within;
+    // A tile on its way through the steps: its first key, whether it needs a
+    // mask, and where its rows are.  In one page (TP): the page, the same for
+    // every lane, and the tile's first row in it; keys behind the last visible
+    // one are out of range of the loads.  Otherwise: key l32's page and row,
+    // where a row of this workgroup may see it.  The page is as the table has
+    // it: it is looked at where the tile is loaded, a step after it is read.
+    struct Tile {
+      int k0, pid, within;
+      bool masked;
     };
     auto look_up = [&](int it) __attribute__((always_inline)) {
-      Place x = {-1, 0};
-      if (it >= nit) return x;
+      const int x = c0 + team + NT * it;
+      Tile t;
+      t.k0 = BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
+      t.masked = (unsigned)(x - f0) >= fn || it >= nit;
+      t.pid = -1;
+      t.within = 0;
       if constexpr (TP) {
-        x.pid = page_of(c, b, tile_key(it), x.within);
+        if (it < nit) {
+          const int pi = (int)div32(c.dv_page, (unsigned)t.k0);
+          t.within = t.k0 - pi * c.page_size;
+          t.pid = c.table ? ((const __attribute__((address_space(4))) int*)trow)[pi] : 0;
+        }
       } else {
-        const int j = tile_key(it) + l32;
-        if (j < sp.hi && (j >= sp.lo || j < p.sinks)) x.pid = page_of(c, b, j, x.within);
+        const int j = t.k0 + l32;
+        if (it < nit && j < sp.hi && (j >= sp.lo || j < p.sinks)) {
+          const int pi = (int)div32(c.dv_page, (unsigned)j);
+          t.within = j - pi * c.page_size;
+          t.pid = c.table ? trow[pi] : 0;
+        }
       }
-      return x;
+      return t;
     };
     uint4 rk[CH], rv[CH];
-    // Loads tile `it` and returns a bit for each of its keys that is read.
-    auto gload = [&](int it, Place x) __attribute__((always_inline)) -> unsigned {
+    // Loads a tile and returns a bit for each of its keys that is read.
+    auto gload = [&](Tile& t) __attribute__((always_inline)) -> unsigned {
       if constexpr (TP) {
-        const int n = x.pid >= 0 ? min(BN, sp.hi - tile_key(it)) : 0;
+        const int n = (unsigned)t.pid < (unsigned)c.pages ? min(BN, sp.hi - t.k0) : 0;
+        const unsigned pid = n > 0 ? t.pid : 0, within = n > 0 ? t.within : 0;
         const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(Kb + (n > 0 ? x.pid * c.k_page + x.within * c.k_row : 0)), (short)0,
-            n > 0 ? (int)sizeof(T) * ((n - 1) * (int)c.k_row + c.d) : 0, fsched::kBufferFlags);
+            (void*)(Kb + (unsigned long)pid * p.k_page32 + (unsigned long)within * p.k_row32), (short)0,
+            n > 0 ? (n - 1) * (int)p.k_row32 + row_bytes : 0, fsched::kBufferFlags);
         const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(Vb + (n > 0 ? x.pid * c.v_page + x.within * c.v_row : 0)), (short)0,
-            n > 0 ? (int)sizeof(T) * ((n - 1) * (int)c.v_row + c.d) : 0, fsched::kBufferFlags);
+            (void*)(Vb + (unsigned long)pid * p.v_page32 + (unsigned long)within * p.v_row32), (short)0,
+            n > 0 ? (n - 1) * (int)p.v_row32 + row_bytes : 0, fsched::kBufferFlags);
         // (left opaque, so that no register holds an offset for each of the loads)
-        int step_k = (TT / CPR) * (int)sizeof(T) * (int)c.k_row, step_v = (TT / CPR) * (int)sizeof(T) * (int)c.v_row;
+        int step_k = (TT / CPR) * (int)p.k_row32, step_v = (TT / CPR) * (int)p.v_row32;
         asm volatile("" : "+s"(step_k), "+s"(step_v));
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, 0));
           rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, 0));
         }
+        t.masked = t.masked || n < BN;
         return low_bits(n);
       } else {
+        const bool in = (unsigned)t.pid < (unsigned)c.pages;
+        const unsigned bits = (unsigned)__builtin_amdgcn_ballot_w64(in);
+        const int pid = in ? t.pid : -1;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           const int ci = min(ttid + TT * i, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
-          const int pg = __shfl(x.pid, r, kWave), wi = __shfl(x.within, r, kWave);
+          const int pg = __shfl(pid, r, kWave), wi = __shfl(t.within, r, kWave);
           const bool ok = pg >= 0 && col < c.d;
-          rk[i] = ld16_or_zero(Kb, (long)pg * c.k_page + (long)wi * c.k_row + col, ok);
-          rv[i] = ld16_or_zero(Vb, (long)pg * c.v_page + (long)wi * c.v_row + col, ok);
+          const T* kp = reinterpret_cast<const T*>(Kb) + (long)pg * c.k_page + (long)wi * c.k_row + col;
+          const T* vp = reinterpret_cast<const T*>(Vb) + (long)pg * c.v_page + (long)wi * c.v_row + col;
+          rk[i] = ld16_or_zero(ok ? kp : reinterpret_cast<const T*>(Kb), 0, ok);
+          rv[i] = ld16_or_zero(ok ? vp : reinterpret_cast<const T*>(Vb), 0, ok);
         }
-        return (unsigned)__builtin_amdgcn_ballot_w64(x.pid >= 0);
+        t.masked = t.masked || bits != ~0u;
+        return bits;
       }
     };
     // Stages the loaded tile.  Where the tile is masked its infinities and NaN
@@ -444,33 +466,35 @@ void paged_attn_kernel(PagedArgs p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) oacc[db][e] = 0.f;
 
+    // K fragments of a tile (16-bit types), and S from them; fp32 reads K as it goes.
+    bf16x8 kf[W32 ? 1 : L::NQ];
+    auto read_k = [&](const T* st) __attribute__((always_inline)) {
+      if constexpr (!W32) {
+#pragma unroll
+        for (int f = 0; f < L::NQ; ++f)
+          kf[f] = *reinterpret_cast<const bf16x8*>(st + l32 * L::LDK + 16 * f + 8 * h32);
+      }
+    };
     auto qk = [&](const T* st, floatx16& sc) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.f;
       if constexpr (W32) {
 #pragma unroll
         for (int f = 0; f < L::NQ / 4; ++f) {
-          const float4 kf = *reinterpret_cast<const float4*>(st + l32 * L::LDK + 8 * f + 4 * h32);
-          sc = Mfma32<float>::mma(kf.x, qf[4 * f], sc);
-          sc = Mfma32<float>::mma(kf.y, qf[4 * f + 1], sc);
-          sc = Mfma32<float>::mma(kf.z, qf[4 * f + 2], sc);
-          sc = Mfma32<float>::mma(kf.w, qf[4 * f + 3], sc);
+          const float4 k4 = *reinterpret_cast<const float4*>(st + l32 * L::LDK + 8 * f + 4 * h32);
+          sc = Mfma32<float>::mma(k4.x, qf[4 * f], sc);
+          sc = Mfma32<float>::mma(k4.y, qf[4 * f + 1], sc);
+          sc = Mfma32<float>::mma(k4.z, qf[4 * f + 2], sc);
+          sc = Mfma32<float>::mma(k4.w, qf[4 * f + 3], sc);
         }
       } else {
-        // Every fragment read is in flight before the first MFMA waits for one.
-        bf16x8 kf[L::NQ];
-#pragma unroll
-        for (int f = 0; f < L::NQ; ++f)
-          kf[f] = *reinterpret_cast<const bf16x8*>(st + l32 * L::LDK + 16 * f + 8 * h32);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int f = 0; f < L::NQ; ++f) sc = mma32_16b<H16>(kf[f], qf[f], sc);
-        __builtin_amdgcn_sched_barrier(0);
       }
     };
     // Masks the scores of keys k0 .., raises the running max and turns S into P.
-    auto softmax = [&](floatx16& sc, int k0, unsigned kvalid) __attribute__((always_inline)) {
-      if (is_masked(k0, kvalid)) {
+    auto softmax = [&](floatx16& sc, int k0, bool masked, unsigned kvalid) __attribute__((always_inline)) {
+      if (masked) {
         const unsigned seen = (row_bits(k0) & kvalid) >> (4 * h32);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -502,93 +526,146 @@ void paged_attn_kernel(PagedArgs p) {
       }
       l_run += rs;
     };
+    // V fragments of d-blocks d0 .. d0 + G - 1 (16-bit types).
+    auto read_v = [&](const T* st, int d0, auto& vf) __attribute__((always_inline)) {
+      constexpr int G = sizeof(vf) / sizeof(vf[0]);
+      const int i16 = lane & 15, g2 = (lane >> 4) & 1;
+      const T* va = st + BN * L::LDK + (4 * h32 + (i16 >> 2)) * L::LDV + 16 * g2 + 4 * (i16 & 3);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int u2 = 0; u2 < 2; ++u2) {
+          const T* a = va + 16 * u2 * L::LDV + 32 * (d0 + g);
+          const shortx4 x = ds_read_tr16_b64_tracked(a), y = ds_read_tr16_b64_tracked(a + 8 * L::LDV);
+          vf[g][u2] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+    // P is rounded to the operands' type for the MFMA; the row sums are of the
+    // unrounded values.
+    auto to_p = [&](const floatx16& sc, bf16x8 (&pf)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u2 = 0; u2 < 2; ++u2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[u2][j] = round16<H16>(sc[8 * u2 + j]);
+    };
+    auto mma_v = [&](const auto& vf, const bf16x8 (&pf)[2], int d0) __attribute__((always_inline)) {
+      constexpr int G = sizeof(vf) / sizeof(vf[0]);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int u2 = 0; u2 < 2; ++u2) oacc[d0 + g] = mma32_16b<H16>(vf[g][u2], pf[u2], oacc[d0 + g]);
+    };
     auto pv = [&](const T* st, const floatx16& sc) __attribute__((always_inline)) {
-      const T* vt = st + BN * L::LDK;
       if constexpr (W32) {
+        const T* vt = st + BN * L::LDK;
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             oacc[db] = Mfma32<float>::mma(vt[(8 * (e >> 2) + 4 * h32 + (e & 3)) * L::LDV + 32 * db + l32], sc[e], oacc[db]);
       } else {
-        // P is rounded to the operands' type for the MFMA; the row sums are of
-        // the unrounded values.
         bf16x8 pf[2];
-#pragma unroll
-        for (int u2 = 0; u2 < 2; ++u2)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) pf[u2][j] = round16<H16>(sc[8 * u2 + j]);
-        const int i16 = lane & 15, g2 = (lane >> 4) & 1;
-        const T* va = vt + (4 * h32 + (i16 >> 2)) * L::LDV + 16 * g2 + 4 * (i16 & 3);
+        to_p(sc, pf);
         // Two d-blocks' fragments are read together before their MFMAs.
         constexpr int G = NDB >= 2 ? 2 : 1;
 #pragma unroll
         for (int d0 = 0; d0 < NDB; d0 += G) {
           bf16x8 vf[G][2];
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int u2 = 0; u2 < 2; ++u2) {
-              const T* a = va + 16 * u2 * L::LDV + 32 * (d0 + g);
-              const shortx4 x = ds_read_tr16_b64_tracked(a), y = ds_read_tr16_b64_tracked(a + 8 * L::LDV);
-              vf[g][u2] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-            }
+          read_v(st, d0, vf);
           __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int u2 = 0; u2 < 2; ++u2) oacc[d0 + g] = mma32_16b<H16>(vf[g][u2], pf[u2], oacc[d0 + g]);
+          mma_v(vf, pf, d0);
         }
       }
     };
 
-    Place at = look_up(0);
-    unsigned kvalid = gload(0, at), kv_next;
-    at = look_up(1);
-    if constexpr (WPT > 1) {
-      // A team's wavefronts share its tiles: two stages, tile it + 1 written to
-      // the other stage between a step's first MFMAs and its softmax, one
-      // barrier a step.
-      auto lds_barrier = [&]() __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wavefront's LDS accesses
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        __builtin_amdgcn_s_barrier();
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      };
-      lstore(stage0, is_masked(tile_key(0), kvalid));
+    // The tile that a step computes, the one that it stages (loaded a step
+    // before) and the one that it loads (looked up a step before).
+    Tile cur = look_up(0), nxt = look_up(1), far;
+    unsigned kv_cur = gload(cur), kv_nxt;
+    // Every wavefront's LDS accesses are done, then all wavefronts meet (with
+    // __syncthreads() the loads in flight would be waited for too).
+    auto lds_barrier = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      __builtin_amdgcn_s_barrier();
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    };
+    if constexpr (WPT > 1 && !W32) {
+      // A team's wavefronts share its tiles, staged one step ahead.  A step's
+      // LDS reads are in flight while others compute: V's go out before the
+      // softmax, the next tile's K before P V.  The barrier between the two
+      // covers tile it + 1's staging, three stages deep: the stage that step
+      // `it` writes was last read by P V of tile it - 2, which every wavefront
+      // had behind it at the barrier of step it - 1.
+      far = look_up(2);
+      lstore(stage0, cur.masked);
       lds_barrier();
-      kv_next = gload(1, at);
-      at = look_up(2);
+      kv_nxt = gload(nxt);
+      read_k(stage0);
+      int st_cur = 0, st_nxt = L::STAGE;
+#pragma unroll 1
+      for (int it = 0; it < nsteps; ++it) {
+        floatx16 sc;
+        bf16x8 vf[NDB][2];
+        qk(stage0 + st_cur, sc);
+        read_v(stage0 + st_cur, 0, vf);
+        __builtin_amdgcn_sched_barrier(0);
+        lstore(stage0 + st_nxt, nxt.masked);
+        const unsigned kv_far = gload(far);
+        const Tile t = look_up(it + 3);
+        __builtin_amdgcn_sched_barrier(0);
+        // (a team's step past its tiles: no key is valid, P is zero)
+        softmax(sc, cur.k0, cur.masked, kv_cur);
+        bf16x8 pf[2];
+        to_p(sc, pf);
+        lds_barrier();
+        read_k(stage0 + st_nxt);
+        __builtin_amdgcn_sched_barrier(0);
+        mma_v(vf, pf, 0);
+        cur = nxt, nxt = far, far = t;
+        kv_cur = kv_nxt, kv_nxt = kv_far;
+        st_cur = st_nxt;
+        st_nxt = st_nxt == 2 * L::STAGE ? 0 : st_nxt + L::STAGE;
+      }
+    } else if constexpr (WPT > 1) {
+      // Two stages, tile it + 1 written to the other stage between a step's
+      // first MFMAs and its softmax, one barrier a step.
+      far = look_up(2);
+      lstore(stage0, cur.masked);
+      lds_barrier();
+      kv_nxt = gload(nxt);
 #pragma unroll 1
       for (int it = 0; it < nsteps; ++it) {
         const T* st = stage0 + (it & 1) * L::STAGE;
-        const int k0 = tile_key(it);
         floatx16 sc;
         if (it < nit) qk(st, sc);
-        lstore(stage0 + ((it + 1) & 1) * L::STAGE, is_masked(tile_key(it + 1), kv_next));
-        const unsigned kv = kvalid;
-        kvalid = kv_next;
-        kv_next = gload(it + 2, at);
-        at = look_up(it + 3);
+        lstore(stage0 + ((it + 1) & 1) * L::STAGE, nxt.masked);
+        const unsigned kv_far = gload(far);
+        const Tile t = look_up(it + 3);
         if (it < nit) {
-          softmax(sc, k0, kv);
+          softmax(sc, cur.k0, cur.masked, kv_cur);
           __builtin_amdgcn_sched_barrier(0);
           pv(st, sc);
         }
         lds_barrier();
+        cur = nxt, nxt = far, far = t;
+        kv_cur = kv_nxt, kv_nxt = kv_far;
       }
     } else {
 #pragma unroll 1
       for (int it = 0; it < nit; ++it) {
-        const int k0 = tile_key(it);
-        lstore(stage0, is_masked(k0, kvalid));
-        const unsigned kv = kvalid;
-        kvalid = gload(it + 1, at);
-        at = look_up(it + 2);
+        lstore(stage0, cur.masked);
+        kv_nxt = gload(nxt);
+        far = look_up(it + 2);
         floatx16 sc;
+        read_k(stage0);
+        __builtin_amdgcn_sched_barrier(0);
         qk(stage0, sc);
-        softmax(sc, k0, kv);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(sc, cur.k0, cur.masked, kv_cur);
         pv(stage0, sc);
+        cur = nxt, nxt = far;
+        kv_cur = kv_nxt;
       }
     }
 
@@ -596,17 +673,25 @@ void paged_attn_kernel(PagedArgs p) {
     if (__syncthreads_or(odd_v)) {
 #pragma unroll 1
       for (int it = 0; it < nit; ++it) {
-        const int k0 = tile_key(it);
+        const int x = c0 + team + NT * it, k0 = BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
         const unsigned vis = row_bits(k0);
+        const int last = min(BN, sp.hi - k0);
+        // (the loop's own rule of what it takes as masked: a tile with a key
+        // that is not read has its others here)
+        bool masked = (unsigned)(x - f0) >= fn || last < BN;
+        for (int kk = 0; kk < last && !TP && !masked; ++kk) {
+          int within;
+          masked = page_of(c, b, k0 + kk, within) < 0;
+        }
+        if (!masked) continue;
 #pragma unroll 1
-        for (int kk = 0; kk < BN; ++kk) {
+        for (int kk = 0; kk < last; ++kk) {
           const int j = k0 + kk;
-          if (j >= sp.hi || (j < sp.lo && j >= p.sinks)) continue;
+          if (j < sp.lo && j >= p.sinks) continue;
           int within;
           const int pid = page_of(c, b, j, within);
-          // (only where the loop left it out: a tile that it took as masked)
-          if (pid < 0 || !is_masked(k0, TP && sp.hi - k0 >= BN ? ~0u : 0u)) continue;
-          const T* vr = Vb + (long)pid * c.v_page + (long)within * c.v_row + 4 * h32;
+          if (pid < 0) continue;
+          const T* vr = reinterpret_cast<const T*>(Vb) + (long)pid * c.v_page + (long)within * c.v_row + 4 * h32;
           const unsigned sees = (unsigned)((int)(vis << (31 - kk)) >> 31);
           // (left opaque, so that no register holds a bound for each of the loads)
           int left = c.d;
@@ -810,7 +895,7 @@ struct Plan {
   size_t bytes;  // workspace
 };
 
-int plan_paged(const char* fn, const CacheArgs& c, int H, int window, int sinks, bool tree, Plan& pl) {
+int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, int sinks, bool tree, Plan& pl) {
   const int group = H / c.kv_heads;
   const long rows = (long)c.max_new * group;
   pl.wide = rows > 32;
@@ -828,16 +913,17 @@ int plan_paged(const char* fn, const CacheArgs& c, int H, int window, int sinks,
   }
   const long key_tiles = (keys + BN - 1) / BN + 1;
   const int cus = cu_count();
-  pl.target = pl.wide ? cus : 2 * cus;
+  pl.target = pl.wide && elem == 4 ? cus : 2 * cus;  // workgroups that fill the card
   pl.min_tiles = pl.wide ? 4 : 8;
   // Split where the row tiles leave workgroups idle, or may be of lengths so
   // different that the longest outlasts the rest (several sequences, or a
   // causal prompt with no window): up to four rounds of them.
   const long rounds = c.batch == 1 && window ? 1 : 4;
-  pl.split = pl.items < rounds * pl.target && key_tiles > 2 * pl.min_tiles;
+  pl.split = pl.items < rounds * (pl.wide ? cus : 2 * cus) && key_tiles > 2 * pl.min_tiles;
   if (pl.split && pl.items * (key_tiles + 1) >= 1L << 31) pl.split = false;
-  // (32-bit byte offsets within a tile)
-  pl.one_page = (!c.table || c.page_size % BN == 0) && c.k_row <= (1L << 21) && c.v_row <= (1L << 21);
+  // (32-bit byte offsets within a tile, and byte strides)
+  pl.one_page = (!c.table || c.page_size % BN == 0) && c.k_row <= (1L << 21) && c.v_row <= (1L << 21) &&
+                c.k_page < (1L << 30) && c.v_page < (1L << 30);
   if (pl.split) {
     pl.grid = pl.target;
     pl.bytes = (size_t)pl.grid * (sizeof(Join) + 2 * (size_t)mr * (pl.dp + 2) * 4);
@@ -874,9 +960,10 @@ int paged_launch(PagedArgs& p, const Plan& pl, hipStream_t st) {
 template <typename T>
 int paged_launch_d(PagedArgs& p, const Plan& pl, hipStream_t st) {
   if (pl.wide) {
-    if (pl.dp == 32) return paged_launch<T, 32, 4, 2>(p, pl, st);
-    if (pl.dp == 64) return paged_launch<T, 64, 4, 2>(p, pl, st);
-    return paged_launch<T, 128, 4, 2>(p, pl, st);
+    constexpr int NT = El<T>::W32 ? 2 : 1;
+    if (pl.dp == 32) return paged_launch<T, 32, 4, NT>(p, pl, st);
+    if (pl.dp == 64) return paged_launch<T, 64, 4, NT>(p, pl, st);
+    return paged_launch<T, 128, 4, NT>(p, pl, st);
   }
   if (pl.dp == 32) return paged_launch<T, 32, 1, 4>(p, pl, st);
   if (pl.dp == 64) return paged_launch<T, 64, 1, 4>(p, pl, st);
@@ -907,7 +994,7 @@ extern "C" size_t nkl_paged_attention_workspace_bytes(const nkl_paged_cache* cac
   CacheArgs c;
   Plan pl;
   if (paged_check("nkl_paged_attention", cache, H, window, sinks, c) || c.batch == 0 || c.rows == 0 || c.max_new == 0 ||
-      plan_paged("nkl_paged_attention", c, H, window, sinks, tree != 0, pl))
+      plan_paged("nkl_paged_attention", c, elem_bytes(cache->dtype), H, window, sinks, tree != 0, pl))
     return 0;
   return pl.bytes;
 }
@@ -931,7 +1018,7 @@ extern "C" int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, 
   if (strides % E || ptrs % 16)
     return set_error(NKL_EINVAL, "%s: strides must be multiples of %d elements, pointers of 16 bytes", fn, E);
   Plan pl;
-  if (const int rc = plan_paged(fn, c, H, window, sinks, tree != nullptr, pl)) return rc;
+  if (const int rc = plan_paged(fn, c, elem_bytes(cache->dtype), H, window, sinks, tree != nullptr, pl)) return rc;
   if (pl.grid * 512 > kMaxGridThreads) return set_error(NKL_EINVAL, "%s: %ld workgroups", fn, pl.grid);
   if (pl.bytes && (!workspace || workspace_bytes < pl.bytes))
     return set_error(NKL_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, pl.bytes,
@@ -948,6 +1035,9 @@ extern "C" int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, 
   p.sinks = sinks < kMaxRows ? sinks : kMaxRows;
   p.scale_log2e = scale * kLog2e;
   p.dv_group = fsched::make_div32((unsigned)p.group);
+  const unsigned el = (unsigned)elem_bytes(cache->dtype);
+  p.k_page32 = (unsigned)c.k_page * el; p.k_row32 = (unsigned)c.k_row * el;
+  p.v_page32 = (unsigned)c.v_page * el; p.v_row32 = (unsigned)c.v_row * el;
   if (pl.split) {
     p.joins = static_cast<Join*>(workspace);
     p.part = reinterpret_cast<float*>(p.joins + pl.grid);
