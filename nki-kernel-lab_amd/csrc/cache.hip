@@ -38,7 +38,7 @@ int cache_args(const char* fn, const nkl_paged_cache* c, bool needs_seqs, CacheA
     return set_error(NKL_EINVAL, "%s: %d rows are not %d for each of %d sequences", fn, c->rows, c->max_new, c->batch);
   if (c->batch > 0 && c->rows > 0 && !c->lens && c->table)
     return set_error(NKL_EINVAL, "%s: null lens", fn);
-  if (!c->table && (c->batch != 1 || c->pages < 1))
+  if (!c->table && c->batch > 0 && (c->batch != 1 || c->pages < 1))
     return set_error(NKL_EINVAL, "%s: no page table: one sequence in one page expected", fn);
   a.table = c->table; a.table_row = c->table_row;
   a.lens = c->lens; a.q_start = c->q_start;
@@ -52,6 +52,13 @@ int cache_args(const char* fn, const nkl_paged_cache* c, bool needs_seqs, CacheA
 namespace {
 
 bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
+
+// Non-temporal stores: see store_vec_nt.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <typename V>
+__device__ __forceinline__ void store_nt(V* p, V v) {
+  __builtin_nontemporal_store(v, p);
+}
 
 // --------------------------------------------------------------- append --
 
@@ -141,8 +148,8 @@ __global__ __launch_bounds__(256) void append_kernel(CacheArgs c, AppendArgs p) 
           y2[e] = x2[e] * co + x1[e] * sn;
         }
         if constexpr (E > 1) {
-          store_vec<E>(dst + ch, y1);
-          store_vec<E>(dst + ch + half, y2);
+          store_vec_nt<E>(dst + ch, y1);
+          store_vec_nt<E>(dst + ch + half, y2);
         } else {
           dst[ch] = from_f32<T>(y1[0]);
           dst[ch + half] = from_f32<T>(y2[0]);
@@ -163,7 +170,7 @@ __global__ __launch_bounds__(256) void append_kernel(CacheArgs c, AppendArgs p) 
           dst = reinterpret_cast<T*>(c.v) + (long)pid * c.v_page + (long)h * c.v_head + (long)within * c.v_row + ch;
         }
         if constexpr (E > 1)
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+          store_nt(reinterpret_cast<u32x4*>(dst), *reinterpret_cast<const u32x4*>(src));
         else
           *dst = *src;
       }
@@ -193,7 +200,7 @@ int append_launch(const CacheArgs& c, AppendArgs p, hipStream_t st) {
 // Pairs of pages that one launch takes in its argument block: a host list
 // needs no device buffer, and no copy that a captured graph would have to
 // keep.
-constexpr int kPairs = 240;
+constexpr int kPairs = 480;
 struct CopyArgs {
   const unsigned char* k;
   const unsigned char* v;
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs p, int layers)
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    if (off[u] >= 0) *reinterpret_cast<V*>(dst + off[u]) = buf[u];
+    if (off[u] >= 0) store_nt(reinterpret_cast<V*>(dst + off[u]), buf[u]);
 }
 
 // --------------------------------------------------------------- accept --
@@ -244,13 +251,13 @@ struct AcceptArgs {
 
 // Workgroup (x, b): columns (a 16-byte piece of every row's (tensor, layer,
 // head)) 256 x .. of sequence b.  A thread owns its column: it reads and
-// writes the path's rows in path order, four loads ahead of their stores.
+// writes the path's rows in path order, a batch of loads ahead of its stores.
 // That is the result of reading every row before any is written: a path
 // ascends strictly from node >= 0, so entry i's node is never below i, and a
 // later entry's node lies above every row written so far.
 template <typename V>
 __global__ __launch_bounds__(256) void accept_kernel(CacheArgs c, AcceptArgs p, int per) {
-  constexpr int N = 256;
+  constexpr int N = 256, A = 16;  // entries in LDS, and a thread's loads in flight
   __shared__ int src_pid[N], src_row[N], dst_pid[N], dst_row[N];
   __shared__ int first_bad;
   const int b = blockIdx.y, tid = threadIdx.x;
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(256) void accept_kernel(CacheArgs c, AcceptArgs p, 
   constexpr int V_ = (int)sizeof(V);
   V* base = nullptr;
   long page = 0, row = 0;
-  if (x < cols) {
+  if (x < cols && c.pages > 0) {
     base = reinterpret_cast<V*>((tensor ? c.v + layer * p.v_layer + head * c.v_head
                                         : c.k + layer * p.k_layer + head * c.k_head)) + piece;
     page = (tensor ? c.v_page : c.k_page) / V_;
@@ -288,14 +295,16 @@ __global__ __launch_bounds__(256) void accept_kernel(CacheArgs c, AcceptArgs p, 
     __syncthreads();
     const int n = first_bad;
     if (base) {
-      for (int j0 = 0; j0 < n; j0 += 4) {
-        V buf[4];
+      for (int j0 = 0; j0 < n; j0 += A) {
+        V buf[A];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j0 + u < n && src_pid[j0 + u] >= 0)
-            buf[u] = base[(long)src_pid[j0 + u] * page + (long)src_row[j0 + u] * row];
+        for (int u = 0; u < A; ++u) {  // (loads that nothing guards go out together: entries past the last read again)
+          const int j = min(j0 + u, n - 1);
+          buf[u] = base[src_pid[j] >= 0 ? (long)src_pid[j] * page + (long)src_row[j] * row : 0];
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < A; ++u)
           if (j0 + u < n && src_pid[j0 + u] >= 0 && dst_pid[j0 + u] >= 0)
             base[(long)dst_pid[j0 + u] * page + (long)dst_row[j0 + u] * row] = buf[u];
       }
@@ -462,12 +471,15 @@ extern "C" int nkl_cache_copy_pages(const nkl_paged_cache* cache, const int* pai
   while (per > 1 && gx * 256 * per * layers * 2 > kMaxGridThreads) per /= 2;
   if (gx * 256 * per * layers * 2 > kMaxGridThreads)
     return set_error(NKL_EINVAL, "nkl_cache_copy_pages: a page of %ld bytes in %d layers", total * (vec ? 16 : el), layers);
+  // (launches of equal length: no short one behind)
+  const long launches = (n + per - 1) / per;
+  per = (n + launches - 1) / launches;
   for (int i = 0; i < n; i += (int)per) {
     const int m = n - i < per ? n - i : (int)per;
     for (int j = 0; j < m; ++j) p.pair[j] = make_int2(pairs[2 * (i + j)], pairs[2 * (i + j) + 1]);
     const dim3 grid((unsigned)gx, (unsigned)(m * layers * 2));
     if (vec)
-      copy_pages_kernel<uint4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
+      copy_pages_kernel<u32x4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
     else if (el == 4)
       copy_pages_kernel<unsigned><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
     else
@@ -501,7 +513,7 @@ extern "C" int nkl_cache_accept(const nkl_paged_cache* cache, const int* paths, 
   const dim3 grid((unsigned)((cols + 255) / 256 > 0 ? (cols + 255) / 256 : 1), (unsigned)c.batch);
   hipStream_t st = (hipStream_t)stream;
   if (vec)
-    accept_kernel<uint4><<<grid, dim3(256), 0, st>>>(c, p, per);
+    accept_kernel<u32x4><<<grid, dim3(256), 0, st>>>(c, p, per);
   else if (el == 4)
     accept_kernel<unsigned><<<grid, dim3(256), 0, st>>>(c, p, per);
   else

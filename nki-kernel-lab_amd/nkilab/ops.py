@@ -16,7 +16,6 @@ what nkilab.model uses.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 
@@ -526,8 +525,8 @@ def _window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torc
     E = 16 // q.element_size()
     q, k, v = (_rows_operand(t, E) for t in (q, k, v))
     out = o if _rows_ok(o, E) else torch.empty((H, S, d), dtype=o.dtype, device=o.device)
-    desc = _lib.PagedCacheDesc(k.data_ptr(), v.data_ptr(), 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), None, 0,
-                               None, None, 1, Hkv, S, d, 1, 1, S, S, dtype_code(q.dtype))
+    desc = _lib.pack_cache(k.data_ptr(), v.data_ptr(), 0, k.stride(0), k.stride(1), 0, v.stride(0), v.stride(1), 0, 0, 0, 0, 1,
+                           Hkv, S, d, 1, 1, S, S, dtype_code(q.dtype))
     _paged_attention(desc, q, (q.stride(1), q.stride(0)), out, (out.stride(1), out.stride(0)), H, w, sinks, None, 0, scale)
     if out is not o:
         o.copy_(out)
@@ -589,11 +588,17 @@ def _rows_operand(t: torch.Tensor, E: int) -> torch.Tensor:
     return t if _rows_ok(t, E) else t.clone(memory_format=torch.contiguous_format)
 
 
-def _on_current_device(fn: str, *tensors: torch.Tensor | None) -> None:
+def _on_current_device(fn: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
     """The kernels run on the current device's current stream: every tensor has to be there."""
-    for t in tensors:
-        if t is not None and not (t.is_cuda and t.get_device() == current_device()):
-            raise ValueError(f"{fn}: a tensor is on {t.device}, which is not the current device")
+    d = first.get_device()
+    if d >= 0 and d == current_device():
+        for t in others:
+            if t is not None and t.get_device() != d:
+                break
+        else:
+            return
+    raise ValueError(f"{fn}: tensors on {sorted({str(t.device) for t in (first, *others) if t is not None})}, every one "
+                     "must be on the current device")
 
 
 def _int32(fn: str, name: str, t: torch.Tensor, shape: tuple) -> None:
@@ -601,44 +606,48 @@ def _int32(fn: str, name: str, t: torch.Tensor, shape: tuple) -> None:
         raise ValueError(f"{fn}: {name} must be int32 {list(shape)} with unit stride, got {t.dtype} {list(t.shape)}")
 
 
-def _cache_tensors(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, layers: bool = False) -> None:
-    dims = (4, 5) if layers else (4,)
-    if k_cache.dim() not in dims or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
-        raise ValueError(f"{fn}: k_cache {tuple(k_cache.shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} "
+def _cache_tensors(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, layers: bool = False) -> tuple:
+    """(shape, k's strides, v's strides) of a cache's tensors, checked."""
+    shape, sk, sv = k_cache.shape, k_cache.stride(), v_cache.stride()
+    n = len(shape)
+    if (n != 4 and not (layers and n == 5)) or shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+        raise ValueError(f"{fn}: k_cache {tuple(shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} "
                          f"{v_cache.dtype} must be equal {'[layers,] ' if layers else ''}[pages, kv_heads, page_size, d]")
-    for t in (k_cache, v_cache):
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            raise ValueError(f"{fn}: the caches' head dim must be contiguous")
+    if (sk[-1] != 1 or sv[-1] != 1) and shape[-1] > 1:
+        raise ValueError(f"{fn}: the caches' head dim must be contiguous")
+    return shape, sk, sv
 
 
 def _cache_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
-                q_start: torch.Tensor | None, rows: int, max_q: int | None) -> _lib.PagedCacheDesc:
-    """The C ABI's description of a cache and a call's new rows, checked."""
-    _cache_tensors(fn, k_cache, v_cache)
-    pages, Hkv, page_size, d = k_cache.shape
-    if page_table.dim() != 2:
-        raise ValueError(f"{fn}: page_table must be [batch, pages of a sequence], got {tuple(page_table.shape)}")
-    B = page_table.shape[0]
-    _int32(fn, "page_table", page_table, page_table.shape)
+                q_start: torch.Tensor | None, rows: int, max_q: int | None) -> tuple[bytes, torch.Size, int]:
+    """The C ABI's description of a cache and a call's new rows (checked), the cache's shape, and max_new."""
+    shape, sk, sv = _cache_tensors(fn, k_cache, v_cache)
+    pages, Hkv, page_size, d = shape
+    ts = page_table.shape
+    if len(ts) != 2:
+        raise ValueError(f"{fn}: page_table must be [batch, pages of a sequence], got {tuple(ts)}")
+    B, cols = ts
+    _int32(fn, "page_table", page_table, ts)
     _int32(fn, "lens", lens, (B,))
+    pstart = 0
     if q_start is not None:
         _int32(fn, "q_start", q_start, (B + 1,))
         if max_q is None:
             raise ValueError(f"{fn}: q_start needs max_q, the most new rows of a sequence")
+        pstart = q_start.data_ptr()
     else:
         each = rows // B if B else 0
         if each * B != rows:
             raise ValueError(f"{fn}: {rows} rows are not a number for each of {B} sequences; q_start expected")
-        if max_q is not None and int(max_q) != each:
+        if max_q is not None and max_q != each:
             raise ValueError(f"{fn}: max_q={max_q}, and {each} rows for each sequence")
         max_q = each
-    if int(max_q) < 0:
+    if max_q < 0:
         raise ValueError(f"{fn}: max_q={max_q} is negative")
-    sk, sv = k_cache.stride(), v_cache.stride()
-    return _lib.PagedCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
-                               page_table.data_ptr(), page_table.stride(0), lens.data_ptr(),
-                               None if q_start is None else q_start.data_ptr(), pages, Hkv, page_size, d,
-                               page_table.shape[1], B, rows, min(int(max_q), rows), dtype_code(k_cache.dtype))
+    max_q = min(int(max_q), rows)
+    return _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
+                           page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), pstart, pages, Hkv, page_size, d,
+                           cols, B, rows, max_q, dtype_code(k_cache.dtype)), shape, max_q
 
 
 def _tree_words(fn: str, tree: torch.Tensor | None, rows: int, max_q: int) -> tuple[int | None, int]:
@@ -702,45 +711,52 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     length and its depth.  Sequences of one call must not share a page that
     either writes."""
     fn = "cache_append_into"
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
-        raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} must be [rows, kv_heads, d] of the caches "
-                         f"{tuple(k_cache.shape)}")
-    if not (k.dtype == v.dtype == k_cache.dtype):
-        raise TypeError(f"{fn}: k {k.dtype}, v {v.dtype} and the caches {k_cache.dtype} must share a dtype")
-    desc = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, k.shape[0], max_q)
-    words, nwords = _tree_words(fn, tree, k.shape[0], desc.max_new)
+    ks = k.shape
+    if len(ks) != 3 or ks != v.shape:
+        raise ValueError(f"{fn}: k {tuple(ks)} and v {tuple(v.shape)} must be equal [rows, kv_heads, d]")
+    rows, Hkv, d = ks
+    desc, shape, max_new = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, rows, max_q)
+    if Hkv != shape[1] or d != shape[3]:
+        raise ValueError(f"{fn}: k {tuple(ks)} must be [rows, kv_heads, d] of the caches {tuple(shape)}")
+    dt = k.dtype
+    if v.dtype is not dt or k_cache.dtype is not dt:
+        raise TypeError(f"{fn}: k {dt}, v {v.dtype} and the caches {k_cache.dtype} must share a dtype")
+    words, nwords = _tree_words(fn, tree, rows, max_new)
     base = 0.0
     if rope_base is not None:
         base = float(rope_base)
         if not base > 1.0:
             raise ValueError(f"{fn}: rope_base {rope_base} must be above 1")
-    H, sq, so = 0, (0, 0), (0, 0)
+    sk, sv = k.stride(), v.stride()
+    packed = d < 2 or (sk[2] == 1 and sv[2] == 1)
+    H, sq, so, pq, po = 0, (0, 0, 1), (0, 0, 1), None, None
     if q is not None or q_out is not None:
         if rope_base is None or q is None or q_out is None:
             raise ValueError(f"{fn}: q, q_out and rope_base go together")
-        if q.dim() != 3 or q.shape != q_out.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-            raise ValueError(f"{fn}: q {tuple(q.shape)} and q_out {tuple(q_out.shape)} must be [{k.shape[0]}, H, "
-                             f"{k.shape[2]}]")
-        if not (q.dtype == q_out.dtype == k.dtype):
-            raise TypeError(f"{fn}: q {q.dtype} and q_out {q_out.dtype} must have k's dtype {k.dtype}")
-        H, sq, so = q.shape[1], q.stride()[:2], q_out.stride()[:2]
-        if H == 0:
-            q = q_out = None
-    for t in (k, v, q, q_out):
-        if t is not None and t.stride(2) != 1 and t.shape[2] > 1:
-            raise ValueError(f"{fn}: the head dim must be contiguous")
+        qs = q.shape
+        if len(qs) != 3 or qs != q_out.shape or qs[0] != rows or qs[2] != d:
+            raise ValueError(f"{fn}: q {tuple(qs)} and q_out {tuple(q_out.shape)} must be [{rows}, H, {d}]")
+        if q.dtype is not dt or q_out.dtype is not dt:
+            raise TypeError(f"{fn}: q {q.dtype} and q_out {q_out.dtype} must have k's dtype {dt}")
+        H = qs[1]
+        if H:
+            sq, so, pq, po = q.stride(), q_out.stride(), q.data_ptr(), q_out.data_ptr()
+            packed = packed and (d < 2 or (sq[2] == 1 and so[2] == 1))
+    if not packed:
+        raise ValueError(f"{fn}: the head dim must be contiguous")
     _on_current_device(fn, k, v, k_cache, v_cache, page_table, lens, q_start, tree, q, q_out)
-    _lib.call("nkl_cache_append", ctypes.byref(desc), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
-              v.stride(1), ptr(q), ptr(q_out), H, *sq, *so, words, nwords, base, stream_handle())
+    rc = _lib.lib().nkl_cache_append(desc, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1], pq, po, H, sq[0], sq[1],
+                                     so[0], so[1], words, nwords, base, stream_handle())
+    if rc:
+        _lib.check("nkl_cache_append", rc)
 
 
-def _layer_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, tuple, tuple, tuple]:
+def _layer_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple:
     """(layers, layer strides, [pages, kv_heads, page_size, d], its strides in both) of caches with or without layers."""
-    _cache_tensors(fn, k_cache, v_cache, layers=True)
-    if k_cache.dim() == 5:
-        return (k_cache.shape[0], k_cache.stride(0), v_cache.stride(0), k_cache.shape[1:], k_cache.stride()[1:4],
-                v_cache.stride()[1:4])
-    return 1, 0, 0, k_cache.shape, k_cache.stride()[:3], v_cache.stride()[:3]
+    shape, sk, sv = _cache_tensors(fn, k_cache, v_cache, layers=True)
+    if len(shape) == 5:
+        return shape[0], sk[0], sv[0], shape[1:], sk[1:], sv[1:]
+    return 1, 0, 0, shape, sk, sv
 
 
 def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs) -> None:
@@ -757,13 +773,15 @@ def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs) -> Non
         return
     if p.ndim != 2 or p.shape[1] != 2 or p.dtype.kind not in "iu":
         raise ValueError(f"{fn}: pairs must be whole numbers [n, 2], got {p.dtype} {list(p.shape)}")
-    if int(p.min()) < 0 or int(p.max()) >= shape[0]:
-        raise ValueError(f"{fn}: pages {int(p.min())} .. {int(p.max())} outside [0, {shape[0]})")
-    p = np.ascontiguousarray(p, dtype=np.int32)
+    i32 = p.astype(np.int32)
+    if (i32 != p).any() or (i32.view(np.uint32) >= shape[0]).any():
+        raise ValueError(f"{fn}: pages outside [0, {shape[0]})")
     _on_current_device(fn, k_cache, v_cache)
-    desc = _lib.PagedCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), *sk, *sv, None, 0, None, None, *shape, 0, 0, 0, 0,
-                               dtype_code(k_cache.dtype))
-    _lib.call("nkl_cache_copy_pages", ctypes.byref(desc), p.ctypes.data, p.shape[0], layers, kl, vl, stream_handle())
+    desc = _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], 0, 0, 0, 0,
+                           *shape, 0, 0, 0, 0, dtype_code(k_cache.dtype))
+    rc = _lib.lib().nkl_cache_copy_pages(desc, i32.ctypes.data, i32.shape[0], layers, kl, vl, stream_handle())
+    if rc:
+        _lib.check("nkl_cache_copy_pages", rc)
 
 
 def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
@@ -780,39 +798,44 @@ def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
     its own."""
     fn = "cache_accept"
     layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
-    if page_table.dim() != 2 or paths.dim() != 2:
-        raise ValueError(f"{fn}: page_table {tuple(page_table.shape)} and paths {tuple(paths.shape)} must have two axes")
-    B = page_table.shape[0]
-    _int32(fn, "page_table", page_table, page_table.shape)
+    ts, ps = page_table.shape, paths.shape
+    if len(ts) != 2 or len(ps) != 2:
+        raise ValueError(f"{fn}: page_table {tuple(ts)} and paths {tuple(ps)} must have two axes")
+    B = ts[0]
+    _int32(fn, "page_table", page_table, ts)
     _int32(fn, "lens", lens, (B,))
-    _int32(fn, "paths", paths, (B, paths.shape[1]))
+    _int32(fn, "paths", paths, (B, ps[1]))
     if (q_start is None) == (n_nodes is None):
         raise ValueError(f"{fn}: either q_start or n_nodes expected")
+    pstart = 0
     if q_start is not None:
         _int32(fn, "q_start", q_start, (B + 1,))
         rows = most = MAX_ROWS
+        pstart = q_start.data_ptr()
     else:
         most = int(n_nodes)
         rows = most * B
         if most < 0 or rows > MAX_ROWS:
             raise ValueError(f"{fn}: n_nodes={n_nodes} for {B} sequences")
     _on_current_device(fn, k_cache, v_cache, page_table, lens, paths, q_start)
-    out = torch.empty_like(lens, memory_format=torch.contiguous_format)
-    desc = _lib.PagedCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), *sk, *sv, page_table.data_ptr(), page_table.stride(0),
-                               lens.data_ptr(), ptr(q_start), *shape, page_table.shape[1], B, rows, most,
-                               dtype_code(k_cache.dtype))
-    _lib.call("nkl_cache_accept", ctypes.byref(desc), paths.data_ptr(), paths.stride(0), paths.shape[1], out.data_ptr(),
-              layers, kl, vl, stream_handle())
+    out = torch.empty((B,), dtype=torch.int32, device=lens.device)
+    desc = _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
+                           page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), pstart, *shape, ts[1], B, rows, most,
+                           dtype_code(k_cache.dtype))
+    rc = _lib.lib().nkl_cache_accept(desc, paths.data_ptr(), paths.stride(0), ps[1], out.data_ptr(), layers, kl, vl,
+                                     stream_handle())
+    if rc:
+        _lib.check("nkl_cache_accept", rc)
     return out
 
 
-def _paged_attention(desc, q, sq, o, so, H: int, window: int, sinks: int, words: int | None, nwords: int,
+def _paged_attention(desc: bytes, q, sq, o, so, H: int, window: int, sinks: int, words: int | None, nwords: int,
                      scale: float) -> None:
     """nkl_paged_attention on operands already checked."""
-    L, ref = _lib.lib(), ctypes.byref(desc)
-    nbytes = L.nkl_paged_attention_workspace_bytes(ref, H, window, sinks, int(words is not None))
+    L = _lib.lib()
+    nbytes = L.nkl_paged_attention_workspace_bytes(desc, H, window, sinks, words is not None)
     ws = workspace(nbytes, q.device) if nbytes else None
-    rc = L.nkl_paged_attention(ref, q.data_ptr(), o.data_ptr(), H, *sq, *so, window, sinks, words, nwords, scale, ptr(ws),
+    rc = L.nkl_paged_attention(desc, q.data_ptr(), o.data_ptr(), H, *sq, *so, window, sinks, words, nwords, scale, ptr(ws),
                                nbytes, stream_handle())
     if rc:
         _lib.check("nkl_paged_attention", rc)
@@ -837,20 +860,21 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
     been freed.  Rows of o that belong to no sequence are left as they are.
     d a multiple of 8 (fp32: 4), at most 128; scale above 0."""
     fn = "paged_attention_into"
-    if q.dim() != 3 or o.shape != q.shape or o.dtype != q.dtype:
-        raise ValueError(f"{fn}: q {tuple(q.shape)} {q.dtype} and o {tuple(o.shape)} {o.dtype} must be equal [rows, H, d]")
-    if q.dtype != k_cache.dtype:
+    qs = q.shape
+    if len(qs) != 3 or o.shape != qs or o.dtype is not q.dtype:
+        raise ValueError(f"{fn}: q {tuple(qs)} {q.dtype} and o {tuple(o.shape)} {o.dtype} must be equal [rows, H, d]")
+    if q.dtype is not k_cache.dtype:
         raise TypeError(f"{fn}: q {q.dtype} and the caches {k_cache.dtype} must share a dtype")
-    desc = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, q.shape[0], max_q)
-    rows, H, d = q.shape
-    if d != desc.d or H < 1 or H % max(desc.kv_heads, 1):
-        raise ValueError(f"{fn}: q {tuple(q.shape)} does not match caches {tuple(k_cache.shape)}")
+    rows, H, d = qs
+    desc, shape, max_new = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, rows, max_q)
+    if d != shape[3] or H < 1 or H % max(shape[1], 1):
+        raise ValueError(f"{fn}: q {tuple(qs)} does not match caches {tuple(shape)}")
     window, sinks = _window_sinks(fn, window, sinks)
-    words, nwords = _tree_words(fn, tree, rows, desc.max_new)
+    words, nwords = _tree_words(fn, tree, rows, max_new)
     if scale is None:
         scale = 1.0 / math.sqrt(d) if d else 1.0
     _on_current_device(fn, q, o, k_cache, v_cache, page_table, lens, q_start, tree)
-    if rows == 0 or desc.max_new == 0:
+    if max_new == 0:
         return o
     E = 16 // q.element_size()
     q = _rows_operand(q, E)

@@ -18,6 +18,17 @@ def desc(**kw):
     return _lib.PagedCacheDesc(*(f[n] for n, _ in _lib.PagedCacheDesc._fields_))
 
 
+def test_packed_description():
+    """The bytes that the operators pass are the structure, field for field."""
+    from nkilab import _lib
+
+    values = list(range(1, len(_lib.PagedCacheDesc._fields_) + 1))
+    packed, d = _lib.pack_cache(*values), _lib.PagedCacheDesc(*values)
+    assert packed == bytes(d)[:len(packed)] and 0 <= ctypes.sizeof(d) - len(packed) < 8
+    # (the library reads the whole structure; what may be missing at its end is padding)
+    assert _lib.PagedCacheDesc.dtype.offset + 4 == len(packed)
+
+
 def attn(d, q=P, o=P, H=8, st=(512, 64, 512, 64), window=0, sinks=0, tree=None, words=0, scale=0.125, ws=None, nb=0):
     from nkilab import _lib
 
