@@ -353,6 +353,7 @@ void paged_attn_kernel(PagedArgs p) {
     }
 
     // ---- staging
+    constexpr bool LANES = TP && WPT > 1;
     const unsigned char* const Kb = c.k + (long)kvh * c.k_head * (long)sizeof(T);
     const unsigned char* const Vb = c.v + (long)kvh * c.v_head * (long)sizeof(T);
     const int* const trow = c.table + (c.table ? (long)b * c.table_row : 0);
@@ -391,6 +392,39 @@ void paged_attn_kernel(PagedArgs p) {
         }
       }
       return t;
+    };
+    // Wavefronts that share their tiles (TP): 64 tiles are looked up at a time,
+    // one a lane -- where their K and V are, the bytes a load may read, and
+    // (flags) the keys that are there with bit 8 set where a mask is needed --
+    // and a step reads its tile's lane: done by a step for itself, on the
+    // scalar unit, this took more instructions than the softmax.  The pages of
+    // the next 64 are on their way meanwhile.
+    struct Lanes {
+      unsigned k_lo, k_hi, v_lo, v_hi;
+      int k_bytes, v_bytes, flags;
+    } lt = {};
+    int pid_next = 0;
+    auto tile_first = [&](int it) __attribute__((always_inline)) {
+      const int x = c0 + team + NT * it;
+      return BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
+    };
+    auto load_pids = [&](int base) __attribute__((always_inline)) {
+      const int it = base + lane;
+      pid_next = !c.table || it >= nit ? 0 : trow[div32(c.dv_page, (unsigned)tile_first(it))];
+    };
+    auto fill_lanes = [&](int base) __attribute__((always_inline)) {
+      const int it = base + lane, x = c0 + team + NT * it, k0 = tile_first(it), pid = pid_next;
+      const int n = it < nit && (unsigned)pid < (unsigned)c.pages ? min(BN, sp.hi - k0) : 0;
+      const unsigned pg = n > 0 ? pid : 0;
+      const unsigned within = n > 0 ? k0 - (int)div32(c.dv_page, (unsigned)k0) * c.page_size : 0;
+      const unsigned long ka = (unsigned long)Kb + (unsigned long)pg * p.k_page32 + (unsigned long)within * p.k_row32;
+      const unsigned long va = (unsigned long)Vb + (unsigned long)pg * p.v_page32 + (unsigned long)within * p.v_row32;
+      lt.k_lo = (unsigned)ka; lt.k_hi = (unsigned)(ka >> 32);
+      lt.v_lo = (unsigned)va; lt.v_hi = (unsigned)(va >> 32);
+      lt.k_bytes = n > 0 ? (n - 1) * (int)p.k_row32 + row_bytes : 0;
+      lt.v_bytes = n > 0 ? (n - 1) * (int)p.v_row32 + row_bytes : 0;
+      lt.flags = n | ((unsigned)(x - f0) >= fn || n < BN ? 256 : 0);
+      load_pids(base + 64);
     };
     uint4 rk[CH], rv[CH];
     // Loads a tile and returns a bit for each of its keys that is read.
@@ -431,6 +465,26 @@ void paged_attn_kernel(PagedArgs p) {
         t.masked = t.masked || bits != ~0u;
         return bits;
       }
+    };
+    // Loads tile `it` by the lanes' list; returns its flags.
+    auto gload_lane = [&](int it) __attribute__((always_inline)) {
+      if ((it & 63) == 0) fill_lanes(it);
+      const int l = it & 63;
+      auto lane_of = [&](unsigned x) __attribute__((always_inline)) { return (unsigned)__builtin_amdgcn_readlane(x, l); };
+      const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(((unsigned long)lane_of(lt.k_hi) << 32) | lane_of(lt.k_lo)), (short)0, (int)lane_of(lt.k_bytes),
+          fsched::kBufferFlags);
+      const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(((unsigned long)lane_of(lt.v_hi) << 32) | lane_of(lt.v_lo)), (short)0, (int)lane_of(lt.v_bytes),
+          fsched::kBufferFlags);
+      int step_k = (TT / CPR) * (int)p.k_row32, step_v = (TT / CPR) * (int)p.v_row32;
+      asm volatile("" : "+s"(step_k), "+s"(step_v));
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, 0));
+        rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, 0));
+      }
+      return (int)lane_of(lt.flags);
     };
     // Stages the loaded tile.  Where the tile is masked its infinities and NaN
     // of V are left out (0 * inf would reach the rows that do not see them) and
@@ -493,8 +547,14 @@ void paged_attn_kernel(PagedArgs p) {
       }
     };
     // Masks the scores of keys k0 .., raises the running max and turns S into P.
+    // (With LANES: tile k0's number instead of its first key, and the keys that
+    // are there instead of a bit for each.)
     auto softmax = [&](floatx16& sc, int k0, bool masked, unsigned kvalid) __attribute__((always_inline)) {
       if (masked) {
+        if constexpr (LANES) {
+          k0 = tile_first(k0);
+          kvalid = low_bits(kvalid);
+        }
         const unsigned seen = (row_bits(k0) & kvalid) >> (4 * h32);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -580,8 +640,13 @@ void paged_attn_kernel(PagedArgs p) {
 
     // The tile that a step computes, the one that it stages (loaded a step
     // before) and the one that it loads (looked up a step before).
-    Tile cur = look_up(0), nxt = look_up(1), far;
-    unsigned kv_cur = gload(cur), kv_nxt;
+    Tile cur, nxt, far;
+    unsigned kv_cur, kv_nxt;
+    if constexpr (!LANES) {
+      cur = look_up(0);
+      nxt = look_up(1);
+      kv_cur = gload(cur);
+    }
     // Every wavefront's LDS accesses are done, then all wavefronts meet (with
     // __syncthreads() the loads in flight would be waited for too).
     auto lds_barrier = [&]() __attribute__((always_inline)) {
@@ -597,10 +662,19 @@ void paged_attn_kernel(PagedArgs p) {
       // covers tile it + 1's staging, three stages deep: the stage that step
       // `it` writes was last read by P V of tile it - 2, which every wavefront
       // had behind it at the barrier of step it - 1.
-      far = look_up(2);
-      lstore(stage0, cur.masked);
+      int fl_cur = 0, fl_nxt = 0, fl_far = 0;
+      if constexpr (LANES) {
+        load_pids(0);
+        fl_cur = gload_lane(0);
+      } else {
+        far = look_up(2);
+      }
+      lstore(stage0, LANES ? fl_cur >= 256 : cur.masked);
       lds_barrier();
-      kv_nxt = gload(nxt);
+      if constexpr (LANES)
+        fl_nxt = gload_lane(1);
+      else
+        kv_nxt = gload(nxt);
       read_k(stage0);
       int st_cur = 0, st_nxt = L::STAGE;
 #pragma unroll 1
@@ -610,20 +684,33 @@ void paged_attn_kernel(PagedArgs p) {
         qk(stage0 + st_cur, sc);
         read_v(stage0 + st_cur, 0, vf);
         __builtin_amdgcn_sched_barrier(0);
-        lstore(stage0 + st_nxt, nxt.masked);
-        const unsigned kv_far = gload(far);
-        const Tile t = look_up(it + 3);
+        lstore(stage0 + st_nxt, LANES ? fl_nxt >= 256 : nxt.masked);
+        unsigned kv_far = 0;
+        Tile t;
+        if constexpr (LANES) {
+          fl_far = gload_lane(it + 2);
+        } else {
+          kv_far = gload(far);
+          t = look_up(it + 3);
+        }
         __builtin_amdgcn_sched_barrier(0);
         // (a team's step past its tiles: no key is valid, P is zero)
-        softmax(sc, cur.k0, cur.masked, kv_cur);
+        if constexpr (LANES)
+          softmax(sc, it, fl_cur >= 256, fl_cur & 255);
+        else
+          softmax(sc, cur.k0, cur.masked, kv_cur);
         bf16x8 pf[2];
         to_p(sc, pf);
         lds_barrier();
         read_k(stage0 + st_nxt);
         __builtin_amdgcn_sched_barrier(0);
         mma_v(vf, pf, 0);
-        cur = nxt, nxt = far, far = t;
-        kv_cur = kv_nxt, kv_nxt = kv_far;
+        if constexpr (LANES) {
+          fl_cur = fl_nxt, fl_nxt = fl_far;
+        } else {
+          cur = nxt, nxt = far, far = t;
+          kv_cur = kv_nxt, kv_nxt = kv_far;
+        }
         st_cur = st_nxt;
         st_nxt = st_nxt == 2 * L::STAGE ? 0 : st_nxt + L::STAGE;
       }
