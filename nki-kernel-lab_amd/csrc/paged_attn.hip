@@ -914,58 +914,97 @@ void paged_attn_kernel(PagedArgs p) {
 }
 
 // Joins the parts of the row tile that begins in range blockIdx.x and ends in
-// another: a wavefront for each of its rows, its lanes over the head dim.
+// another; DP / 4 lanes to a row, four columns each.  Row tiles of 32 rows (few
+// new tokens, up to hundreds of parts): a workgroup's four wavefronts take every
+// fourth part of the same rows and meet in LDS.  Row tiles of 128 rows (a few
+// parts each): every wavefront has its own rows, four times over.
+constexpr int kJoinPasses = 4;
+template <int DP, int MR>
+constexpr int join_rows() {
+  return 64 / (DP / 4) * (MR == 32 ? 1 : 4 * kJoinPasses);
+}
+
 template <typename T, int DP, int MR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
+  constexpr bool SHARE = MR == 32;
+  constexpr int LPR = DP / 4, RPW = 64 / LPR;  // lanes a row, rows a wavefront
+  constexpr int A = 8;                         // parts in flight
+  __shared__ float4 xo[SHARE ? 4 : 1][64];
+  __shared__ float2 xm[SHARE ? 4 : 1][64];
   const CacheArgs& c = p.c;
   const Join jn = p.joins[blockIdx.x];
   const int n = jn.parts;
   if (n == 0) return;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int r = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + wid), row = jn.r0 + r;
+  const int col = 4 * (lane % LPR);
   const Seq s = seq_of(c, jn.b);
-  if (row >= s.use * p.group) return;
+  const int nrows = s.use * p.group - jn.r0;
   // Part i is slot 0 of range blockIdx.x + i, the first slot 1.
   auto part_of = [&](int i) __attribute__((always_inline)) {
     return p.part + (2L * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0)) * part_floats<DP, MR>();
   };
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, part_of(i)[MR * DP + 2 * r]);
-  m = wave_max(m);
-  constexpr int PL = DP >= 64 ? DP / 64 : 1;
-  float l = 0.f, acc[PL] = {};
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    float w = 0.f;
-    if (i0 + lane < n) {
-      const float2 x = *reinterpret_cast<const float2*>(part_of(i0 + lane) + MR * DP + 2 * r);
-      w = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m);
-      l += x.y * w;
-    }
-    const int cnt = min(64, n - i0);
-    for (int i1 = 0; i1 < cnt; i1 += 4) {  // four parts' loads in flight (past the last: again, weight 0)
-      float x[4][PL], wi[4];
+#pragma unroll 1
+  for (int pass = 0; pass < (SHARE ? 1 : kJoinPasses); ++pass) {
+    const int r = (int)blockIdx.y * join_rows<DP, MR>() + (SHARE ? 0 : (pass * 4 + wid) * RPW) + lane / LPR;
+    const bool ok = r < nrows;  // (rows past the last are not in the parts either: their loads repeat row 0)
+    const int rl = ok ? r : 0;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int i_first = SHARE ? wid : 0, i_step = SHARE ? 4 : 1;
+    for (int i0 = i_first; i0 < n; i0 += A * i_step) {
+      float2 ml[A];
+      float4 x[A];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = min(i1 + i, cnt - 1);
-        wi[i] = i1 + i < cnt ? __shfl(w, j, kWave) : 0.f;
-        const float* pr = part_of(i0 + j) + (long)r * DP;
-#pragma unroll
-        for (int k = 0; k < PL; ++k) x[i][k] = PL * lane + k < DP ? pr[PL * lane + k] : 0.f;
+      for (int k = 0; k < A; ++k) {  // (past the last part: the first again)
+        const int i = i0 + k * i_step;
+        const float* pt = part_of(i < n ? i : i_first);
+        ml[k] = *reinterpret_cast<const float2*>(pt + MR * DP + 2 * rl);
+        x[k] = *reinterpret_cast<const float4*>(pt + (long)rl * DP + col);
       }
+      float mn = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (wi[i] > 0.f)
+      for (int k = 0; k < A; ++k) {
+        if (i0 + k * i_step < n) mn = fmaxf(mn, ml[k].x);
+      }
+      const float w0 = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+      m = mn;
+      l *= w0;
+      acc.x *= w0; acc.y *= w0; acc.z *= w0; acc.w *= w0;
 #pragma unroll
-          for (int k = 0; k < PL; ++k) acc[k] = fmaf(x[i][k], wi[i], acc[k]);
+      for (int k = 0; k < A; ++k) {
+        if (i0 + k * i_step >= n) break;
+        // (a part with no score above -inf has weight 0, and keeps a NaN that way)
+        const float w = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - m);
+        l = fmaf(ml[k].y, w, l);
+        acc.x = fmaf(x[k].x, w, acc.x); acc.y = fmaf(x[k].y, w, acc.y);
+        acc.z = fmaf(x[k].z, w, acc.z); acc.w = fmaf(x[k].w, w, acc.w);
+      }
+    }
+    if constexpr (SHARE) {
+      xm[wid][lane] = make_float2(m, l);
+      xo[wid][lane] = acc;
+      __syncthreads();
+      if (wid > 0) return;
+      m = fmaxf(fmaxf(xm[0][lane].x, xm[1][lane].x), fmaxf(xm[2][lane].x, xm[3][lane].x));
+      l = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 y = xm[w][lane];
+        const float f = y.x == -INFINITY ? 0.f : fast_exp2(y.x - m);
+        const float4 o = xo[w][lane];
+        l = fmaf(y.y, f, l);
+        acc.x = fmaf(o.x, f, acc.x); acc.y = fmaf(o.y, f, acc.y);
+        acc.z = fmaf(o.z, f, acc.z); acc.w = fmaf(o.w, f, acc.w);
+      }
+    }
+    if (ok && col < c.d) {
+      const float linv = l == 0.f ? 0.f : 1.f / l;
+      const int row = jn.r0 + r, ri = (int)div32(p.dv_group, (unsigned)row), head = jn.kvh * p.group + row - ri * p.group;
+      const float y[4] = {acc.x * linv, acc.y * linv, acc.z * linv, acc.w * linv};
+      store_vec<4>(reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h + col, y);
     }
   }
-  l = wave_sum(l);
-  const float linv = l == 0.f ? 0.f : 1.f / l;
-  const int ri = (int)div32(p.dv_group, (unsigned)row), head = jn.kvh * p.group + row - ri * p.group;
-  T* orow = reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h;
-#pragma unroll
-  for (int k = 0; k < PL; ++k)
-    if (PL * lane + k < c.d) orow[PL * lane + k] = from_f32<T>(acc[k] * linv);
 }
 
 // ------------------------------------------------------------------ host --
@@ -1038,7 +1077,8 @@ int paged_launch(PagedArgs& p, const Plan& pl, hipStream_t st) {
   }
   if (pl.split) {
     const long rows = (long)p.c.max_new * p.group;
-    const dim3 jgrid((unsigned)pl.grid, (unsigned)(((rows < 32 * WPT ? rows : 32 * WPT) + 3) / 4));
+    constexpr int J = join_rows<DP, 32 * WPT>();
+    const dim3 jgrid((unsigned)pl.grid, (unsigned)(((rows < 32 * WPT ? rows : 32 * WPT) + J - 1) / J));
     paged_join_kernel<T, DP, 32 * WPT><<<jgrid, dim3(256), 0, st>>>(p);
   }
   return check_launch("nkl_paged_attention");
