@@ -180,7 +180,34 @@ struct El<float> {
   static constexpr bool W32 = true, H = false;
 };
 
-template <typename T, int DP, int WPT, int NT>
+// Tiles that the buffer unit copies to LDS (WPT > 1, 16-bit types, a tile in one
+// page): rows of DP elements without gaps, a row's 16-byte chunks swizzled --
+// logical chunk c of row r sits at chunk c ^ swz(r) -- so that sixteen rows'
+// chunk c (a K fragment's read) and four rows' four chunks of a d-block (a V
+// fragment's) lie in banks of their own.
+template <int DP>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (DP == 128) return 4 * (r & 3) + 2 * ((r >> 2) & 1) + ((r >> 3) & 1);
+  if constexpr (DP == 64) return 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1) + ((r >> 3) & 1);
+  return (r >> 2) & 3;
+}
+
+// LDS reads that the compiler does not track (it would make them wait for every
+// copy in flight): their results go through a wait before any use.
+template <int OFF>
+__device__ __forceinline__ bf16x8 lds_b128(unsigned a) {
+  bf16x8 r;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF));
+  return r;
+}
+template <int OFF>
+__device__ __forceinline__ shortx4 lds_tr64(unsigned a) {
+  shortx4 r;
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF));
+  return r;
+}
+
+template <typename T, int DP, int WPT, int NT, bool TP>
 struct Lay {
   static constexpr bool W32 = El<T>::W32;
   static constexpr int MR = 32 * WPT, THREADS = 64 * WPT * NT, TT = 64 * WPT;
@@ -198,7 +225,13 @@ struct Lay {
   // finish (team t finishes those with db % NT == t), 4 KB each.
   static constexpr int ML = NT * WPT * 64 * 8;
   static constexpr int XO = NT > 1 ? NT * WPT * NDB * 4096 : 0;
-  static constexpr int BYTES0 = NT * TEAM * (int)sizeof(T);
+  // Copied tiles: bytes of a tensor's, copies a wavefront (two copy K, two V),
+  // stages.
+  static constexpr bool COPY = TP && WPT > 1;
+  static constexpr int ROWB = DP * (int)sizeof(T), TILEB = BN * ROWB;
+  static constexpr int NCP = TILEB / 2048;
+  static constexpr int CSTAGES = 4;
+  static constexpr int BYTES0 = COPY ? CSTAGES * 2 * TILEB : NT * TEAM * (int)sizeof(T);
   static constexpr int BYTES = BYTES0 > ML + XO ? BYTES0 : ML + XO;
   static_assert(BYTES <= 160 * 1024, "LDS");
 };
@@ -225,10 +258,10 @@ constexpr long part_floats() {
 template <typename T, int DP, int WPT, int NT, bool TP, bool SPLIT>
 __global__ __launch_bounds__(64 * WPT * NT) __attribute__((amdgpu_waves_per_eu(El<T>::W32 && WPT == 1 && DP == 128 ? 1 : 2)))
 void paged_attn_kernel(PagedArgs p) {
-  using L = Lay<T, DP, WPT, NT>;
+  using L = Lay<T, DP, WPT, NT, TP>;
   constexpr bool W32 = L::W32, H16 = El<T>::H;
   constexpr int MR = L::MR, TT = L::TT, CPR = L::CPR, CH = L::CH, NDB = L::NDB, E = L::E;
-  __shared__ __align__(16) unsigned char smem[L::BYTES];
+  __shared__ __align__(1024) unsigned char smem[L::BYTES];  // (fragment addresses are formed by XOR within 256 bytes)
 
   const CacheArgs& c = p.c;
 
@@ -277,7 +310,7 @@ void paged_attn_kernel(PagedArgs p) {
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int team = wid / WPT, wq = wid % WPT, ttid = tid % TT;
     const int h32 = lane >> 5, l32 = lane & 31;
-    T* const stage0 = reinterpret_cast<T*>(smem) + team * L::TEAM;
+    T* const stage0 = reinterpret_cast<T*>(smem) + (L::COPY ? 0 : team * L::TEAM);
     // This thread's chunks of a tile in one page: byte offsets from the tile's
     // first row, columns past d out of range.
     int voff_k, voff_v;
@@ -353,7 +386,8 @@ void paged_attn_kernel(PagedArgs p) {
     }
 
     // ---- staging
-    constexpr bool LANES = TP && WPT > 1;
+    constexpr bool LANES = L::COPY;
+    static_assert(!LANES || (WPT == 4 && NT == 1), "four wavefronts copy a tile");
     const unsigned char* const Kb = c.k + (long)kvh * c.k_head * (long)sizeof(T);
     const unsigned char* const Vb = c.v + (long)kvh * c.v_head * (long)sizeof(T);
     const int* const trow = c.table + (c.table ? (long)b * c.table_row : 0);
@@ -400,31 +434,55 @@ void paged_attn_kernel(PagedArgs p) {
     // scalar unit, this took more instructions than the softmax.  The pages of
     // the next 64 are on their way meanwhile.
     struct Lanes {
-      unsigned k_lo, k_hi, v_lo, v_hi;
-      int k_bytes, v_bytes, flags;
+      unsigned lo, hi;
+      int bytes, flags;
     } lt = {};
     int pid_next = 0;
     auto tile_first = [&](int it) __attribute__((always_inline)) {
-      const int x = c0 + team + NT * it;
+      const int x = c0 + it;
       return BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
     };
     auto load_pids = [&](int base) __attribute__((always_inline)) {
       const int it = base + lane;
       pid_next = !c.table || it >= nit ? 0 : trow[div32(c.dv_page, (unsigned)tile_first(it))];
     };
+    const bool copies_v = wq >= 2;
     auto fill_lanes = [&](int base) __attribute__((always_inline)) {
-      const int it = base + lane, x = c0 + team + NT * it, k0 = tile_first(it), pid = pid_next;
+      const int it = base + lane, x = c0 + it, k0 = tile_first(it), pid = pid_next;
       const int n = it < nit && (unsigned)pid < (unsigned)c.pages ? min(BN, sp.hi - k0) : 0;
       const unsigned pg = n > 0 ? pid : 0;
       const unsigned within = n > 0 ? k0 - (int)div32(c.dv_page, (unsigned)k0) * c.page_size : 0;
-      const unsigned long ka = (unsigned long)Kb + (unsigned long)pg * p.k_page32 + (unsigned long)within * p.k_row32;
-      const unsigned long va = (unsigned long)Vb + (unsigned long)pg * p.v_page32 + (unsigned long)within * p.v_row32;
-      lt.k_lo = (unsigned)ka; lt.k_hi = (unsigned)(ka >> 32);
-      lt.v_lo = (unsigned)va; lt.v_hi = (unsigned)(va >> 32);
-      lt.k_bytes = n > 0 ? (n - 1) * (int)p.k_row32 + row_bytes : 0;
-      lt.v_bytes = n > 0 ? (n - 1) * (int)p.v_row32 + row_bytes : 0;
+      const unsigned long at = (unsigned long)(copies_v ? Vb : Kb) +
+                               (unsigned long)pg * (copies_v ? p.v_page32 : p.k_page32) +
+                               (unsigned long)within * (copies_v ? p.v_row32 : p.k_row32);
+      lt.lo = (unsigned)at;
+      lt.hi = (unsigned)(at >> 32);
+      lt.bytes = n > 0 ? (n - 1) * (int)(copies_v ? p.v_row32 : p.k_row32) + row_bytes : 0;
       lt.flags = n | ((unsigned)(x - f0) >= fn || n < BN ? 256 : 0);
       load_pids(base + 64);
+    };
+    // Copies this wavefront's part of tile `it` to LDS (lane l's 16 bytes at the
+    // copy's place + 16 l; past the last tile nothing is read, and zeros are
+    // written); returns the tile's flags.
+    unsigned lds0 = 0;
+    int coff[L::NCP > 0 ? L::NCP : 1];
+    auto copy_tile = [&](int it) __attribute__((always_inline)) {
+      if ((it & 63) == 0) fill_lanes(it);
+      const int l = it & 63;
+      auto lane_of = [&](unsigned x) __attribute__((always_inline)) { return (unsigned)__builtin_amdgcn_readlane(x, l); };
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(((unsigned long)lane_of(lt.hi) << 32) | lane_of(lt.lo)), (short)0, (int)lane_of(lt.bytes),
+          fsched::kBufferFlags);
+      const unsigned dst = lds0 + (it % L::CSTAGES) * 2 * L::TILEB + wq * L::NCP * 1024;
+#pragma unroll
+      for (int i = 0; i < L::NCP; ++i) {
+        // (Through locals: written inline in the builtin's arguments they make
+        // the host pass drop the kernel's launch stub without a diagnostic.)
+        const int off = coff[i];
+        const unsigned at = dst + i * 1024;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_ptr(at), 16, off, 0, 0, 0);
+      }
+      return (int)lane_of(lt.flags);
     };
     uint4 rk[CH], rv[CH];
     // Loads a tile and returns a bit for each of its keys that is read.
@@ -465,26 +523,6 @@ void paged_attn_kernel(PagedArgs p) {
         t.masked = t.masked || bits != ~0u;
         return bits;
       }
-    };
-    // Loads tile `it` by the lanes' list; returns its flags.
-    auto gload_lane = [&](int it) __attribute__((always_inline)) {
-      if ((it & 63) == 0) fill_lanes(it);
-      const int l = it & 63;
-      auto lane_of = [&](unsigned x) __attribute__((always_inline)) { return (unsigned)__builtin_amdgcn_readlane(x, l); };
-      const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(((unsigned long)lane_of(lt.k_hi) << 32) | lane_of(lt.k_lo)), (short)0, (int)lane_of(lt.k_bytes),
-          fsched::kBufferFlags);
-      const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(((unsigned long)lane_of(lt.v_hi) << 32) | lane_of(lt.v_lo)), (short)0, (int)lane_of(lt.v_bytes),
-          fsched::kBufferFlags);
-      int step_k = (TT / CPR) * (int)p.k_row32, step_v = (TT / CPR) * (int)p.v_row32;
-      asm volatile("" : "+s"(step_k), "+s"(step_v));
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, 0));
-        rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, 0));
-      }
-      return (int)lane_of(lt.flags);
     };
     // Stages the loaded tile.  Where the tile is masked its infinities and NaN
     // of V are left out (0 * inf would reach the rows that do not see them) and
@@ -655,26 +693,123 @@ void paged_attn_kernel(PagedArgs p) {
       __builtin_amdgcn_s_barrier();
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
     };
-    if constexpr (WPT > 1 && !W32) {
-      // A team's wavefronts share its tiles, staged one step ahead.  A step's
-      // LDS reads are in flight while others compute: V's go out before the
-      // softmax, the next tile's K before P V.  The barrier between the two
-      // covers tile it + 1's staging, three stages deep: the stage that step
-      // `it` writes was last read by P V of tile it - 2, which every wavefront
-      // had behind it at the barrier of step it - 1.
-      int fl_cur = 0, fl_nxt = 0, fl_far = 0;
-      if constexpr (LANES) {
-        load_pids(0);
-        fl_cur = gload_lane(0);
-      } else {
-        far = look_up(2);
+    if constexpr (LANES) {
+      // The wavefronts share their tiles, copied three steps ahead of use into
+      // four stages.  A step's LDS reads are in flight while others compute:
+      // V's go out before the softmax, the next tile's K before P V.  One
+      // barrier a step, between the two: before it each wavefront waits for its
+      // own copies of tile it + 1 and for its reads of V, so that behind it the
+      // whole tile is there, and the stage of tile `it` is free for the copies
+      // that step it + 1 starts.
+      {
+        lds0 = opaque_lds_addr(smem);
+        const int row_b = (int)(copies_v ? p.v_row32 : p.k_row32);
+#pragma unroll
+        for (int i = 0; i < L::NCP; ++i) {
+          const int r = ((wq & 1) * L::NCP + i) * (64 / CPR) + lane / CPR, ch = (lane % CPR) ^ swz<DP>(r);
+          coff[i] = ch * E < c.d ? r * row_b + 16 * ch : 0x40000000;
+        }
       }
-      lstore(stage0, LANES ? fl_cur >= 256 : cur.masked);
+      // This lane's places in a stage: K row l32, chunk 2 f + h32 at
+      // ka ^ 32 f; V rows r and r + 8 (then 16 further), d-block db at
+      // va ^ 64 db.
+      const unsigned ka = l32 * L::ROWB + ((h32 ^ swz<DP>(l32)) << 4);
+      unsigned va[2];
+      {
+        const int i16 = lane & 15, g2 = (lane >> 4) & 1, r = 4 * h32 + (i16 >> 2), ch = 2 * g2 + ((i16 & 3) >> 1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          va[k] = L::TILEB + (r + 8 * k) * L::ROWB + ((ch ^ swz<DP>(r + 8 * k)) << 4) + (i16 & 1) * 8;
+      }
+      auto read_kf = [&](unsigned st) __attribute__((always_inline)) {
+        const unsigned a = st + ka;
+#pragma unroll
+        for (int f = 0; f < L::NQ; ++f) kf[f] = lds_b128<0>(a ^ (32 * f));
+      };
+      auto tie_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int f = 0; f < L::NQ; ++f) lds_wait_tie(kf[f]);
+      };
+      load_pids(0);
+      int fl_cur = copy_tile(0), fl_nxt = copy_tile(1), fl_far = copy_tile(2);
+      fsched::wait_vm<2 * L::NCP>();
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      __builtin_amdgcn_s_barrier();
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      read_kf(lds0);
+      tie_k();
+#pragma unroll 1
+      for (int it = 0; it < nsteps; ++it) {
+        const unsigned st = lds0 + (it % L::CSTAGES) * 2 * L::TILEB;
+        const bool masked = fl_cur >= 256;
+        floatx16 sc;
+        qk(nullptr, sc);
+        if (masked) {
+          // V's infinities and NaN leave a masked tile (see lstore): every
+          // thread looks at its chunks.
+#pragma unroll
+          for (int i = 0; i < (L::TILEB + 4095) / 4096; ++i) {
+            const unsigned a = st + L::TILEB + min(tid * 16 + i * 4096, L::TILEB - 16);
+            bf16x8 v = lds_b128<0>(a);
+            lds_wait_tie(v);
+            uint4 w = __builtin_bit_cast(uint4, v);
+            const uint4 odd = make_uint4(not_finite<T>(w.x), not_finite<T>(w.y), not_finite<T>(w.z), not_finite<T>(w.w));
+            if (odd.x | odd.y | odd.z | odd.w) {
+              odd_v = 1;
+              w = make_uint4(w.x & ~odd.x, w.y & ~odd.y, w.z & ~odd.z, w.w & ~odd.w);
+              v = __builtin_bit_cast(bf16x8, w);
+              asm volatile("ds_write_b128 %0, %1" ::"v"(a), "v"(v) : "memory");
+            }
+          }
+          lds_barrier();
+        }
+        shortx4 vr[NDB][4];  // (left as they are read until the wait: no copy of a register may precede it)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const unsigned a = (st + va[0]) ^ (64 * db), b2 = (st + va[1]) ^ (64 * db);
+          vr[db][0] = lds_tr64<0>(a);
+          vr[db][1] = lds_tr64<0>(b2);
+          vr[db][2] = lds_tr64<16 * L::ROWB>(a);
+          vr[db][3] = lds_tr64<16 * L::ROWB>(b2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const int fl = copy_tile(it + 3);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(sc, it, masked, fl_cur & 255);
+        bf16x8 pf[2];
+        to_p(sc, pf);
+        bf16x8 vf[NDB][2];
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[db][k]));
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            vf[db][k] = __builtin_bit_cast(
+                bf16x8, __builtin_shufflevector(vr[db][2 * k], vr[db][2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+        fsched::wait_vm<2 * L::NCP>();  // tiles it + 2 and it + 3 may still be on their way
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_barrier();
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        read_kf(lds0 + ((it + 1) % L::CSTAGES) * 2 * L::TILEB);
+        __builtin_amdgcn_sched_barrier(0);
+        mma_v(vf, pf, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        tie_k();
+        fl_cur = fl_nxt, fl_nxt = fl_far, fl_far = fl;
+      }
+      // (the copies past the last tile write zeros: they land before LDS is used again)
+      __builtin_amdgcn_s_waitcnt(0);
+    } else if constexpr (WPT > 1 && !W32) {
+      // As above with tiles staged through registers, one step ahead and three
+      // stages deep: the stage that step `it` writes was last read by P V of
+      // tile it - 2, which every wavefront had behind it at the barrier of
+      // step it - 1.
+      far = look_up(2);
+      lstore(stage0, cur.masked);
       lds_barrier();
-      if constexpr (LANES)
-        fl_nxt = gload_lane(1);
-      else
-        kv_nxt = gload(nxt);
+      kv_nxt = gload(nxt);
       read_k(stage0);
       int st_cur = 0, st_nxt = L::STAGE;
 #pragma unroll 1
@@ -684,33 +819,20 @@ void paged_attn_kernel(PagedArgs p) {
         qk(stage0 + st_cur, sc);
         read_v(stage0 + st_cur, 0, vf);
         __builtin_amdgcn_sched_barrier(0);
-        lstore(stage0 + st_nxt, LANES ? fl_nxt >= 256 : nxt.masked);
-        unsigned kv_far = 0;
-        Tile t;
-        if constexpr (LANES) {
-          fl_far = gload_lane(it + 2);
-        } else {
-          kv_far = gload(far);
-          t = look_up(it + 3);
-        }
+        lstore(stage0 + st_nxt, nxt.masked);
+        const unsigned kv_far = gload(far);
+        const Tile t = look_up(it + 3);
         __builtin_amdgcn_sched_barrier(0);
         // (a team's step past its tiles: no key is valid, P is zero)
-        if constexpr (LANES)
-          softmax(sc, it, fl_cur >= 256, fl_cur & 255);
-        else
-          softmax(sc, cur.k0, cur.masked, kv_cur);
+        softmax(sc, cur.k0, cur.masked, kv_cur);
         bf16x8 pf[2];
         to_p(sc, pf);
         lds_barrier();
         read_k(stage0 + st_nxt);
         __builtin_amdgcn_sched_barrier(0);
         mma_v(vf, pf, 0);
-        if constexpr (LANES) {
-          fl_cur = fl_nxt, fl_nxt = fl_far;
-        } else {
-          cur = nxt, nxt = far, far = t;
-          kv_cur = kv_nxt, kv_nxt = kv_far;
-        }
+        cur = nxt, nxt = far, far = t;
+        kv_cur = kv_nxt, kv_nxt = kv_far;
         st_cur = st_nxt;
         st_nxt = st_nxt == 2 * L::STAGE ? 0 : st_nxt + L::STAGE;
       }
