@@ -70,7 +70,7 @@ struct PagedArgs {
   // a range.  joins: one for each range.
   float* part;
   Join* joins;
-  int target, min_tiles;
+  int target, min_tiles, setup, align;
   int tiles_max;  // row tiles of the longest sequence
   int per_xcd;    // not split: items per XCD
 };
@@ -104,16 +104,27 @@ __device__ __forceinline__ Span span_of(const PagedArgs& p, const Seq& s, int r0
   return x;
 }
 
-// Split schedule.  A row tile of a K/V head holds as many units as it has key
-// tiles (one where it sees nothing: its zeros are to be written), numbered by
-// sequence, row tile and K/V head.  The units are cut into ranges of equal
-// length, one a workgroup, so that ragged lengths leave no workgroup behind;
-// only a range's first and last segment can be part of a row tile.
+// Split schedule.  A row tile of a K/V head (an item) costs `setup` units and
+// then one for each of its key tiles (one where it sees nothing: its zeros are
+// to be written).  The items' units, by sequence, row tile and K/V head, are
+// cut into ranges of equal length, one a workgroup, so that ragged lengths
+// leave no workgroup behind; only a range's first and last segment can be part
+// of an item.  `setup` is what a segment costs beside its tiles (Q's load, the
+// first tile's latency, the stores): without it the ranges with the most and
+// shortest items end last (16 trees of 64 nodes: 98 us in the median, 133 at
+// the end).  Where workgroups are many to an item (`align`), an item fills
+// ranges of its own instead, and no range has two segments.
+__device__ __forceinline__ int item_units(const PagedArgs& p, int nt, int len) {
+  const int n = p.setup + max(nt, 1);
+  return p.align && len > 0 ? (int)((unsigned)(n + len - 1) / (unsigned)len) * len : n;
+}
+
+// Units of a sequence; len > 0: with its items aligned to ranges of that length.
 template <int MR>
-__device__ __forceinline__ int seq_units(const PagedArgs& p, const Seq& s) {
+__device__ __forceinline__ int seq_units(const PagedArgs& p, const Seq& s, int len) {
   int sum = 0;
   const int rows = s.use * p.group;
-  for (int r0 = 0; r0 < rows; r0 += MR) sum += max(span_of(p, s, r0, MR).nt, 1);
+  for (int r0 = 0; r0 < rows; r0 += MR) sum += item_units(p, span_of(p, s, r0, MR).nt, len);
   return sum * p.c.kv_heads;
 }
 
@@ -124,26 +135,34 @@ __device__ __forceinline__ int seq_units(const PagedArgs& p, const Seq& s) {
 template <int MR>
 __device__ __forceinline__ void find_range(const PagedArgs& p, int w, int& len, int& u, int& u1, int& b, int& first) {
   const int lane = threadIdx.x & 63, batch = p.c.batch;
-  auto scan = [&](int b0) __attribute__((always_inline)) {  // units of sequences b0 .. b0 + lane
-    int x = b0 + lane < batch ? seq_units<MR>(p, seq_of(p.c, b0 + lane)) : 0;
+  auto scan = [&](int b0, int al) __attribute__((always_inline)) {  // units of sequences b0 .. b0 + lane
+    int x = b0 + lane < batch ? seq_units<MR>(p, seq_of(p.c, b0 + lane), al) : 0;
     for (int o = 1; o < 64 && o < batch; o <<= 1) {
       const int y = __shfl_up(x, o, kWave);
       if (lane >= o) x += y;
     }
     return x;
   };
-  int incl = scan(0);
-  int total = __builtin_amdgcn_readlane(incl, 63 < batch ? 63 : batch - 1);
-  for (int b0 = 64; b0 < batch; b0 += 64)
-    total += __builtin_amdgcn_readlane(scan(b0), batch - b0 > 64 ? 63 : batch - b0 - 1);
+  auto sum_of = [&](int al, int incl) __attribute__((always_inline)) {
+    int total = __builtin_amdgcn_readlane(incl, 63 < batch ? 63 : batch - 1);
+    for (int b0 = 64; b0 < batch; b0 += 64)
+      total += __builtin_amdgcn_readlane(scan(b0, al), batch - b0 > 64 ? 63 : batch - b0 - 1);
+    return total;
+  };
+  int incl = scan(0, 0);
+  int total = sum_of(0, incl);
   len = max((int)(((long)total + p.target - 1) / p.target), p.min_tiles);
+  if (p.align) {
+    incl = scan(0, len);
+    total = sum_of(len, incl);
+  }
   u = (int)min((long)w * len, (long)total);
   u1 = (int)min((long)u + len, (long)total);
   first = 0;
   b = batch;
   if (u >= u1) return;
   for (int b0 = 0; b0 < batch; b0 += 64) {
-    if (b0 > 0) incl = scan(b0);
+    if (b0 > 0) incl = scan(b0, len);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(b0 + lane < batch && u < first + incl);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -268,7 +287,7 @@ void paged_attn_kernel(PagedArgs p) {
   // ---- this workgroup's units: a range of them, or one row tile's
   int b, kvh, r0;
   int len = 1, u = 0, u1 = 1;
-  int skip = 0;  // key tiles of the row tile before the range
+  int skip = 0;  // units of the item before the range
   Seq s;
   if constexpr (SPLIT) {
     int first;
@@ -280,13 +299,13 @@ void paged_attn_kernel(PagedArgs p) {
     s = seq_of(c, b);
     int x = u - first;
     for (r0 = 0;; r0 += MR) {
-      const int nt = max(span_of(p, s, r0, MR).nt, 1);
-      if (x < nt * c.kv_heads) {
-        kvh = x / nt;
-        skip = x - kvh * nt;
+      const int n = item_units(p, span_of(p, s, r0, MR).nt, len);
+      if (x < n * c.kv_heads) {
+        kvh = x / n;
+        skip = x - kvh * n;
         break;
       }
-      x -= nt * c.kv_heads;
+      x -= n * c.kv_heads;
     }
   } else {
     // Workgroups are dealt to the 8 XCDs in turn: item (id % 8) per_xcd + id / 8
@@ -322,9 +341,15 @@ void paged_attn_kernel(PagedArgs p) {
 
     // ---- the segment: key tiles c0 .. c1 - 1 of row tile r0, K/V head kvh
     const Span sp = span_of(p, s, r0, MR);
-    const int c0 = skip;
-    const int c1 = SPLIT ? min(sp.nt, skip + (u1 - u)) : sp.nt;
+    // (the item's units: its setup, then its tiles)
+    const int c0 = SPLIT ? max(0, skip - p.setup) : 0;
+    const int c1 = SPLIT ? min(sp.nt, skip + (u1 - u) - p.setup) : sp.nt;
     const bool whole = !SPLIT || (c0 == 0 && c1 == sp.nt);
+    if (SPLIT && (c1 < c0 || (c1 == c0 && sp.nt > 0))) {
+      // The range ends in the item's setup.
+      if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
+      return;
+    }
 
     // ---- this lane's row
     const int nrows = s.use * p.group;
@@ -1001,7 +1026,7 @@ void paged_attn_kernel(PagedArgs p) {
       // row tile begins here and goes on in the next ranges: slot 1, and the
       // entry by which the second kernel finds its parts.
       if (c0 == 0 && threadIdx.x == 0)
-        p.joins[blockIdx.x] = {b, kvh, r0, (u + sp.nt - 1) / len - (int)blockIdx.x + 1};
+        p.joins[blockIdx.x] = {b, kvh, r0, (u - skip + p.setup + sp.nt - 1) / len - (int)blockIdx.x + 1};
       float* part = p.part + (2L * blockIdx.x + (c0 > 0 ? 0 : 1)) * part_floats<DP, MR>();
       const int r = 32 * wq + l32;
 #pragma unroll
@@ -1017,7 +1042,7 @@ void paged_attn_kernel(PagedArgs p) {
 
     if constexpr (!SPLIT) break;
     // ---- the range's next segment: the next K/V head, row tile or sequence
-    u += max(c1 - c0, 1);
+    u += item_units(p, sp.nt, len) - skip;
     if (u >= u1) {
       if ((whole || c0 > 0) && threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
       break;
@@ -1138,7 +1163,7 @@ struct Plan {
   int tiles_max; // row tiles of the longest sequence
   long items;    // row tiles at most
   bool one_page; // a key tile lies in one page
-  int target, min_tiles;
+  int target, min_tiles, setup, align;
   long grid;
   size_t bytes;  // workspace
 };
@@ -1168,12 +1193,20 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   // causal prompt with no window): up to four rounds of them.
   const long rounds = c.batch == 1 && window ? 1 : 4;
   pl.split = pl.items < rounds * (pl.wide ? cus : 2 * cus) && key_tiles > 2 * pl.min_tiles;
-  if (pl.split && pl.items * (key_tiles + 1) >= 1L << 31) pl.split = false;
+  // Four ranges and more to an item: items of their own ranges, which are then
+  // no more than the workgroups with one range less to each item.
+  pl.align = pl.items * 4 <= pl.target;
+  pl.setup = pl.align ? 0 : 8;
+  pl.grid = pl.target;
+  if (pl.align) {
+    pl.target -= (int)pl.items;
+    pl.min_tiles = 4;
+  }
+  if (pl.split && pl.items * (key_tiles + pl.setup + pl.grid) >= 1L << 30) pl.split = false;
   // (32-bit byte offsets within a tile, and byte strides)
   pl.one_page = (!c.table || c.page_size % BN == 0) && c.k_row <= (1L << 21) && c.v_row <= (1L << 21) &&
                 c.k_page < (1L << 30) && c.v_page < (1L << 30);
   if (pl.split) {
-    pl.grid = pl.target;
     pl.bytes = (size_t)pl.grid * (sizeof(Join) + 2 * (size_t)mr * (pl.dp + 2) * 4);
   } else {
     pl.grid = (pl.items + 7) / 8 * 8;
@@ -1293,6 +1326,8 @@ extern "C" int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, 
   }
   p.target = pl.target;
   p.min_tiles = pl.min_tiles;
+  p.setup = pl.setup;
+  p.align = pl.align;
   p.tiles_max = pl.tiles_max;
   p.per_xcd = (int)(pl.grid / 8);
   hipStream_t st = (hipStream_t)stream;
