@@ -199,8 +199,8 @@ struct El<float> {
   static constexpr bool W32 = true, H = false;
 };
 
-// Tiles that the buffer unit copies to LDS (WPT > 1, 16-bit types, a tile in one
-// page): rows of DP elements without gaps, a row's 16-byte chunks swizzled --
+// Tiles that the buffer unit copies to LDS (one team of four wavefronts, 16-bit
+// types, a tile in one page): rows of DP elements without gaps, a row's 16-byte chunks swizzled --
 // logical chunk c of row r sits at chunk c ^ swz(r) -- so that sixteen rows'
 // chunk c (a K fragment's read) and four rows' four chunks of a d-block (a V
 // fragment's) lie in banks of their own.
@@ -246,7 +246,7 @@ struct Lay {
   static constexpr int XO = NT > 1 ? NT * WPT * NDB * 4096 : 0;
   // Copied tiles: bytes of a tensor's, copies a wavefront (two copy K, two V),
   // stages.
-  static constexpr bool COPY = TP && WPT > 1;
+  static constexpr bool COPY = TP && WPT > 1 && NT == 1;
   static constexpr int ROWB = DP * (int)sizeof(T), TILEB = BN * ROWB;
   static constexpr int NCP = TILEB / 2048;
   static constexpr int CSTAGES = 4;
@@ -412,7 +412,7 @@ void paged_attn_kernel(PagedArgs p) {
 
     // ---- staging
     constexpr bool LANES = L::COPY;
-    static_assert(!LANES || (WPT == 4 && NT == 1), "four wavefronts copy a tile");
+    static_assert(!LANES || WPT == 4, "four wavefronts copy a tile");
     const unsigned char* const Kb = c.k + (long)kvh * c.k_head * (long)sizeof(T);
     const unsigned char* const Vb = c.v + (long)kvh * c.v_head * (long)sizeof(T);
     const int* const trow = c.table + (c.table ? (long)b * c.table_row : 0);
@@ -1215,26 +1215,26 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   return NKL_OK;
 }
 
-template <typename T, int DP, int WPT, int NT>
+// DIRECT: of the plans that are not split only.
+template <typename T, int DP, int WPT, int NT, bool DIRECT = false>
 int paged_launch(PagedArgs& p, const Plan& pl, hipStream_t st) {
   const dim3 grid((unsigned)pl.grid), block(64 * WPT * NT);
-  constexpr bool TP = !El<T>::W32;
-  if (TP && pl.one_page) {
-    if (pl.split)
-      paged_attn_kernel<T, DP, WPT, NT, TP, true><<<grid, block, 0, st>>>(p);
-    else
-      paged_attn_kernel<T, DP, WPT, NT, TP, false><<<grid, block, 0, st>>>(p);
-  } else {
-    if (pl.split)
-      paged_attn_kernel<T, DP, WPT, NT, false, true><<<grid, block, 0, st>>>(p);
-    else
-      paged_attn_kernel<T, DP, WPT, NT, false, false><<<grid, block, 0, st>>>(p);
-  }
-  if (pl.split) {
+  auto run = [&](auto one_page, auto split) {
+    paged_attn_kernel<T, DP, WPT, NT, decltype(one_page)::value, decltype(split)::value><<<grid, block, 0, st>>>(p);
+  };
+  constexpr std::integral_constant<bool, !El<T>::W32> kOnePage{};
+  constexpr std::integral_constant<bool, false> kNo{};
+  constexpr std::integral_constant<bool, !DIRECT> kSplit{};
+  if (pl.split && !DIRECT) {
+    if (kOnePage && pl.one_page) run(kOnePage, kSplit);
+    else run(kNo, kSplit);
     const long rows = (long)p.c.max_new * p.group;
     constexpr int J = join_rows<DP, 32 * WPT>();
     const dim3 jgrid((unsigned)pl.grid, (unsigned)(((rows < 32 * WPT ? rows : 32 * WPT) + J - 1) / J));
     paged_join_kernel<T, DP, 32 * WPT><<<jgrid, dim3(256), 0, st>>>(p);
+  } else {
+    if (kOnePage && pl.one_page) run(kOnePage, kNo);
+    else run(kNo, kNo);
   }
   return check_launch("nkl_paged_attention");
 }
@@ -1242,7 +1242,16 @@ int paged_launch(PagedArgs& p, const Plan& pl, hipStream_t st) {
 template <typename T>
 int paged_launch_d(PagedArgs& p, const Plan& pl, hipStream_t st) {
   if (pl.wide) {
+    // One team a workgroup lets two workgroups of a CU run out of step (their
+    // LDS reads, MFMAs and exps overlap: 32 x 16384 x 128 1.35 -> 1.21 ms).
+    // Where a CU has one workgroup at most, two teams of it share the keys
+    // (16 x 2048 x 128 under a window of 512: 29 -> 26 us).
     constexpr int NT = El<T>::W32 ? 2 : 1;
+    if (!pl.split && pl.items <= cu_count()) {
+      if (pl.dp == 32) return paged_launch<T, 32, 4, 2, !El<T>::W32>(p, pl, st);
+      if (pl.dp == 64) return paged_launch<T, 64, 4, 2, !El<T>::W32>(p, pl, st);
+      return paged_launch<T, 128, 4, 2, !El<T>::W32>(p, pl, st);
+    }
     if (pl.dp == 32) return paged_launch<T, 32, 4, NT>(p, pl, st);
     if (pl.dp == 64) return paged_launch<T, 64, 4, NT>(p, pl, st);
     return paged_launch<T, 128, 4, NT>(p, pl, st);
