@@ -1,0 +1,268 @@
+"""A paged K/V cache: which pages each sequence has, and the tensors they are in.
+
+``PagePool`` keeps the books on the host: sequences are lists of page ids,
+pages are counted, and forked sequences share theirs until one of them writes.
+``PagedCache`` adds the tensors ([layers, pages, kv_heads, page_size, d]) and
+runs the copies its pool asks for; ``nkilab.ops`` writes to them and attends
+over them, ``nkilab.model.nki_decode`` runs a decoder block over them.  The
+reference has no cache (its block attends over one prompt, model.py:59-67).
+
+    cache = PagedCache(pages=1024, kv_heads=8, head_dim=128, layers=24)
+    seq = cache.add()
+    step = cache.step([seq], [len(prompt)])        # rows for the prompt
+    x = nki_decode(block, x, cache, step, layer)   # for every layer
+    step = cache.step([seq], [16], tree=parents)   # a tree of 16 drafted tokens
+    ...
+    cache.accept(step, [[0, 3, 7]])                # the path that was accepted
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import ops
+
+
+class OutOfPages(RuntimeError):
+    """No free page is left for what was asked; nothing has changed."""
+
+
+class PagePool:
+    """Pages and sequences, on the host."""
+
+    def __init__(self, pages: int, page_size: int):
+        if pages < 1 or page_size < 1:
+            raise ValueError(f"PagePool: pages={pages} and page_size={page_size} must be at least 1")
+        self.pages, self.page_size = int(pages), int(page_size)
+        self._free = list(range(self.pages - 1, -1, -1))  # taken from the end: the lowest first
+        self._users = [0] * self.pages
+        self._tables: dict[int, list[int]] = {}
+        self._lens: dict[int, int] = {}
+        self._floor: dict[int, int] = {}  # the length a sequence had when it last gave up pages
+        self._next = 0
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        seq, self._next = self._next, self._next + 1
+        self._tables[seq], self._lens[seq], self._floor[seq] = [], 0, 0
+        return seq
+
+    def length(self, seq: int) -> int:
+        return self._lens[seq]
+
+    def pages_of(self, seq: int) -> list[int]:
+        """The sequence's pages in order; -1 where one was released."""
+        return list(self._tables[seq])
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self) -> int:
+        p = self._free.pop()
+        self._users[p] = 1
+        return p
+
+    def _drop(self, page: int) -> None:
+        if page < 0:
+            return
+        self._users[page] -= 1
+        if self._users[page] == 0:
+            self._free.append(page)
+
+    def fork(self, seq: int) -> int:
+        """A sequence with the same rows, in the same pages until either writes."""
+        new = self.add()
+        self._tables[new], self._lens[new] = list(self._tables[seq]), self._lens[seq]
+        self._floor[new] = self._floor[seq]
+        for p in self._tables[new]:
+            if p >= 0:
+                self._users[p] += 1
+        return new
+
+    def free(self, seq: int) -> None:
+        """Ends a sequence; pages that no other has are free again."""
+        for p in self._tables.pop(seq):
+            self._drop(p)
+        del self._lens[seq], self._floor[seq]
+
+    def own(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> list[tuple[int, int]]:
+        """Gives each sequence pages of its own for rows starts[i] .. ends[i] - 1 and
+        that length.  Returns the (from, to) copies that are to be made first; the
+        rows before starts[i] are kept, those from there on with `keep` only."""
+        ps = self.page_size
+        if len(set(seqs)) != len(seqs):
+            raise ValueError(f"a sequence is named twice: {seqs}")
+        users = dict()  # pages' users as they will be
+        need = 0
+        for seq, start, end in zip(seqs, starts, ends):
+            table = self._tables[seq]
+            for i in range(start // ps, -(-end // ps) if end > start else 0):
+                if i >= len(table):
+                    need += 1
+                    continue
+                p = table[i]
+                if p < 0:
+                    raise ValueError(f"sequence {seq}: rows {i * ps} .. were released")
+                left = users.get(p, self._users[p])
+                if left > 1:
+                    need += 1
+                    users[p] = left - 1
+        if need > len(self._free):
+            raise OutOfPages(f"{need} pages needed, {len(self._free)} of {self.pages} free")
+        copies = []
+        for seq, start, end in zip(seqs, starts, ends):
+            table = self._tables[seq]
+            for i in range(start // ps, -(-end // ps) if end > start else 0):
+                if i >= len(table):
+                    table.append(self._take())
+                elif self._users[table[i]] > 1:
+                    old, new = table[i], self._take()
+                    self._users[old] -= 1
+                    table[i] = new
+                    if keep or i * ps < start:
+                        copies.append((old, new))
+            self._lens[seq] = max(end, 0)
+        return copies
+
+    def trim(self, seq: int, length: int) -> None:
+        """Cuts a sequence to its first `length` rows (no fewer than it had when
+        pages were last released: its next tokens would look for them)."""
+        if not self._floor[seq] <= length <= self._lens[seq]:
+            raise ValueError(f"sequence {seq}: length {length} outside [{self._floor[seq]}, {self._lens[seq]}]")
+        table = self._tables[seq]
+        while len(table) > -(-length // self.page_size):
+            self._drop(table.pop())
+        self._lens[seq] = length
+
+    def release(self, seq: int, window: int, sinks: int = 0) -> int:
+        """Gives up the pages that no later token sees under a window: those whose
+        rows are all at least `window` before the sequence's next position and
+        none of the first `sinks`.  Returns how many."""
+        if window < 1 or sinks < 0:
+            raise ValueError(f"window={window} must be at least 1 and sinks={sinks} at least 0")
+        ps, table, n = self.page_size, self._tables[seq], 0
+        for i in range(-(-sinks // ps), max(0, (self._lens[seq] - window + 1) // ps)):
+            if table[i] >= 0:
+                self._drop(table[i])
+                table[i] = -1
+                n += 1
+        if n:
+            self._floor[seq] = self._lens[seq]
+        return n
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Moves the pages in use to the lowest ids.  Returns the copies."""
+        used = [p for p in range(self.pages) if self._users[p]]
+        low = [p for p in range(len(used)) if not self._users[p]]
+        moves = dict(zip([p for p in used if p >= len(used)], low))
+        for table in self._tables.values():
+            table[:] = [moves.get(p, p) for p in table]
+        for a, b in moves.items():
+            self._users[b], self._users[a] = self._users[a], 0
+        self._free = list(range(self.pages - 1, len(used) - 1, -1))
+        return list(moves.items())
+
+
+@dataclass
+class CacheStep:
+    """The new rows of some sequences, as the operators take them (device
+    tensors), and as the cache knows them."""
+    seqs: list[int]
+    counts: list[int]
+    table: torch.Tensor      # int32 [batch, columns]
+    lens: torch.Tensor       # int32 [batch], with the new rows
+    q_start: torch.Tensor    # int32 [batch + 1]
+    max_q: int
+    tree: torch.Tensor | None = None
+
+    @property
+    def rows(self) -> int:
+        return sum(self.counts)
+
+
+class PagedCache(PagePool):
+    """K and V of every layer in pages, and the sequences they belong to."""
+
+    def __init__(self, pages: int, kv_heads: int, head_dim: int, layers: int = 1, page_size: int = 64,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str | None = None):
+        super().__init__(pages, page_size)
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        device = torch.device("cuda") if device is None else device
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+
+    def _copy(self, copies: list[tuple[int, int]]) -> None:
+        if copies:
+            ops.cache_copy_pages(self.k, self.v, copies)
+
+    def _tensor(self, rows) -> torch.Tensor:
+        return torch.tensor(rows, dtype=torch.int32).to(self.k.device)
+
+    def step(self, seqs: list[int], counts: list[int], tree: list[list[int]] | None = None) -> CacheStep:
+        """Makes room for counts[i] new rows of sequence seqs[i] (shared pages that
+        they touch are copied) and describes them.  tree: each sequence's drafted
+        tree as its nodes' parents (see ``ops.tree_mask``)."""
+        seqs, counts = list(seqs), [int(n) for n in counts]
+        if len(seqs) != len(counts) or any(n < 0 for n in counts):
+            raise ValueError(f"step: {len(seqs)} sequences and counts {counts}")
+        if tree is not None and [len(p) for p in tree] != counts:
+            raise ValueError(f"step: trees of {[len(p) for p in tree]} nodes for counts {counts}")
+        old = [self._lens[s] for s in seqs]
+        self._copy(self.own(seqs, old, [a + n for a, n in zip(old, counts)]))
+        width = max([len(self._tables[s]) for s in seqs] + [1])
+        start = [0]
+        for n in counts:
+            start.append(start[-1] + n)
+        # One upload: the table's rows, the lengths, the offsets.
+        flat = [p for s in seqs for p in self._tables[s] + [-1] * (width - len(self._tables[s]))]
+        B, nt = len(seqs), len(flat)
+        dev = self._tensor(flat + [self._lens[s] for s in seqs] + start + ([p for t in tree for p in t] if tree else []))
+        step = CacheStep(seqs, counts, dev[:nt].view(B, width), dev[nt:nt + B], dev[nt + B:nt + 2 * B + 1],
+                         max(counts + [0]))
+        if tree is not None:
+            step.tree = ops.tree_mask(dev[nt + 2 * B + 1:], q_start=step.q_start, max_q=step.max_q)
+        return step
+
+    def accept(self, step: CacheStep, paths: list[list[int]]) -> None:
+        """Keeps the accepted path of each sequence's rows of `step` (its latest),
+        strictly ascending nodes, and drops the others."""
+        if len(paths) != len(step.seqs):
+            raise ValueError(f"accept: {len(paths)} paths for {len(step.seqs)} sequences")
+        for s, n, path in zip(step.seqs, step.counts, paths):
+            if any(a >= b for a, b in zip([-1] + path, path + [n])):
+                raise ValueError(f"accept: path {path} does not ascend within [0, {n})")
+        lens = [self._lens[s] for s in step.seqs]
+        ctx = [a - n for a, n in zip(lens, step.counts)]
+        moved = [list(p) != list(range(len(p))) for p in paths]
+        if any(moved):
+            table = step.table
+            copies = self.own(step.seqs, ctx, lens, keep=True)
+            if copies:  # forked since the step
+                self._copy(copies)
+                rows = [self._tables[s] + [-1] * (table.shape[1] - len(self._tables[s])) for s in step.seqs]
+                table = self._tensor(rows)
+            width = max(len(p) for p in paths)
+            ops.cache_accept(self.k, self.v, table, step.lens,
+                             self._tensor([list(p) + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start)
+        for s, c, path in zip(step.seqs, ctx, paths):
+            self.trim(s, c + len(path))
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Moves the pages in use to the lowest ids, so that the others are one
+        stretch at the end.  Steps made before have stale tables."""
+        moves = super().compact()
+        self._copy(moves)
+        return moves
+
+    def append(self, layer: int, step: CacheStep, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None, rope_base: float | None = None) -> None:
+        """``ops.cache_append_into`` of the step's rows in a layer."""
+        ops.cache_append_into(k, v, self.k[layer], self.v[layer], step.table, step.lens, step.q_start, step.max_q,
+                              step.tree, q, q_out, rope_base)
+
+    def attention_into(self, layer: int, step: CacheStep, q: torch.Tensor, o: torch.Tensor, window: int | None = None,
+                       sinks: int = 0, scale: float | None = None) -> torch.Tensor:
+        """``ops.paged_attention_into`` of the step's rows in a layer."""
+        return ops.paged_attention_into(q, o, self.k[layer], self.v[layer], step.table, step.lens, step.q_start,
+                                        step.max_q, window, sinks, step.tree, scale)

@@ -24,6 +24,9 @@ Differences from the reference's host glue, none of which changes the math:
   * ``BlockConfig(n_kv_heads=..., rope_base=...)`` adds grouped-query
     attention and rotary embeddings, which the reference lacks (README.md:89);
     both default off, giving the reference's block;
+  * ``BlockConfig(window=..., sinks=...)`` adds a sliding window with first
+    tokens that stay visible, and ``nki_decode`` runs the block over a paged
+    cache (nkilab.cache): single tokens, chunks of prompts, drafted trees;
   * ``compute_dtype="bfloat16"`` runs the block in bf16 with an fp32 residual
     stream (the GEMMs that feed the residual emit fp32).  The default keeps
     the reference's behaviour: everything in x's dtype.
@@ -50,6 +53,7 @@ import torch.nn.functional as F
 
 from . import ops
 from ._tensors import from_device, to_device
+from .cache import CacheStep, PagedCache
 
 
 @dataclass
@@ -61,6 +65,8 @@ class BlockConfig:
     # Options the reference lacks (README.md:89); the defaults keep its block.
     n_kv_heads: int | None = None   # grouped-query attention: K/V heads (dividing n_heads)
     rope_base: float | None = None  # rotary embedding of q and k (rotate-half layout)
+    window: int | None = None       # sliding window: token i sees the keys j <= i with j > i - window or j < sinks
+    sinks: int = 0                  # first tokens that stay visible under the window
 
     @property
     def head_dim(self) -> int:
@@ -127,7 +133,12 @@ class DecoderBlock(nn.Module):
             q, k = rope_reference(q, self.cfg.rope_base), rope_reference(k, self.cfg.rope_base)
         if Hkv != H:
             k, v = (t.repeat_interleave(H // Hkv, dim=0) for t in (k, v))
-        attn = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        if self.cfg.window is None:
+            attn = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        else:
+            i = torch.arange(S, device=x.device)
+            seen = (i[None] <= i[:, None]) & ((i[None] > i[:, None] - self.cfg.window) | (i[None] < self.cfg.sinks))
+            attn = F.scaled_dot_product_attention(q, k, v, attn_mask=seen)
         x = x + self.wo(attn.transpose(0, 1).reshape(S, d))
         h = self.norm2(x)
         return x + self.wd(F.silu(self.wg(h)) * self.wu(h))
@@ -229,7 +240,8 @@ def _split_forward(block: DecoderBlock, xt: torch.Tensor, attention_variant: str
         ops.rope_into(q, q, cfg.rope_base)
         ops.rope_into(k, k, cfg.rope_base)
     a = torch.empty((S, d), dtype=f32, device=dev)
-    ops.attention_into(q, k, v, a.view(S, H, hd).transpose(0, 1), variant=attention_variant)
+    ops.attention_into(q, k, v, a.view(S, H, hd).transpose(0, 1), variant=attention_variant, window=cfg.window,
+                       sinks=cfg.sinks)
     x1 = torch.empty((S, d), dtype=f32, device=dev)
     linear(a, "wo", x1, residual=xt)
     h2 = torch.empty((S, d), dtype=f32, device=dev)
@@ -261,15 +273,69 @@ def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipeline
         if xt.dtype != torch.float32:
             raise ValueError("nki_forward: compute_dtype='split' needs an fp32 x")
         return from_device(_split_forward(block, xt, attention_variant), kind)
-    dev = xt.device
     S, d = xt.shape
-    H, hd = cfg.n_heads, cfg.head_dim
-    rdt = xt.dtype
+    H, hd, Hkv = cfg.n_heads, cfg.head_dim, cfg.kv_heads
+
+    def attend(qkv: torch.Tensor, a: torch.Tensor) -> None:
+        q, k, v = _heads(qkv, 0, H, hd), _heads(qkv, d, Hkv, hd), _heads(qkv, d + Hkv * hd, Hkv, hd)
+        if cfg.rope_base is not None:  # in place on the q and k columns of qkv
+            ops.rope_into(q, q, cfg.rope_base)
+            ops.rope_into(k, k, cfg.rope_base)
+        ops.attention_into(q, k, v, _heads(a, 0, H, hd), variant=attention_variant, window=cfg.window, sinks=cfg.sinks)
+
+    return from_device(_forward(block, xt, _compute_dtype("nki_forward", xt.dtype, compute_dtype), attend), kind)
+
+
+def nki_decode(block: DecoderBlock, x, cache: PagedCache, step: CacheStep, layer: int = 0, compute_dtype=None):
+    """The block over new tokens and a cache of the ones before them: x
+    [step.rows, d_model] holds the new rows of the step's sequences one after
+    another (single tokens, prompts, chunks of them, or drafted trees), whose K
+    (rotated) and V rows go to `layer` of the cache, and which attend over it.
+    A prompt in one step gives what nki_forward gives; compute_dtype as there
+    ("split" apart), and the cache's dtype is the compute dtype.  With a tree in
+    the step a token sees the context and its ancestors, and is at the context's
+    length and its depth.  Every layer's call takes the same step."""
+    cfg = block.cfg
+    xt, kind = to_device(x)
+    if compute_dtype == SPLIT:
+        raise ValueError("nki_decode: compute_dtype='split' is not supported")
+    cdt = _compute_dtype("nki_decode", xt.dtype, compute_dtype)
+    n, d = xt.shape
+    H, hd, Hkv = cfg.n_heads, cfg.head_dim, cfg.kv_heads
+    if n != step.rows:
+        raise ValueError(f"nki_decode: x has {n} rows, the step {step.rows}")
+    if cache.k.dtype != cdt or cache.k.shape[2] != Hkv or cache.k.shape[4] != hd:
+        raise ValueError(f"nki_decode: a cache of {cache.k.dtype} [{cache.k.shape[2]} heads, {cache.k.shape[4]}] for "
+                         f"{cdt} [{Hkv}, {hd}]")
+
+    def attend(qkv: torch.Tensor, a: torch.Tensor) -> None:
+        q, k, v = (_heads(qkv, c, h, hd).transpose(0, 1) for c, h in ((0, H), (d, Hkv), (d + Hkv * hd, Hkv)))
+        if cfg.rope_base is None:
+            cache.append(layer, step, k, v)
+        else:  # q in place on its columns of qkv
+            cache.append(layer, step, k, v, q, q, cfg.rope_base)
+        cache.attention_into(layer, step, q, a.view(n, H, hd), cfg.window, cfg.sinks)
+
+    return from_device(_forward(block, xt, cdt, attend), kind)
+
+
+def _compute_dtype(fn: str, rdt: torch.dtype, compute_dtype) -> torch.dtype:
+    """The type of the GEMM and attention operands for a residual stream of rdt."""
     cdt = rdt if compute_dtype is None else _DTYPES[compute_dtype]
     if cdt == torch.float32 and rdt == torch.bfloat16:
-        raise ValueError("nki_forward: fp32 compute on a bf16 residual stream is not supported")
+        raise ValueError(f"{fn}: fp32 compute on a bf16 residual stream is not supported")
     if cdt == torch.float16 and rdt != torch.float32:
-        raise ValueError("nki_forward: compute_dtype='float16' needs an fp32 x")
+        raise ValueError(f"{fn}: compute_dtype='float16' needs an fp32 x")
+    return cdt
+
+
+def _forward(block: DecoderBlock, xt: torch.Tensor, cdt: torch.dtype, attend) -> torch.Tensor:
+    """The block with operands of type cdt; attend(qkv, a) fills a [S, d_model]
+    with the attention of the projected rows qkv [S, d_model + 2 kv_heads hd]."""
+    cfg = block.cfg
+    dev = xt.device
+    S, d = xt.shape
+    rdt = xt.dtype
 
     def weight(n):
         return _device_param(block, n, _weight(block, n), cdt, dev)
@@ -279,16 +345,10 @@ def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipeline
 
     h = torch.empty((S, d), dtype=cdt, device=dev)
     ops.rmsnorm_into(xt, g1, h, cfg.eps)
-    Hkv = cfg.kv_heads
-    kvd = Hkv * hd
-    qkv = torch.empty((S, d + 2 * kvd), dtype=cdt, device=dev)
+    qkv = torch.empty((S, d + 2 * cfg.kv_heads * cfg.head_dim), dtype=cdt, device=dev)
     ops.linear_into(h, weight("wqkv"), qkv)
-    q, k, v = _heads(qkv, 0, H, hd), _heads(qkv, d, Hkv, hd), _heads(qkv, d + kvd, Hkv, hd)
-    if cfg.rope_base is not None:  # in place on the q and k columns of qkv
-        ops.rope_into(q, q, cfg.rope_base)
-        ops.rope_into(k, k, cfg.rope_base)
     a = torch.empty((S, d), dtype=cdt, device=dev)
-    ops.attention_into(q, k, v, _heads(a, 0, H, hd), variant=attention_variant)
+    attend(qkv, a)
     x1 = torch.empty((S, d), dtype=rdt, device=dev)
     ops.linear_into(a, weight("wo"), x1, residual=xt)
     h2 = torch.empty((S, d), dtype=cdt, device=dev)
@@ -301,4 +361,4 @@ def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipeline
         ops.gate_up_into(h2, weight("wg"), weight("wu"), act)
     out = torch.empty((S, d), dtype=rdt, device=dev)
     ops.linear_into(act, weight("wd"), out, residual=x1)
-    return from_device(out, kind)
+    return out
