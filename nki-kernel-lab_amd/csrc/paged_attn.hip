@@ -509,6 +509,9 @@ void paged_attn_kernel(PagedArgs p) {
       }
       return (int)lane_of(lt.flags);
     };
+    // Non-temporal loads where no other workgroup reads the keys (reads of 1 GiB
+    // in random blocks of 8 KB: 6.0 -> 6.8 TB/s).
+    constexpr int kPolicy = WPT == 1 ? 2 : 0;
     uint4 rk[CH], rv[CH];
     // Loads a tile and returns a bit for each of its keys that is read.
     auto gload = [&](Tile& t) __attribute__((always_inline)) -> unsigned {
@@ -526,8 +529,8 @@ void paged_attn_kernel(PagedArgs p) {
         asm volatile("" : "+s"(step_k), "+s"(step_v));
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-          rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, 0));
-          rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, 0));
+          rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, kPolicy));
+          rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, kPolicy));
         }
         t.masked = t.masked || n < BN;
         return low_bits(n);
@@ -1186,13 +1189,17 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   }
   const long key_tiles = (keys + BN - 1) / BN + 1;
   const int cus = cu_count();
-  pl.target = pl.wide && elem == 4 ? cus : 2 * cus;  // workgroups that fill the card
+  // Workgroups that fill the card.  Up to 32 rows: as many as have 64 KB of
+  // tiles on their way in each CU; with twice that the loads queue for longer
+  // than they gain (64 single tokens over 16384 rows, d = 128: 168 us with one
+  // workgroup a CU, 178 with two, 186 with four).
+  pl.target = pl.wide ? (elem == 4 ? cus : 2 * cus) : cus * (pl.dp * elem >= 256 ? 1 : 256 / (pl.dp * elem));
   pl.min_tiles = pl.wide ? 4 : 8;
   // Split where the row tiles leave workgroups idle, or may be of lengths so
   // different that the longest outlasts the rest (several sequences, or a
   // causal prompt with no window): up to four rounds of them.
   const long rounds = c.batch == 1 && window ? 1 : 4;
-  pl.split = pl.items < rounds * (pl.wide ? cus : 2 * cus) && key_tiles > 2 * pl.min_tiles;
+  pl.split = pl.items < rounds * cus * (pl.wide ? 1 : 2) && key_tiles > 2 * pl.min_tiles;
   // Four ranges and more to an item: items of their own ranges, which are then
   // no more than the workgroups with one range less to each item.
   pl.align = pl.items * 4 <= pl.target;
