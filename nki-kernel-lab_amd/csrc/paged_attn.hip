@@ -268,7 +268,9 @@ __device__ __forceinline__ unsigned not_finite(unsigned w) {
   }
 }
 
-// State of a share in the workspace: MR rows of DP floats, then MR (m, l).
+// A part's state in the workspace: for each wavefront and d-block four chunks of
+// four columns a lane (1 KB together), then (m, l) of each row.  Rows past the
+// last are left out.
 template <int DP, int MR>
 constexpr long part_floats() {
   return (long)MR * (DP + 2);
@@ -1031,16 +1033,17 @@ void paged_attn_kernel(PagedArgs p) {
       if (c0 == 0 && threadIdx.x == 0)
         p.joins[blockIdx.x] = {b, kvh, r0, (u - skip + p.setup + sp.nt - 1) / len - (int)blockIdx.x + 1};
       float* part = p.part + (2L * blockIdx.x + (c0 > 0 ? 0 : 1)) * part_floats<DP, MR>();
-      const int r = 32 * wq + l32;
+      if (row_ok) {
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
-        if (NT == 1 || db % NT == team)
+        for (int db = 0; db < NDB; ++db)
+          if (NT == 1 || db % NT == team)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4*>(part + r * DP + 32 * db + 8 * k + 4 * h32) =
-                make_float4(oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]);
-      if (team == 0 && h32 == 0)
-        *reinterpret_cast<float2*>(part + MR * DP + 2 * r) = make_float2(m_run, l_tot);
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<float4*>(part + ((wq * NDB + db) * 4 + k) * 256 + lane * 4) =
+                  make_float4(oacc[db][4 * k], oacc[db][4 * k + 1], oacc[db][4 * k + 2], oacc[db][4 * k + 3]);
+        if (team == 0 && h32 == 0)
+          *reinterpret_cast<float2*>(part + MR * DP + 2 * (32 * wq + l32)) = make_float2(m_run, l_tot);
+      }
     }
 
     if constexpr (!SPLIT) break;
@@ -1064,21 +1067,19 @@ void paged_attn_kernel(PagedArgs p) {
 }
 
 // Joins the parts of the row tile that begins in range blockIdx.x and ends in
-// another; DP / 4 lanes to a row, four columns each.  Row tiles of 32 rows (few
-// new tokens, up to hundreds of parts): a workgroup's four wavefronts take every
-// fourth part of the same rows and meet in LDS.  Row tiles of 128 rows (a few
-// parts each): every wavefront has its own rows, four times over.
-constexpr int kJoinPasses = 4;
+// another, a chunk of 32 rows and 8 columns at a time, laid out over a wavefront
+// as the parts are.  Row tiles of 32 rows (few new tokens, up to hundreds of
+// parts): a workgroup's four wavefronts take every fourth part of one chunk and
+// meet in LDS.  Row tiles of 128 rows (a few parts each): a chunk a wavefront.
 template <int DP, int MR>
-constexpr int join_rows() {
-  return 64 / (DP / 4) * (MR == 32 ? 1 : 4 * kJoinPasses);
+constexpr int join_chunks() {
+  return MR / 32 * (DP / 8);
 }
 
 template <typename T, int DP, int MR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   constexpr bool SHARE = MR == 32;
-  constexpr int LPR = DP / 4, RPW = 64 / LPR;  // lanes a row, rows a wavefront
-  constexpr int A = 8;                         // parts in flight
+  constexpr int A = 8;  // parts in flight
   __shared__ float4 xo[SHARE ? 4 : 1][64];
   __shared__ float2 xm[SHARE ? 4 : 1][64];
   const CacheArgs& c = p.c;
@@ -1086,20 +1087,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   const int n = jn.parts;
   if (n == 0) return;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int col = 4 * (lane % LPR);
+  const int chunk = SHARE ? blockIdx.y : blockIdx.y * 4 + wid;  // (wavefront, d-block, k)
   const Seq s = seq_of(c, jn.b);
   const int nrows = s.use * p.group - jn.r0;
-  // Part i is slot 0 of range blockIdx.x + i, the first slot 1.
-  auto part_of = [&](int i) __attribute__((always_inline)) {
-    return p.part + (2L * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0)) * part_floats<DP, MR>();
-  };
-#pragma unroll 1
-  for (int pass = 0; pass < (SHARE ? 1 : kJoinPasses); ++pass) {
-    const int r = (int)blockIdx.y * join_rows<DP, MR>() + (SHARE ? 0 : (pass * 4 + wid) * RPW) + lane / LPR;
-    const bool ok = r < nrows;  // (rows past the last are not in the parts either: their loads repeat row 0)
-    const int rl = ok ? r : 0;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int r = 32 * (chunk / (DP / 8)) + (lane & 31), col = 8 * (chunk % (DP / 8)) + 4 * (lane >> 5);
+  const bool ok = r < nrows && col < c.d;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ok) {
+    // Part i is slot 0 of range blockIdx.x + i, the first slot 1.
+    auto part_of = [&](int i) __attribute__((always_inline)) {
+      return p.part + (2L * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0)) * part_floats<DP, MR>();
+    };
     const int i_first = SHARE ? wid : 0, i_step = SHARE ? 4 : 1;
     for (int i0 = i_first; i0 < n; i0 += A * i_step) {
       float2 ml[A];
@@ -1108,14 +1107,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
       for (int k = 0; k < A; ++k) {  // (past the last part: the first again)
         const int i = i0 + k * i_step;
         const float* pt = part_of(i < n ? i : i_first);
-        ml[k] = *reinterpret_cast<const float2*>(pt + MR * DP + 2 * rl);
-        x[k] = *reinterpret_cast<const float4*>(pt + (long)rl * DP + col);
+        ml[k] = *reinterpret_cast<const float2*>(pt + MR * DP + 2 * r);
+        x[k] = *reinterpret_cast<const float4*>(pt + chunk * 256 + lane * 4);
       }
       float mn = m;
 #pragma unroll
-      for (int k = 0; k < A; ++k) {
+      for (int k = 0; k < A; ++k)
         if (i0 + k * i_step < n) mn = fmaxf(mn, ml[k].x);
-      }
       const float w0 = m == -INFINITY ? 0.f : fast_exp2(m - mn);
       m = mn;
       l *= w0;
@@ -1130,30 +1128,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
         acc.z = fmaf(x[k].z, w, acc.z); acc.w = fmaf(x[k].w, w, acc.w);
       }
     }
-    if constexpr (SHARE) {
-      xm[wid][lane] = make_float2(m, l);
-      xo[wid][lane] = acc;
-      __syncthreads();
-      if (wid > 0) return;
-      m = fmaxf(fmaxf(xm[0][lane].x, xm[1][lane].x), fmaxf(xm[2][lane].x, xm[3][lane].x));
-      l = 0.f;
-      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  if constexpr (SHARE) {
+    xm[wid][lane] = make_float2(m, l);
+    xo[wid][lane] = acc;
+    __syncthreads();
+    if (wid > 0) return;
+    m = fmaxf(fmaxf(xm[0][lane].x, xm[1][lane].x), fmaxf(xm[2][lane].x, xm[3][lane].x));
+    l = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float2 y = xm[w][lane];
-        const float f = y.x == -INFINITY ? 0.f : fast_exp2(y.x - m);
-        const float4 o = xo[w][lane];
-        l = fmaf(y.y, f, l);
-        acc.x = fmaf(o.x, f, acc.x); acc.y = fmaf(o.y, f, acc.y);
-        acc.z = fmaf(o.z, f, acc.z); acc.w = fmaf(o.w, f, acc.w);
-      }
+    for (int w = 0; w < 4; ++w) {
+      const float2 y = xm[w][lane];
+      const float f = y.x == -INFINITY ? 0.f : fast_exp2(y.x - m);
+      const float4 o = xo[w][lane];
+      l = fmaf(y.y, f, l);
+      acc.x = fmaf(o.x, f, acc.x); acc.y = fmaf(o.y, f, acc.y);
+      acc.z = fmaf(o.z, f, acc.z); acc.w = fmaf(o.w, f, acc.w);
     }
-    if (ok && col < c.d) {
-      const float linv = l == 0.f ? 0.f : 1.f / l;
-      const int row = jn.r0 + r, ri = (int)div32(p.dv_group, (unsigned)row), head = jn.kvh * p.group + row - ri * p.group;
-      const float y[4] = {acc.x * linv, acc.y * linv, acc.z * linv, acc.w * linv};
-      store_vec<4>(reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h + col, y);
-    }
+  }
+  if (ok) {
+    const float linv = l == 0.f ? 0.f : 1.f / l;
+    const int row = jn.r0 + r, ri = (int)div32(p.dv_group, (unsigned)row), head = jn.kvh * p.group + row - ri * p.group;
+    const float y[4] = {acc.x * linv, acc.y * linv, acc.z * linv, acc.w * linv};
+    store_vec<4>(reinterpret_cast<T*>(p.o) + (long)(s.t0 + ri) * p.o_t + (long)head * p.o_h + col, y);
   }
 }
 
@@ -1203,7 +1201,7 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   // Four ranges and more to an item: items of their own ranges, which are then
   // no more than the workgroups with one range less to each item.
   pl.align = pl.items * 4 <= pl.target;
-  pl.setup = pl.align ? 0 : 8;
+  pl.setup = pl.align ? 0 : elem == 4 ? 3 : 12;  // (an fp32 tile takes three times as long)
   pl.grid = pl.target;
   if (pl.align) {
     pl.target -= (int)pl.items;
@@ -1235,9 +1233,7 @@ int paged_launch(PagedArgs& p, const Plan& pl, hipStream_t st) {
   if (pl.split && !DIRECT) {
     if (kOnePage && pl.one_page) run(kOnePage, kSplit);
     else run(kNo, kSplit);
-    const long rows = (long)p.c.max_new * p.group;
-    constexpr int J = join_rows<DP, 32 * WPT>();
-    const dim3 jgrid((unsigned)pl.grid, (unsigned)(((rows < 32 * WPT ? rows : 32 * WPT) + J - 1) / J));
+    const dim3 jgrid((unsigned)pl.grid, (unsigned)(join_chunks<DP, 32 * WPT>() / (WPT == 1 ? 1 : 4)));
     paged_join_kernel<T, DP, 32 * WPT><<<jgrid, dim3(256), 0, st>>>(p);
   } else {
     if (kOnePage && pl.one_page) run(kOnePage, kNo);
