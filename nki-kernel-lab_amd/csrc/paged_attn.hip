@@ -48,7 +48,8 @@ using fsched::Div32;
 using fsched::div32;
 using fsched::kRescaleSlack;
 
-constexpr int BN = 32;  // keys per tile
+constexpr int BN = 32;            // keys per tile
+constexpr int kMasked = 1 << 16;  // flag of a looked-up tile: it needs a mask
 
 // A row tile whose keys are split: it begins in a range, and has `parts` parts.
 struct Join {
@@ -65,7 +66,8 @@ struct PagedArgs {
   int H, group, window, sinks;  // window 0: none
   float scale_log2e;
   Div32 dv_group;
-  unsigned k_page32, k_row32, v_page32, v_row32;  // byte strides, where a tile lies in one page
+  unsigned k_page32, k_row32, v_page32, v_row32;  // byte strides, where half tiles lie in one page
+  int same_rows;                                  // K's and V's page and row strides are the same
   // Split over keys (part != nullptr): workgroups, and the fewest key tiles of
   // a range.  joins: one for each range.
   float* part;
@@ -200,7 +202,7 @@ struct El<float> {
 };
 
 // Tiles that the buffer unit copies to LDS (one team of four wavefronts, 16-bit
-// types, a tile in one page): rows of DP elements without gaps, a row's 16-byte chunks swizzled --
+// types, half tiles in one page): rows of DP elements without gaps, a row's 16-byte chunks swizzled --
 // logical chunk c of row r sits at chunk c ^ swz(r) -- so that sixteen rows'
 // chunk c (a K fragment's read) and four rows' four chunks of a d-block (a V
 // fragment's) lie in banks of their own.
@@ -255,6 +257,15 @@ struct Lay {
   static_assert(BYTES <= 160 * 1024, "LDS");
 };
 
+// 16 bytes at p where ok, else zeros (p is valid either way); NT: non-temporal.
+template <bool NT, typename T>
+__device__ __forceinline__ uint4 ld16_policy(const T* p, bool ok) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4* q = reinterpret_cast<const u32x4*>(p);
+  const u32x4 v = NT ? __builtin_nontemporal_load(q) : *q;
+  return ok ? make_uint4(v.x, v.y, v.z, v.w) : make_uint4(0, 0, 0, 0);
+}
+
 // All ones in the elements of w (one of 32 bits or two of 16) that are
 // infinite or NaN: an exponent of ones carries into the sign's place.
 template <typename T>
@@ -277,7 +288,7 @@ constexpr long part_floats() {
 }
 
 template <typename T, int DP, int WPT, int NT, bool TP, bool SPLIT>
-__global__ __launch_bounds__(64 * WPT * NT) __attribute__((amdgpu_waves_per_eu(El<T>::W32 && WPT == 1 && DP == 128 ? 1 : 2)))
+__global__ __launch_bounds__(64 * WPT * NT) __attribute__((amdgpu_waves_per_eu(WPT == 1 && DP == 128 && (El<T>::W32 || SPLIT) ? 1 : 2)))
 void paged_attn_kernel(PagedArgs p) {
   using L = Lay<T, DP, WPT, NT, TP>;
   constexpr bool W32 = L::W32, H16 = El<T>::H;
@@ -332,13 +343,13 @@ void paged_attn_kernel(PagedArgs p) {
     const int team = wid / WPT, wq = wid % WPT, ttid = tid % TT;
     const int h32 = lane >> 5, l32 = lane & 31;
     T* const stage0 = reinterpret_cast<T*>(smem) + (L::COPY ? 0 : team * L::TEAM);
-    // This thread's chunks of a tile in one page: byte offsets from the tile's
-    // first row, columns past d out of range.
+    // This thread's first chunk of a tile whose halves lie in one page each: byte
+    // offsets from the half's first row, columns past d out of range.
     int voff_k, voff_v;
     {
       const int ci = min(ttid, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
-      voff_k = col < c.d ? r * (int)p.k_row32 + col * (int)sizeof(T) : 0x40000000;
-      voff_v = col < c.d ? r * (int)p.v_row32 + col * (int)sizeof(T) : 0x40000000;
+      voff_k = col < c.d ? r % (BN / 2) * (int)p.k_row32 + col * (int)sizeof(T) : 0x40000000;
+      voff_v = col < c.d ? r % (BN / 2) * (int)p.v_row32 + col * (int)sizeof(T) : 0x40000000;
     }
 
     // ---- the segment: key tiles c0 .. c1 - 1 of row tile r0, K/V head kvh
@@ -422,75 +433,88 @@ void paged_attn_kernel(PagedArgs p) {
     const int nit = (c1 - c0 - team + NT - 1) / NT;  // this team's tiles
     const int nsteps = (c1 - c0 + NT - 1) / NT;      // the workgroup's steps
     // A tile on its way through the steps: its first key, whether it needs a
-    // mask, and where its rows are.  In one page (TP): the page, the same for
-    // every lane, and the tile's first row in it; keys behind the last visible
-    // one are out of range of the loads.  Otherwise: key l32's page and row,
-    // where a row of this workgroup may see it.  The page is as the table has
+    // mask, and where its rows are.  Halves in one page (TP): each half's page,
+    // the same for every lane, and its first row in it; keys behind the last
+    // visible one are out of range of the loads.  Otherwise: key l32's page and
+    // row, where a row of this workgroup may see it.  A page is as the table has
     // it: it is looked at where the tile is loaded, a step after it is read.
     struct Tile {
-      int k0, pid, within;
+      int k0, pid[2], within[2];
       bool masked;
+    };
+    // Whether keys j .. j + 15 hold one that a row of this workgroup may see.
+    auto half_seen = [&](int j) __attribute__((always_inline)) {
+      return j < sp.hi && (j + BN / 2 > sp.lo || j < p.sinks);
     };
     auto look_up = [&](int it) __attribute__((always_inline)) {
       const int x = c0 + team + NT * it;
       Tile t;
       t.k0 = BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
       t.masked = (unsigned)(x - f0) >= fn || it >= nit;
-      t.pid = -1;
-      t.within = 0;
-      if constexpr (TP) {
-        if (it < nit) {
-          const int pi = (int)div32(c.dv_page, (unsigned)t.k0);
-          t.within = t.k0 - pi * c.page_size;
-          t.pid = c.table ? ((const __attribute__((address_space(4))) int*)trow)[pi] : 0;
-        }
-      } else {
-        const int j = t.k0 + l32;
-        if (it < nit && j < sp.hi && (j >= sp.lo || j < p.sinks)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        t.pid[h] = -1;
+        t.within[h] = 0;
+        const int j = t.k0 + (TP ? BN / 2 * h : l32);
+        if (TP ? it < nit && half_seen(j) : h == 0 && it < nit && j < sp.hi && (j >= sp.lo || j < p.sinks)) {
           const int pi = (int)div32(c.dv_page, (unsigned)j);
-          t.within = j - pi * c.page_size;
-          t.pid = c.table ? trow[pi] : 0;
+          t.within[h] = j - pi * c.page_size;
+          if constexpr (TP)
+            t.pid[h] = c.table ? ((const __attribute__((address_space(4))) int*)trow)[pi] : 0;
+          else
+            t.pid[h] = c.table ? trow[pi] : 0;
         }
       }
       return t;
     };
-    // Wavefronts that share their tiles (TP): 64 tiles are looked up at a time,
-    // one a lane -- where their K and V are, the bytes a load may read, and
-    // (flags) the keys that are there with bit 8 set where a mask is needed --
-    // and a step reads its tile's lane: done by a step for itself, on the
-    // scalar unit, this took more instructions than the softmax.  The pages of
-    // the next 64 are on their way meanwhile.
+    // Wavefronts that share copied tiles: 64 tiles are looked up at a time, one a
+    // lane -- where this wavefront's half of the tile's K or V is and the bytes
+    // that may be read there, and (flags) the keys that are there of each half,
+    // with bit 16 where a mask is needed -- and a step reads its tile's lane:
+    // done by a step for itself, on the scalar unit, this took more
+    // instructions than the softmax.  The pages of the next 64 are on their way
+    // meanwhile.
     struct Lanes {
       unsigned lo, hi;
       int bytes, flags;
     } lt = {};
-    int pid_next = 0;
+    int pid_next[2] = {-1, -1};
     auto tile_first = [&](int it) __attribute__((always_inline)) {
       const int x = c0 + it;
       return BN * (x < sp.ns ? x : x - sp.ns + sp.m0);
     };
     auto load_pids = [&](int base) __attribute__((always_inline)) {
       const int it = base + lane;
-      pid_next = !c.table || it >= nit ? 0 : trow[div32(c.dv_page, (unsigned)tile_first(it))];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = tile_first(it) + BN / 2 * h;
+        pid_next[h] = -1;
+        if (it < nit && half_seen(j)) pid_next[h] = c.table ? trow[div32(c.dv_page, (unsigned)j)] : 0;
+      }
     };
     const bool copies_v = wq >= 2;
+    const int my_half = wq & 1;
     auto fill_lanes = [&](int base) __attribute__((always_inline)) {
-      const int it = base + lane, x = c0 + it, k0 = tile_first(it), pid = pid_next;
-      const int n = it < nit && (unsigned)pid < (unsigned)c.pages ? min(BN, sp.hi - k0) : 0;
-      const unsigned pg = n > 0 ? pid : 0;
-      const unsigned within = n > 0 ? k0 - (int)div32(c.dv_page, (unsigned)k0) * c.page_size : 0;
+      const int it = base + lane, x = c0 + it, k0 = tile_first(it);
+      int n[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        n[h] = (unsigned)pid_next[h] < (unsigned)c.pages ? min(BN / 2, sp.hi - k0 - BN / 2 * h) : 0;
+      const int mine = my_half ? n[1] : n[0], j = k0 + BN / 2 * my_half;
+      const unsigned pg = mine > 0 ? (my_half ? pid_next[1] : pid_next[0]) : 0;
+      const unsigned within = mine > 0 ? j - (int)div32(c.dv_page, (unsigned)j) * c.page_size : 0;
+      const unsigned row_b = copies_v ? p.v_row32 : p.k_row32;
       const unsigned long at = (unsigned long)(copies_v ? Vb : Kb) +
-                               (unsigned long)pg * (copies_v ? p.v_page32 : p.k_page32) +
-                               (unsigned long)within * (copies_v ? p.v_row32 : p.k_row32);
+                               (unsigned long)pg * (copies_v ? p.v_page32 : p.k_page32) + (unsigned long)within * row_b;
       lt.lo = (unsigned)at;
       lt.hi = (unsigned)(at >> 32);
-      lt.bytes = n > 0 ? (n - 1) * (int)(copies_v ? p.v_row32 : p.k_row32) + row_bytes : 0;
-      lt.flags = n | ((unsigned)(x - f0) >= fn || n < BN ? 256 : 0);
+      lt.bytes = mine > 0 ? (mine - 1) * (int)row_b + row_bytes : 0;
+      lt.flags = n[0] | (n[1] << 8) | ((unsigned)(x - f0) >= fn || n[0] + n[1] < BN ? kMasked : 0);
       load_pids(base + 64);
     };
-    // Copies this wavefront's part of tile `it` to LDS (lane l's 16 bytes at the
-    // copy's place + 16 l; past the last tile nothing is read, and zeros are
-    // written); returns the tile's flags.
+    // Copies this wavefront's half of tile `it`'s K or V to LDS (lane l's 16 bytes
+    // at the copy's place + 16 l; past the last tile nothing is read, and zeros
+    // are written); returns the tile's flags.
     unsigned lds0 = 0;
     int coff[L::NCP > 0 ? L::NCP : 1];
     auto copy_tile = [&](int it) __attribute__((always_inline)) {
@@ -517,42 +541,51 @@ void paged_attn_kernel(PagedArgs p) {
     uint4 rk[CH], rv[CH];
     // Loads a tile and returns a bit for each of its keys that is read.
     auto gload = [&](Tile& t) __attribute__((always_inline)) -> unsigned {
+      unsigned bits = 0;
       if constexpr (TP) {
-        const int n = (unsigned)t.pid < (unsigned)c.pages ? min(BN, sp.hi - t.k0) : 0;
-        const unsigned pid = n > 0 ? t.pid : 0, within = n > 0 ? t.within : 0;
-        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(Kb + (unsigned long)pid * p.k_page32 + (unsigned long)within * p.k_row32), (short)0,
-            n > 0 ? (n - 1) * (int)p.k_row32 + row_bytes : 0, fsched::kBufferFlags);
-        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(Vb + (unsigned long)pid * p.v_page32 + (unsigned long)within * p.v_row32), (short)0,
-            n > 0 ? (n - 1) * (int)p.v_row32 + row_bytes : 0, fsched::kBufferFlags);
         // (left opaque, so that no register holds an offset for each of the loads)
-        int step_k = (TT / CPR) * (int)p.k_row32, step_v = (TT / CPR) * (int)p.v_row32;
-        asm volatile("" : "+s"(step_k), "+s"(step_v));
+        int row_k = (int)p.k_row32, row_v = (int)p.v_row32;
+        asm volatile("" : "+s"(row_k), "+s"(row_v));
+        __amdgpu_buffer_rsrc_t ks[2], vs[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int n = (unsigned)t.pid[h] < (unsigned)c.pages ? min(BN / 2, sp.hi - t.k0 - BN / 2 * h) : 0;
+          const unsigned pid = n > 0 ? t.pid[h] : 0, within = n > 0 ? t.within[h] : 0;
+          ks[h] = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(Kb + (unsigned long)pid * p.k_page32 + (unsigned long)within * p.k_row32), (short)0,
+              n > 0 ? (n - 1) * row_k + row_bytes : 0, fsched::kBufferFlags);
+          vs[h] = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(Vb + (unsigned long)pid * p.v_page32 + (unsigned long)within * p.v_row32), (short)0,
+              n > 0 ? (n - 1) * row_v + row_bytes : 0, fsched::kBufferFlags);
+          bits |= low_bits(n) << (BN / 2 * h);
+        }
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-          rk[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ks, voff_k + i * step_k, 0, kPolicy));
-          rv[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vs, voff_v + i * step_v, 0, kPolicy));
+          // (a wavefront's 64 chunks are 4, 8 or 16 rows of one half)
+          const int h = min(wq * 64 + TT * i, BN * CPR - 1) / CPR >= BN / 2;
+          const int r = (TT / CPR) * i % (BN / 2);
+          rk[i] = __builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(h ? ks[1] : ks[0], voff_k + r * row_k, 0, kPolicy));
+          rv[i] = __builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(h ? vs[1] : vs[0], voff_v + r * row_v, 0, kPolicy));
         }
-        t.masked = t.masked || n < BN;
-        return low_bits(n);
       } else {
-        const bool in = (unsigned)t.pid < (unsigned)c.pages;
-        const unsigned bits = (unsigned)__builtin_amdgcn_ballot_w64(in);
-        const int pid = in ? t.pid : -1;
+        // A key's place is made by its lane and handed to those that load it.
+        const bool in = (unsigned)t.pid[0] < (unsigned)c.pages;
+        bits = (unsigned)__builtin_amdgcn_ballot_w64(in);
+        const long ko = in ? (long)t.pid[0] * c.k_page + (long)t.within[0] * c.k_row : -1;
+        const long vo = in ? (long)t.pid[0] * c.v_page + (long)t.within[0] * c.v_row : -1;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           const int ci = min(ttid + TT * i, BN * CPR - 1), r = ci / CPR, col = (ci % CPR) * E;
-          const int pg = __shfl(pid, r, kWave), wi = __shfl(t.within, r, kWave);
-          const bool ok = pg >= 0 && col < c.d;
-          const T* kp = reinterpret_cast<const T*>(Kb) + (long)pg * c.k_page + (long)wi * c.k_row + col;
-          const T* vp = reinterpret_cast<const T*>(Vb) + (long)pg * c.v_page + (long)wi * c.v_row + col;
-          rk[i] = ld16_or_zero(ok ? kp : reinterpret_cast<const T*>(Kb), 0, ok);
-          rv[i] = ld16_or_zero(ok ? vp : reinterpret_cast<const T*>(Vb), 0, ok);
+          const long kr = __shfl(ko, r, kWave), vr = p.same_rows ? kr : __shfl(vo, r, kWave);
+          const bool ok = kr >= 0 && col < c.d;
+          rk[i] = ld16_policy<WPT == 1>(reinterpret_cast<const T*>(Kb) + (ok ? kr + col : 0), ok);
+          rv[i] = ld16_policy<WPT == 1>(reinterpret_cast<const T*>(Vb) + (ok ? vr + col : 0), ok);
         }
-        t.masked = t.masked || bits != ~0u;
-        return bits;
       }
+      t.masked = t.masked || bits != ~0u;
+      return bits;
     };
     // Stages the loaded tile.  Where the tile is masked its infinities and NaN
     // of V are left out (0 * inf would reach the rows that do not see them) and
@@ -615,13 +648,13 @@ void paged_attn_kernel(PagedArgs p) {
       }
     };
     // Masks the scores of keys k0 .., raises the running max and turns S into P.
-    // (With LANES: tile k0's number instead of its first key, and the keys that
-    // are there instead of a bit for each.)
+    // (With LANES: tile k0's number instead of its first key, and its flags
+    // instead of a bit for each key.)
     auto softmax = [&](floatx16& sc, int k0, bool masked, unsigned kvalid) __attribute__((always_inline)) {
       if (masked) {
         if constexpr (LANES) {
           k0 = tile_first(k0);
-          kvalid = low_bits(kvalid);
+          kvalid = low_bits(kvalid & 255) | (low_bits(kvalid >> 8 & 255) << (BN / 2));
         }
         const unsigned seen = (row_bits(k0) & kvalid) >> (4 * h32);
 #pragma unroll
@@ -736,7 +769,7 @@ void paged_attn_kernel(PagedArgs p) {
         const int row_b = (int)(copies_v ? p.v_row32 : p.k_row32);
 #pragma unroll
         for (int i = 0; i < L::NCP; ++i) {
-          const int r = ((wq & 1) * L::NCP + i) * (64 / CPR) + lane / CPR, ch = (lane % CPR) ^ swz<DP>(r);
+          const int r = i * (64 / CPR) + lane / CPR, ch = (lane % CPR) ^ swz<DP>(r);
           coff[i] = ch * E < c.d ? r * row_b + 16 * ch : 0x40000000;
         }
       }
@@ -771,7 +804,7 @@ void paged_attn_kernel(PagedArgs p) {
 #pragma unroll 1
       for (int it = 0; it < nsteps; ++it) {
         const unsigned st = lds0 + (it % L::CSTAGES) * 2 * L::TILEB;
-        const bool masked = fl_cur >= 256;
+        const bool masked = fl_cur >= kMasked;
         floatx16 sc;
         qk(nullptr, sc);
         if (masked) {
@@ -805,7 +838,7 @@ void paged_attn_kernel(PagedArgs p) {
         __builtin_amdgcn_sched_barrier(0);
         const int fl = copy_tile(it + 3);
         __builtin_amdgcn_sched_barrier(0);
-        softmax(sc, it, masked, fl_cur & 255);
+        softmax(sc, it, masked, fl_cur);
         bf16x8 pf[2];
         to_p(sc, pf);
         bf16x8 vf[NDB][2];
@@ -918,7 +951,7 @@ void paged_attn_kernel(PagedArgs p) {
         // (the loop's own rule of what it takes as masked: a tile with a key
         // that is not read has its others here)
         bool masked = (unsigned)(x - f0) >= fn || last < BN;
-        for (int kk = 0; kk < last && !TP && !masked; ++kk) {
+        for (int kk = 0; kk < last && !masked; ++kk) {
           int within;
           masked = page_of(c, b, k0 + kk, within) < 0;
         }
@@ -1163,7 +1196,7 @@ struct Plan {
   bool split;
   int tiles_max; // row tiles of the longest sequence
   long items;    // row tiles at most
-  bool one_page; // a key tile lies in one page
+  bool one_page; // each half of a key tile lies in one page
   int target, min_tiles, setup, align;
   long grid;
   size_t bytes;  // workspace
@@ -1209,7 +1242,7 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   }
   if (pl.split && pl.items * (key_tiles + pl.setup + pl.grid) >= 1L << 30) pl.split = false;
   // (32-bit byte offsets within a tile, and byte strides)
-  pl.one_page = (!c.table || c.page_size % BN == 0) && c.k_row <= (1L << 21) && c.v_row <= (1L << 21) &&
+  pl.one_page = (!c.table || c.page_size % (BN / 2) == 0) && c.k_row <= (1L << 21) && c.v_row <= (1L << 21) &&
                 c.k_page < (1L << 30) && c.v_page < (1L << 30);
   if (pl.split) {
     pl.bytes = (size_t)pl.grid * (sizeof(Join) + 2 * (size_t)mr * (pl.dp + 2) * 4);
@@ -1332,6 +1365,7 @@ extern "C" int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, 
   const unsigned el = (unsigned)elem_bytes(cache->dtype);
   p.k_page32 = (unsigned)c.k_page * el; p.k_row32 = (unsigned)c.k_row * el;
   p.v_page32 = (unsigned)c.v_page * el; p.v_row32 = (unsigned)c.v_row * el;
+  p.same_rows = c.k_page == c.v_page && c.k_row == c.v_row;
   if (pl.split) {
     p.joins = static_cast<Join*>(workspace);
     p.part = reinterpret_cast<float*>(p.joins + pl.grid);
