@@ -69,10 +69,27 @@ struct AppendArgs {
   const unsigned long long* tree;
   int tree_words, H, rope;
   double log2_base;
-  int groups;  // workgroups per sequence
+  int groups;  // workgroups per sequence; 0: one per packed row
 };
 
-// Workgroup (b, g): new rows TPB g .. of sequence b.  First the rows' angles,
+// The sequence that packed row t is of, by a 64-way search over the offsets
+// (batch: none): every lane looks at one offset a round.
+__device__ __forceinline__ int seq_of_row(const CacheArgs& c, int t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = c.batch;  // it is one of lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const bool at_or_before = lane * step < n && c.q_start[lo + lane * step] <= t;
+    const unsigned long long m = __builtin_amdgcn_ballot_w64(at_or_before);
+    if (!m) return c.batch;
+    const int l = 63 - __builtin_clzll(m);
+    lo += l * step;
+    n = min(step, n - l * step);
+  }
+  return lo;
+}
+
+// Workgroup (b, g): new rows TPB g .. of sequence b (or one packed row).  First the rows' angles,
 // a thread to each: position times frequency in 64 bits and reduced there (a
 // 32-bit product is off by position * 2^-24 radians, a quarter of a turn at
 // position 2^24), sine and cosine of the remainder in 32, once for every head.
@@ -80,9 +97,18 @@ struct AppendArgs {
 template <typename T, int E, int TPB>
 __global__ __launch_bounds__(256) void append_kernel(CacheArgs c, AppendArgs p) {
   extern __shared__ float cs[];  // [TPB][half] (cos, sin)
-  const int b = blockIdx.x / p.groups, i0 = (int)(blockIdx.x % p.groups) * TPB;
+  int b, i0;
+  if (p.groups) {
+    b = blockIdx.x / p.groups;
+    i0 = (int)(blockIdx.x % p.groups) * TPB;
+  } else {
+    b = seq_of_row(c, blockIdx.x);
+    if (b >= c.batch) return;
+    i0 = (int)blockIdx.x - c.q_start[b];
+    if (i0 < 0) return;
+  }
   const Seq s = seq_of(c, b);
-  const int cnt = min(TPB, s.use - i0);
+  const int cnt = min(p.groups ? TPB : 1, s.use - i0);
   if (cnt <= 0) return;
   const int half = c.d / 2, tid = threadIdx.x;
   if (p.rope) {
@@ -182,10 +208,14 @@ template <typename T, int E>
 int append_launch(const CacheArgs& c, AppendArgs p, hipStream_t st) {
   // Four rows a workgroup where that still fills the card (its 256 threads
   // then hold the angles of a 128-wide head's rows, one each), else one.
-  const bool four = (long)c.batch * c.max_new >= 8L * cu_count();
+  // Where the sequences' rows differ so much that most of these would be past
+  // their sequence's last (one prompt among single tokens): a workgroup a row.
+  const long places = (long)c.batch * c.max_new;
+  const bool sparse = c.q_start && places > 4L * c.rows + 4L * cu_count();
+  const bool four = !sparse && places >= 8L * cu_count();
   const int tpb = four ? 4 : 1;
-  p.groups = (c.max_new + tpb - 1) / tpb;
-  const long grid = (long)c.batch * p.groups;
+  p.groups = sparse ? 0 : (c.max_new + tpb - 1) / tpb;
+  const long grid = sparse ? c.rows : (long)c.batch * p.groups;
   if (grid * 256 > kMaxGridThreads) return set_error(NKL_EINVAL, "nkl_cache_append: %ld workgroups", grid);
   const size_t lds = p.rope ? (size_t)tpb * c.d * sizeof(float) : 0;
   if (four)

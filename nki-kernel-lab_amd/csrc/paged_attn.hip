@@ -1209,7 +1209,14 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   pl.dp = c.d <= 32 ? 32 : c.d <= 64 ? 64 : 128;
   const int mr = pl.wide ? 128 : 32;
   const long tiles = (rows + mr - 1) / mr;
-  pl.items = tiles * c.kv_heads * c.batch;
+  // Row tiles: at most the longest sequence's for each, and at most the rows
+  // hold with a part tile for each sequence.  Far fewer than the first (one
+  // prompt among single tokens) and a workgroup for each place in the longest
+  // sequence's stead would mostly find nothing to do: the ranges below are cut
+  // over the tiles that there are.
+  const long places = tiles * c.batch, held = (long)c.rows * group / mr + c.batch;
+  const bool sparse = c.q_start && places > 2 * held;
+  pl.items = (places < held ? places : held) * c.kv_heads;
   if (tiles > (1L << 24) || pl.items > (1L << 30)) return set_error(NKL_EINVAL, "%s: %ld tiles of rows", fn, pl.items);
   pl.tiles_max = (int)tiles;
   // Key tiles of a tile of rows, at most.
@@ -1230,7 +1237,7 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   // different that the longest outlasts the rest (several sequences, or a
   // causal prompt with no window): up to four rounds of them.
   const long rounds = c.batch == 1 && window ? 1 : 4;
-  pl.split = pl.items < rounds * cus * (pl.wide ? 1 : 2) && key_tiles > 2 * pl.min_tiles;
+  pl.split = sparse || (pl.items < rounds * cus * (pl.wide ? 1 : 2) && key_tiles > 2 * pl.min_tiles);
   // Four ranges and more to an item: items of their own ranges, which are then
   // no more than the workgroups with one range less to each item.
   pl.align = pl.items * 4 <= pl.target;
@@ -1247,7 +1254,7 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   if (pl.split) {
     pl.bytes = (size_t)pl.grid * (sizeof(Join) + 2 * (size_t)mr * (pl.dp + 2) * 4);
   } else {
-    pl.grid = (pl.items + 7) / 8 * 8;
+    pl.grid = (places * c.kv_heads + 7) / 8 * 8;
     pl.bytes = 0;
   }
   return NKL_OK;
@@ -1351,6 +1358,10 @@ extern "C" int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, 
     return set_error(NKL_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, pl.bytes,
                      workspace ? workspace_bytes : (size_t)0);
   if (pl.bytes && (size_t)workspace % 16) return set_error(NKL_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  if (c.pages == 0) {  // (loads that nothing guards read the first row of a cache: of no pages, Q's)
+    p.c.k = p.c.v = const_cast<unsigned char*>(static_cast<const unsigned char*>(q));
+    p.c.k_page = p.c.k_head = p.c.k_row = p.c.v_page = p.c.v_head = p.c.v_row = 0;
+  }
   p.q = static_cast<const unsigned char*>(q);
   p.o = static_cast<unsigned char*>(o);
   p.q_t = q_row; p.q_h = q_head; p.o_t = o_row; p.o_h = o_head;

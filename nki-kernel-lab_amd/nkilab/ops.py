@@ -517,6 +517,7 @@ def _window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torc
     if spec.path != "flash":
         raise ValueError(f"attention: variant {spec.name!r} has no window; one of the flash variants expected")
     w, sinks = _window_sinks("attention", window, sinks)
+    _on_current_device("attention", q, k, v, o)
     if S == 0 or H == 0:
         return o
     if d == 0:
@@ -653,8 +654,8 @@ def _cache_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_tabl
         raise ValueError(f"{fn}: max_q={max_q} is negative")
     max_q = min(int(max_q), rows)
     return _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
-                           page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), pstart, pages, Hkv, page_size, d,
-                           cols, B, rows, max_q, dtype_code(k_cache.dtype)), shape, max_q
+                           page_table.data_ptr() if cols else lens.data_ptr(),  # (no columns: any address, never read)
+                           page_table.stride(0), lens.data_ptr(), pstart, pages, Hkv, page_size, d, cols, B, rows, max_q, dtype_code(k_cache.dtype)), shape, max_q
 
 
 def _tree_words(fn: str, tree: torch.Tensor | None, rows: int, max_q: int) -> tuple[int | None, int]:
@@ -836,7 +837,8 @@ def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
     _on_current_device(fn, k_cache, v_cache, page_table, lens, paths, q_start)
     out = torch.empty((B,), dtype=torch.int32, device=lens.device)
     desc = _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
-                           page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), pstart, *shape, ts[1], B, rows, most,
+                           page_table.data_ptr() if ts[1] else lens.data_ptr(), page_table.stride(0), lens.data_ptr(),
+                           pstart, *shape, ts[1], B, rows, most,
                            dtype_code(k_cache.dtype))
     rc = _lib.lib().nkl_cache_accept(desc, paths.data_ptr(), paths.stride(0), ps[1], out.data_ptr(), layers, kl, vl,
                                      stream_handle())
@@ -874,7 +876,8 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
     sees nothing gets zeros.  Keys a row does not see take no part, whatever
     they hold; pages that no row of the call sees are not read, and may have
     been freed.  Rows of o that belong to no sequence are left as they are.
-    d a multiple of 8 (fp32: 4), at most 128; scale above 0."""
+    d a multiple of 8 (fp32: 4), at most 128; the caches' strides too, and
+    their first elements on 16 bytes; scale above 0; at most 65535 sequences."""
     fn = "paged_attention_into"
     qs = q.shape
     if len(qs) != 3 or o.shape != qs or o.dtype is not q.dtype:

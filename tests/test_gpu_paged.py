@@ -650,3 +650,146 @@ def test_tree_mask_ends_at_bad_parents():
     assert m.shape == (5000, 79)
     pop = torch.tensor([[bin(w % 2 ** 64).count("1") for w in r] for r in m[::499].tolist()]).sum(dim=1)
     assert pop.tolist() == [i + 1 for i in range(0, 5000, 499)]
+
+
+# ------------------------------------------------------------- odd batches --
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_one_prompt_among_single_tokens(dtype):
+    """Sequences whose new rows differ a hundredfold, more of them than a wavefront has lanes."""
+    from nkilab import ops
+
+    news = [1] * 40 + [150] + [0] + [1] * 60
+    lens = [5 + 3 * i for i in range(40)] + [170] + [7] + [1 + i for i in range(60)]
+    b = Batch(22, lens, news, 4, 2, 64, 16, dtype)
+    for window, sinks in ((None, 0), (50, 2)):
+        out = ops.paged_attention(b.q, *b.args(), q_start=b.q_start, max_q=b.max_q, window=window, sinks=sinks)
+        b.check(out, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("batch", [1, 63, 64, 65, 200, 4100])
+def test_append_of_one_prompt_among_single_tokens(batch):
+    """Rows placed by a search over the offsets, empty sequences among them."""
+    from nkilab import ops
+
+    rng = random.Random(batch)
+    news = [rng.choice((0, 1, 1, 2)) for _ in range(batch)]
+    news[batch // 2] = 700
+    lens = [n + rng.randint(0, 3) for n in news]
+    b = Batch(23, lens, news, 1, 1, 32, 16, "fp32")
+    T = b.starts[-1]
+    k, v = (torch.randn(T + 3, 1, 32, device="cuda") for _ in range(2))  # 3 rows of no sequence
+    want_k, want_v = b.kc.cpu().clone(), b.vc.cpu().clone()
+    for s in range(batch):
+        for i in range(news[s]):
+            p, o = R.table_rows(b.table_host[s], 16, b.pages, lens[s] - news[s] + i)
+            want_k[p, :, o], want_v[p, :, o] = k[b.starts[s] + i].cpu(), v[b.starts[s] + i].cpu()
+    ops.cache_append_into(k, v, *b.args(), q_start=b.q_start, max_q=b.max_q)
+    assert torch.equal(b.kc.cpu(), want_k) and torch.equal(b.vc.cpu(), want_v)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_nothing_to_do(dtype):
+    """No sequences, no rows, no columns, no pages."""
+    from nkilab import ops
+
+    dt = DT[dtype]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kc, vc = (torch.randn(4, 2, 16, 64, device="cuda").to(dt) for _ in range(2))
+    none = torch.empty(0, 2, 64, dtype=dt, device="cuda")
+    table0, lens0 = torch.empty(0, 3, **i32), torch.empty(0, **i32)
+    assert ops.paged_attention(none, kc, vc, table0, lens0).shape == (0, 2, 64)
+    assert ops.paged_attention(none, kc, vc, table0, lens0, q_start=torch.zeros(1, **i32), max_q=0).shape == (0, 2, 64)
+    ops.cache_append_into(none, none, kc, vc, table0, lens0)
+    assert ops.cache_accept(kc, vc, table0, lens0, torch.empty(0, 2, **i32), n_nodes=3).shape == (0,)
+    assert ops.tree_mask(torch.empty(0, **i32), batch=2).shape == (0, 1)
+    q = torch.randn(2, 4, 64, device="cuda").to(dt)
+    lens = torch.tensor([9, 3], **i32)
+    # a table of no columns, and a cache of no pages, hold no keys
+    assert not ops.paged_attention(q, kc, vc, torch.empty(2, 0, **i32), lens).any()
+    assert not ops.paged_attention(q, kc[:0], vc[:0], torch.zeros(2, 3, **i32), lens).any()
+    many = torch.randn(200, 4, 64, device="cuda").to(dt)
+    assert not ops.paged_attention(many, kc[:0], vc[:0], torch.zeros(2, 300, **i32), lens).any()
+    before = kc.clone()
+    ops.cache_append_into(q[:, :2], q[:, :2], kc, vc, torch.empty(2, 0, **i32), lens)
+    ops.cache_append_into(q[:, :2], q[:, :2], kc[:0], vc[:0], torch.zeros(2, 3, **i32), lens)
+    paths = torch.tensor([[1], [0]], **i32)
+    assert ops.cache_accept(kc, vc, torch.empty(2, 0, **i32), lens, paths, n_nodes=2).tolist() == [8, 2]
+    assert ops.cache_accept(kc[:0], vc[:0], torch.zeros(2, 3, **i32), lens, paths, n_nodes=2).tolist() == [8, 2]
+    assert torch.equal(kc, before)
+    assert ops.attention(none.transpose(0, 1), none.transpose(0, 1), none.transpose(0, 1), window=4).shape == (2, 0, 64)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_output_over_the_queries(dtype):
+    """o may be q: whole row tiles and split ones."""
+    from nkilab import ops
+
+    for lens, news in (([3000, 40], [1, 1]), ([900, 333], [200, 33])):
+        b = Batch(24, lens, news, 8, 2, 64, 16, dtype)
+        want = ops.paged_attention(b.q, *b.args(), q_start=b.q_start, max_q=b.max_q)
+        got = b.q.clone()
+        ops.paged_attention_into(got, got, *b.args(), q_start=b.q_start, max_q=b.max_q)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("page", [1, 8, 16, 48, 4096])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_page_sizes(page, dtype):
+    """Pages of one row, smaller than a tile's half, of halves and tiles, and longer than the sequences."""
+    from nkilab import ops
+
+    for lens, news in (([300, 33, 64], [1, 1, 1]), ([170, 600], [70, 130])):
+        b = Batch(25, lens, news, 6, 3, 128, page, dtype)
+        for window, sinks in ((None, 0), (37, 20)):
+            out = ops.paged_attention(b.q, *b.args(), q_start=b.q_start, max_q=b.max_q, window=window, sinks=sinks)
+            b.check(out, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("d", [8, 24, 40, 72, 104, 120])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_head_dims(d, dtype):
+    from nkilab import ops
+
+    for lens, news in (([300, 33], [1, 1]), ([170, 90], [70, 5])):
+        b = Batch(26, lens, news, 4, 2, d, 32, dtype)
+        poison(b, float("nan"))
+        out = ops.paged_attention(b.q, *b.args(), q_start=b.q_start, max_q=b.max_q)
+        ref = R.attention(b.q.float().cpu(), b.kc.float().cpu(), b.vc.float().cpu(), b.table_host, b.lens_host, b.starts)
+        close(out, ref, dtype, 5.0)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_infinities_in_split_keys(dtype):
+    """V's infinities and NaN where keys are split over workgroups and pages are
+    halves of tiles: the rows that see them have them, the others do not."""
+    from nkilab import ops
+
+    b = Batch(27, [2500, 2500], [3, 70], 4, 2, 64, 16, dtype)
+    for s, j, col, value in ((0, 2497, 3, float("inf")), (0, 2498, 4, float("nan")), (1, 2460, 5, float("-inf")),
+                             (1, 10, 6, float("inf"))):
+        p, o = R.table_rows(b.table_host[s], 16, b.pages, j)
+        b.vc[p, 0, o, col] = value
+    for window, sinks in ((None, 0), (2000, 16)):
+        out = ops.paged_attention(b.q, *b.args(), q_start=b.q_start, max_q=b.max_q, window=window, sinks=sinks)
+        got = out.double().cpu().numpy()
+        with np.errstate(invalid="ignore"):
+            ref = b.ref(window=window, sinks=sinks)
+        bad = ~np.isfinite(ref)
+        assert bad.any() and np.array_equal(got[bad], ref[bad], equal_nan=True)
+        assert np.abs(got[~bad] - ref[~bad]).max() <= TOL[dtype] * 5
+
+
+def test_all_scores_nan():
+    """A row whose every visible score is NaN is NaN, also where one part of its keys has nothing else."""
+    from nkilab import ops
+
+    b = Batch(28, [2500], [2], 2, 1, 64, 16, "bf16")
+    b.q[0] = float("nan")
+    out = ops.paged_attention(b.q, *b.args())
+    assert out[0].isnan().all() and out[1].isfinite().all()
+    b.q[0] = 1.0
+    p, o = R.table_rows(b.table_host[0], 16, b.pages, 5)
+    b.kc[p, 0, o] = float("nan")
+    assert ops.paged_attention(b.q, *b.args()).isnan().all()
+    assert ops.paged_attention(b.q, *b.args(), window=2000).isfinite().all()
