@@ -19,21 +19,29 @@
 // 32 w .. of the tile, team t takes the 32-key tiles t, t + NT, ... of the
 // workgroup's share.  Per key tile, with 32x32 MFMAs,
 //     S^T[32 keys x 32 rows] = K . Q^T,   O^T[d x 32 rows] += V^T . P^T
-// as in flash_bf16.hip, whose operand layouts these are.  K and V go global ->
-// VGPR -> LDS, loaded one tile ahead of use; the page of a tile's rows is
-// looked up one tile ahead of that.  A one-wavefront team shares its tiles
-// with no other: it needs no barrier, and one LDS stage.
+// as in flash_bf16.hip, whose operand layouts these are.  Tiles of up to 32
+// rows (single tokens, small trees) are bound by reading the keys: four
+// one-wavefront teams, each with key tiles of its own, K and V global -> VGPR ->
+// LDS one tile ahead of use, no barrier (64 single tokens over up to 16384 rows,
+// 32/8 heads, d = 128, window 4096, bf16: 5.9 TB/s of keys; reads alone of
+// random 8 KB reach 6.8).  Tiles of 128 rows (prompts, large trees) are bound by
+// the matrix cores and the exps beside them: four wavefronts share key tiles
+// that the buffer unit copies to LDS three steps ahead (32 x 16384 x 128, 8 K/V
+// heads, window 4096, fp16: 1.07 ms, 0.90 PFLOP/s, where the library's 8192^3
+// product runs at 1.11).  fp32, and pages that are no multiple of 16 rows, go
+// through VGPRs in both.
 //
-// Masked keys take no part whatever their bits: a key that is not a row of
-// the sequence is neither read nor looked up; a score is replaced, not added
-// to; and a tile with masked keys whose V holds infinities or NaN takes its
-// finite values and the others apart (0 * inf would reach every row).
+// Masked keys take no part whatever their bits: a key that no row of the
+// workgroup sees is not looked up; a score is replaced, not added to; and V's
+// infinities and NaN are taken out of a tile with masked keys (0 * inf would
+// reach every row) and given, after the loop, to the rows that see them.
 //
-// Split.  Where the tiles of rows are few, their keys are cut into shares of
-// equal length, one workgroup each, whose states (max, sum, O) the second
-// kernel joins.  Every workgroup finds its share from the lengths on the
-// device: nothing about them needs to be known where the call is made, so a
-// captured graph can be replayed with other lengths.
+// Split.  Where the tiles of rows are few, or differ much, the keys are cut
+// into ranges of equal cost, one workgroup each, and the second kernel joins
+// the states (max, sum, O) of row tiles that more than one range holds.  Every
+// workgroup finds its range from the lengths on the device: nothing about them
+// needs to be known where the call is made, so a captured graph can be replayed
+// with other lengths, and no counter or flag outlives a call.
 #include <math.h>
 
 #include <type_traits>
@@ -588,8 +596,8 @@ void paged_attn_kernel(PagedArgs p) {
       return bits;
     };
     // Stages the loaded tile.  Where the tile is masked its infinities and NaN
-    // of V are left out (0 * inf would reach the rows that do not see them) and
-    // counted, to be given to the rows that see them after the loop.
+    // of V are left out and noted, to be given to the rows that see them after
+    // the loop.
     unsigned odd_v = 0;
     auto lstore = [&](T* st, bool masked) __attribute__((always_inline)) {
       if (masked) {
