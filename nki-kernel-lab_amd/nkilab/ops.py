@@ -16,9 +16,10 @@ what nkilab.model uses.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from dataclasses import dataclass
+from itertools import chain
 
 import numpy as np
 import torch
@@ -776,23 +777,28 @@ def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs) -> Non
     layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
     if isinstance(pairs, torch.Tensor) and pairs.is_cuda:
         raise ValueError(f"{fn}: pairs are read on the host: a list, an array or a CPU tensor expected")
-    if isinstance(pairs, (list, tuple)):  # (three times as fast as an array made of them)
-        try:
-            flat = [x for a, b in pairs for x in (a, b)]
-        except (TypeError, ValueError):
-            raise ValueError(f"{fn}: pairs must be whole numbers [n, 2]") from None
-    else:
-        p = np.asarray(pairs)
-        if p.size and (p.ndim != 2 or p.shape[1] != 2):
-            raise ValueError(f"{fn}: pairs must be whole numbers [n, 2], got {list(p.shape)}")
-        flat = p.ravel().tolist()
+    try:  # (packed by struct: a thousand pairs in a third of the time that an array made of them takes)
+        if isinstance(pairs, (list, tuple)):
+            flat = list(chain.from_iterable(pairs))
+            whole = not pairs or set(map(len, pairs)) == {2}
+        else:
+            p = np.asarray(pairs)
+            whole = p.size == 0 or (p.ndim == 2 and p.shape[1] == 2 and p.dtype.kind in "iu")
+            flat = p.ravel().tolist()
+        ids = struct.pack(f"{len(flat)}i", *flat)
+    except (TypeError, struct.error):
+        whole = False
+    if not whole:
+        raise ValueError(f"{fn}: pairs must be whole numbers [n, 2]")
     if not flat:
         return
-    if not all(isinstance(x, (int, np.integer)) for x in flat):
-        raise ValueError(f"{fn}: pairs must be whole numbers")
-    if min(flat) < 0 or max(flat) >= shape[0]:
-        raise ValueError(f"{fn}: pages {min(flat)} .. {max(flat)} outside [0, {shape[0]})")
-    ids = (ctypes.c_int * len(flat))(*flat)
+    if len(flat) < 64:
+        low, high = min(flat), max(flat)
+    else:
+        view = np.frombuffer(ids, np.int32)
+        low, high = int(view.min()), int(view.max())
+    if low < 0 or high >= shape[0]:
+        raise ValueError(f"{fn}: pages {low} .. {high} outside [0, {shape[0]})")
     _on_current_device(fn, k_cache, v_cache)
     desc = _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], 0, 0, 0, 0,
                            *shape, 0, 0, 0, 0, dtype_code(k_cache.dtype))

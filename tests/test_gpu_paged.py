@@ -793,3 +793,29 @@ def test_all_scores_nan():
     b.kc[p, 0, o] = float("nan")
     assert ops.paged_attention(b.q, *b.args()).isnan().all()
     assert ops.paged_attention(b.q, *b.args(), window=2000).isfinite().all()
+
+
+@pytest.mark.parametrize("page", [64, 8])
+def test_offsets_past_4_gib(page):
+    """Byte offsets past 32 bits and element offsets past 31, in both kinds of loads."""
+    from nkilab import ops
+
+    d = 128
+    pages = 2 ** 32 // (2 * 2 * page * d) + 50  # two heads of bf16
+    kc = torch.empty(pages, 2, page, d, dtype=torch.bfloat16, device="cuda")
+    vc = torch.empty_like(kc)
+    for lens, news in (([3 * page], [2]), ([3 * page], [3 * page])):
+        b = Batch(29, lens, news, 4 if news == [2] else 40, 2, d, page, "bf16")
+        ids = [pages - 1, pages // 2 + 1, pages - 40]
+        for i, src in zip(ids, b.table_host[0]):
+            kc[i], vc[i] = b.kc[src], b.vc[src]
+        table = torch.tensor([ids], dtype=torch.int32).cuda()
+        b.check(ops.paged_attention(b.q, kc, vc, table, b.lens))
+    new = torch.randn(2, 2, d, device="cuda").bfloat16()
+    ops.cache_append_into(new, new, kc, vc, table, b.lens)
+    at = page - 2
+    assert torch.equal(kc[ids[2], :, at:].transpose(0, 1), new) and torch.equal(vc[ids[2], :, at:].transpose(0, 1), new)
+    ops.cache_copy_pages(kc, vc, [(ids[2], 0), (5, ids[0])])
+    assert torch.equal(kc[0], kc[ids[2]]) and torch.equal(vc[ids[0]], vc[5])
+    ops.cache_accept(kc, vc, table, b.lens, torch.tensor([[1]], dtype=torch.int32).cuda(), n_nodes=2)
+    assert torch.equal(vc[ids[2], :, at], new[1])
