@@ -856,11 +856,14 @@ def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
 def _paged_attention(desc: bytes, q, sq, o, so, H: int, window: int, sinks: int, words: int | None, nwords: int,
                      scale: float) -> None:
     """nkl_paged_attention on operands already checked."""
-    L = _lib.lib()
-    nbytes = L.nkl_paged_attention_workspace_bytes(desc, H, window, sinks, words is not None)
-    ws = workspace(nbytes, q.device) if nbytes else None
-    rc = L.nkl_paged_attention(desc, q.data_ptr(), o.data_ptr(), H, *sq, *so, window, sinks, words, nwords, scale, ptr(ws),
-                               nbytes, stream_handle())
+    L, pq, po, st = _lib.lib(), q.data_ptr(), o.data_ptr(), stream_handle()
+    # Short calls need no workspace; the call says so before it launches anything.
+    rc = L.nkl_paged_attention(desc, pq, po, H, sq[0], sq[1], so[0], so[1], window, sinks, words, nwords, scale, None, 0, st)
+    if rc == _lib.EWORKSPACE:
+        nbytes = L.nkl_paged_attention_workspace_bytes(desc, H, window, sinks, words is not None)
+        ws = workspace(nbytes, q.device)
+        rc = L.nkl_paged_attention(desc, pq, po, H, sq[0], sq[1], so[0], so[1], window, sinks, words, nwords, scale,
+                                   ws.data_ptr(), nbytes, st)
     if rc:
         _lib.check("nkl_paged_attention", rc)
 
@@ -904,7 +907,7 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
     E = 16 // q.element_size()
     q = _rows_operand(q, E)
     out = o if _rows_ok(o, E) else o.clone(memory_format=torch.contiguous_format)
-    _paged_attention(desc, q, q.stride()[:2], out, out.stride()[:2], H, window, sinks, words, nwords, float(scale))
+    _paged_attention(desc, q, q.stride(), out, out.stride(), H, window, sinks, words, nwords, float(scale))
     if out is not o:
         o.copy_(out)
     return o
