@@ -1244,8 +1244,14 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   // Split where the row tiles leave workgroups idle, or may be of lengths so
   // different that the longest outlasts the rest (several sequences, or a
   // causal prompt with no window): up to four rounds of them.
+  // Few key tiles are worked off in the time of the second launch (8 us; a key
+  // tile takes a workgroup 0.4 us of 32 rows, 0.6 of 128, three times that in
+  // fp32): 16 nodes over 1000 rows, 16.2 us in one launch and 18.2 in two, over
+  // 2000 25.1 and 18.5; 4 x 600 under a window of 512 20.7 and 21.5,
+  // 4 x 900 under 900 26.3 and 25.0.
   const long rounds = c.batch == 1 && window ? 1 : 4;
-  pl.split = sparse || (pl.items < rounds * cus * (pl.wide ? 1 : 2) && key_tiles > 2 * pl.min_tiles);
+  const long worth = elem == 4 ? 8 : pl.wide ? 22 : 40;
+  pl.split = sparse || (pl.items < rounds * cus * (pl.wide ? 1 : 2) && key_tiles > worth);
   // Four ranges and more to an item: items of their own ranges, which are then
   // no more than the workgroups with one range less to each item.
   pl.align = pl.items * 4 <= pl.target;

@@ -819,3 +819,22 @@ def test_offsets_past_4_gib(page):
     assert torch.equal(kc[0], kc[ids[2]]) and torch.equal(vc[ids[0]], vc[5])
     ops.cache_accept(kc, vc, table, b.lens, torch.tensor([[1]], dtype=torch.int32).cuda(), n_nodes=2)
     assert torch.equal(vc[ids[2], :, at], new[1])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("tree", [False, True])
+def test_split_keys_of_many_sequences(dtype, tree):
+    """More sequences than a wavefront has lanes, from no rows to long ones, in ranges over their keys."""
+    from nkilab import ops
+
+    lens = [(37 * i * i) % 2100 for i in range(70)]
+    news = [min(n, 1 + i % 3) for i, n in enumerate(lens)]
+    b = Batch(30, lens, news, 2, 1, 32, 32, dtype)
+    kw, bits = dict(q_start=b.q_start, max_q=b.max_q, window=1500, sinks=33), None
+    if tree:
+        parents = [[-1, 0, 0][:n] for n in news]
+        kw["tree"] = ops.tree_mask(torch.tensor(sum(parents, []), dtype=torch.int32).cuda(), q_start=b.q_start,
+                                   max_q=b.max_q)
+        bits = sum((R.tree_bits(p) for p in parents), [])
+        bits = [row + [0] * (3 - len(row)) for row in bits]
+    b.check(ops.paged_attention(b.q, *b.args(), **kw), window=1500, sinks=33, bits=bits)
