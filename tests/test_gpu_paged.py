@@ -838,3 +838,39 @@ def test_split_keys_of_many_sequences(dtype, tree):
         bits = sum((R.tree_bits(p) for p in parents), [])
         bits = [row + [0] * (3 - len(row)) for row in bits]
     b.check(ops.paged_attention(b.q, *b.args(), **kw), window=1500, sinks=33, bits=bits)
+
+
+@pytest.mark.parametrize("news", [1, 70])
+def test_two_captured_graphs_share_no_workspace(news):
+    """Calls whose keys are split, captured twice and replayed side by side on two
+    streams, over lengths that change between replays."""
+    from nkilab import ops
+
+    first, second = (Batch(s, [6000, 300], [news] * 2, 4, 1, 64, 64, "bf16") for s in (31, 32))
+    graphs = []
+    for b in (first, second):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            ops.paged_attention(b.q, *b.args())
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = ops.paged_attention(b.q, *b.args())
+        graphs.append((g, s, out))
+    for lens in ([6000, 300], [5000, 100], [news, 299], [3001, 256]):
+        want = []
+        for b in (first, second):
+            b.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+            want.append(ops.paged_attention(b.q, *b.args()))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, s, _out in graphs:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for (_g, _s, out), w in zip(graphs, want):
+            assert torch.equal(out, w)
+    first.lens_host = lens
+    first.check(graphs[0][2])
