@@ -174,7 +174,9 @@ class CacheStep:
     lens: torch.Tensor       # int32 [batch], with the new rows
     q_start: torch.Tensor    # int32 [batch + 1]
     max_q: int
-    tree: torch.Tensor | None = None
+    tree: torch.Tensor | None
+    ends: list[int]          # the sequences' lengths with the new rows
+    moved: int               # how often the cache had been compacted
 
     @property
     def rows(self) -> int:
@@ -191,6 +193,7 @@ class PagedCache(PagePool):
         device = torch.device("cuda") if device is None else device
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)
+        self._moved = 0
 
     def _copy(self, copies: list[tuple[int, int]]) -> None:
         if copies:
@@ -219,10 +222,14 @@ class PagedCache(PagePool):
         B, nt = len(seqs), len(flat)
         dev = self._tensor(flat + [self._lens[s] for s in seqs] + start + ([p for t in tree for p in t] if tree else []))
         step = CacheStep(seqs, counts, dev[:nt].view(B, width), dev[nt:nt + B], dev[nt + B:nt + 2 * B + 1],
-                         max(counts + [0]))
+                         max(counts + [0]), None, [self._lens[s] for s in seqs], self._moved)
         if tree is not None:
             step.tree = ops.tree_mask(dev[nt + 2 * B + 1:], q_start=step.q_start, max_q=step.max_q)
         return step
+
+    def _check(self, fn: str, step: CacheStep) -> None:
+        if step.moved != self._moved:
+            raise ValueError(f"{fn}: the step's table is stale, the cache has been compacted since")
 
     def accept(self, step: CacheStep, paths: list[list[int]]) -> None:
         """Keeps the accepted path of each sequence's rows of `step` (its latest),
@@ -232,7 +239,10 @@ class PagedCache(PagePool):
         for s, n, path in zip(step.seqs, step.counts, paths):
             if any(a >= b for a, b in zip([-1] + path, path + [n])):
                 raise ValueError(f"accept: path {path} does not ascend within [0, {n})")
+        self._check("accept", step)
         lens = [self._lens[s] for s in step.seqs]
+        if lens != step.ends:
+            raise ValueError(f"accept: the step left lengths {step.ends}, and they are {lens}: not the latest step")
         ctx = [a - n for a, n in zip(lens, step.counts)]
         moved = [list(p) != list(range(len(p))) for p in paths]
         if any(moved):
@@ -250,19 +260,22 @@ class PagedCache(PagePool):
 
     def compact(self) -> list[tuple[int, int]]:
         """Moves the pages in use to the lowest ids, so that the others are one
-        stretch at the end.  Steps made before have stale tables."""
+        stretch at the end.  Steps made before a move are refused from then on."""
         moves = super().compact()
+        self._moved += bool(moves)
         self._copy(moves)
         return moves
 
     def append(self, layer: int, step: CacheStep, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                q_out: torch.Tensor | None = None, rope_base: float | None = None) -> None:
         """``ops.cache_append_into`` of the step's rows in a layer."""
+        self._check("append", step)
         ops.cache_append_into(k, v, self.k[layer], self.v[layer], step.table, step.lens, step.q_start, step.max_q,
                               step.tree, q, q_out, rope_base)
 
     def attention_into(self, layer: int, step: CacheStep, q: torch.Tensor, o: torch.Tensor, window: int | None = None,
                        sinks: int = 0, scale: float | None = None) -> torch.Tensor:
         """``ops.paged_attention_into`` of the step's rows in a layer."""
+        self._check("attention_into", step)
         return ops.paged_attention_into(q, o, self.k[layer], self.v[layer], step.table, step.lens, step.q_start,
                                         step.max_q, window, sinks, step.tree, scale)

@@ -296,3 +296,35 @@ def test_windowed_block_forward(variant):
         block_close(nki_forward(block, x.cuda(), attention_variant=variant), want, torch.float32)
         block_close(nki_forward(block, x.cuda(), compute_dtype="split"), want, torch.float32)
         assert np.allclose(nki_forward(block, x.numpy()), want.numpy(), atol=1e-3)
+
+
+def test_stale_steps_are_refused():
+    """A step is of use until its cache is compacted, and accepted once, as the
+    latest of its sequences."""
+    from nkilab.cache import PagedCache
+
+    cache = PagedCache(16, 1, 8, page_size=4, dtype=torch.float32, device="cpu")
+    cache._copy = lambda copies: None
+    a, b = cache.add(), cache.add()
+    cache.step([a], [9])
+    old = cache.step([b], [3])
+    new = cache.step([b], [5])
+    with pytest.raises(ValueError, match="latest"):
+        cache.accept(old, [[0]])
+    assert cache.length(b) == 8
+    cache.accept(new, [[0, 1]])
+    assert cache.length(b) == 5
+    with pytest.raises(ValueError, match="latest"):
+        cache.accept(new, [[0, 1]])
+    step = cache.step([b], [2])
+    assert cache.compact() == []  # nothing moved: the step stands
+    cache.accept(step, [[0]])
+    step = cache.step([b], [2])
+    cache.free(a)
+    assert cache.compact()
+    x = torch.zeros(2, 1, 8)
+    for call in (lambda: cache.accept(step, [[0]]), lambda: cache.append(0, step, x, x),
+                 lambda: cache.attention_into(0, step, x, x)):
+        with pytest.raises(ValueError, match="stale"):
+            call()
+    assert cache.length(b) == 8
