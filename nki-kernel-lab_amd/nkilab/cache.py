@@ -244,6 +244,10 @@ class PagedCache(PagePool):
         if lens != step.ends:
             raise ValueError(f"accept: the step left lengths {step.ends}, and they are {lens}: not the latest step")
         ctx = [a - n for a, n in zip(lens, step.counts)]
+        for s, c, path in zip(step.seqs, ctx, paths):
+            if c + len(path) < self._floor[s]:
+                raise ValueError(f"accept: sequence {s} gave up pages at length {self._floor[s]}, the path leaves "
+                                 f"{c + len(path)}; release pages after a path is accepted")
         moved = [list(p) != list(range(len(p))) for p in paths]
         if any(moved):
             table = step.table

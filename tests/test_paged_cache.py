@@ -328,3 +328,20 @@ def test_stale_steps_are_refused():
         with pytest.raises(ValueError, match="stale"):
             call()
     assert cache.length(b) == 8
+
+
+def test_accept_after_a_release_changes_nothing():
+    """A path that would leave a sequence shorter than when it gave up pages is
+    refused before any sequence is changed."""
+    from nkilab.cache import PagedCache
+
+    cache = PagedCache(16, 1, 8, page_size=4, dtype=torch.float32, device="cpu")
+    a, b = cache.add(), cache.add()
+    step = cache.step([a, b], [12, 20])
+    assert cache.release(b, 8) == 3
+    books = [cache.pages_of(s) for s in (a, b)]
+    with pytest.raises(ValueError, match="gave up pages"):
+        cache.accept(step, [list(range(5)), list(range(7))])
+    assert [cache.length(s) for s in (a, b)] == [12, 20] and [cache.pages_of(s) for s in (a, b)] == books
+    cache.accept(step, [list(range(5)), list(range(20))])
+    assert [cache.length(s) for s in (a, b)] == [5, 20]
