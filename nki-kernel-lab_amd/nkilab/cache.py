@@ -234,6 +234,7 @@ class PagedCache(PagePool):
     def accept(self, step: CacheStep, paths: list[list[int]]) -> None:
         """Keeps the accepted path of each sequence's rows of `step` (its latest),
         strictly ascending nodes, and drops the others."""
+        paths = [[int(i) for i in p] for p in paths]
         if len(paths) != len(step.seqs):
             raise ValueError(f"accept: {len(paths)} paths for {len(step.seqs)} sequences")
         for s, n, path in zip(step.seqs, step.counts, paths):
@@ -248,7 +249,7 @@ class PagedCache(PagePool):
             if c + len(path) < self._floor[s]:
                 raise ValueError(f"accept: sequence {s} gave up pages at length {self._floor[s]}, the path leaves "
                                  f"{c + len(path)}; release pages after a path is accepted")
-        moved = [list(p) != list(range(len(p))) for p in paths]
+        moved = [p != list(range(len(p))) for p in paths]
         if any(moved):
             table = step.table
             copies = self.own(step.seqs, ctx, lens, keep=True)
@@ -258,7 +259,7 @@ class PagedCache(PagePool):
                 table = self._tensor(rows)
             width = max(len(p) for p in paths)
             ops.cache_accept(self.k, self.v, table, step.lens,
-                             self._tensor([list(p) + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start)
+                             self._tensor([p + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start)
         for s, c, path in zip(step.seqs, ctx, paths):
             self.trim(s, c + len(path))
 

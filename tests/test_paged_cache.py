@@ -345,3 +345,17 @@ def test_accept_after_a_release_changes_nothing():
     assert [cache.length(s) for s in (a, b)] == [12, 20] and [cache.pages_of(s) for s in (a, b)] == books
     cache.accept(step, [list(range(5)), list(range(20))])
     assert [cache.length(s) for s in (a, b)] == [5, 20]
+
+
+@pytest.mark.parametrize("kind", [list, tuple, np.array, torch.tensor])
+def test_accept_takes_any_sequence_of_nodes(kind):
+    from nkilab.cache import PagedCache
+
+    cache = PagedCache(4, 1, 8, page_size=4, dtype=torch.float32, device="cpu")
+    a = cache.add()
+    step = cache.step([a], [6])
+    for bad in ([1, 0], [0, 6], [-1, 0], [2, 2]):
+        with pytest.raises(ValueError, match="ascend"):
+            cache.accept(step, [kind(bad)])
+    cache.accept(step, [kind([0, 1, 2])])
+    assert cache.length(a) == 3
