@@ -211,6 +211,9 @@ class PagedCache(PagePool):
             raise ValueError(f"step: {len(seqs)} sequences and counts {counts}")
         if tree is not None and [len(p) for p in tree] != counts:
             raise ValueError(f"step: trees of {[len(p) for p in tree]} nodes for counts {counts}")
+        for t in tree or []:
+            if not all(-1 <= p < i for i, p in enumerate(t)):
+                raise ValueError(f"step: parents {t} must be nodes before their own, or -1")
         old = [self._lens[s] for s in seqs]
         self._copy(self.own(seqs, old, [a + n for a, n in zip(old, counts)]))
         width = max([len(self._tables[s]) for s in seqs] + [1])

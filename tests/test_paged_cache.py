@@ -359,3 +359,14 @@ def test_accept_takes_any_sequence_of_nodes(kind):
             cache.accept(step, [kind(bad)])
     cache.accept(step, [kind([0, 1, 2])])
     assert cache.length(a) == 3
+
+
+@pytest.mark.parametrize("parents", [[0, 0], [-1, 1], [-2, 0], [-1, 0, 5]])
+def test_trees_that_are_none_are_refused(parents):
+    from nkilab.cache import PagedCache
+
+    cache = PagedCache(4, 1, 8, page_size=4, dtype=torch.float32, device="cpu")
+    a = cache.add()
+    with pytest.raises(ValueError, match="parents"):
+        cache.step([a], [len(parents)], tree=[parents])
+    assert cache.length(a) == 0 and cache.free_pages() == 4
