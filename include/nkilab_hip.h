@@ -477,11 +477,24 @@ int nkl_tree_mask(const int* parents, const int* q_start, int batch, int rows,
                   int n_each, void* words, int tree_words, void* stream);
 
 /*
+ * The same under a window: of its ancestors a node has the bits of those whose
+ * positions lie within `window` of its own, and of those at positions below
+ * `sinks` (lens as in nkl_paged_cache; null without sinks).  window 0: every
+ * one.  nkl_paged_attention with these words and the same window and sinks gives
+ * each node what it would see as the last row of a sequence that ends in its
+ * branch; nkl_cache_append takes the words without a window, for their depths.
+ */
+int nkl_tree_mask_window(const int* parents, const int* q_start, const int* lens,
+                         int batch, int rows, int n_each, int window, int sinks,
+                         void* words, int tree_words, void* stream);
+
+/*
  * Attention of the new rows over the cache (which holds their K and V already):
  * q, o: [rows, H, d], H a multiple of kv_heads; query head h reads K/V head
  * h / (H / kv_heads).  Row i of n, at position pos, sees the keys j <= pos with
  * j > pos - window or j < sinks (window 0: every key).  With a tree it sees the
- * new rows whose bits are set in its mask words, and of the rows before them
+ * new rows whose bits are set in its mask words (whatever the window: trees
+ * deeper than it take nkl_tree_mask_window's words), and of the rows before them
  * those within the window of position lens[b] - n - 1 + (nodes it sees), and the
  * sinks.  A row that sees nothing gets zeros; keys that a row does not see take
  * no part, whatever they hold, and pages that no row of a call sees are not

@@ -358,29 +358,46 @@ __global__ __launch_bounds__(256) void accept_kernel(CacheArgs c, AcceptArgs p, 
 // One workgroup a sequence, one thread a node: the node's ancestors are
 // walked towards the root (their indices fall, or the walk ends), a word of
 // the mask in a register at a time.  Bound by the walk's dependent loads.
-__global__ __launch_bounds__(256) void tree_mask_kernel(const int* parents, const int* q_start, int rows, int n_each,
-                                                        unsigned long long* words, int W) {
+//
+// Under a window a node of depth D keeps the ancestor `up` steps above it where
+// up < window, or where that ancestor, at position ctx + D - up, is one of the
+// sinks (D takes a walk of its own).
+__global__ __launch_bounds__(256) void tree_mask_kernel(const int* parents, const int* q_start, const int* lens, int rows,
+                                                        int n_each, int window, int sinks, unsigned long long* words,
+                                                        int W) {
   constexpr int N = 4096;  // parents held in LDS; longer trees read the rest from memory
   __shared__ int par[N];
   const int b = blockIdx.x;
-  int t0 = b * n_each, n = n_each;
+  int t0 = b * n_each, n = n_each, n_all = n;
   if (q_start) {
     t0 = q_start[b];
     n = q_start[b + 1] - t0;
     if (t0 < 0 || t0 > rows || n < 0) n = 0;
+    n_all = n;
     n = n == 0 ? 0 : min(n, rows - t0);
   }
   for (int i = threadIdx.x; i < min(n, N); i += 256) par[i] = parents[t0 + i];
   __syncthreads();
+  auto above = [&](int j) __attribute__((always_inline)) {  // j's parent, -1 at a root
+    const int a = j < N ? par[j] : parents[t0 + j];
+    return a < j ? a : -1;
+  };
+  // Sinks among the nodes: those at depths below this (0: none).
+  const long below = sinks > 0 ? sinks - (min(max(0, lens[b]), kMaxRows) - (long)n_all) : 0;
+  const int sink_depth = (int)max(0L, min(below, (long)kMaxRows));
   for (int i = threadIdx.x; i < n; i += 256) {
     unsigned long long* out = words + (long)(t0 + i) * W;
-    int w = W - 1, j = i;
+    int w = W - 1, j = i, up = 0, depth = 0;  // j is `up` steps above i, and the node itself at `depth`
+    if (sink_depth > 0)
+      for (int a = above(i); a >= 0; a = above(a)) ++depth;
     unsigned long long bits = 0;
     while (w >= 0) {
       if (j >= 0 && (j >> 6) >= w) {
-        if ((j >> 6) == w) bits |= 1ull << (j & 63);  // (a node past the words has no bit)
-        const int up = j < N ? par[j] : parents[t0 + j];
-        j = up < j ? up : -1;
+        // (a node past the words has no bit)
+        const bool seen = window == 0 || up < window || (sink_depth > 0 && depth - up < sink_depth);
+        if ((j >> 6) == w && seen) bits |= 1ull << (j & 63);
+        j = above(j);
+        ++up;
       } else {
         out[w--] = bits;
         bits = 0;
@@ -558,16 +575,23 @@ extern "C" int nkl_cache_accept(const nkl_paged_cache* cache, const int* paths, 
   return check_launch("nkl_cache_accept");
 }
 
-extern "C" int nkl_tree_mask(const int* parents, const int* q_start, int batch, int rows, int n_each, void* words,
-                             int tree_words, void* stream) {
+extern "C" int nkl_tree_mask_window(const int* parents, const int* q_start, const int* lens, int batch, int rows,
+                                    int n_each, int window, int sinks, void* words, int tree_words, void* stream) {
   if (batch < 0 || rows < 0 || n_each < 0 || tree_words < 1)
     return set_error(NKL_EINVAL, "nkl_tree_mask: batch=%d rows=%d n_each=%d tree_words=%d", batch, rows, n_each, tree_words);
+  if (window < 0 || sinks < 0 || (window == 0 && sinks > 0))
+    return set_error(NKL_EINVAL, "nkl_tree_mask: window=%d, sinks=%d", window, sinks);
   if (!q_start && (long)batch * n_each != rows)
     return set_error(NKL_EINVAL, "nkl_tree_mask: %d rows are not %d for each of %d sequences", rows, n_each, batch);
   if (batch == 0 || rows == 0) return NKL_OK;
-  if (!parents || !words) return set_error(NKL_EINVAL, "nkl_tree_mask: null pointer");
+  if (!parents || !words || (sinks > 0 && !lens)) return set_error(NKL_EINVAL, "nkl_tree_mask: null pointer");
   if ((long)batch * 256 > kMaxGridThreads) return set_error(NKL_EINVAL, "nkl_tree_mask: batch=%d", batch);
   tree_mask_kernel<<<dim3((unsigned)batch), dim3(256), 0, (hipStream_t)stream>>>(
-      parents, q_start, rows, n_each, static_cast<unsigned long long*>(words), tree_words);
+      parents, q_start, lens, rows, n_each, window, sinks, static_cast<unsigned long long*>(words), tree_words);
   return check_launch("nkl_tree_mask");
+}
+
+extern "C" int nkl_tree_mask(const int* parents, const int* q_start, int batch, int rows, int n_each, void* words,
+                             int tree_words, void* stream) {
+  return nkl_tree_mask_window(parents, q_start, nullptr, batch, rows, n_each, 0, 0, words, tree_words, stream);
 }

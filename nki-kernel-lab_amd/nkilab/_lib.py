@@ -85,6 +85,7 @@ SIGNATURES = {
     "nkl_cache_copy_pages": (_c_int, [_cache_p, _vp, _c_int, _c_int, _c_long, _c_long, _vp]),
     "nkl_cache_accept": (_c_int, [_cache_p, _vp, _c_long, _c_int, _vp, _c_int, _c_long, _c_long, _vp]),
     "nkl_tree_mask": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
+    "nkl_tree_mask_window": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
     "nkl_paged_attention_workspace_bytes": (_c_size, [_cache_p, _c_int, _c_int, _c_int, _c_int]),
     "nkl_paged_attention": (_c_int, [_cache_p, _vp, _vp, _c_int, _c_long, _c_long, _c_long, _c_long, _c_int, _c_int, _vp,
                                      _c_int, _c_float, _vp, _c_size, _vp]),

@@ -164,6 +164,14 @@ class PagePool:
         return list(moves.items())
 
 
+def _depth(parents: list[int]) -> int:
+    """Nodes of a tree's longest branch."""
+    depths = []
+    for p in parents:
+        depths.append(1 + (depths[p] if p >= 0 else 0))
+    return max(depths, default=0)
+
+
 @dataclass
 class CacheStep:
     """The new rows of some sequences, as the operators take them (device
@@ -174,7 +182,9 @@ class CacheStep:
     lens: torch.Tensor       # int32 [batch], with the new rows
     q_start: torch.Tensor    # int32 [batch + 1]
     max_q: int
-    tree: torch.Tensor | None
+    tree: torch.Tensor | None     # mask words, as ops.tree_mask has them without a window
+    parents: torch.Tensor | None  # the trees' parents, packed
+    depth: int                    # nodes of the longest branch
     ends: list[int]          # the sequences' lengths with the new rows
     moved: int               # how often the cache had been compacted
 
@@ -225,9 +235,11 @@ class PagedCache(PagePool):
         B, nt = len(seqs), len(flat)
         dev = self._tensor(flat + [self._lens[s] for s in seqs] + start + ([p for t in tree for p in t] if tree else []))
         step = CacheStep(seqs, counts, dev[:nt].view(B, width), dev[nt:nt + B], dev[nt + B:nt + 2 * B + 1],
-                         max(counts + [0]), None, [self._lens[s] for s in seqs], self._moved)
+                         max(counts + [0]), None, None, 0, [self._lens[s] for s in seqs], self._moved)
         if tree is not None:
-            step.tree = ops.tree_mask(dev[nt + 2 * B + 1:], q_start=step.q_start, max_q=step.max_q)
+            step.parents = dev[nt + 2 * B + 1:]
+            step.depth = max(map(_depth, tree), default=0)
+            step.tree = ops.tree_mask(step.parents, q_start=step.q_start, max_q=step.max_q)
         return step
 
     def _check(self, fn: str, step: CacheStep) -> None:
@@ -283,7 +295,12 @@ class PagedCache(PagePool):
 
     def attention_into(self, layer: int, step: CacheStep, q: torch.Tensor, o: torch.Tensor, window: int | None = None,
                        sinks: int = 0, scale: float | None = None) -> torch.Tensor:
-        """``ops.paged_attention_into`` of the step's rows in a layer."""
+        """``ops.paged_attention_into`` of the step's rows in a layer.  A drafted
+        node sees its branch as the row of a prompt would: under a window, the
+        ancestors within it and the sinks."""
         self._check("attention_into", step)
+        tree = step.tree
+        if tree is not None and window is not None and step.depth > window:
+            tree = ops.tree_mask(step.parents, step.q_start, step.max_q, window=window, sinks=sinks, lens=step.lens)
         return ops.paged_attention_into(q, o, self.k[layer], self.v[layer], step.table, step.lens, step.q_start,
-                                        step.max_q, window, sinks, step.tree, scale)
+                                        step.max_q, window, sinks, tree, scale)

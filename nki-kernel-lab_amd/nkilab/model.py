@@ -293,8 +293,8 @@ def nki_decode(block: DecoderBlock, x, cache: PagedCache, step: CacheStep, layer
     (rotated) and V rows go to `layer` of the cache, and which attend over it.
     A prompt in one step gives what nki_forward gives; compute_dtype as there
     ("split" apart), and the cache's dtype is the compute dtype.  With a tree in
-    the step a token sees the context and its ancestors, and is at the context's
-    length and its depth.  Every layer's call takes the same step."""
+    the step a token sees the context and its ancestors (under a window those
+    within it, and the sinks), and is at the context's length and its depth.  Every layer's call takes the same step."""
     cfg = block.cfg
     xt, kind = to_device(x)
     if compute_dtype == SPLIT:

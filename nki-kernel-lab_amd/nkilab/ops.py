@@ -670,14 +670,21 @@ def _tree_words(fn: str, tree: torch.Tensor | None, rows: int, max_q: int) -> tu
     return tree.data_ptr(), tree.shape[1]
 
 
-def tree_mask(parents: torch.Tensor, q_start: torch.Tensor | None = None, max_q: int | None = None,
-              batch: int = 1) -> torch.Tensor:
+def tree_mask(parents: torch.Tensor, q_start: torch.Tensor | None = None, max_q: int | None = None, batch: int = 1,
+              window: int | None = None, sinks: int = 0, lens: torch.Tensor | None = None) -> torch.Tensor:
     """Mask words [rows, words] (int64, bit i % 64 of word i // 64 for node i) of
     drafted trees: node t sees itself and its ancestors.  parents: int32 [rows],
     each node's parent as an index within its own sequence's nodes, below the
     node's (-1: a root, which hangs off the context).  q_start: int32
     [batch + 1], the sequences' first rows, with max_q their most nodes;
-    without it, rows / batch nodes each."""
+    without it, rows / batch nodes each.
+
+    With a window a node sees, of its ancestors, those whose positions lie
+    within `window` of its own, and those at positions below `sinks` (which
+    takes lens: int32 [batch], each sequence's rows with its nodes).
+    ``paged_attention`` takes new rows by their bits, so trees deeper than its
+    window take these words; ``cache_append_into``, which counts a node's depth
+    in them, takes the words without a window."""
     fn = "tree_mask"
     rows = parents.shape[0] if parents.dim() == 1 else -1
     _int32(fn, "parents", parents, (rows,))
@@ -692,11 +699,17 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor | None = None, max_q:
         if each * batch != rows or (max_q is not None and int(max_q) != each):
             raise ValueError(f"{fn}: {rows} nodes are not a number (max_q={max_q}) for each of {batch} sequences")
         max_q = each
-    _on_current_device(fn, parents, q_start)
+    window, sinks = _window_sinks(fn, window, sinks)
+    if sinks:
+        if lens is None:
+            raise ValueError(f"{fn}: sinks need lens, the sequences' rows")
+        _int32(fn, "lens", lens, (batch,))
+    _on_current_device(fn, parents, q_start, lens)
     # (rows that belong to no sequence see nothing)
     words = (torch.empty if q_start is None else torch.zeros)((rows, max(1, -(-int(max_q) // 64))), dtype=torch.int64,
                                                               device=parents.device)
-    _lib.call("nkl_tree_mask", ptr(parents), ptr(q_start), batch, rows, each, ptr(words), words.shape[1], stream_handle())
+    _lib.call("nkl_tree_mask_window", ptr(parents), ptr(q_start), ptr(lens), batch, rows, each, window, sinks, ptr(words),
+              words.shape[1], stream_handle())
     return words
 
 
@@ -880,7 +893,8 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
     New row i of n, at position p = lens[b] - n + i, sees the keys j <= p: all
     of them, or with a window those with j > p - window or j < sinks.  With a
     tree (``tree_mask``'s words, or any bits: bit i lets it see new row i) it
-    sees those new rows, and of the rows before them those in the window of
+    sees those new rows (whatever the window, which ``tree_mask`` takes for trees
+    deeper than it), and of the rows before them those in the window of
     position lens[b] - n - 1 + (new rows it sees), and the sinks.  A row that
     sees nothing gets zeros.  Keys a row does not see take no part, whatever
     they hold; pages that no row of the call sees are not read, and may have
