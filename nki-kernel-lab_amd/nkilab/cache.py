@@ -86,44 +86,56 @@ class PagePool:
             self._drop(p)
         del self._lens[seq], self._floor[seq]
 
-    def own(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> list[tuple[int, int]]:
-        """Gives each sequence pages of its own for rows starts[i] .. ends[i] - 1 and
-        that length.  Returns the (from, to) copies that are to be made first; the
-        rows before starts[i] are kept, those from there on with `keep` only."""
+    def _plan(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> "_Plan":
+        """What `own` will do; nothing changes."""
         ps = self.page_size
         if len(set(seqs)) != len(seqs):
             raise ValueError(f"a sequence is named twice: {seqs}")
         users = dict()  # pages' users as they will be
-        need = 0
+        wanted = []     # (sequence, place in its table, the page that is there and to be kept)
         for seq, start, end in zip(seqs, starts, ends):
             table = self._tables[seq]
             for i in range(start // ps, -(-end // ps) if end > start else 0):
                 if i >= len(table):
-                    need += 1
+                    wanted.append((seq, i, None))
                     continue
                 p = table[i]
                 if p < 0:
                     raise ValueError(f"sequence {seq}: rows {i * ps} .. were released")
                 left = users.get(p, self._users[p])
                 if left > 1:
-                    need += 1
+                    wanted.append((seq, i, p if keep or i * ps < start else None))
                     users[p] = left - 1
-        if need > len(self._free):
-            raise OutOfPages(f"{need} pages needed, {len(self._free)} of {self.pages} free")
-        copies = []
-        for seq, start, end in zip(seqs, starts, ends):
+        if len(wanted) > len(self._free):
+            raise OutOfPages(f"{len(wanted)} pages needed, {len(self._free)} of {self.pages} free")
+        new = self._free[len(self._free) - len(wanted):][::-1]  # as _take hands them out
+        return _Plan([(seq, i, page) for (seq, i, _), page in zip(wanted, new)],
+                     [(old, page) for (_, _, old), page in zip(wanted, new) if old is not None],
+                     {seq: max(end, 0) for seq, end in zip(seqs, ends)})
+
+    def _planned(self, plan: "_Plan") -> dict[int, list[int]]:
+        """The tables of the plan's sequences as they will be."""
+        tables = {seq: list(self._tables[seq]) for seq in plan.lens}
+        for seq, i, page in plan.pages:
+            tables[seq][i:i + 1] = [page]
+        return tables
+
+    def _apply(self, plan: "_Plan") -> None:
+        for seq, i, page in plan.pages:
+            assert self._take() == page
             table = self._tables[seq]
-            for i in range(start // ps, -(-end // ps) if end > start else 0):
-                if i >= len(table):
-                    table.append(self._take())
-                elif self._users[table[i]] > 1:
-                    old, new = table[i], self._take()
-                    self._users[old] -= 1
-                    table[i] = new
-                    if keep or i * ps < start:
-                        copies.append((old, new))
-            self._lens[seq] = max(end, 0)
-        return copies
+            if i < len(table):
+                self._users[table[i]] -= 1
+            table[i:i + 1] = [page]
+        self._lens.update(plan.lens)
+
+    def own(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> list[tuple[int, int]]:
+        """Gives each sequence pages of its own for rows starts[i] .. ends[i] - 1 and
+        that length.  Returns the (from, to) copies that are to be made first; the
+        rows before starts[i] are kept, those from there on with `keep` only."""
+        plan = self._plan(seqs, starts, ends, keep)
+        self._apply(plan)
+        return plan.copies
 
     def trim(self, seq: int, length: int) -> None:
         """Cuts a sequence to its first `length` rows (no fewer than it had when
@@ -151,17 +163,32 @@ class PagePool:
             self._floor[seq] = self._lens[seq]
         return n
 
-    def compact(self) -> list[tuple[int, int]]:
-        """Moves the pages in use to the lowest ids.  Returns the copies."""
+    def _moves(self) -> dict[int, int]:
+        """The copies of a compaction: every page in use that is not among the lowest, to the lowest free ones."""
         used = [p for p in range(self.pages) if self._users[p]]
         low = [p for p in range(len(used)) if not self._users[p]]
-        moves = dict(zip([p for p in used if p >= len(used)], low))
+        return dict(zip([p for p in used if p >= len(used)], low))
+
+    def _rename(self, moves: dict[int, int]) -> None:
         for table in self._tables.values():
             table[:] = [moves.get(p, p) for p in table]
         for a, b in moves.items():
             self._users[b], self._users[a] = self._users[a], 0
-        self._free = list(range(self.pages - 1, len(used) - 1, -1))
+        self._free = [p for p in range(self.pages - 1, -1, -1) if not self._users[p]]
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Moves the pages in use to the lowest ids.  Returns the copies."""
+        moves = self._moves()
+        self._rename(moves)
         return list(moves.items())
+
+
+@dataclass
+class _Plan:
+    """Pages that sequences are to be given, decided before anything changes."""
+    pages: list[tuple[int, int, int]]  # (sequence, place in its table, page), in the order that they are taken
+    copies: list[tuple[int, int]]      # (from, to), made before the plan is applied
+    lens: dict[int, int]
 
 
 def _depth(parents: list[int]) -> int:
@@ -225,21 +252,28 @@ class PagedCache(PagePool):
             if not all(-1 <= p < i for i, p in enumerate(t)):
                 raise ValueError(f"step: parents {t} must be nodes before their own, or -1")
         old = [self._lens[s] for s in seqs]
-        self._copy(self.own(seqs, old, [a + n for a, n in zip(old, counts)]))
-        width = max([len(self._tables[s]) for s in seqs] + [1])
+        ends = [a + n for a, n in zip(old, counts)]
+        # The books change once everything that may be refused is done.
+        plan = self._plan(seqs, old, ends)
+        tables = self._planned(plan)
+        self._copy(plan.copies)
+        width = max([len(tables[s]) for s in seqs] + [1])
         start = [0]
         for n in counts:
             start.append(start[-1] + n)
         # One upload: the table's rows, the lengths, the offsets.
-        flat = [p for s in seqs for p in self._tables[s] + [-1] * (width - len(self._tables[s]))]
+        flat = []
+        for s in seqs:
+            flat += tables[s] + [-1] * (width - len(tables[s]))
         B, nt = len(seqs), len(flat)
-        dev = self._tensor(flat + [self._lens[s] for s in seqs] + start + ([p for t in tree for p in t] if tree else []))
+        dev = self._tensor(flat + ends + start + ([p for t in tree for p in t] if tree else []))
         step = CacheStep(seqs, counts, dev[:nt].view(B, width), dev[nt:nt + B], dev[nt + B:nt + 2 * B + 1],
-                         max(counts + [0]), None, None, 0, [self._lens[s] for s in seqs], self._moved)
+                         max(counts + [0]), None, None, 0, ends, self._moved)
         if tree is not None:
             step.parents = dev[nt + 2 * B + 1:]
             step.depth = max(map(_depth, tree), default=0)
             step.tree = ops.tree_mask(step.parents, q_start=step.q_start, max_q=step.max_q)
+        self._apply(plan)
         return step
 
     def _check(self, fn: str, step: CacheStep) -> None:
@@ -267,24 +301,26 @@ class PagedCache(PagePool):
         moved = [p != list(range(len(p))) for p in paths]
         if any(moved):
             table = step.table
-            copies = self.own(step.seqs, ctx, lens, keep=True)
-            if copies:  # forked since the step
-                self._copy(copies)
-                rows = [self._tables[s] + [-1] * (table.shape[1] - len(self._tables[s])) for s in step.seqs]
-                table = self._tensor(rows)
+            plan = self._plan(step.seqs, ctx, lens, keep=True)
+            if plan.copies:  # forked since the step
+                self._copy(plan.copies)
+                rows = self._planned(plan)
+                table = self._tensor([rows[s] + [-1] * (table.shape[1] - len(rows[s])) for s in step.seqs])
             width = max(len(p) for p in paths)
             ops.cache_accept(self.k, self.v, table, step.lens,
                              self._tensor([p + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start)
+            self._apply(plan)
         for s, c, path in zip(step.seqs, ctx, paths):
             self.trim(s, c + len(path))
 
     def compact(self) -> list[tuple[int, int]]:
         """Moves the pages in use to the lowest ids, so that the others are one
         stretch at the end.  Steps made before a move are refused from then on."""
-        moves = super().compact()
+        moves = self._moves()
+        self._copy(list(moves.items()))
+        self._rename(moves)
         self._moved += bool(moves)
-        self._copy(moves)
-        return moves
+        return list(moves.items())
 
     def append(self, layer: int, step: CacheStep, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                q_out: torch.Tensor | None = None, rope_base: float | None = None) -> None:
