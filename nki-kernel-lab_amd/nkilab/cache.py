@@ -41,11 +41,21 @@ class PagePool:
         self._lens: dict[int, int] = {}
         self._floor: dict[int, int] = {}  # the length a sequence had when it last gave up pages
         self._next = 0
+        # Counts what happens to sequences; and its values when each last changed
+        # its length, and when rows or pages of it last went.
+        self._clock = 0
+        self._resized: dict[int, int] = {}
+        self._cut: dict[int, int] = {}
+
+    def _note(self, when: dict[int, int], seq: int) -> None:
+        self._clock += 1
+        when[seq] = self._clock
 
     def add(self) -> int:
         """A new, empty sequence."""
         seq, self._next = self._next, self._next + 1
         self._tables[seq], self._lens[seq], self._floor[seq] = [], 0, 0
+        self._resized[seq] = self._cut[seq] = self._clock
         return seq
 
     def length(self, seq: int) -> int:
@@ -84,7 +94,8 @@ class PagePool:
         """Ends a sequence; pages that no other has are free again."""
         for p in self._tables.pop(seq):
             self._drop(p)
-        del self._lens[seq], self._floor[seq]
+        del self._lens[seq], self._floor[seq], self._resized[seq], self._cut[seq]
+        self._clock += 1
 
     def _plan(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> "_Plan":
         """What `own` will do; nothing changes."""
@@ -126,8 +137,11 @@ class PagePool:
             table = self._tables[seq]
             if i < len(table):
                 self._users[table[i]] -= 1
+                self._note(self._cut, seq)
             table[i:i + 1] = [page]
-        self._lens.update(plan.lens)
+        for seq, n in plan.lens.items():
+            self._lens[seq] = n
+            self._note(self._resized, seq)
 
     def own(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> list[tuple[int, int]]:
         """Gives each sequence pages of its own for rows starts[i] .. ends[i] - 1 and
@@ -145,6 +159,9 @@ class PagePool:
         table = self._tables[seq]
         while len(table) > -(-length // self.page_size):
             self._drop(table.pop())
+        if length < self._lens[seq]:
+            self._note(self._resized, seq)
+            self._note(self._cut, seq)
         self._lens[seq] = length
 
     def release(self, seq: int, window: int, sinks: int = 0) -> int:
@@ -212,8 +229,10 @@ class CacheStep:
     tree: torch.Tensor | None     # mask words, as ops.tree_mask has them without a window
     parents: torch.Tensor | None  # the trees' parents, packed
     depth: int                    # nodes of the longest branch
-    ends: list[int]          # the sequences' lengths with the new rows
-    moved: int               # how often the cache had been compacted
+    resized: list[int]       # when the cache last changed the sequences' lengths,
+    cut: list[int]           # when it last took rows or pages from them,
+    moved: int               # how often it had been compacted,
+    checked: int             # and when the step last stood
 
     @property
     def rows(self) -> int:
@@ -242,7 +261,9 @@ class PagedCache(PagePool):
     def step(self, seqs: list[int], counts: list[int], tree: list[list[int]] | None = None) -> CacheStep:
         """Makes room for counts[i] new rows of sequence seqs[i] (shared pages that
         they touch are copied) and describes them.  tree: each sequence's drafted
-        tree as its nodes' parents (see ``ops.tree_mask``)."""
+        tree as its nodes' parents (see ``ops.tree_mask``).  A step stands, also
+        when later ones are made, until one of its sequences ends or gives up
+        rows or pages, or pages are moved; calls with it are refused from then on."""
         seqs, counts = list(seqs), [int(n) for n in counts]
         if len(seqs) != len(counts) or any(n < 0 for n in counts):
             raise ValueError(f"step: {len(seqs)} sequences and counts {counts}")
@@ -268,31 +289,43 @@ class PagedCache(PagePool):
         B, nt = len(seqs), len(flat)
         dev = self._tensor(flat + ends + start + ([p for t in tree for p in t] if tree else []))
         step = CacheStep(seqs, counts, dev[:nt].view(B, width), dev[nt:nt + B], dev[nt + B:nt + 2 * B + 1],
-                         max(counts + [0]), None, None, 0, ends, self._moved)
+                         max(counts + [0]), None, None, 0, [], [], self._moved, 0)
         if tree is not None:
             step.parents = dev[nt + 2 * B + 1:]
             step.depth = max(map(_depth, tree), default=0)
             step.tree = ops.tree_mask(step.parents, q_start=step.q_start, max_q=step.max_q)
         self._apply(plan)
+        step.resized, step.cut, step.checked = ([self._resized[s] for s in seqs], [self._cut[s] for s in seqs], self._clock)
         return step
 
     def _check(self, fn: str, step: CacheStep) -> None:
+        """The step's rows are where its table has them, in pages of its sequences' own."""
+        if step.checked == self._clock:
+            return  # (nothing has happened since it last stood)
+        self._check_moved(fn, step)
+        for s, at in zip(step.seqs, step.cut):
+            if self._cut.get(s) != at:
+                raise ValueError(f"{fn}: the step's table is stale, sequence {s} has ended or given up rows or pages since")
+        step.checked = self._clock
+
+    def _check_moved(self, fn: str, step: CacheStep) -> None:
         if step.moved != self._moved:
             raise ValueError(f"{fn}: the step's table is stale, the cache has been compacted since")
 
     def accept(self, step: CacheStep, paths: list[list[int]]) -> None:
         """Keeps the accepted path of each sequence's rows of `step` (its latest),
-        strictly ascending nodes, and drops the others."""
+        strictly ascending nodes, and drops the others.  Once for a step."""
         paths = [[int(i) for i in p] for p in paths]
         if len(paths) != len(step.seqs):
             raise ValueError(f"accept: {len(paths)} paths for {len(step.seqs)} sequences")
         for s, n, path in zip(step.seqs, step.counts, paths):
             if any(a >= b for a, b in zip([-1] + path, path + [n])):
                 raise ValueError(f"accept: path {path} does not ascend within [0, {n})")
-        self._check("accept", step)
+        self._check_moved("accept", step)
+        for s, at in zip(step.seqs, step.resized):
+            if self._resized.get(s) != at:
+                raise ValueError(f"accept: sequence {s} has ended, or changed its length since: not its latest step")
         lens = [self._lens[s] for s in step.seqs]
-        if lens != step.ends:
-            raise ValueError(f"accept: the step left lengths {step.ends}, and they are {lens}: not the latest step")
         ctx = [a - n for a, n in zip(lens, step.counts)]
         for s, c, path in zip(step.seqs, ctx, paths):
             if c + len(path) < self._floor[s]:
@@ -312,6 +345,7 @@ class PagedCache(PagePool):
             self._apply(plan)
         for s, c, path in zip(step.seqs, ctx, paths):
             self.trim(s, c + len(path))
+            self._note(self._resized, s)  # (a step is accepted once, also where the whole of it is)
 
     def compact(self) -> list[tuple[int, int]]:
         """Moves the pages in use to the lowest ids, so that the others are one
@@ -320,6 +354,7 @@ class PagedCache(PagePool):
         self._copy(list(moves.items()))
         self._rename(moves)
         self._moved += bool(moves)
+        self._clock += 1
         return list(moves.items())
 
     def append(self, layer: int, step: CacheStep, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,

@@ -61,3 +61,88 @@ def test_a_refused_call_leaves_the_books_alone(call):
         with pytest.raises(ValueError, match="current device"):
             run()
         assert books(cache) == before
+
+
+def refused(cache, step, *calls):
+    """The calls of a step that no longer stands, refused before any operator is asked."""
+    x = torch.zeros(step.rows, 1, 8)
+    path = [[0][:n] for n in step.counts]
+    run = dict(accept=lambda: cache.accept(step, path), append=lambda: cache.append(0, step, x, x),
+               attention_into=lambda: cache.attention_into(0, step, x, x))
+    before = books(cache)
+    for name in calls:
+        with pytest.raises(ValueError, match="latest" if name == "accept" else "stale"):
+            run[name]()
+    assert books(cache) == before
+
+
+def stands(cache, step):
+    """append and attention_into get as far as the operators, which refuse tensors on the CPU."""
+    x = torch.zeros(step.rows, 1, 8)
+    for call in (lambda: cache.append(0, step, x, x), lambda: cache.attention_into(0, step, x, x)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+
+
+def test_steps_of_equal_lengths_are_told_apart():
+    """A sequence that is back at the length which an earlier step left."""
+    cache = make_cache()
+    a, b = cache.add(), cache.add()
+    cache.step([a], [10])
+    old = cache.step([a], [4])
+    cache.accept(old, [[0, 1]])
+    new = cache.step([a], [2])
+    assert cache.length(a) == 14
+    refused(cache, old, "accept", "append", "attention_into")
+    stands(cache, new)
+    cache.trim(a, 10)  # its page goes to another sequence, and the length comes back
+    cache.step([b], [5])
+    later = cache.step([a], [4])
+    assert cache.length(a) == 14
+    refused(cache, old, "accept", "append", "attention_into")
+    refused(cache, new, "accept", "append", "attention_into")
+    cache.accept(later, [[0]])
+    refused(cache, later, "accept", "append", "attention_into")
+
+
+def test_steps_of_ended_sequences_are_refused():
+    cache = make_cache()
+    a, b = cache.add(), cache.add()
+    both = cache.step([a, b], [4, 4])
+    alone = cache.step([b], [2])
+    cache.free(a)
+    c = cache.add()
+    cache.step([c], [4])  # a's page
+    refused(cache, both, "accept", "append", "attention_into")
+    stands(cache, alone)
+    cache.accept(alone, [[0]])
+
+
+def test_steps_whose_page_became_a_forks_are_refused():
+    """The step's last page was shared with a fork, and its sequence got a copy when it went on."""
+    cache = make_cache()
+    cache._copy = lambda copies: None
+    a = cache.add()
+    step = cache.step([a], [6])
+    f = cache.fork(a)
+    stands(cache, step)
+    more = cache.step([f], [1])  # (the fork's copy: a's pages are as they were)
+    stands(cache, step)
+    stands(cache, more)
+    cache.fork(a)
+    cache.step([a], [1])
+    refused(cache, step, "accept", "append", "attention_into")
+
+
+def test_steps_made_ahead_stand():
+    """Chunks planned one after another are run in that order, and the last is accepted."""
+    cache = make_cache()
+    a, b = cache.add(), cache.add()
+    steps = [cache.step([a, b], n) for n in ((5, 1), (3, 6), (2, 0))]
+    for step in steps:
+        stands(cache, step)
+    for step in steps[:-1]:
+        refused(cache, step, "accept")
+    cache.accept(steps[-1], [[0, 1], []])
+    assert (cache.length(a), cache.length(b)) == (10, 7)
+    refused(cache, steps[-1], "accept")  # once
