@@ -167,7 +167,8 @@ class PagePool:
     def release(self, seq: int, window: int, sinks: int = 0) -> int:
         """Gives up the pages that no later token sees under a window: those whose
         rows are all at least `window` before the sequence's next position and
-        none of the first `sinks`.  Returns how many."""
+        none of the first `sinks`.  Returns how many.  (Tokens before the next may
+        see more: it is called once the latest step has been run.)"""
         if window < 1 or sinks < 0:
             raise ValueError(f"window={window} must be at least 1 and sinks={sinks} at least 0")
         ps, table, n = self.page_size, self._tables[seq], 0
@@ -178,6 +179,7 @@ class PagePool:
                 n += 1
         if n:
             self._floor[seq] = self._lens[seq]
+            self._note(self._cut, seq)
         return n
 
     def _moves(self) -> dict[int, int]:

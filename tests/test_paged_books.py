@@ -146,3 +146,19 @@ def test_steps_made_ahead_stand():
     cache.accept(steps[-1], [[0, 1], []])
     assert (cache.length(a), cache.length(b)) == (10, 7)
     refused(cache, steps[-1], "accept")  # once
+
+
+def test_steps_made_before_a_release_are_refused():
+    """Pages that no later token sees may be ones that the step's own tokens see:
+    the row before the next sees one row more."""
+    cache = make_cache()
+    a, b = cache.add(), cache.add()
+    cache.step([a], [7])
+    step = cache.step([a], [4])
+    assert cache.release(a, 30) == 0
+    stands(cache, step)  # (nothing was given up)
+    assert cache.release(a, 4) == 2
+    cache.step([b], [8])  # the pages that the window of the step's rows begins in
+    refused(cache, step, "append", "attention_into")
+    cache.accept(step, [[0, 1, 2, 3]])
+    assert cache.length(a) == 11
