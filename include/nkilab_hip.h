@@ -461,7 +461,7 @@ int nkl_cache_copy_pages(const nkl_paged_cache* cache, const int* pairs, int n,
  * read before any is written, in each layer, and new_lens[b] = ctx + the path's
  * length.  A path is a strictly ascending list of nodes in [0, n): it ends
  * at its first entry that is not one (-1 by custom), or after path_cols.
- * A sequence's pages from ctx on must be its own.
+ * No other sequence may have a page that rows are moved to.
  */
 int nkl_cache_accept(const nkl_paged_cache* cache, const int* paths,
                      long path_row, int path_cols, int* new_lens, int layers,

@@ -333,10 +333,13 @@ class PagedCache(PagePool):
             if c + len(path) < self._floor[s]:
                 raise ValueError(f"accept: sequence {s} gave up pages at length {self._floor[s]}, the path leaves "
                                  f"{c + len(path)}; release pages after a path is accepted")
-        moved = [p != list(range(len(p))) for p in paths]
-        if any(moved):
+        stay = [sum(i == node for i, node in enumerate(p)) for p in paths]  # (an ascending path's first: in place already)
+        if any(m < len(p) for m, p in zip(stay, paths)):
             table = step.table
-            plan = self._plan(step.seqs, ctx, lens, keep=True)
+            # Pages of its own for the rows that move; those that they come from are only read.
+            plan = self._plan(step.seqs, [c + m for c, m in zip(ctx, stay)], [c + len(p) for c, p in zip(ctx, paths)],
+                              keep=True)
+            plan.lens = dict(zip(step.seqs, lens))  # (until the others are dropped)
             if plan.copies:  # forked since the step
                 self._copy(plan.copies)
                 rows = self._planned(plan)

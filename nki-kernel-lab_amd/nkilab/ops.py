@@ -830,8 +830,8 @@ def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
     lens: int32 [batch], rows with the nodes.  paths: int32 [batch, columns],
     strictly ascending nodes, ended by the first entry that is not (-1 by
     custom).  The nodes of each sequence: q_start (int32 [batch + 1]), or
-    n_nodes for every one.  A sequence's pages from its first node on must be
-    its own."""
+    n_nodes for every one.  No other sequence may have a page that rows are
+    moved to (those that they come from are only read)."""
     fn = "cache_accept"
     layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
     ts, ps = page_table.shape, paths.shape

@@ -162,3 +162,51 @@ def test_steps_made_before_a_release_are_refused():
     refused(cache, step, "append", "attention_into")
     cache.accept(step, [[0, 1, 2, 3]])
     assert cache.length(a) == 11
+
+
+def test_accept_copies_no_page_that_it_only_reads(monkeypatch):
+    """After a fork the sequence gets pages of its own for its path's rows alone."""
+    from nkilab import ops
+
+    cache = make_cache(pages=4)
+    copies, moves = [], []
+    cache._copy = copies.extend
+    monkeypatch.setattr(ops, "cache_accept", lambda k, v, table, lens, paths, **kw: moves.append((table.tolist(), paths.tolist())))
+    a = cache.add()
+    cache.step([a], [4])
+    step = cache.step([a], [8])  # three pages of four
+    f = cache.fork(a)
+    cache.accept(step, [[0, 2]])
+    assert copies == [(1, 3)] and moves == [([[0, 3, 2]], [[0, 2]])]
+    assert cache.pages_of(a) == [0, 3] and cache.pages_of(f) == [0, 1, 2]
+    assert (cache.length(a), cache.length(f), cache.free_pages()) == (6, 12, 0)
+    # a path whose rows end where they begin needs no page at all
+    step = cache.step([f], [0])
+    cache.accept(step, [[]])
+    with pytest.raises(ValueError):
+        cache.accept(step, [[]])
+
+
+@pytest.mark.gpu
+def test_accept_of_both_forks_reads_shared_pages():
+    """Two sequences that share a step's pages keep paths of different lengths: a
+    page that one only reads is not the one that the other writes."""
+    from nkilab.cache import PagedCache
+
+    import paged_reference as R
+
+    cache = PagedCache(12, 1, 8, page_size=4, dtype=torch.float32)
+    a = cache.add()
+    rows = torch.randn(30, 1, 8, device="cuda")
+    head = cache.step([a], [5])
+    cache.append(0, head, rows[:5], rows[:5])
+    f = cache.fork(a)
+    both = cache.step([a, f], [12, 12])
+    cache.append(0, both, rows[5:29], rows[5:29])
+    g = cache.fork(f)
+    cache.accept(both, [[1, 9], [0, 2, 5, 6, 8, 11]])
+    at = lambda s: torch.stack([cache.k[0, p, :, o] for p, o in  # noqa: E731
+                                (R.table_rows(cache.pages_of(s), 4, 12, j) for j in range(cache.length(s)))])
+    assert torch.equal(at(a), rows[[0, 1, 2, 3, 4, 6, 14]])
+    assert torch.equal(at(f), rows[[0, 1, 2, 3, 4] + [17 + i for i in (0, 2, 5, 6, 8, 11)]])
+    assert torch.equal(at(g), torch.cat((rows[:5], rows[17:29])))
