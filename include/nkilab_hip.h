@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define NKL_ABI_VERSION 1
+#define NKL_ABI_VERSION 2
 
 enum { NKL_F32 = 0, NKL_BF16 = 1, NKL_F16 = 2 };
 
@@ -432,7 +432,7 @@ typedef struct {
 /*
  * Writes new K and V rows to the cache and, with rope_base != 0, rotates K on
  * the way and q into q_out (which may be q): rotate-half layout as nkl_rope,
- * but each row by its own position and with the angle in 64 bits.  With a tree
+ * but each row by its own position and with the base and the angle in 64 bits.  With a tree
  * (mask words as nkl_tree_mask makes them) a node's position is lens[b] - n - 1
  * + the nodes it sees.  k, v: [rows, kv_heads, d], q, q_out: [rows, H, d], with
  * element strides; H = 0 and null pointers for no q.  d even (and at most 1024)
@@ -443,7 +443,7 @@ int nkl_cache_append(const nkl_paged_cache* cache, const void* k, const void* v,
                      long k_row, long k_head, long v_row, long v_head,
                      const void* q, void* q_out, int H, long q_row, long q_head,
                      long qo_row, long qo_head, const void* tree,
-                     int tree_words, float rope_base, void* stream);
+                     int tree_words, double rope_base, void* stream);
 
 /*
  * Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, K and V, in each of

@@ -413,16 +413,16 @@ using namespace nkl;
 
 extern "C" int nkl_cache_append(const nkl_paged_cache* cache, const void* k, const void* v, long k_row, long k_head,
                                 long v_row, long v_head, const void* q, void* q_out, int H, long q_row, long q_head,
-                                long qo_row, long qo_head, const void* tree, int tree_words, float rope_base,
+                                long qo_row, long qo_head, const void* tree, int tree_words, double rope_base,
                                 void* stream) {
   CacheArgs c;
   if (const int rc = cache_args("nkl_cache_append", cache, true, c)) return rc;
-  if (rope_base != 0.f && (!(rope_base > 1.f) || !isfinite(rope_base)))
+  if (rope_base != 0.0 && (!(rope_base > 1.0) || !isfinite(rope_base)))
     return set_error(NKL_EINVAL, "nkl_cache_append: rotary base %g must be finite and > 1 (0: none)", rope_base);
-  if (rope_base != 0.f && c.d % 2) return set_error(NKL_EINVAL, "nkl_cache_append: rotary head dim %d must be even", c.d);
-  if (rope_base != 0.f && c.d > 1024)
+  if (rope_base != 0.0 && c.d % 2) return set_error(NKL_EINVAL, "nkl_cache_append: rotary head dim %d must be even", c.d);
+  if (rope_base != 0.0 && c.d > 1024)
     return set_error(NKL_EINVAL, "nkl_cache_append: rotary head dim %d above 1024", c.d);
-  if ((q || q_out || H) && rope_base == 0.f)
+  if ((q || q_out || H) && rope_base == 0.0)
     return set_error(NKL_EINVAL, "nkl_cache_append: q is rotated, and there is no rotary base");
   if (H < 0 || (H > 0) != (q != nullptr) || (H > 0) != (q_out != nullptr))
     if (!(H > 0 && cache->rows == 0)) return set_error(NKL_EINVAL, "nkl_cache_append: q, q_out and H=%d do not match", H);
@@ -441,8 +441,8 @@ extern "C" int nkl_cache_append(const nkl_paged_cache* cache, const void* k, con
   p.tree = static_cast<const unsigned long long*>(tree);
   p.tree_words = tree_words;
   p.H = H;
-  p.rope = rope_base != 0.f;
-  p.log2_base = p.rope ? log2((double)rope_base) : 0.0;
+  p.rope = rope_base != 0.0;
+  p.log2_base = p.rope ? log2(rope_base) : 0.0;
   const int E = 16 / elem_bytes(cache->dtype);
   long strides = c.k_page | c.k_head | c.k_row | c.v_page | c.v_head | c.v_row | k_row | k_head | v_row | v_head | c.d;
   if (H) strides |= q_row | q_head | qo_row | qo_head;

@@ -15,9 +15,10 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 F32, BF16, F16 = 0, 1, 2
 GEMM_BLOCKED, GEMM_NAIVE = 0, 1
 EINVAL, EWORKSPACE = -1, -4
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 _c_int, _c_long, _c_float, _c_size = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_size_t
+_c_double = ctypes.c_double
 _vp = ctypes.c_void_p
 
 
@@ -81,7 +82,7 @@ SIGNATURES = {
     "nkl_attention_naive": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_int, _c_long, _c_long,
                                      _c_long, _c_long, _c_long, _c_long, _c_long, _c_long, _c_float, _c_int, _vp]),
     "nkl_cache_append": (_c_int, [_cache_p, _vp, _vp, _c_long, _c_long, _c_long, _c_long, _vp, _vp, _c_int, _c_long,
-                                  _c_long, _c_long, _c_long, _vp, _c_int, _c_float, _vp]),
+                                  _c_long, _c_long, _c_long, _vp, _c_int, _c_double, _vp]),
     "nkl_cache_copy_pages": (_c_int, [_cache_p, _vp, _c_int, _c_int, _c_long, _c_long, _vp]),
     "nkl_cache_accept": (_c_int, [_cache_p, _vp, _c_long, _c_int, _vp, _c_int, _c_long, _c_long, _vp]),
     "nkl_tree_mask": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
