@@ -407,9 +407,11 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
  * A call brings `rows` new rows, those of sequence b at rows
  * q_start[b] .. q_start[b + 1] - 1 of its packed tensors (q_start null: max_new
  * each).  max_new is the most that a sequence brings: rows past it, and rows
- * behind the last sequence's, are left as they are.  lens[b] counts the
- * sequence's rows with its new ones, which are its last: new row i of n is at
- * position lens[b] - n + i.  (A position below 0 has no row.)
+ * behind the last sequence's, are left as they are.  Offsets ascend within the
+ * packed rows: of sequences for which they do not, the rows that there are count,
+ * and a packed row that two sequences name gets the result of either.
+ * lens[b] counts the sequence's rows with its new ones, which are its last: new
+ * row i of n is at position lens[b] - n + i.  (A position below 0 has no row.)
  *
  * table, lens and q_start are device arrays, read by the kernels only, so a
  * captured graph can be replayed with other contents.  A table addresses at

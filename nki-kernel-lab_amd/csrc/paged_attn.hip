@@ -126,7 +126,7 @@ __device__ __forceinline__ Span span_of(const PagedArgs& p, const Seq& s, int r0
 // ranges of its own instead, and no range has two segments.
 __device__ __forceinline__ int item_units(const PagedArgs& p, int nt, int len) {
   const int n = p.setup + max(nt, 1);
-  return p.align && len > 0 ? (int)((unsigned)(n + len - 1) / (unsigned)len) * len : n;
+  return len > 0 ? (int)((unsigned)(n + len - 1) / (unsigned)len) * len : n;
 }
 
 // Units of a sequence; len > 0: with its items aligned to ranges of that length.
@@ -139,32 +139,42 @@ __device__ __forceinline__ int seq_units(const PagedArgs& p, const Seq& s, int l
 }
 
 // Where workgroup w's range lies: its units [u, u1), the sequence that u is of
-// and that sequence's first unit.  Every lane of a wavefront takes a sequence
-// (64 at a time); the results are the same in all of them.  The plan refuses
-// calls of 2^31 units.
+// and that sequence's first unit, and the length that items are aligned to (0:
+// none).  Every lane of a wavefront takes a sequence (64 at a time); the results
+// are the same in all of them.  The plan takes the packed rows to be of one
+// sequence each: it allows for the items of so many rows, and for under 2^30
+// units.  Offsets that overlap may bring more of both, so sums stop there, and
+// items are aligned only where their ranges then fit the grid.
 template <int MR>
-__device__ __forceinline__ void find_range(const PagedArgs& p, int w, int& len, int& u, int& u1, int& b, int& first) {
+__device__ __forceinline__ void find_range(const PagedArgs& p, int w, int& len, int& al, int& u, int& u1, int& b,
+                                           int& first) {
+  constexpr int kMost = (1 << 30) - 1;
   const int lane = threadIdx.x & 63, batch = p.c.batch;
   auto scan = [&](int b0, int al) __attribute__((always_inline)) {  // units of sequences b0 .. b0 + lane
     int x = b0 + lane < batch ? seq_units<MR>(p, seq_of(p.c, b0 + lane), al) : 0;
     for (int o = 1; o < 64 && o < batch; o <<= 1) {
       const int y = __shfl_up(x, o, kWave);
-      if (lane >= o) x += y;
+      if (lane >= o) x = min(x + y, kMost);
     }
     return x;
   };
   auto sum_of = [&](int al, int incl) __attribute__((always_inline)) {
     int total = __builtin_amdgcn_readlane(incl, 63 < batch ? 63 : batch - 1);
     for (int b0 = 64; b0 < batch; b0 += 64)
-      total += __builtin_amdgcn_readlane(scan(b0, al), batch - b0 > 64 ? 63 : batch - b0 - 1);
+      total = min(total + __builtin_amdgcn_readlane(scan(b0, al), batch - b0 > 64 ? 63 : batch - b0 - 1), kMost);
     return total;
   };
   int incl = scan(0, 0);
   int total = sum_of(0, incl);
   len = max((int)(((long)total + p.target - 1) / p.target), p.min_tiles);
+  al = 0;
   if (p.align) {
-    incl = scan(0, len);
-    total = sum_of(len, incl);
+    const int incl_al = scan(0, len), total_al = sum_of(len, incl_al);
+    if (total_al <= (long)gridDim.x * len) {
+      al = len;
+      incl = incl_al;
+      total = total_al;
+    }
   }
   u = (int)min((long)w * len, (long)total);
   u1 = (int)min((long)u + len, (long)total);
@@ -172,7 +182,7 @@ __device__ __forceinline__ void find_range(const PagedArgs& p, int w, int& len, 
   b = batch;
   if (u >= u1) return;
   for (int b0 = 0; b0 < batch; b0 += 64) {
-    if (b0 > 0) incl = scan(b0, len);
+    if (b0 > 0) incl = scan(b0, al);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(b0 + lane < batch && u < first + incl);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -307,12 +317,12 @@ void paged_attn_kernel(PagedArgs p) {
 
   // ---- this workgroup's units: a range of them, or one row tile's
   int b, kvh, r0;
-  int len = 1, u = 0, u1 = 1;
+  int len = 1, al = 0, u = 0, u1 = 1;
   int skip = 0;  // units of the item before the range
   Seq s;
   if constexpr (SPLIT) {
     int first;
-    find_range<MR>(p, blockIdx.x, len, u, u1, b, first);
+    find_range<MR>(p, blockIdx.x, len, al, u, u1, b, first);
     if (u >= u1) {
       if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
       return;
@@ -320,7 +330,7 @@ void paged_attn_kernel(PagedArgs p) {
     s = seq_of(c, b);
     int x = u - first;
     for (r0 = 0;; r0 += MR) {
-      const int n = item_units(p, span_of(p, s, r0, MR).nt, len);
+      const int n = item_units(p, span_of(p, s, r0, MR).nt, al);
       if (x < n * c.kv_heads) {
         kvh = x / n;
         skip = x - kvh * n;
@@ -1071,8 +1081,9 @@ void paged_attn_kernel(PagedArgs p) {
       // A range's first segment, if its row tile began before: slot 0.  Else the
       // row tile begins here and goes on in the next ranges: slot 1, and the
       // entry by which the second kernel finds its parts.
+      // (cut off at the grid: see find_range's sums)
       if (c0 == 0 && threadIdx.x == 0)
-        p.joins[blockIdx.x] = {b, kvh, r0, (u - skip + p.setup + sp.nt - 1) / len - (int)blockIdx.x + 1};
+        p.joins[blockIdx.x] = {b, kvh, r0, min((u - skip + p.setup + sp.nt - 1) / len + 1, (int)gridDim.x) - (int)blockIdx.x};
       float* part = p.part + (2L * blockIdx.x + (c0 > 0 ? 0 : 1)) * part_floats<DP, MR>();
       if (row_ok) {
 #pragma unroll
@@ -1089,7 +1100,7 @@ void paged_attn_kernel(PagedArgs p) {
 
     if constexpr (!SPLIT) break;
     // ---- the range's next segment: the next K/V head, row tile or sequence
-    u += item_units(p, sp.nt, len) - skip;
+    u += item_units(p, sp.nt, al) - skip;
     if (u >= u1) {
       if ((whole || c0 > 0) && threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
       break;
