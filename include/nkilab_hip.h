@@ -461,8 +461,9 @@ int nkl_cache_copy_pages(const nkl_paged_cache* cache, const int* pairs, int n,
  * Keeps the accepted path of each sequence's new rows: with ctx = lens[b] - n,
  * row ctx + paths[b path_row + i] moves to row ctx + i, as if every row were
  * read before any is written, in each layer, and new_lens[b] = ctx + the path's
- * length.  A path is a strictly ascending list of nodes in [0, n): it ends
- * at its first entry that is not one (-1 by custom), or after path_cols.
+ * length (apart from lens, which all of the call reads).  A path is a strictly
+ * ascending list of nodes in [0, n): it ends at its first entry that is not one
+ * (-1 by custom), or after path_cols.
  * No other sequence may have a page that rows are moved to.
  */
 int nkl_cache_accept(const nkl_paged_cache* cache, const int* paths,

@@ -553,6 +553,8 @@ extern "C" int nkl_cache_accept(const nkl_paged_cache* cache, const int* paths, 
   if (!c.table || !c.lens) return set_error(NKL_EINVAL, "nkl_cache_accept: null page table or lens");
   if (!new_lens || (path_cols > 0 && !paths)) return set_error(NKL_EINVAL, "nkl_cache_accept: null pointer");
   if (layers > 0 && c.pages > 0 && (!c.k || !c.v)) return set_error(NKL_EINVAL, "nkl_cache_accept: null cache pointer");
+  if ((size_t)new_lens < (size_t)(c.lens + c.batch) && (size_t)c.lens < (size_t)(new_lens + c.batch))
+    return set_error(NKL_EINVAL, "nkl_cache_accept: new_lens must lie apart from lens");
   if (c.batch > 65535) return set_error(NKL_EINVAL, "nkl_cache_accept: batch=%d above 65535", c.batch);
   const int el = elem_bytes(cache->dtype);
   AcceptArgs p{paths, path_row, path_cols, new_lens, k_layer * el, v_layer * el, layers};

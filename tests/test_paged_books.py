@@ -210,3 +210,18 @@ def test_accept_of_both_forks_reads_shared_pages():
     assert torch.equal(at(a), rows[[0, 1, 2, 3, 4, 6, 14]])
     assert torch.equal(at(f), rows[[0, 1, 2, 3, 4] + [17 + i for i in (0, 2, 5, 6, 8, 11)]])
     assert torch.equal(at(g), torch.cat((rows[:5], rows[17:29])))
+
+
+def test_accept_writes_lengths_apart_from_those_it_reads():
+    """Every workgroup of a sequence reads its length, and one writes the new one:
+    in the same place, the others might read that."""
+    import ctypes
+
+    from nkilab import _lib
+
+    d = _lib.PagedCacheDesc(k=P, v=P, k_page=4096, k_head=1024, k_row=64, v_page=4096, v_head=1024, v_row=64, table=P,
+                            table_row=8, lens=P + 400, q_start=None, pages=10, kv_heads=4, page_size=16, d=64, table_cols=8,
+                            batch=3, rows=0, max_new=0, dtype=1)
+    for new in (P + 400, P + 400 + 8, P + 400 - 8):
+        assert _lib.lib().nkl_cache_accept(ctypes.byref(d), P, 4, 4, new, 1, 0, 0, None) == -1
+        assert b"new_lens" in _lib.lib().nkl_last_error_string()
