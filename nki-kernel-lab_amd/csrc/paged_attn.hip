@@ -27,8 +27,8 @@
 // random 8 KB reach 6.8).  Tiles of 128 rows (prompts, large trees) are bound by
 // the matrix cores and the exps beside them: four wavefronts share key tiles
 // that the buffer unit copies to LDS three steps ahead (32 x 16384 x 128, 8 K/V
-// heads, window 4096, fp16: 1.07 ms, 0.90 PFLOP/s, where the library's 8192^3
-// product runs at 1.11).  fp32, and pages that are no multiple of 16 rows, go
+// heads, window 4096, fp16: 1.04-1.10 ms on different boxes, 0.87-0.93 PFLOP/s,
+// where the library's 8192^3 product runs at 1.16-1.19).  fp32, and pages that are no multiple of 16 rows, go
 // through VGPRs in both.
 //
 // Masked keys take no part whatever their bits: a key that no row of the
@@ -1083,7 +1083,8 @@ void paged_attn_kernel(PagedArgs p) {
       // entry by which the second kernel finds its parts.
       // (cut off at the grid: see find_range's sums)
       if (c0 == 0 && threadIdx.x == 0)
-        p.joins[blockIdx.x] = {b, kvh, r0, min((u - skip + p.setup + sp.nt - 1) / len + 1, (int)gridDim.x) - (int)blockIdx.x};
+        p.joins[blockIdx.x] = {b, kvh, r0,
+                               min((u - skip + p.setup + sp.nt - 1) / len + 1, (int)gridDim.x) - (int)blockIdx.x};
       float* part = p.part + (2L * blockIdx.x + (c0 > 0 ? 0 : 1)) * part_floats<DP, MR>();
       if (row_ok) {
 #pragma unroll
@@ -1259,9 +1260,12 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int H, int window, 
   // causal prompt with no window): up to four rounds of them.
   // Few key tiles are worked off in the time of the second launch (8 us; a key
   // tile takes a workgroup 0.4 us of 32 rows, 0.6 of 128, three times that in
-  // fp32): 16 nodes over 1000 rows, 16.2 us in one launch and 18.2 in two, over
-  // 2000 25.1 and 18.5; 4 x 600 under a window of 512 20.7 and 21.5,
-  // 4 x 900 under 900 26.3 and 25.0.
+  // fp32).  One launch and two, us: 16 nodes, 16 heads x 128 bf16, over 1000 rows
+  // 16.1 and 20.6, 1500 20.5 and 18.1, 2000 25.1 and 18.4; 4 prompts of 300, 16
+  // heads x 128 bf16, 15.1 and 29; 4 fp32 tokens, 8 heads x 128, over 200 rows
+  // 20.8 and 21.6, 400 34.3 and 22.8.  (Key tiles are counted from the table's
+  // columns and the window.  Prompts with row tiles for more than half the card
+  // would gain from one launch for longer: 4 of 900 take 38.7 and 57.)
   const long rounds = c.batch == 1 && window ? 1 : 4;
   const long worth = elem == 4 ? 8 : pl.wide ? 22 : 40;
   pl.split = sparse || (pl.items < rounds * cus * (pl.wide ? 1 : 2) && key_tiles > worth);

@@ -11,7 +11,7 @@ reference has no cache (its block attends over one prompt, model.py:59-67).
     seq = cache.add()
     step = cache.step([seq], [len(prompt)])        # rows for the prompt
     x = nki_decode(block, x, cache, step, layer)   # for every layer
-    step = cache.step([seq], [16], tree=parents)   # a tree of 16 drafted tokens
+    step = cache.step([seq], [16], tree=[parents]) # a tree of 16 drafted tokens
     ...
     cache.accept(step, [[0, 3, 7]])                # the path that was accepted
 """
@@ -81,7 +81,8 @@ class PagePool:
             self._free.append(page)
 
     def fork(self, seq: int) -> int:
-        """A sequence with the same rows, in the same pages until either writes."""
+        """A sequence with the same rows, in the same pages until either writes (rows
+        that a step has yet to bring are copied as they are)."""
         new = self.add()
         self._tables[new], self._lens[new] = list(self._tables[seq]), self._lens[seq]
         self._floor[new] = self._floor[seq]

@@ -656,7 +656,8 @@ def _cache_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_tabl
     max_q = min(int(max_q), rows)
     return _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
                            page_table.data_ptr() if cols else lens.data_ptr(),  # (no columns: any address, never read)
-                           page_table.stride(0), lens.data_ptr(), pstart, pages, Hkv, page_size, d, cols, B, rows, max_q, dtype_code(k_cache.dtype)), shape, max_q
+                           page_table.stride(0), lens.data_ptr(), pstart, pages, Hkv, page_size, d, cols, B, rows, max_q,
+                           dtype_code(k_cache.dtype)), shape, max_q
 
 
 def _tree_words(fn: str, tree: torch.Tensor | None, rows: int, max_q: int) -> tuple[int | None, int]:
