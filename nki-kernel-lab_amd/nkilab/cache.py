@@ -68,11 +68,6 @@ class PagePool:
     def free_pages(self) -> int:
         return len(self._free)
 
-    def _take(self) -> int:
-        p = self._free.pop()
-        self._users[p] = 1
-        return p
-
     def _drop(self, page: int) -> None:
         if page < 0:
             return
@@ -120,7 +115,7 @@ class PagePool:
                     users[p] = left - 1
         if len(wanted) > len(self._free):
             raise OutOfPages(f"{len(wanted)} pages needed, {len(self._free)} of {self.pages} free")
-        new = self._free[len(self._free) - len(wanted):][::-1]  # as _take hands them out
+        new = self._free[len(self._free) - len(wanted):][::-1]  # from the end
         return _Plan([(seq, i, page) for (seq, i, _), page in zip(wanted, new)],
                      [(old, page) for (_, _, old), page in zip(wanted, new) if old is not None],
                      {seq: max(end, 0) for seq, end in zip(seqs, ends)})
@@ -133,8 +128,9 @@ class PagePool:
         return tables
 
     def _apply(self, plan: "_Plan") -> None:
+        del self._free[len(self._free) - len(plan.pages):]
         for seq, i, page in plan.pages:
-            assert self._take() == page
+            self._users[page] = 1
             table = self._tables[seq]
             if i < len(table):
                 self._users[table[i]] -= 1

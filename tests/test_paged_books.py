@@ -225,3 +225,19 @@ def test_accept_writes_lengths_apart_from_those_it_reads():
     for new in (P + 400, P + 400 + 8, P + 400 - 8):
         assert _lib.lib().nkl_cache_accept(ctypes.byref(d), P, 4, 4, new, 1, 0, 0, None) == -1
         assert b"new_lens" in _lib.lib().nkl_last_error_string()
+
+
+def test_books_need_no_assertions():
+    """The same pages where Python runs without them."""
+    import os
+    import subprocess
+    import sys
+
+    import nkilab
+
+    code = ("from nkilab.cache import PagePool; p = PagePool(8, 4); a = p.add(); p.own([a], [0], [9]); b = p.fork(a); "
+            "print(p.own([a, b], [9, 9], [13, 10]), p.pages_of(a), p.pages_of(b), p.free_pages())")
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(nkilab.__file__)))
+    out = [subprocess.run([sys.executable, *flags, "-c", code], env=env, capture_output=True, text=True, check=True).stdout
+           for flags in ([], ["-O"])]
+    assert out[0] == out[1] == "[(2, 3)] [0, 1, 3, 4] [0, 1, 2] 3\n"
