@@ -137,8 +137,9 @@ class PagePool:
                 self._note(self._cut, seq)
             table[i:i + 1] = [page]
         for seq, n in plan.lens.items():
-            self._lens[seq] = n
-            self._note(self._resized, seq)
+            if n != self._lens[seq]:
+                self._lens[seq] = n
+                self._note(self._resized, seq)
 
     def own(self, seqs: list[int], starts: list[int], ends: list[int], keep: bool = False) -> list[tuple[int, int]]:
         """Gives each sequence pages of its own for rows starts[i] .. ends[i] - 1 and
@@ -345,9 +346,10 @@ class PagedCache(PagePool):
             ops.cache_accept(self.k, self.v, table, step.lens,
                              self._tensor([p + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start)
             self._apply(plan)
-        for s, c, path in zip(step.seqs, ctx, paths):
+        for s, n, c, path in zip(step.seqs, step.counts, ctx, paths):
             self.trim(s, c + len(path))
-            self._note(self._resized, s)  # (a step is accepted once, also where the whole of it is)
+            if n:  # (once, also where the whole of it is accepted)
+                self._note(self._resized, s)
 
     def compact(self) -> list[tuple[int, int]]:
         """Moves the pages in use to the lowest ids, so that the others are one

@@ -183,8 +183,7 @@ def test_accept_copies_no_page_that_it_only_reads(monkeypatch):
     # a path whose rows end where they begin needs no page at all
     step = cache.step([f], [0])
     cache.accept(step, [[]])
-    with pytest.raises(ValueError):
-        cache.accept(step, [[]])
+    assert (cache.length(f), cache.free_pages()) == (12, 0)
 
 
 @pytest.mark.gpu
@@ -241,3 +240,17 @@ def test_books_need_no_assertions():
     out = [subprocess.run([sys.executable, *flags, "-c", code], env=env, capture_output=True, text=True, check=True).stdout
            for flags in ([], ["-O"])]
     assert out[0] == out[1] == "[(2, 3)] [0, 1, 3, 4] [0, 1, 2] 3\n"
+
+
+def test_a_step_that_brings_a_sequence_nothing_leaves_its_draft_open():
+    """Drafted nodes are accepted after a step of the batch in which their sequence had no rows."""
+    cache = make_cache()
+    a, b = cache.add(), cache.add()
+    draft = cache.step([a], [5])
+    other = cache.step([a, b], [0, 3])
+    stands(cache, draft)
+    cache.accept(other, [[], [0, 1]])
+    stands(cache, draft)
+    cache.accept(draft, [[0, 1]])
+    assert (cache.length(a), cache.length(b)) == (2, 2)
+    refused(cache, draft, "accept", "append", "attention_into")
