@@ -27,7 +27,7 @@
 // random 8 KB reach 6.8).  Tiles of 128 rows (prompts, large trees) are bound by
 // the matrix cores and the exps beside them: four wavefronts share key tiles
 // that the buffer unit copies to LDS three steps ahead (32 x 16384 x 128, 8 K/V
-// heads, window 4096, fp16: 1.04-1.10 ms on different boxes, 0.87-0.93 PFLOP/s,
+// heads, window 4096, fp16: 1.04-1.10 ms on different cards, 0.87-0.93 PFLOP/s,
 // where the library's 8192^3 product runs at 1.16-1.19).  fp32, and pages that are no multiple of 16 rows, go
 // through VGPRs in both.
 //

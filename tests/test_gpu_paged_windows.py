@@ -74,3 +74,45 @@ def test_masks_under_a_window(dtype, window, sinks):
             rows = slice(b.starts[s], b.starts[s + 1])
             err = float((out[rows].float() - chunk[rows].float()).abs().max())
             assert err <= 2 * TOL[dtype] * float(b.vc.float().abs().max())
+
+
+def test_captured_step_of_a_deep_tree():
+    """A layer's calls for a tree deeper than the window, captured once and
+    replayed over other rows, with eager calls between."""
+    from nkilab.cache import PagedCache
+
+    cache = PagedCache(40, 2, 64, layers=2, page_size=16, dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(61)
+    r = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()  # noqa: E731
+    cache.k.zero_()
+    cache.v.zero_()
+    a, b = cache.add(), cache.add()
+    cache.step([a, b], [30, 5])
+    step = cache.step([a, b], [12, 7], tree=[list(range(-1, 11)), [-1, 0, 0, 1, 3, 4, 5]])
+    k, v, q = r(19, 2, 64), r(19, 2, 64), r(19, 4, 64)
+    o = torch.empty_like(q)
+
+    def layer(i):
+        turned = torch.empty_like(q)
+        cache.append(i, step, k, v, q, turned, 10000.0)
+        cache.attention_into(i, step, turned, o, window=4, sinks=8)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        layer(0)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        layer(0)
+    for _ in range(4):
+        for t in (k, v, q):
+            t.copy_(r(*t.shape))
+        cache.k[0, :, :, 3], cache.v[0, :, :, 3] = r(40, 2, 64), r(40, 2, 64)
+        cache.k[1], cache.v[1] = cache.k[0], cache.v[0]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = o.clone()
+        layer(1)
+        assert torch.equal(got, o) and torch.equal(cache.k[0], cache.k[1])
