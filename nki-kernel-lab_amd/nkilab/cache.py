@@ -338,7 +338,7 @@ class PagedCache(PagePool):
             plan = self._plan(step.seqs, [c + m for c, m in zip(ctx, stay)], [c + len(p) for c, p in zip(ctx, paths)],
                               keep=True)
             plan.lens = dict(zip(step.seqs, lens))  # (until the others are dropped)
-            if plan.copies:  # forked since the step
+            if plan.copies or any(self._cut[s] != at for s, at in zip(step.seqs, step.cut)):  # forked since the step
                 self._copy(plan.copies)
                 rows = self._planned(plan)
                 table = self._tensor([rows[s] + [-1] * (table.shape[1] - len(rows[s])) for s in step.seqs])

@@ -254,3 +254,20 @@ def test_a_step_that_brings_a_sequence_nothing_leaves_its_draft_open():
     cache.accept(draft, [[0, 1]])
     assert (cache.length(a), cache.length(b)) == (2, 2)
     refused(cache, draft, "accept", "append", "attention_into")
+
+
+def test_accept_moves_rows_where_they_are_now(monkeypatch):
+    """A sequence that was given pages of its own since the step: its table of now counts."""
+    from nkilab import ops
+
+    cache = make_cache()
+    cache._copy = lambda copies: None
+    tables = []
+    monkeypatch.setattr(ops, "cache_accept", lambda k, v, table, lens, paths, **kw: tables.append(table.tolist()))
+    a = cache.add()
+    step = cache.step([a], [6])
+    f = cache.fork(a)
+    assert cache.own([a], [0], [6], keep=True) == [(0, 2), (1, 3)]
+    refused(cache, step, "append", "attention_into")
+    cache.accept(step, [[1, 3]])
+    assert tables == [[[2, 3]]] and cache.pages_of(f) == [0, 1]
