@@ -78,8 +78,9 @@ class PagePool:
     def fork(self, seq: int) -> int:
         """A sequence with the same rows, in the same pages until either writes (rows
         that a step has yet to bring are copied as they are)."""
+        table = list(self._tables[seq])
         new = self.add()
-        self._tables[new], self._lens[new] = list(self._tables[seq]), self._lens[seq]
+        self._tables[new], self._lens[new] = table, self._lens[seq]
         self._floor[new] = self._floor[seq]
         for p in self._tables[new]:
             if p >= 0:

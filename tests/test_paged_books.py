@@ -271,3 +271,12 @@ def test_accept_moves_rows_where_they_are_now(monkeypatch):
     refused(cache, step, "append", "attention_into")
     cache.accept(step, [[1, 3]])
     assert tables == [[[2, 3]]] and cache.pages_of(f) == [0, 1]
+
+
+def test_a_fork_of_no_sequence_adds_none():
+    cache = make_cache()
+    a = cache.add()
+    before = books(cache)
+    with pytest.raises(KeyError):
+        cache.fork(a + 1)
+    assert books(cache) == before and cache.add() == a + 1
