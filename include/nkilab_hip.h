@@ -395,6 +395,32 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
              void* stream);
 
 /*
+ * Rotary embedding from a table: pair i < pairs of a row at position t rotates
+ * by t freq[i] radians (|freq| <= 1, in 64 bits), scaled by `magnitude`: elements
+ * (i, i + pairs) of a head, or (2 i, 2 i + 1) interleaved.  A HOST structure,
+ * read before the call returns.
+ */
+#define NKL_ROTARY_PAIRS 128
+typedef struct {
+  int pairs, interleaved;
+  double magnitude;
+  double freq[NKL_ROTARY_PAIRS];
+} nkl_rotary;
+
+/*
+ * x [H, S, d] rotated into y (strides of heads and rows, elements together):
+ * row s at positions[s] (int32, or int64 with positions64; null: pos0 + s),
+ * positions within 2^31.  Elements past the 2 * pairs first of a head are
+ * copied.  transposed: by -angle, which takes the gradient of y to x's.  y may be
+ * x, with its strides.  Angles in 64 bits, products in fp32, one rounding per
+ * output.  Does not depend on, or replace, nkl_rope's fp32 angles.
+ */
+int nkl_rotary_apply(const nkl_rotary* rotary, const void* x, void* y, int H,
+                     int S, int d, long x_sh, long x_ss, long y_sh, long y_ss,
+                     const void* positions, int positions64, long pos0,
+                     int transposed, int dtype, void* stream);
+
+/*
  * ---- The paged cache.  No counterpart in the reference, whose block has no
  * cache (nkilab/model.py:59-67 attends over one prompt).
  *

@@ -35,6 +35,10 @@ class PagedCacheDesc(ctypes.Structure):
 pack_cache = struct.Struct("@PPqqqqqqPqPP9i").pack
 _cache_p = _vp
 
+ROTARY_PAIRS = 128
+# nkl_rotary: pairs, interleaved, magnitude, frequencies.
+pack_rotary = struct.Struct(f"@2id{ROTARY_PAIRS}d").pack
+
 # name -> (restype, argtypes); mirrors include/nkilab_hip.h one for one.
 SIGNATURES = {
     "nkl_abi_version": (_c_int, []),
@@ -75,6 +79,8 @@ SIGNATURES = {
                                          _c_int, _vp]),
     "nkl_rope": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_long, _c_long, _c_long, _c_long, _c_int, _c_float,
                           _c_int, _vp]),
+    "nkl_rotary_apply": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_long, _c_long, _c_long, _c_long, _vp, _c_int,
+                                  _c_long, _c_int, _c_int, _vp]),
     "nkl_flash_attn_configure": (_c_int, [_c_int, _c_int, _c_int, _c_int]),
     "nkl_flash_attn_configure_polls": (_c_int, [_c_int]),
     "nkl_flash_attn_plan_check": (_c_int, [_c_int, _c_int, _c_int, _c_int, _vp]),

@@ -282,6 +282,116 @@ def rope(x, base: float = 10000.0, pos0: int = 0):
     return from_device(rope_into(tx, y, base, pos0), kind)
 
 
+@dataclass(frozen=True)
+class Rotary:
+    """How the elements of a head rotate with their position: pair i of the
+    first `dim` elements by position * frequency(i), which is base^(-2 i / dim)
+    unless scaled.  Pairs are (i, i + dim / 2), or (2 i, 2 i + 1) interleaved.
+
+    scaling, for contexts `factor` times as long as the `original` one (in
+    positions) that a model was trained for:
+      "linear"  every frequency divided by factor;
+      "base"    the base times factor^(dim / (dim - 2)): the lowest frequency
+                divided by factor, the highest kept;
+      "parts"   the pairs that turn more than high_turns (32) times over the
+                original context kept, those that turn less than low_turns (1)
+                times divided by factor, a linear ramp over the pairs' numbers
+                between; the rotated elements times 0.1 ln(factor) + 1;
+      "bands"   the same with the ramp over the turns themselves (high_turns
+                4), and no factor of the elements.
+    magnitude replaces the factor of the rotated elements.
+
+    An object is made once and kept: it holds its table of frequencies."""
+    dim: int
+    base: float = 10000.0
+    interleaved: bool = False
+    scaling: str | None = None
+    factor: float = 1.0
+    original: int = 0
+    low_turns: float | None = None
+    high_turns: float | None = None
+    magnitude: float | None = None
+
+    def __post_init__(self):
+        dim, base, factor = self.dim, float(self.base), float(self.factor)
+        if dim < 2 or dim % 2 or dim > 2 * _lib.ROTARY_PAIRS:
+            raise ValueError(f"Rotary: dim={dim} must be even, within [2, {2 * _lib.ROTARY_PAIRS}]")
+        if not (1.0 < base < math.inf):
+            raise ValueError(f"Rotary: base={self.base} must be above 1")
+        if self.scaling not in (None, "linear", "base", "parts", "bands"):
+            raise ValueError(f"Rotary: scaling {self.scaling!r}; one of 'linear', 'base', 'parts', 'bands' expected")
+        if not (1.0 <= factor < math.inf) or (self.scaling is None and factor != 1.0):
+            raise ValueError(f"Rotary: factor={self.factor} must be at least 1 (and 1 without scaling)")
+        freq = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+        magnitude = 1.0
+        if self.scaling == "linear":
+            freq = [f / factor for f in freq]
+        elif self.scaling == "base" and dim > 2:
+            stretched = base * factor ** (dim / (dim - 2))
+            freq = [stretched ** (-2.0 * i / dim) for i in range(dim // 2)]
+        elif self.scaling in ("parts", "bands"):
+            low = 1.0 if self.low_turns is None else float(self.low_turns)
+            high = (32.0 if self.scaling == "parts" else 4.0) if self.high_turns is None else float(self.high_turns)
+            if self.original < 1 or not (0.0 < low < high < math.inf):
+                raise ValueError(f"Rotary: scaling {self.scaling!r} needs the original context ({self.original}) and "
+                                 f"0 < low_turns ({low}) < high_turns ({high})")
+            if self.scaling == "parts":
+                def pair(turns):  # the (fractional) number of the pair that turns so often
+                    return dim * math.log(self.original / (2 * math.pi * turns)) / (2 * math.log(base))
+
+                first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), dim - 1)
+                kept = [1 - min(1.0, max(0.0, (i - first) / max(last - first, 0.001))) for i in range(dim // 2)]
+                magnitude = 0.1 * math.log(factor) + 1
+            else:
+                kept = [min(1.0, max(0.0, (self.original * f / (2 * math.pi) - low) / (high - low))) for f in freq]
+            freq = [f * k + f / factor * (1 - k) for f, k in zip(freq, kept)]
+        if self.magnitude is not None:
+            magnitude = float(self.magnitude)
+            if not math.isfinite(magnitude):
+                raise ValueError(f"Rotary: magnitude={self.magnitude}")
+        object.__setattr__(self, "frequencies", tuple(freq))
+        object.__setattr__(self, "gain", magnitude)
+        object.__setattr__(self, "_packed", _lib.pack_rotary(dim // 2, int(self.interleaved), magnitude, *freq,
+                                                             *([0.0] * (_lib.ROTARY_PAIRS - dim // 2))))
+
+
+def rotary_into(x: torch.Tensor, y: torch.Tensor, rotary: Rotary, positions: torch.Tensor | None = None, pos0: int = 0,
+                grad: bool = False) -> torch.Tensor:
+    """x [H, S, d] rotated into y (which may be x) as `rotary` says: row s by
+    positions[s] (int32 or int64 [S], within 2^31) or pos0 + s.  Elements past
+    rotary.dim are copied.  Any strides along H and S; d contiguous.
+    grad: the transposed map, which takes the gradient of y (as x) to x's."""
+    fn = "rotary_into"
+    if x.dim() != 3 or y.shape != x.shape or x.dtype != y.dtype:
+        raise ValueError(f"{fn}: x {tuple(x.shape)} {x.dtype} and y {tuple(y.shape)} {y.dtype} must be equal [H, S, d]")
+    H, S, d = x.shape
+    sx, sy = x.stride(), y.stride()
+    if d > 1 and (sx[2] != 1 or sy[2] != 1):
+        raise ValueError(f"{fn}: the head dim must be contiguous")
+    wide = 0
+    if positions is not None:
+        if positions.shape != (S,) or positions.dtype not in (torch.int32, torch.int64) or (S > 1 and positions.stride(0) != 1):
+            raise ValueError(f"{fn}: positions must be int32 or int64 [{S}] with unit stride, got {positions.dtype} "
+                             f"{list(positions.shape)}")
+        if pos0:
+            raise ValueError(f"{fn}: either positions or pos0")
+        wide = int(positions.dtype is torch.int64)
+    _on_current_device(fn, x, y, positions)
+    rc = _lib.lib().nkl_rotary_apply(rotary._packed, x.data_ptr(), y.data_ptr(), H, S, d, sx[0], sx[1], sy[0], sy[1],
+                                     ptr(positions), wide, int(pos0), int(grad), dtype_code(x.dtype), stream_handle())
+    if rc:
+        _lib.check("nkl_rotary_apply", rc)
+    return y
+
+
+def rotary(x, rotary: Rotary, positions=None, pos0: int = 0, grad: bool = False):
+    """``rotary_into`` a new array of x's kind (NumPy or torch; positions too)."""
+    tx, kind = to_device(x)
+    if positions is not None and not (isinstance(positions, torch.Tensor) and positions.is_cuda):
+        positions = torch.as_tensor(positions).to(tx.device)
+    return from_device(rotary_into(tx, torch.empty_like(tx), rotary, positions, pos0, grad), kind)
+
+
 # ------------------------------------------------------------- row ops --
 
 def _as_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
