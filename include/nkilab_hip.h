@@ -395,6 +395,31 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
              void* stream);
 
 /*
+ * y[M, N] = x[M, K] W^T (+ residual) for 4-bit weights, W[n, k] = s[n, g] (q[n, k]
+ * - z[n, g]) with g = k / group (32, 64 or a multiple of 128 columns).  Sums in
+ * fp32, weights never rounded, one rounding per output.
+ *
+ * packed: tiles of 16 rows x 128 columns in the order [ceil(N / 16)][ceil(K / 128)],
+ * 1 KB each: bytes 16 l + 4 s .. + 3 (l < 64, s < 4) are a little-endian word with
+ * the codes of row l % 16, columns 32 s + 8 (l / 16) + j, j < 8: j = 0, 2, 4, 6 in
+ * its lower half's nibbles from the lowest up, 1, 3, 5, 7 in its upper half's.
+ * Rows and columns past N and K are there, with any codes.
+ * scales: [ceil(N / 16)][G][16], G = the groups of ceil(K / 128) * 128 columns for
+ * groups below 128, else ceil(K / group); scales of rows past N are 0 or any
+ * finite number.  zeros: the same in bytes (0 .. 15), or null: 8 throughout.
+ * glu: y = silu(x Wg^T) * (x Wu^T), tiles alternate between Wg and Wu (2 ceil(N /
+ * 16) of them; scales and zeros likewise); the products are not rounded between.
+ *
+ * x, y, residual: rows of elements together (ldx, ldy, ldr elements apart).  dt:
+ * x's dtype; dt_scale, dt_out (y and residual): dt or NKL_F32.  y may be the
+ * residual.  A row of x with an infinity or NaN gives NaN.  No workspace.
+ */
+int nkl_gemm_w4(const void* x, const void* packed, const void* scales,
+                const void* zeros, void* y, const void* residual, int M, int N,
+                int K, int group, long ldx, long ldy, long ldr, int glu, int dt,
+                int dt_scale, int dt_out, void* stream);
+
+/*
  * Rotary embedding from a table: pair i < pairs of a row at position t rotates
  * by t freq[i] radians (|freq| <= 1, in 64 bits), scaled by `magnitude`: elements
  * (i, i + pairs) of a head, or (2 i, 2 i + 1) interleaved.  A HOST structure,

@@ -258,6 +258,159 @@ def stack_k(w: torch.Tensor) -> torch.Tensor:
     return torch.cat((w, w), dim=1).contiguous()
 
 
+# ------------------------------------------------------- 4-bit weights --
+
+@dataclass(frozen=True)
+class W4Weight:
+    """A weight [n, k] in 4 bits as the kernels take it (``pack_w4``): W[n, k] =
+    scale[n, g] * (code[n, k] - zero[n, g]), g = k // group.  paired: a gate and
+    an up weight, both [n, k] (``pair_w4``)."""
+    packed: torch.Tensor         # int32 [tiles of 16 rows, chunks of 128 columns, 64, 4]
+    scales: torch.Tensor         # [tiles, groups, 16]
+    zeros: torch.Tensor | None   # uint8 [tiles, groups, 16]; None: 8 throughout
+    n: int
+    k: int
+    group: int
+    paired: bool = False
+
+
+def _w4_group(fn: str, group: int) -> None:
+    if group not in (32, 64) and (group < 128 or group % 128):
+        raise ValueError(f"{fn}: group={group}; 32, 64 or a multiple of 128 columns expected")
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, group: int = 128) -> W4Weight:
+    """Lays out 4-bit codes (uint8 [N, K], 0 .. 15) with a scale for each row and
+    `group` columns (fp32, bf16 or fp16 [N, ceil(K / group)]) and zeros (the
+    codes that stand for 0: uint8, as scales; None: 8).  Once per weight."""
+    fn = "pack_w4"
+    _w4_group(fn, group)
+    if codes.dim() != 2 or codes.dtype is not torch.uint8 or 0 in codes.shape:
+        raise ValueError(f"{fn}: codes must be uint8 [N, K], got {codes.dtype} {list(codes.shape)}")
+    N, K = codes.shape
+    G = -(-K // group)
+    dtype_code(scales.dtype)
+    if scales.shape != (N, G) or (zeros is not None and (zeros.shape != (N, G) or zeros.dtype is not torch.uint8)):
+        raise ValueError(f"{fn}: scales {list(scales.shape)} and zeros (uint8) must be [{N}, {G}]")
+    if int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
+        raise ValueError(f"{fn}: codes and zeros must lie within 0 .. 15")
+    Nt, Kc = -(-N // 16), -(-K // 128)
+    c = torch.nn.functional.pad(codes, (0, 128 * Kc - K, 0, 16 * Nt - N))
+    # [tile, row, chunk, word, lane group, code] -> [tile, chunk, lane group, row, word, code]
+    c = c.view(Nt, 16, Kc, 4, 4, 8).permute(0, 2, 4, 1, 3, 5).reshape(Nt, Kc, 64, 4, 8)
+    words = torch.zeros((Nt, Kc, 64, 4), dtype=torch.int64, device=c.device)
+    for j in range(8):
+        words |= c[..., j].to(torch.int64) << (4 * (j // 2) + 16 * (j % 2))
+    words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    groups = Kc * (128 // group) if group < 128 else G
+    tiles = lambda t: (torch.nn.functional.pad(t, (0, groups - G, 0, 16 * Nt - N))  # noqa: E731
+                       .view(Nt, 16, groups).transpose(1, 2).contiguous())
+    return W4Weight(words, tiles(scales), None if zeros is None else tiles(zeros), N, K, group)
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype | None = None) -> W4Weight:
+    """A weight [N, K] in 4 bits: each row's groups scaled so that their largest
+    values keep their places (with zeros: their least and largest), and rounded
+    to the nearest code.  Scales of scale_dtype (w's)."""
+    fn = "quantize_w4"
+    _w4_group(fn, group)
+    if w.dim() != 2 or 0 in w.shape:
+        raise ValueError(f"{fn}: w {tuple(w.shape)} must be [N, K]")
+    N, K = w.shape
+    sdt = w.dtype if scale_dtype is None else scale_dtype
+    dtype_code(sdt)
+    G = -(-K // group)
+    x = torch.nn.functional.pad(w.detach().float(), (0, G * group - K)).view(N, G, group)
+    hi, lo = x.amax(dim=2).clamp(min=0), x.amin(dim=2).clamp(max=0)
+    s = (hi - lo) / 15 if zeros else torch.maximum(hi / 7, lo / -8)
+    s = torch.where(s > 0, s, torch.ones_like(s)).to(sdt)
+    sf = s.float().clamp(min=torch.finfo(sdt).tiny)  # (a scale that its type has none of holds zeros)
+    z = (-lo / sf).round().clamp(0, 15) if zeros else torch.full_like(sf, 8.0)
+    q = ((x / sf[:, :, None]).round() + z[:, :, None]).clamp(0, 15).to(torch.uint8)
+    return pack_w4(q.view(N, G * group)[:, :K], s, z.to(torch.uint8) if zeros else None, group)
+
+
+def pair_w4(gate: W4Weight, up: W4Weight) -> W4Weight:
+    """The weight that ``linear_w4_swiglu_into`` takes: the tiles of two weights
+    of one shape, group and scale dtype in turn."""
+    a, b = ((w.n, w.k, w.group, w.scales.dtype, w.zeros is None, w.paired) for w in (gate, up))
+    if a != b or gate.paired:
+        raise ValueError(f"pair_w4: weights of (n, k, group, scales' dtype, no zeros, paired) {a} and {b}")
+    mix = lambda s, t: torch.stack((s, t), dim=1).reshape(-1, *s.shape[1:])  # noqa: E731
+    return W4Weight(mix(gate.packed, up.packed), mix(gate.scales, up.scales),
+                    None if gate.zeros is None else mix(gate.zeros, up.zeros), gate.n, gate.k, gate.group, True)
+
+
+def unpack_w4(w: W4Weight) -> torch.Tensor:
+    """The values of an unpaired weight, fp32 [n, k]."""
+    if w.paired:
+        raise ValueError("unpack_w4: a pair of weights")
+    Nt, Kc = w.packed.shape[:2]
+    codes = torch.stack([(w.packed >> (4 * (j // 2) + 16 * (j % 2))) & 15 for j in range(8)], dim=-1)
+    codes = codes.view(Nt, Kc, 4, 16, 4, 8).permute(0, 3, 1, 4, 2, 5).reshape(16 * Nt, 128 * Kc)
+    spread = lambda t: (t.transpose(1, 2).reshape(16 * Nt, -1).float()  # noqa: E731
+                        .repeat_interleave(w.group, dim=1)[:, :128 * Kc][:w.n, :w.k])
+    return (codes[:w.n, :w.k].float() - (8.0 if w.zeros is None else spread(w.zeros))) * spread(w.scales)
+
+
+def _linear_w4(fn: str, a: torch.Tensor, w: W4Weight, c: torch.Tensor, residual: torch.Tensor | None) -> torch.Tensor:
+    sa, sc = a.shape, c.shape
+    if len(sa) != 2 or len(sc) != 2 or sa[1] != w.k or sc[0] != sa[0] or sc[1] != w.n:
+        raise ValueError(f"{fn}: a {tuple(sa)} and output {tuple(sc)} do not match a weight [{w.n}, {w.k}]")
+    M, K = sa
+    dt, ds, do = a.dtype, w.scales.dtype, c.dtype
+    if (ds is not dt and ds is not torch.float32) or (do is not dt and do is not torch.float32):
+        raise TypeError(f"{fn}: scales of {ds} and an output of {do} for activations of {dt}: theirs or float32 expected")
+    ta, tc = a.stride(), c.stride()
+    if M > 1 and tc[0] < w.n or w.n > 1 and tc[1] != 1:
+        raise ValueError(f"{fn}: the output must be a row-major [M, N] tensor")
+    if K > 1 and ta[1] != 1 or M > 1 and ta[0] < K:
+        a = a.contiguous()
+        ta = a.stride()
+    pr, ldr = None, 0
+    if residual is not None:
+        if residual.shape != sc or residual.dtype is not do:
+            raise ValueError(f"{fn}: residual {tuple(residual.shape)} {residual.dtype} does not match the output "
+                             f"{tuple(sc)} {do}")
+        if w.n > 1 and residual.stride(1) != 1 or M > 1 and residual.stride(0) < w.n:
+            residual = residual.contiguous()
+        pr, ldr = residual.data_ptr(), max(residual.stride(0), 0)
+    _on_current_device(fn, a, w.packed, c, residual)
+    zeros = w.zeros
+    rc = _lib.lib().nkl_gemm_w4(a.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(),
+                                None if zeros is None else zeros.data_ptr(), c.data_ptr(), pr, M, w.n, K, w.group,
+                                ta[0], tc[0], ldr, w.paired, dtype_code(dt), dtype_code(ds), dtype_code(do),
+                                stream_handle())
+    if rc:
+        _lib.check("nkl_gemm_w4", rc)
+    return c
+
+
+def linear_w4_into(a: torch.Tensor, w: W4Weight, c: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """c = a @ w^T (+ residual) for a 4-bit weight; a [M, k] of any of the three
+    dtypes, c [M, n] (which may be the residual) of a's or fp32, the weight's
+    scales likewise.  The weight's values are not rounded: sums are of codes
+    times a in fp32, scaled group by group, and rounded once.  A row of a with
+    an infinity or NaN gives NaN."""
+    if w.paired:
+        raise ValueError("linear_w4_into: a pair of weights; linear_w4_swiglu_into takes those")
+    return _linear_w4("linear_w4_into", a, w, c, residual)
+
+
+def linear_w4_swiglu_into(a: torch.Tensor, w: W4Weight, c: torch.Tensor) -> torch.Tensor:
+    """c = silu(a @ gate^T) * (a @ up^T) for ``pair_w4(gate, up)`` in one pass; the
+    products are not rounded between."""
+    if not w.paired:
+        raise ValueError("linear_w4_swiglu_into: pair_w4's weight expected")
+    return _linear_w4("linear_w4_swiglu_into", a, w, c, None)
+
+
+def linear_w4(a, w: W4Weight):
+    """a @ w^T in a new array of a's kind and dtype."""
+    t, kind = to_device(a)
+    return from_device(linear_w4_into(t, w, t.new_empty((t.shape[0], w.n))), kind)
+
+
 # ---------------------------------------------------------------- RoPE --
 
 def rope_into(x: torch.Tensor, y: torch.Tensor, base: float = 10000.0, pos0: int = 0) -> torch.Tensor:
