@@ -39,7 +39,7 @@ extern "C" {
 
 #define NKL_ABI_VERSION 2
 
-enum { NKL_F32 = 0, NKL_BF16 = 1, NKL_F16 = 2 };
+enum { NKL_F32 = 0, NKL_BF16 = 1, NKL_F16 = 2, NKL_E4M3 = 3 };
 
 enum {
   NKL_OK = 0,
@@ -569,6 +569,67 @@ int nkl_paged_attention(const nkl_paged_cache* cache, const void* q, void* o,
                         int window, int sinks, const void* tree, int tree_words,
                         float scale, void* workspace, size_t workspace_bytes,
                         void* stream);
+
+/*
+ * ---- The paged cache in 8 bits.
+ *
+ * cache->dtype NKL_E4M3: k and v hold OCP e4m3 codes (4 exponent and 3 fraction
+ * bits, no infinity), and scales an exponent byte s for each page and K/V head of
+ * each: row j's value is its code times 2^(s - 127), s < 255.  Codes' strides are
+ * multiples of 16 elements, their addresses of 16 bytes, d of 16.
+ */
+typedef struct {
+  unsigned char* k;
+  unsigned char* v;
+  long k_page, k_head, v_page, v_head;
+} nkl_cache_scales;
+
+/*
+ * nkl_cache_append with rotary a table (null: no rotation, then no q) and, for a
+ * cache of 8 bits, rows of dtype `dtype` taken to codes (others: dtype is the
+ * cache's, scales null).  Rows are rotated in 64 bits and rounded once.
+ * 8 bits: a page whose first rows these are gets the smallest exponent with
+ * which they stay within 448, s within 17 .. 246; one that holds rows before the
+ * new ones its own or, if that is larger, theirs, and its rows before are brought
+ * to it (rounded once where they become subnormal).  Codes are the nearest, ties
+ * to even.  Infinities and NaN become NaN and do not count for the exponent; what
+ * exceeds the largest exponent saturates.  Rows behind the new ones in their last
+ * page hold nothing of meaning afterwards.
+ */
+int nkl_cache_write(const nkl_paged_cache* cache, const nkl_cache_scales* scales,
+                    const void* k, const void* v, long k_row, long k_head,
+                    long v_row, long v_head, const void* q, void* q_out, int H,
+                    long q_row, long q_head, long qo_row, long qo_head,
+                    const void* tree, int tree_words, const nkl_rotary* rotary,
+                    int dtype, void* stream);
+
+/*
+ * nkl_cache_accept for a cache of 8 bits (paths of at most 1024 nodes; scales'
+ * layers k_scale_layer and v_scale_layer bytes apart): a page that rows move to
+ * gets the largest exponent of the pages they come from, and its own if it keeps
+ * rows before them; codes follow it.
+ */
+int nkl_cache_accept8(const nkl_paged_cache* cache, const nkl_cache_scales* scales,
+                      const int* paths, long path_row, int path_cols,
+                      int* new_lens, int layers, long k_layer, long v_layer,
+                      long k_scale_layer, long v_scale_layer, void* stream);
+
+/*
+ * nkl_paged_attention over a cache of 8 bits, for q and o of dtype `dtype`
+ * (strides in its elements, on 16 bytes): scores and sums are of the codes'
+ * values, taken to q's type -- exactly to bf16 and fp32 for exponent bytes 17 ..
+ * 246, to fp16 rounded where they leave its range of normal numbers, at most
+ * 65504 in magnitude.  The workspace's size depends on dtype too.
+ */
+size_t nkl_paged_attention8_workspace_bytes(const nkl_paged_cache* cache, int H,
+                                            int window, int sinks, int tree,
+                                            int dtype);
+int nkl_paged_attention8(const nkl_paged_cache* cache,
+                         const nkl_cache_scales* scales, int dtype,
+                         const void* q, void* o, int H, long q_row, long q_head,
+                         long o_row, long o_head, int window, int sinks,
+                         const void* tree, int tree_words, float scale,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -9,9 +9,9 @@
 
 namespace nkl {
 
-int cache_args(const char* fn, const nkl_paged_cache* c, bool needs_seqs, CacheArgs& a) {
+int cache_args(const char* fn, const nkl_paged_cache* c, bool needs_seqs, CacheArgs& a, bool e4m3) {
   if (!c) return set_error(NKL_EINVAL, "%s: null cache", fn);
-  if (c->dtype != NKL_F32 && c->dtype != NKL_BF16 && c->dtype != NKL_F16)
+  if (c->dtype != NKL_F32 && c->dtype != NKL_BF16 && c->dtype != NKL_F16 && !(e4m3 && c->dtype == NKL_E4M3))
     return set_error(NKL_EDTYPE, "%s: unsupported dtype %d", fn, c->dtype);
   if (c->pages < 0 || c->kv_heads < 1 || c->page_size < 1 || c->d < 1)
     return set_error(NKL_EINVAL, "%s: pages=%d kv_heads=%d page_size=%d d=%d", fn, c->pages, c->kv_heads, c->page_size,
@@ -487,7 +487,7 @@ int check_pairs(const int* pairs, int n, int pages) {
 extern "C" int nkl_cache_copy_pages(const nkl_paged_cache* cache, const int* pairs, int n, int layers, long k_layer,
                                     long v_layer, void* stream) {
   CacheArgs c;
-  if (const int rc = cache_args("nkl_cache_copy_pages", cache, false, c)) return rc;
+  if (const int rc = cache_args("nkl_cache_copy_pages", cache, false, c, true)) return rc;
   if (n < 0 || layers < 0 || k_layer < 0 || v_layer < 0)
     return set_error(NKL_EINVAL, "nkl_cache_copy_pages: negative n=%d, layers=%d or layer stride", n, layers);
   if (n == 0 || layers == 0) return NKL_OK;
@@ -538,6 +538,8 @@ extern "C" int nkl_cache_copy_pages(const nkl_paged_cache* cache, const int* pai
       copy_pages_kernel<u32x4><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
     else if (el == 4)
       copy_pages_kernel<unsigned><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
+    else if (el == 1)
+      copy_pages_kernel<unsigned char><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
     else
       copy_pages_kernel<unsigned short><<<grid, dim3(256), 0, (hipStream_t)stream>>>(p, layers);
     if (const int rc = check_launch("nkl_cache_copy_pages")) return rc;

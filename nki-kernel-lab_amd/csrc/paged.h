@@ -61,9 +61,9 @@ __device__ __forceinline__ int page_of(const CacheArgs& c, int b, int j, int& wi
 }
 
 // Host side: checks a cache description and fills CacheArgs (NKL_OK or a
-// status with the error set).
-int cache_args(const char* fn, const nkl_paged_cache* c, bool needs_seqs, CacheArgs& a);
+// status with the error set).  e4m3: a cache of 8 bits is taken too.
+int cache_args(const char* fn, const nkl_paged_cache* c, bool needs_seqs, CacheArgs& a, bool e4m3 = false);
 
-inline int elem_bytes(int dtype) { return dtype == NKL_F32 ? 4 : 2; }
+inline int elem_bytes(int dtype) { return dtype == NKL_F32 ? 4 : dtype == NKL_E4M3 ? 1 : 2; }
 
 }  // namespace nkl

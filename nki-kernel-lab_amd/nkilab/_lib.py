@@ -12,7 +12,7 @@ import struct
 LIB_NAME = "libnkilab_hip.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 GEMM_BLOCKED, GEMM_NAIVE = 0, 1
 EINVAL, EWORKSPACE = -1, -4
 ABI_VERSION = 2
@@ -34,6 +34,9 @@ class PagedCacheDesc(ctypes.Structure):
 # structure takes; null pointers are 0.  (Its parameter takes either.)
 pack_cache = struct.Struct("@PPqqqqqqPqPP9i").pack
 _cache_p = _vp
+
+# nkl_cache_scales as bytes.
+pack_scales = struct.Struct("@PPqqqq").pack
 
 ROTARY_PAIRS = 128
 # nkl_rotary: pairs, interleaved, magnitude, frequencies.
@@ -93,6 +96,13 @@ SIGNATURES = {
                                   _c_long, _c_long, _c_long, _vp, _c_int, _c_double, _vp]),
     "nkl_cache_copy_pages": (_c_int, [_cache_p, _vp, _c_int, _c_int, _c_long, _c_long, _vp]),
     "nkl_cache_accept": (_c_int, [_cache_p, _vp, _c_long, _c_int, _vp, _c_int, _c_long, _c_long, _vp]),
+    "nkl_cache_write": (_c_int, [_cache_p, _vp, _vp, _vp, _c_long, _c_long, _c_long, _c_long, _vp, _vp, _c_int, _c_long,
+                                 _c_long, _c_long, _c_long, _vp, _c_int, _vp, _c_int, _vp]),
+    "nkl_cache_accept8": (_c_int, [_cache_p, _vp, _vp, _c_long, _c_int, _vp, _c_int, _c_long, _c_long, _c_long, _c_long,
+                                   _vp]),
+    "nkl_paged_attention8_workspace_bytes": (_c_size, [_cache_p, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "nkl_paged_attention8": (_c_int, [_cache_p, _vp, _c_int, _vp, _vp, _c_int, _c_long, _c_long, _c_long, _c_long, _c_int,
+                                      _c_int, _vp, _c_int, _c_float, _vp, _c_size, _vp]),
     "nkl_tree_mask": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
     "nkl_tree_mask_window": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
     "nkl_paged_attention_workspace_bytes": (_c_size, [_cache_p, _c_int, _c_int, _c_int, _c_int]),

@@ -241,7 +241,8 @@ class CacheStep:
 
 
 class PagedCache(PagePool):
-    """K and V of every layer in pages, and the sequences they belong to."""
+    """K and V of every layer in pages, and the sequences they belong to.  dtype
+    torch.float8_e4m3fn: in 8 bits, with a scale for each page and head."""
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, layers: int = 1, page_size: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str | None = None):
@@ -250,11 +251,19 @@ class PagedCache(PagePool):
         device = torch.device("cuda") if device is None else device
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)
+        # In 8 bits: exponents of each layer's pages and heads (a page gets its
+        # own with its first rows).
+        self.k_scale = self.v_scale = None
+        if dtype is ops.E4M3:
+            self.k_scale, self.v_scale = (torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2))
         self._moved = 0
 
     def _copy(self, copies: list[tuple[int, int]]) -> None:
         if copies:
-            ops.cache_copy_pages(self.k, self.v, copies)
+            ops.cache_copy_pages(self.k, self.v, copies, self.k_scale, self.v_scale)
+
+    def _layer_scales(self, layer: int) -> dict:
+        return {} if self.k_scale is None else {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer]}
 
     def _tensor(self, rows) -> torch.Tensor:
         return torch.tensor(rows, dtype=torch.int32).to(self.k.device)
@@ -345,7 +354,8 @@ class PagedCache(PagePool):
                 table = self._tensor([rows[s] + [-1] * (table.shape[1] - len(rows[s])) for s in step.seqs])
             width = max(len(p) for p in paths)
             ops.cache_accept(self.k, self.v, table, step.lens,
-                             self._tensor([p + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start)
+                             self._tensor([p + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start,
+                             k_scale=self.k_scale, v_scale=self.v_scale)
             self._apply(plan)
         for s, n, c, path in zip(step.seqs, step.counts, ctx, paths):
             self.trim(s, c + len(path))
@@ -363,11 +373,11 @@ class PagedCache(PagePool):
         return list(moves.items())
 
     def append(self, layer: int, step: CacheStep, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
-               q_out: torch.Tensor | None = None, rope_base: float | None = None) -> None:
+               q_out: torch.Tensor | None = None, rope_base: float | None = None, rotary: ops.Rotary | None = None) -> None:
         """``ops.cache_append_into`` of the step's rows in a layer."""
         self._check("append", step)
         ops.cache_append_into(k, v, self.k[layer], self.v[layer], step.table, step.lens, step.q_start, step.max_q,
-                              step.tree, q, q_out, rope_base)
+                              step.tree, q, q_out, rope_base, rotary, **self._layer_scales(layer))
 
     def attention_into(self, layer: int, step: CacheStep, q: torch.Tensor, o: torch.Tensor, window: int | None = None,
                        sinks: int = 0, scale: float | None = None) -> torch.Tensor:
@@ -379,4 +389,4 @@ class PagedCache(PagePool):
         if tree is not None and window is not None and step.depth > window:
             tree = ops.tree_mask(step.parents, step.q_start, step.max_q, window=window, sinks=sinks, lens=step.lens)
         return ops.paged_attention_into(q, o, self.k[layer], self.v[layer], step.table, step.lens, step.q_start,
-                                        step.max_q, window, sinks, tree, scale)
+                                        step.max_q, window, sinks, tree, scale, **self._layer_scales(layer))

@@ -19,6 +19,7 @@ from __future__ import annotations
 import math
 import struct
 from dataclasses import dataclass
+from functools import lru_cache
 from itertools import chain
 
 import numpy as np
@@ -842,6 +843,32 @@ def attention(q, k, v, variant: str = "flash_pipelined", scale: float | None = N
 # ---------------------------------------------------------- paged cache --
 
 MAX_ROWS = 1 << 30  # rows a page table addresses at most, and new rows of a call
+E4M3 = torch.float8_e4m3fn  # codes of a cache in 8 bits
+
+
+def _cache_code(dt: torch.dtype) -> int:
+    return _lib.E4M3 if dt is E4M3 else dtype_code(dt)
+
+
+def _scales(fn: str, k_cache: torch.Tensor, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> bytes | None:
+    """The C ABI's description of the scales of a cache in 8 bits (None: of another), checked."""
+    if k_cache.dtype is not E4M3:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{fn}: scales belong to a cache of {E4M3}, this one is of {k_cache.dtype}")
+        return None
+    want = k_cache.shape[:-2]
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is None or t.dtype is not torch.uint8 or t.shape != want:
+            raise ValueError(f"{fn}: {name} must be uint8 {list(want)}, the exponents of a cache of {E4M3}; got "
+                             f"{None if t is None else (t.dtype, list(t.shape))}")
+    sk, sv = k_scale.stride(), v_scale.stride()
+    return _lib.pack_scales(k_scale.data_ptr(), v_scale.data_ptr(), sk[-2], sk[-1], sv[-2], sv[-1])
+
+
+@lru_cache(maxsize=64)
+def _rope(d: int, base: float) -> "Rotary":
+    """The table that a rotary base stands for."""
+    return Rotary(d, base)
 
 
 def _rows_ok(t: torch.Tensor, E: int) -> bool:
@@ -920,7 +947,7 @@ def _cache_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_tabl
     return _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
                            page_table.data_ptr() if cols else lens.data_ptr(),  # (no columns: any address, never read)
                            page_table.stride(0), lens.data_ptr(), pstart, pages, Hkv, page_size, d, cols, B, rows, max_q,
-                           dtype_code(k_cache.dtype)), shape, max_q
+                           _cache_code(k_cache.dtype)), shape, max_q
 
 
 def _tree_words(fn: str, tree: torch.Tensor | None, rows: int, max_q: int) -> tuple[int | None, int]:
@@ -980,7 +1007,8 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor | None = None, max_q:
 def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       page_table: torch.Tensor, lens: torch.Tensor, q_start: torch.Tensor | None = None,
                       max_q: int | None = None, tree: torch.Tensor | None = None, q: torch.Tensor | None = None,
-                      q_out: torch.Tensor | None = None, rope_base: float | None = None) -> None:
+                      q_out: torch.Tensor | None = None, rope_base: float | None = None, rotary: "Rotary | None" = None,
+                      k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
     """Writes new K and V rows (k, v: [rows, kv_heads, d]) to a paged cache
     (k_cache, v_cache: [pages, kv_heads, page_size, d], any strides, d
     contiguous), in one launch with their rotary embedding.
@@ -995,7 +1023,17 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     [rows, H, d] into q_out, which may be q): rotate-half layout, angles in 64
     bits.  tree (``tree_mask``'s words): a node's position is the context's
     length and its depth.  Sequences of one call must not share a page that
-    either writes."""
+    either writes.
+
+    rotary (in rope_base's place): any ``Rotary`` of the head, rows rotated in 64
+    bits and rounded once.
+
+    A cache in 8 bits (float8_e4m3fn, d and strides multiples of 16) takes rows
+    of any of the three dtypes, and k_scale and v_scale, uint8 [pages,
+    kv_heads]: a value is its code times 2^(scale - 127), the scale its page's and
+    head's.  A page gets the smallest scale with which its rows stay within
+    448; where that rises with the new rows, the codes of the rows before
+    them follow (rounded again only where they become subnormal)."""
     fn = "cache_append_into"
     ks = k.shape
     if len(ks) != 3 or ks != v.shape:
@@ -1005,8 +1043,11 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     if Hkv != shape[1] or d != shape[3]:
         raise ValueError(f"{fn}: k {tuple(ks)} must be [rows, kv_heads, d] of the caches {tuple(shape)}")
     dt = k.dtype
-    if v.dtype is not dt or k_cache.dtype is not dt:
+    scales = _scales(fn, k_cache, k_scale, v_scale)
+    if v.dtype is not dt or (scales is None and k_cache.dtype is not dt):
         raise TypeError(f"{fn}: k {dt}, v {v.dtype} and the caches {k_cache.dtype} must share a dtype")
+    if rotary is not None and rope_base is not None:
+        raise ValueError(f"{fn}: either rope_base or rotary")
     words, nwords = _tree_words(fn, tree, rows, max_new)
     base = 0.0
     if rope_base is not None:
@@ -1017,8 +1058,8 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     packed = d < 2 or (sk[2] == 1 and sv[2] == 1)
     H, sq, so, pq, po = 0, (0, 0, 1), (0, 0, 1), None, None
     if q is not None or q_out is not None:
-        if rope_base is None or q is None or q_out is None:
-            raise ValueError(f"{fn}: q, q_out and rope_base go together")
+        if (rope_base is None and rotary is None) or q is None or q_out is None:
+            raise ValueError(f"{fn}: q, q_out and rope_base or rotary go together")
         qs = q.shape
         if len(qs) != 3 or qs != q_out.shape or qs[0] != rows or qs[2] != d:
             raise ValueError(f"{fn}: q {tuple(qs)} and q_out {tuple(q_out.shape)} must be [{rows}, H, {d}]")
@@ -1031,6 +1072,17 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     if not packed:
         raise ValueError(f"{fn}: the head dim must be contiguous")
     _on_current_device(fn, k, v, k_cache, v_cache, page_table, lens, q_start, tree, q, q_out)
+    if scales is not None or rotary is not None:
+        if scales is not None:
+            _on_current_device(fn, k_scale, v_scale)
+        if rotary is None and rope_base is not None:
+            rotary = _rope(d, base)
+        rc = _lib.lib().nkl_cache_write(desc, scales, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1], pq, po, H,
+                                        sq[0], sq[1], so[0], so[1], words, nwords,
+                                        None if rotary is None else rotary._packed, dtype_code(dt), stream_handle())
+        if rc:
+            _lib.check("nkl_cache_write", rc)
+        return
     rc = _lib.lib().nkl_cache_append(desc, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1], pq, po, H, sq[0], sq[1],
                                      so[0], so[1], words, nwords, base, stream_handle())
     if rc:
@@ -1045,13 +1097,16 @@ def _layer_desc(fn: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple:
     return 1, 0, 0, shape, sk, sv
 
 
-def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs) -> None:
+def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs, k_scale: torch.Tensor | None = None,
+                     v_scale: torch.Tensor | None = None) -> None:
     """Copies pages of a cache ([pages, kv_heads, page_size, d], or with a
     leading axis of layers, in each): pairs is a list of (from, to) page ids on
     the host (or an integer array [n, 2]).  A page that is written twice, or
-    both read and written, is refused."""
+    both read and written, is refused.  Of a cache in 8 bits the scales
+    ([layers,] pages, kv_heads) are copied with it."""
     fn = "cache_copy_pages"
     layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
+    scales = _scales(fn, k_cache, k_scale, v_scale)
     if isinstance(pairs, torch.Tensor) and pairs.is_cuda:
         raise ValueError(f"{fn}: pairs are read on the host: a list, an array or a CPU tensor expected")
     try:  # (packed by struct: a thousand pairs in a third of the time that an array made of them takes)
@@ -1076,16 +1131,23 @@ def cache_copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs) -> Non
         low, high = int(view.min()), int(view.max())
     if low < 0 or high >= shape[0]:
         raise ValueError(f"{fn}: pages {low} .. {high} outside [0, {shape[0]})")
-    _on_current_device(fn, k_cache, v_cache)
+    _on_current_device(fn, k_cache, v_cache, k_scale, v_scale)
     desc = _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], 0, 0, 0, 0,
-                           *shape, 0, 0, 0, 0, dtype_code(k_cache.dtype))
+                           *shape, 0, 0, 0, 0, _cache_code(k_cache.dtype))
     rc = _lib.lib().nkl_cache_copy_pages(desc, ids, len(flat) // 2, layers, kl, vl, stream_handle())
+    if rc == 0 and scales is not None:  # the scales as a cache of one-byte rows
+        tk, tv = k_scale.stride(), v_scale.stride()
+        desc = _lib.pack_cache(k_scale.data_ptr(), v_scale.data_ptr(), tk[-2], tk[-1], 0, tv[-2], tv[-1], 0, 0, 0, 0, 0,
+                               shape[0], shape[1], 1, 1, 0, 0, 0, 0, _lib.E4M3)
+        rc = _lib.lib().nkl_cache_copy_pages(desc, ids, len(flat) // 2, layers, tk[0] if len(tk) == 3 else 0,
+                                             tv[0] if len(tv) == 3 else 0, stream_handle())
     if rc:
         _lib.check("nkl_cache_copy_pages", rc)
 
 
 def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
-                 paths: torch.Tensor, q_start: torch.Tensor | None = None, n_nodes: int | None = None) -> torch.Tensor:
+                 paths: torch.Tensor, q_start: torch.Tensor | None = None, n_nodes: int | None = None,
+                 k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Keeps the accepted path of each sequence's newest rows (the nodes of a
     drafted tree): row paths[b, i] of them moves to row i, in every layer of
     the caches ([layers,] pages, kv_heads, page_size, d), and the sequence's
@@ -1095,9 +1157,14 @@ def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
     strictly ascending nodes, ended by the first entry that is not (-1 by
     custom).  The nodes of each sequence: q_start (int32 [batch + 1]), or
     n_nodes for every one.  No other sequence may have a page that rows are
-    moved to (those that they come from are only read)."""
+    moved to (those that they come from are only read).
+
+    In a cache of 8 bits (with its scales, [layers,] pages, kv_heads; paths of at
+    most 1024 columns) a page that rows move to gets the largest scale of those
+    it then holds rows of, and its codes follow."""
     fn = "cache_accept"
     layers, kl, vl, shape, sk, sv = _layer_desc(fn, k_cache, v_cache)
+    scales = _scales(fn, k_cache, k_scale, v_scale)
     ts, ps = page_table.shape, paths.shape
     if len(ts) != 2 or len(ps) != 2:
         raise ValueError(f"{fn}: page_table {tuple(ts)} and paths {tuple(ps)} must have two axes")
@@ -1117,17 +1184,37 @@ def cache_accept(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
         rows = most * B
         if most < 0 or rows > MAX_ROWS:
             raise ValueError(f"{fn}: n_nodes={n_nodes} for {B} sequences")
-    _on_current_device(fn, k_cache, v_cache, page_table, lens, paths, q_start)
+    _on_current_device(fn, k_cache, v_cache, page_table, lens, paths, q_start, k_scale, v_scale)
     out = torch.empty((B,), dtype=torch.int32, device=lens.device)
     desc = _lib.pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
                            page_table.data_ptr() if ts[1] else lens.data_ptr(), page_table.stride(0), lens.data_ptr(),
                            pstart, *shape, ts[1], B, rows, most,
-                           dtype_code(k_cache.dtype))
-    rc = _lib.lib().nkl_cache_accept(desc, paths.data_ptr(), paths.stride(0), ps[1], out.data_ptr(), layers, kl, vl,
-                                     stream_handle())
+                           _cache_code(k_cache.dtype))
+    if scales is not None:
+        five = k_scale.dim() == 3
+        rc = _lib.lib().nkl_cache_accept8(desc, scales, paths.data_ptr(), paths.stride(0), ps[1], out.data_ptr(), layers, kl,
+                                          vl, k_scale.stride(0) if five else 0, v_scale.stride(0) if five else 0,
+                                          stream_handle())
+    else:
+        rc = _lib.lib().nkl_cache_accept(desc, paths.data_ptr(), paths.stride(0), ps[1], out.data_ptr(), layers, kl, vl,
+                                         stream_handle())
     if rc:
         _lib.check("nkl_cache_accept", rc)
     return out
+
+
+def _paged_attention8(desc: bytes, scales: bytes, q, sq, o, so, H: int, window: int, sinks: int, words: int | None,
+                      nwords: int, scale: float) -> None:
+    """nkl_paged_attention8 on operands already checked."""
+    L, st, dt = _lib.lib(), stream_handle(), dtype_code(q.dtype)
+    args = (desc, scales, dt, q.data_ptr(), o.data_ptr(), H, sq[0], sq[1], so[0], so[1], window, sinks, words, nwords, scale)
+    # (as below)
+    rc = L.nkl_paged_attention8(*args, None, 0, st)
+    if rc == _lib.EWORKSPACE:
+        nbytes = L.nkl_paged_attention8_workspace_bytes(desc, H, window, sinks, words is not None, dt)
+        rc = L.nkl_paged_attention8(*args, workspace(nbytes, q.device).data_ptr(), nbytes, st)
+    if rc:
+        _lib.check("nkl_paged_attention8", rc)
 
 
 def _paged_attention(desc: bytes, q, sq, o, so, H: int, window: int, sinks: int, words: int | None, nwords: int,
@@ -1148,7 +1235,8 @@ def _paged_attention(desc: bytes, q, sq, o, so, H: int, window: int, sinks: int,
 def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                          page_table: torch.Tensor, lens: torch.Tensor, q_start: torch.Tensor | None = None,
                          max_q: int | None = None, window: int | None = None, sinks: int = 0,
-                         tree: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+                         tree: torch.Tensor | None = None, scale: float | None = None, k_scale: torch.Tensor | None = None,
+                         v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of new tokens over a paged cache that holds their K and V rows
     already (``cache_append_into``), into o; q, o: [rows, H, d], H a multiple of
     the caches' kv_heads (query head h reads K/V head h // (H / kv_heads)).
@@ -1164,12 +1252,18 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
     they hold; pages that no row of the call sees are not read, and may have
     been freed.  Rows of o that belong to no sequence are left as they are.
     d a multiple of 8 (fp32: 4), at most 128; the caches' strides too, and
-    their first elements on 16 bytes; scale above 0; at most 65535 sequences."""
+    their first elements on 16 bytes; scale above 0; at most 65535 sequences.
+
+    A cache in 8 bits comes with k_scale and v_scale (``cache_append_into``); q
+    and o are of any of the three dtypes, d and the caches' strides multiples
+    of 16.  Codes' values are exact in bf16 and fp32; in fp16 those outside its
+    normal numbers are rounded, to 65504 at most."""
     fn = "paged_attention_into"
     qs = q.shape
     if len(qs) != 3 or o.shape != qs or o.dtype is not q.dtype:
         raise ValueError(f"{fn}: q {tuple(qs)} {q.dtype} and o {tuple(o.shape)} {o.dtype} must be equal [rows, H, d]")
-    if q.dtype is not k_cache.dtype:
+    scales = _scales(fn, k_cache, k_scale, v_scale)
+    if scales is None and q.dtype is not k_cache.dtype:
         raise TypeError(f"{fn}: q {q.dtype} and the caches {k_cache.dtype} must share a dtype")
     rows, H, d = qs
     desc, shape, max_new = _cache_desc(fn, k_cache, v_cache, page_table, lens, q_start, rows, max_q)
@@ -1179,13 +1273,16 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
     words, nwords = _tree_words(fn, tree, rows, max_new)
     if scale is None:
         scale = 1.0 / math.sqrt(d) if d else 1.0
-    _on_current_device(fn, q, o, k_cache, v_cache, page_table, lens, q_start, tree)
+    _on_current_device(fn, q, o, k_cache, v_cache, page_table, lens, q_start, tree, k_scale, v_scale)
     if max_new == 0:
         return o
     E = 16 // q.element_size()
     q = _rows_operand(q, E)
     out = o if _rows_ok(o, E) else o.clone(memory_format=torch.contiguous_format)
-    _paged_attention(desc, q, q.stride(), out, out.stride(), H, window, sinks, words, nwords, float(scale))
+    if scales is not None:
+        _paged_attention8(desc, scales, q, q.stride(), out, out.stride(), H, window, sinks, words, nwords, float(scale))
+    else:
+        _paged_attention(desc, q, q.stride(), out, out.stride(), H, window, sinks, words, nwords, float(scale))
     if out is not o:
         o.copy_(out)
     return o
@@ -1194,8 +1291,9 @@ def paged_attention_into(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     lens: torch.Tensor, q_start: torch.Tensor | None = None, max_q: int | None = None,
                     window: int | None = None, sinks: int = 0, tree: torch.Tensor | None = None,
-                    scale: float | None = None) -> torch.Tensor:
+                    scale: float | None = None, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_attention_into`` a new tensor (whose rows that belong to no
     sequence, if there are any, hold nothing of meaning)."""
     return paged_attention_into(q, torch.empty(q.shape, dtype=q.dtype, device=q.device), k_cache, v_cache, page_table,
-                                lens, q_start, max_q, window, sinks, tree, scale)
+                                lens, q_start, max_q, window, sinks, tree, scale, k_scale, v_scale)
