@@ -27,6 +27,11 @@ Differences from the reference's host glue, none of which changes the math:
   * ``BlockConfig(window=..., sinks=...)`` adds a sliding window with first
     tokens that stay visible, and ``nki_decode`` runs the block over a paged
     cache (nkilab.cache): single tokens, chunks of prompts, drafted trees;
+  * ``BlockConfig(rotary=ops.Rotary(...))`` rotates q and k by a table of
+    frequencies (either layout, part of the head, stretched contexts);
+  * ``weights=quantize_block(block)`` multiplies by 4-bit weights instead of
+    the block's own, and a cache of torch.float8_e4m3fn holds K and V in 8
+    bits: the two streams that bound a decode step;
   * ``compute_dtype="bfloat16"`` runs the block in bf16 with an fp32 residual
     stream (the GEMMs that feed the residual emit fp32).  The default keeps
     the reference's behaviour: everything in x's dtype.
@@ -67,6 +72,7 @@ class BlockConfig:
     rope_base: float | None = None  # rotary embedding of q and k (rotate-half layout)
     window: int | None = None       # sliding window: token i sees the keys j <= i with j > i - window or j < sinks
     sinks: int = 0                  # first tokens that stay visible under the window
+    rotary: ops.Rotary | None = None  # rotary embedding by a table of frequencies (in rope_base's place)
 
     @property
     def head_dim(self) -> int:
@@ -87,6 +93,19 @@ def rope_reference(x: torch.Tensor, base: float, pos0: int = 0) -> torch.Tensor:
     c, s = torch.cos(a), torch.sin(a)
     x1, x2 = x[..., :half].float(), x[..., half:].float()
     return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1).to(x.dtype)
+
+
+def rotary_reference(x: torch.Tensor, rotary: ops.Rotary, pos0: int = 0) -> torch.Tensor:
+    """``ops.rotary`` of x [..., S, d] in PyTorch, differentiable: the eager block's."""
+    S, n = x.shape[-2], rotary.dim
+    f = torch.tensor(rotary.frequencies, dtype=torch.float64, device=x.device)
+    a = (pos0 + torch.arange(S, dtype=torch.float64, device=x.device))[:, None] * f
+    c, s = (rotary.gain * torch.cos(a)).float(), (rotary.gain * torch.sin(a)).float()
+    h = x[..., :n].float()
+    x1, x2 = (h[..., 0::2], h[..., 1::2]) if rotary.interleaved else h.chunk(2, dim=-1)
+    y1, y2 = x1 * c - x2 * s, x2 * c + x1 * s
+    y = torch.stack((y1, y2), dim=-1).flatten(-2) if rotary.interleaved else torch.cat((y1, y2), dim=-1)
+    return torch.cat((y.to(x.dtype), x[..., n:]), dim=-1)
 
 
 class RMSNorm(nn.Module):
@@ -113,6 +132,9 @@ class DecoderBlock(nn.Module):
         self.norm2 = RMSNorm(d, cfg.eps)
         if cfg.n_heads % cfg.kv_heads:
             raise ValueError(f"BlockConfig: n_kv_heads={cfg.n_kv_heads} must divide n_heads={cfg.n_heads}")
+        if cfg.rotary is not None and (cfg.rope_base is not None or cfg.rotary.dim > cfg.head_dim):
+            raise ValueError(f"BlockConfig: rotary of {cfg.rotary.dim} elements for heads of {cfg.head_dim}, and "
+                             f"rope_base={cfg.rope_base}: either, within the head")
         self.wqkv = nn.Linear(d, d + 2 * cfg.kv_heads * cfg.head_dim, bias=False)
         self.wo = nn.Linear(d, d, bias=False)
         self.wg = nn.Linear(d, f, bias=False)
@@ -131,6 +153,8 @@ class DecoderBlock(nn.Module):
         k, v = (t.reshape(S, Hkv, hd).transpose(0, 1) for t in qkv[:, d:].chunk(2, dim=-1))
         if self.cfg.rope_base is not None:
             q, k = rope_reference(q, self.cfg.rope_base), rope_reference(k, self.cfg.rope_base)
+        if self.cfg.rotary is not None:
+            q, k = rotary_reference(q, self.cfg.rotary), rotary_reference(k, self.cfg.rotary)
         if Hkv != H:
             k, v = (t.repeat_interleave(H // Hkv, dim=0) for t in (k, v))
         if self.cfg.window is None:
@@ -209,6 +233,27 @@ def _stacked_weight(block: nn.Module, name: str, dev: torch.device) -> torch.Ten
     return t
 
 
+def quantize_block(block: DecoderBlock, group: int = 128, zeros: bool = False,
+                   device: torch.device | str = "cuda") -> dict[str, ops.W4Weight]:
+    """The block's projections in 4 bits (``ops.quantize_w4``; fp32 scales, which go
+    with every compute dtype), as ``nki_forward`` and ``nki_decode`` take them:
+    "wqkv", "wo", "gate_up" (``ops.pair_w4``) and "wd".  Made once; a user with
+    codes of their own packs them by ``ops.pack_w4`` under the same names."""
+    q = {n: ops.quantize_w4(_weight(block, n).detach().to(device), group, zeros, torch.float32)
+         for n in ("wqkv", "wo", "wg", "wu", "wd")}
+    return {"wqkv": q["wqkv"], "wo": q["wo"], "gate_up": ops.pair_w4(q["wg"], q["wu"]), "wd": q["wd"]}
+
+
+def _check_weights(fn: str, block: DecoderBlock, weights) -> None:
+    cfg = block.cfg
+    d, f = cfg.d_model, cfg.d_ff
+    want = {"wqkv": (d + 2 * cfg.kv_heads * cfg.head_dim, d, False), "wo": (d, d, False), "gate_up": (f, d, True),
+            "wd": (d, f, False)}
+    got = {n: (w.n, w.k, w.paired) for n, w in weights.items()}
+    if got != want:
+        raise ValueError(f"{fn}: 4-bit weights (n, k, paired) {got} for a block of {want}")
+
+
 def _split_forward(block: DecoderBlock, xt: torch.Tensor, attention_variant: str) -> torch.Tensor:
     """The block with fp32 activations and bf16-MFMA projections over hi/lo
     operand pairs (compute_dtype="split")."""
@@ -239,6 +284,9 @@ def _split_forward(block: DecoderBlock, xt: torch.Tensor, attention_variant: str
     if cfg.rope_base is not None:
         ops.rope_into(q, q, cfg.rope_base)
         ops.rope_into(k, k, cfg.rope_base)
+    if cfg.rotary is not None:
+        qk = _heads(qkv, 0, H + Hkv, hd)
+        ops.rotary_into(qk, qk, cfg.rotary)
     a = torch.empty((S, d), dtype=f32, device=dev)
     ops.attention_into(q, k, v, a.view(S, H, hd).transpose(0, 1), variant=attention_variant, window=cfg.window,
                        sinks=cfg.sinks)
@@ -257,7 +305,8 @@ def _split_forward(block: DecoderBlock, xt: torch.Tensor, attention_variant: str
     return out
 
 
-def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipelined", compute_dtype=None):
+def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipelined", compute_dtype=None,
+                weights: dict[str, ops.W4Weight] | None = None):
     """The same block with every heavy op on the HIP kernels (model.py:70-89).
 
     x: [S, d_model] as NumPy or torch (CPU or GPU); returns the same kind.
@@ -266,10 +315,16 @@ def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipeline
     dtype, "float16" (fp32 x only) for fp16 operands (within 1e-3 of the fp32
     block at bf16 cost), or "split" (fp32 x only) for fp32 activations with
     the projections on bf16 MFMA over hi/lo operand pairs.
+    weights: 4-bit weights (``quantize_block``) in place of the block's own; the
+    gate and up products are then not rounded before their SwiGLU.
     """
     cfg = block.cfg
     xt, kind = to_device(x)
+    if weights is not None:
+        _check_weights("nki_forward", block, weights)
     if compute_dtype == SPLIT:
+        if weights is not None:
+            raise ValueError("nki_forward: compute_dtype='split' has no 4-bit weights")
         if xt.dtype != torch.float32:
             raise ValueError("nki_forward: compute_dtype='split' needs an fp32 x")
         return from_device(_split_forward(block, xt, attention_variant), kind)
@@ -281,18 +336,24 @@ def nki_forward(block: DecoderBlock, x, attention_variant: str = "flash_pipeline
         if cfg.rope_base is not None:  # in place on the q and k columns of qkv
             ops.rope_into(q, q, cfg.rope_base)
             ops.rope_into(k, k, cfg.rope_base)
+        if cfg.rotary is not None:
+            qk = _heads(qkv, 0, H + Hkv, hd)
+            ops.rotary_into(qk, qk, cfg.rotary)
         ops.attention_into(q, k, v, _heads(a, 0, H, hd), variant=attention_variant, window=cfg.window, sinks=cfg.sinks)
 
-    return from_device(_forward(block, xt, _compute_dtype("nki_forward", xt.dtype, compute_dtype), attend), kind)
+    return from_device(_forward(block, xt, _compute_dtype("nki_forward", xt.dtype, compute_dtype), attend, weights), kind)
 
 
-def nki_decode(block: DecoderBlock, x, cache: PagedCache, step: CacheStep, layer: int = 0, compute_dtype=None):
+def nki_decode(block: DecoderBlock, x, cache: PagedCache, step: CacheStep, layer: int = 0, compute_dtype=None,
+               weights: dict[str, ops.W4Weight] | None = None):
     """The block over new tokens and a cache of the ones before them: x
     [step.rows, d_model] holds the new rows of the step's sequences one after
     another (single tokens, prompts, chunks of them, or drafted trees), whose K
     (rotated) and V rows go to `layer` of the cache, and which attend over it.
     A prompt in one step gives what nki_forward gives; compute_dtype as there
-    ("split" apart), and the cache's dtype is the compute dtype.  With a tree in
+    ("split" apart), and the cache's dtype is the compute dtype, or
+    torch.float8_e4m3fn (a prompt then gives what the rounded K and V rows do);
+    weights as there.  With a tree in
     the step a token sees the context and its ancestors (under a window those
     within it, and the sinks), and is at the context's length and its depth.  Every layer's call takes the same step."""
     cfg = block.cfg
@@ -304,19 +365,21 @@ def nki_decode(block: DecoderBlock, x, cache: PagedCache, step: CacheStep, layer
     H, hd, Hkv = cfg.n_heads, cfg.head_dim, cfg.kv_heads
     if n != step.rows:
         raise ValueError(f"nki_decode: x has {n} rows, the step {step.rows}")
-    if cache.k.dtype != cdt or cache.k.shape[2] != Hkv or cache.k.shape[4] != hd:
+    if weights is not None:
+        _check_weights("nki_decode", block, weights)
+    if (cache.k.dtype != cdt and cache.k.dtype is not ops.E4M3) or cache.k.shape[2] != Hkv or cache.k.shape[4] != hd:
         raise ValueError(f"nki_decode: a cache of {cache.k.dtype} [{cache.k.shape[2]} heads, {cache.k.shape[4]}] for "
                          f"{cdt} [{Hkv}, {hd}]")
 
     def attend(qkv: torch.Tensor, a: torch.Tensor) -> None:
         q, k, v = (_heads(qkv, c, h, hd).transpose(0, 1) for c, h in ((0, H), (d, Hkv), (d + Hkv * hd, Hkv)))
-        if cfg.rope_base is None:
+        if cfg.rope_base is None and cfg.rotary is None:
             cache.append(layer, step, k, v)
         else:  # q in place on its columns of qkv
-            cache.append(layer, step, k, v, q, q, cfg.rope_base)
+            cache.append(layer, step, k, v, q, q, cfg.rope_base, cfg.rotary)
         cache.attention_into(layer, step, q, a.view(n, H, hd), cfg.window, cfg.sinks)
 
-    return from_device(_forward(block, xt, cdt, attend), kind)
+    return from_device(_forward(block, xt, cdt, attend, weights), kind)
 
 
 def _compute_dtype(fn: str, rdt: torch.dtype, compute_dtype) -> torch.dtype:
@@ -329,9 +392,11 @@ def _compute_dtype(fn: str, rdt: torch.dtype, compute_dtype) -> torch.dtype:
     return cdt
 
 
-def _forward(block: DecoderBlock, xt: torch.Tensor, cdt: torch.dtype, attend) -> torch.Tensor:
+def _forward(block: DecoderBlock, xt: torch.Tensor, cdt: torch.dtype, attend,
+             weights: dict[str, ops.W4Weight] | None = None) -> torch.Tensor:
     """The block with operands of type cdt; attend(qkv, a) fills a [S, d_model]
-    with the attention of the projected rows qkv [S, d_model + 2 kv_heads hd]."""
+    with the attention of the projected rows qkv [S, d_model + 2 kv_heads hd].
+    weights: in 4 bits, checked."""
     cfg = block.cfg
     dev = xt.device
     S, d = xt.shape
@@ -340,25 +405,32 @@ def _forward(block: DecoderBlock, xt: torch.Tensor, cdt: torch.dtype, attend) ->
     def weight(n):
         return _device_param(block, n, _weight(block, n), cdt, dev)
 
+    def linear(a: torch.Tensor, n: str, out: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if weights is not None:
+            return ops.linear_w4_into(a, weights[n], out, residual)
+        return ops.linear_into(a, weight(n), out, residual)
+
     g1 = _device_param(block, "norm1", _weight(block, "norm1"), rdt, dev)
     g2 = _device_param(block, "norm2", _weight(block, "norm2"), rdt, dev)
 
     h = torch.empty((S, d), dtype=cdt, device=dev)
     ops.rmsnorm_into(xt, g1, h, cfg.eps)
     qkv = torch.empty((S, d + 2 * cfg.kv_heads * cfg.head_dim), dtype=cdt, device=dev)
-    ops.linear_into(h, weight("wqkv"), qkv)
+    linear(h, "wqkv", qkv)
     a = torch.empty((S, d), dtype=cdt, device=dev)
     attend(qkv, a)
     x1 = torch.empty((S, d), dtype=rdt, device=dev)
-    ops.linear_into(a, weight("wo"), x1, residual=xt)
+    linear(a, "wo", x1, xt)
     h2 = torch.empty((S, d), dtype=cdt, device=dev)
     ops.rmsnorm_into(x1, g2, h2, cfg.eps)
     act = torch.empty((S, cfg.d_ff), dtype=cdt, device=dev)
-    if cdt in (torch.bfloat16, torch.float16) and cfg.d_ff % ops.GATE_UP_GROUP == 0 and d % 8 == 0:
+    if weights is not None:
+        ops.linear_w4_swiglu_into(h2, weights["gate_up"], act)
+    elif cdt in (torch.bfloat16, torch.float16) and cfg.d_ff % ops.GATE_UP_GROUP == 0 and d % 8 == 0:
         # gate, up and SwiGLU in one GEMM over the packed weight (same values)
         ops.gemm_swiglu_into(h2, _packed_gate_up(block, dev, cdt), act)
     else:
         ops.gate_up_into(h2, weight("wg"), weight("wu"), act)
     out = torch.empty((S, d), dtype=rdt, device=dev)
-    ops.linear_into(act, weight("wd"), out, residual=x1)
+    linear(act, "wd", out, x1)
     return out

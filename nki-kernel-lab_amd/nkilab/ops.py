@@ -274,6 +274,20 @@ class W4Weight:
     group: int
     paired: bool = False
 
+    def __post_init__(self):
+        _w4_group("W4Weight", self.group)
+        Kc = -(-self.k // 128)
+        tiles = -(-self.n // 16) * (2 if self.paired else 1)
+        groups = Kc * (128 // self.group) if self.group < 128 else -(-self.k // self.group)
+        shapes = {"packed": (self.packed, torch.int32, (tiles, Kc, 64, 4)),
+                  "scales": (self.scales, self.scales.dtype, (tiles, groups, 16)),
+                  "zeros": (self.zeros, torch.uint8, (tiles, groups, 16))}
+        dtype_code(self.scales.dtype)
+        for name, (t, dt, shape) in shapes.items():
+            if t is not None and (t.shape != shape or t.dtype is not dt or not t.is_contiguous() or t.device != self.packed.device):
+                raise ValueError(f"W4Weight: {name} must be a contiguous {dt} {list(shape)} with the packed codes, got "
+                                 f"{t.dtype} {list(t.shape)} on {t.device}")
+
 
 def _w4_group(fn: str, group: int) -> None:
     if group not in (32, 64) and (group < 128 or group % 128):
