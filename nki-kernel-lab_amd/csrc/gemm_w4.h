@@ -158,19 +158,16 @@ __device__ __forceinline__ void w4_fragments(const W4Raw<T>& r, bf16x8 (&f)[W4Ac
     f[0] = __builtin_bit_cast(bf16x8, r.v[0]);
 }
 
-// Four rows' scales.
+// Four rows' scales as they lie.
 template <typename S>
-__device__ __forceinline__ void w4_scales(const S* p, float (&s)[4]) {
-  if constexpr (sizeof(S) == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
-  } else {
-    typedef S s4 __attribute__((ext_vector_type(4)));
-    const s4 v = *reinterpret_cast<const s4*>(p);
+struct W4Scales {
+  typedef S s4 __attribute__((ext_vector_type(4)));
+  s4 v;
+  __device__ __forceinline__ void get(float (&s)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = (float)v[i];
   }
-}
+};
 
 // Four outputs n .. n + 3 of row m, with the residual.
 template <typename O>
