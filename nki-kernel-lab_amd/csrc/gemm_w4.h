@@ -41,6 +41,7 @@ struct W4Args {
   long ldx, ldy, ldr;
   int M, N, K, chunks, groups;
   fsched::Div32 dv_gc;  // chunks of a group (groups of 128 and more)
+  int fold_shift;       // folds below 128 columns: log2 of those in a group
   int y_f32;            // y and the residual are fp32
   int tiles;            // tiles of 16 packed rows
   int whole;            // rows of y and of the residual begin on four elements' boundary
@@ -66,25 +67,24 @@ __device__ __forceinline__ floatx4 mma16_16b(bf16x8 a, bf16x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight codes as 16 + q.
+// Eight codes as 16 + q.  The two constants in registers (kept there by an empty
+// asm: as literals they would make two instructions of each and-or).
 template <bool H>
-__device__ __forceinline__ bf16x8 w4_operand(unsigned w) {
-  u32x4 r;
-  if constexpr (H) {
-    constexpr unsigned kMask = 0x03c003c0u, k16 = 0x4c004c00u;
-    r.x = ((w << 6) & kMask) | k16;
-    r.y = ((w << 2) & kMask) | k16;
-    r.z = ((w >> 2) & kMask) | k16;
-    r.w = ((w >> 6) & kMask) | k16;
-  } else {
-    constexpr unsigned kMask = 0x00780078u, k16 = 0x41804180u;
-    r.x = ((w << 3) & kMask) | k16;
-    r.y = ((w >> 1) & kMask) | k16;
-    r.z = ((w >> 5) & kMask) | k16;
-    r.w = ((w >> 9) & kMask) | k16;
+struct W4Decode {
+  unsigned mask = H ? 0x03c003c0u : 0x00780078u, k16 = H ? 0x4c004c00u : 0x41804180u;
+  __device__ __forceinline__ W4Decode() {
+    asm volatile("" : "+s"(mask));
+    asm volatile("" : "+v"(k16));
   }
-  return __builtin_bit_cast(bf16x8, r);
-}
+  __device__ __forceinline__ bf16x8 operator()(unsigned w) const {
+    u32x4 r;
+    r.x = ((w << (H ? 6 : 3)) & mask) | k16;
+    r.y = ((H ? w << 2 : w >> 1) & mask) | k16;
+    r.z = ((w >> (H ? 2 : 5)) & mask) | k16;
+    r.w = ((w >> (H ? 6 : 9)) & mask) | k16;
+    return __builtin_bit_cast(bf16x8, r);
+  }
+};
 
 template <bool H>
 __device__ __forceinline__ bf16x8 w4_ones() {
@@ -200,7 +200,7 @@ __device__ __forceinline__ void w4_store(const W4Args& p, int m, int n, const fl
 
 // Gate times sigmoid(gate) times up; far below zero the sigmoid's exponential
 // overflows to infinity and its reciprocal is zero.
-__device__ __forceinline__ float w4_swiglu(float g, float u) { return g / (1.0f + fast_exp2(-g * kLog2e)) * u; }
+__device__ __forceinline__ float w4_swiglu(float g, float u) { return silu(g) * u; }
 
 // One type's launches (gemm_w4_bf16.hip and so on).
 struct W4Plan {

@@ -75,6 +75,7 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
     if constexpr (kAhead) load_x(wid, x);
   }
   const bf16x8 ones = w4_ones<H>();
+  const W4Decode<H> decode;
   const floatx4 zero4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int c = wid; c < p.chunks; c += KW) {
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
     for (int s = 0; s < 4; ++s) {
       bf16x8 wf[NF];
 #pragma unroll
-      for (int nf = 0; nf < NF; ++nf) wf[nf] = w4_operand<H>(w[nf][s]);
+      for (int nf = 0; nf < NF; ++nf) wf[nf] = decode(w[nf][s]);
 #pragma unroll
       for (int mf = 0; mf < MF; ++mf) {
         bf16x8 xf[NS];
@@ -163,14 +164,28 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
 
 // LDS reads that the compiler does not track (it would make them wait for every
 // copy in flight): their results go through a wait before any use.
+template <int OFF>
 __device__ __forceinline__ bf16x8 w4_lds_b128(unsigned a) {
   bf16x8 r;
-  asm volatile("ds_read_b128 %0, %1" : "=v"(r) : "v"(a));
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF));
   return r;
 }
-template <int N>
-__device__ __forceinline__ void w4_lds_wait(bf16x8& x) {
-  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(x) : "i"(N));
+template <int FIRST, int STEP, int N, typename F>
+__device__ __forceinline__ void w4_static_for(F&& f) {
+  if constexpr (N > 0) {
+    f(std::integral_constant<int, FIRST>{});
+    w4_static_for<FIRST + STEP, STEP, N - 1>(f);
+  }
+}
+template <int OFF>
+__device__ __forceinline__ unsigned w4_lds_b32(unsigned a) {
+  unsigned r;
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF));
+  return r;
+}
+template <typename V>
+__device__ __forceinline__ void w4_lds_wait(V& x) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x));
 }
 
 // Many rows: a workgroup's four wavefronts, two by two, take BM rows of x by 128
@@ -180,12 +195,13 @@ __device__ __forceinline__ void w4_lds_wait(bf16x8& x) {
 // reads lie in banks of their own), and so are the eight tiles of W.  Bound by the matrix cores and the vector unit together: beside 16
 // MFMAs of 16 cycles and 4 of the row sums a step has 32 operations on codes,
 // and a group 128 on sums, of 4 cycles each.
-template <typename T, typename S, int MF, bool GLU, int FS, bool ZEROS>
+template <typename T, typename S, int MF, bool GLU, int FS>
 __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks, int nblocks, int per_xcd) {
   constexpr int NS = W4Act<T>::NS, NF = 4, GC = 4 / FS, EB = (int)sizeof(T);
   constexpr int BM = 32 * MF, ROWB = 128 * EB, XSTAGE = BM * ROWB, CPL = XSTAGE / 4096;  // copies a wavefront
   constexpr int STAGE = XSTAGE + 8 * 1024;                                               // x, then eight tiles of W
   constexpr int RPC = 1024 / ROWB, PPR = ROWB / 16;  // rows a copy, pieces a row
+  constexpr int XR = EB / 2;  // reads a fragment
   constexpr bool H = W4Act<T>::H;
   __shared__ __align__(1024) unsigned char smem[2 * STAGE];
   // Workgroups are dealt to the 8 XCDs in turn: each takes a stretch of the
@@ -233,31 +249,51 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
     }
   };
 
-  // (one base for all tiles of the wavefront: those past the last read the last's)
+  // (tiles past the last read the last's)
   unsigned sbase[NF];
 #pragma unroll
-  for (int nf = 0; nf < NF; ++nf) sbase[nf] = (unsigned)min(t0 + nf, p.tiles - 1) * p.groups * 16;
-  const S* const scales = reinterpret_cast<const S*>(p.scales);
+  for (int nf = 0; nf < NF; ++nf) sbase[nf] = (unsigned)min(t0 + nf, p.tiles - 1) * p.groups;
   floatx4 acc[MF][NF], accg[MF][NF], ax[MF];
 #pragma unroll
   for (int mf = 0; mf < MF; ++mf)
 #pragma unroll
     for (int nf = 0; nf < NF; ++nf) acc[mf][nf] = floatx4{0.f, 0.f, 0.f, 0.f};
   const bf16x8 ones = w4_ones<H>();
+  const W4Decode<H> decode;
   const floatx4 zero4 = {0.f, 0.f, 0.f, 0.f};
-  // This lane's piece of fragment (mf, step s): at xa[mf] ^ (s << 6) -- fp32: two
-  // of them, at ^ (s << 7) and ^ 16.
-  unsigned xa[MF];
-#pragma unroll
-  for (int mf = 0; mf < MF; ++mf) {
-    const int r = 16 * MF * wm + 16 * mf + l16;
-    xa[mf] = r * ROWB + (((EB == 4 ? 2 * lg : lg) ^ l16) << 4);
-  }
+  // This lane's piece of fragment (mf, step s): at (xa ^ (s << 6)) + 16 rows for
+  // each mf -- fp32: two of them, at ^ (s << 7) and ^ 16.
+  const unsigned xa = (16 * MF * wm + l16) * ROWB + (((EB == 4 ? 2 * lg : lg) ^ l16) << 4);
 
-  // (a group's scales, on their way while its steps run)
-  W4Scales<S> sc[NF];
-  unsigned zc[NF];
+  // Scales of a chunk's groups, and of the next chunk's first one: loaded before
+  // the copies of the next chunk, which a wait for them would else be one for.
+  W4Scales<S> sc[GC + 1][NF];
+  // Row sums of four folds, those of fold lg of them in this lane.
+  float xs[MF];
+#pragma unroll
+  for (int mf = 0; mf < MF; ++mf) xs[mf] = 0.f;
+  auto load_scales = [&](int f, W4Scales<S> (&to)[NF]) __attribute__((always_inline)) {
+    const int g = min(FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)f) : f >> p.fold_shift, p.groups - 1);
+    const unsigned mine = 4 * lg * (unsigned)sizeof(S);
+#pragma unroll
+    for (int nf = 0; nf < NF; ++nf)
+      to[nf] = *reinterpret_cast<const W4Scales<S>*>(p.scales + (size_t)(sbase[nf] + g) * (16 * sizeof(S)) + mine);
+  };
+  // A fold of tile nf: its fp32 sums, scaled, into the outputs; and its share of the row sums.
+  auto fold = [&](int nf, const W4Scales<S>& sx, bool mine) __attribute__((always_inline)) {
+    float sf[4];
+    sx.get(sf);
+#pragma unroll
+    for (int mf = 0; mf < MF; ++mf)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[mf][nf][i] = fmaf(sf[i], accg[mf][nf][i], acc[mf][nf][i]);
+    // (here: left until later, sums of several groups would wait in registers)
+#pragma unroll
+    for (int mf = 0; mf < MF; ++mf) asm volatile("" : "+v"(acc[mf][nf]));
+    if (nf < MF) xs[nf] = mine ? ax[nf][0] : xs[nf];
+  };
   copy(0);
+  load_scales(0, sc[0]);
 #pragma unroll 1
   for (int c = 0; c < p.chunks; ++c) {
     // This wavefront's copies are done, then every wavefront's; and none reads
@@ -267,83 +303,96 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     const bool more = c + 1 < p.chunks;
+#pragma unroll
+    for (int g = 1; g <= GC; ++g) load_scales(c * GC + g, sc[g]);
     if (more) copy(c + 1);
     const unsigned stage = lds0 + (c & 1) * STAGE;
-    constexpr int XR = EB / 2;  // reads a fragment
     bf16x8 xr[2][MF][XR];
     auto read_x = [&](int s, bf16x8 (&x)[MF][XR]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int mf = 0; mf < MF; ++mf)
-#pragma unroll
-        for (int k = 0; k < XR; ++k) x[mf][k] = w4_lds_b128((stage + xa[mf]) ^ ((s << (EB == 4 ? 7 : 6)) | (k << 4)));
+      for (int k = 0; k < XR; ++k) {
+        const unsigned a = (stage + xa) ^ ((s << (EB == 4 ? 7 : 6)) | (k << 4));
+        w4_static_for<0, 1, MF>([&](auto mf) { x[mf.value][k] = w4_lds_b128<mf.value * 16 * ROWB>(a); });
+      }
     };
-    read_x(0, xr[0]);
-    bf16x8 w[NF];
+    unsigned w[2][NF];
+    auto read_w = [&](auto s, unsigned (&to)[NF]) __attribute__((always_inline)) {
+      const unsigned a = stage + wn * NF * 1024 + lane * 16;
+      w4_static_for<0, 1, NF>([&](auto nf) { to[nf.value] = w4_lds_b32<XSTAGE + nf.value * 1024 + s.value * 4>(a); });
+    };
+    auto wait_step = [&](unsigned (&ws)[NF], bf16x8 (&x)[MF][XR]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int nf = 0; nf < NF; ++nf) w[nf] = w4_lds_b128(stage + XSTAGE + (wn * NF + nf) * 1024 + lane * 16);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (s % FS == 0) {
-        const int g = FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)c) : c * GC + s / FS;
-#pragma unroll
-        for (int nf = 0; nf < NF; ++nf) {
-          const unsigned at = sbase[nf] + g * 16;
-          sc[nf] = *reinterpret_cast<const W4Scales<S>*>(scales + at + 4 * lg);
-          zc[nf] = ZEROS ? *reinterpret_cast<const unsigned*>(p.zeros + at + 4 * lg) : 0x08080808u;
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (s < 3) read_x(s + 1, xr[(s + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-      // (LDS returns in order: what was read for the next step may be on its way)
-      constexpr int kNext = MF * XR;
+      for (int nf = 0; nf < NF; ++nf) w4_lds_wait(ws[nf]);
 #pragma unroll
       for (int mf = 0; mf < MF; ++mf)
 #pragma unroll
-        for (int k = 0; k < XR; ++k) {
-          if (s == 0)
-            w4_lds_wait<0>(xr[0][mf][k]);
-          else if (s < 3)
-            w4_lds_wait<kNext>(xr[s & 1][mf][k]);
-          else
-            w4_lds_wait<0>(xr[s & 1][mf][k]);
-        }
-      if (s == 0) {
-#pragma unroll
-        for (int nf = 0; nf < NF; ++nf) w4_lds_wait<0>(w[nf]);
+        for (int k = 0; k < XR; ++k) w4_lds_wait(x[mf][k]);
+    };
+    read_w(std::integral_constant<int, 0>{}, w[0]);
+    read_x(0, xr[0]);
+    wait_step(w[0], xr[0]);
+    bf16x8 wf = decode(w[0][0]);
+    // A step's MFMAs go out tile by tile, and between a tile's the vector unit
+    // makes the next tile's operand and folds the one before.
+    w4_static_for<0, 1, 4>([&](auto step) __attribute__((always_inline)) {
+      constexpr int s = step.value;
+      if constexpr (s < 3) {
+        read_w(std::integral_constant<int, s + 1>{}, w[(s + 1) & 1]);
+        read_x(s + 1, xr[(s + 1) & 1]);
       }
-      bf16x8 wf[NF];
-#pragma unroll
-      for (int nf = 0; nf < NF; ++nf) wf[nf] = w4_operand<H>(__builtin_bit_cast(u32x4, w[nf])[s]);
+      bf16x8 xf[MF][NS];
 #pragma unroll
       for (int mf = 0; mf < MF; ++mf) {
-        bf16x8 xf[NS];
         if constexpr (EB == 4) {
-          w4_split(__builtin_bit_cast(u32x4, xr[s & 1][mf][0]), __builtin_bit_cast(u32x4, xr[s & 1][mf][1]), xf);
+          w4_split(__builtin_bit_cast(u32x4, xr[s & 1][mf][0]), __builtin_bit_cast(u32x4, xr[s & 1][mf][1]), xf[mf]);
         } else {
-          xf[0] = xr[s & 1][mf][0];
+          xf[mf][0] = xr[s & 1][mf][0];
         }
+      }
+      const bool ends = (s + 1) % FS == 0;
+#pragma unroll
+      for (int nf = 0; nf < NF; ++nf) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
           const bool first = s % FS == 0 && k == 0;
-          ax[mf] = mma16_16b<H>(ones, xf[k], first ? zero4 : ax[mf]);
+          if (nf < MF) ax[nf] = mma16_16b<H>(ones, xf[nf][k], first ? zero4 : ax[nf]);
 #pragma unroll
-          for (int nf = 0; nf < NF; ++nf)
-            accg[mf][nf] = mma16_16b<H>(wf[nf], xf[k], first ? zero4 : accg[mf][nf]);
+          for (int mf = 0; mf < MF; ++mf) accg[mf][nf] = mma16_16b<H>(wf, xf[mf][k], first ? zero4 : accg[mf][nf]);
+        }
+        if (nf < NF - 1) wf = decode(w[s & 1][nf + 1]);
+        if (nf > 0 && ends) fold(nf - 1, sc[s / FS][nf - 1], lg == ((c * GC + s / FS) & 3));
+        if (nf == 0 && s > 0 && s % FS == 0)
+          fold(NF - 1, sc[(s - 1) / FS][NF - 1], lg == ((c * GC + (s - 1) / FS) & 3));
+#pragma unroll
+        for (int i = 0; i < (MF + 1) * NS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA,
+          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // and vector operations behind it
         }
       }
-      if ((s + 1) % FS == 0) {
-#pragma unroll
-        for (int nf = 0; nf < NF; ++nf) {
-          float zz[4], sf[4];
-          sc[nf].get(sf);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) zz[i] = 16.f + (float)((zc[nf] >> (8 * i)) & 255u);
-#pragma unroll
-          for (int mf = 0; mf < MF; ++mf) w4_fold(acc[mf][nf], accg[mf][nf], ax[mf][0], sf, zz);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (s < 3) {
+        wait_step(w[(s + 1) & 1], xr[(s + 1) & 1]);
+        wf = decode(w[(s + 1) & 1][0]);
       }
+    });
+    fold(NF - 1, sc[3 / FS][NF - 1], lg == ((c * GC + 3 / FS) & 3));
+#pragma unroll
+    for (int nf = 0; nf < NF; ++nf) sc[0][nf] = sc[GC][nf];
+    // Four folds' row sums times -s (16 + z), in fp32 on the matrix unit.
+    const int folds = (c + 1) * GC;
+    if ((folds & 3) == 0 || !more) {
+      const int f = ((folds - 1) & ~3) + lg;
+      const unsigned g = min(FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)f) : f >> p.fold_shift, p.groups - 1);
+#pragma unroll
+      for (int nf = 0; nf < NF; ++nf) {
+        const size_t at = (size_t)(sbase[nf] + g) * 16 + l16;
+        const float t = -to_f32(reinterpret_cast<const S*>(p.scales)[at]) * (16.f + (p.zeros ? (float)p.zeros[at] : 8.f));
+#pragma unroll
+        for (int mf = 0; mf < MF; ++mf) acc[mf][nf] = __builtin_amdgcn_mfma_f32_16x16x4f32(t, xs[mf], acc[mf][nf], 0, 0, 0);
+      }
+#pragma unroll
+      for (int mf = 0; mf < MF; ++mf) xs[mf] = 0.f;
     }
   }
   // ---- the outputs: four columns of a row a lane and fragment
@@ -371,11 +420,7 @@ int w4_tiles_launch(const W4Args& p, hipStream_t st) {
   const int mblocks = (p.M + 32 * MF - 1) / (32 * MF), nblocks = (p.tiles + 7) / 8;
   const long items = (long)mblocks * nblocks, per_xcd = (items + 7) / 8;
   if (8 * per_xcd * 256 > kMaxGridThreads) return set_error(NKL_EINVAL, "nkl_gemm_w4: %ld tiles", items);
-  const dim3 grid((unsigned)(8 * per_xcd));
-  if (p.zeros)
-    w4_tiles_kernel<T, S, MF, GLU, FS, true><<<grid, dim3(256), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
-  else
-    w4_tiles_kernel<T, S, MF, GLU, FS, false><<<grid, dim3(256), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
+  w4_tiles_kernel<T, S, MF, GLU, FS><<<dim3((unsigned)(8 * per_xcd)), dim3(256), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
   return check_launch("nkl_gemm_w4");
 }
 
@@ -407,8 +452,12 @@ int w4_launch_fold(const W4Args& p, const W4Plan& pl, hipStream_t st) {
   const bool copies = p.M > 64 && p.K % (16 / (int)sizeof(T)) == 0 && p.ldx % (16 / (int)sizeof(T)) == 0 &&
                       (size_t)p.x % 16 == 0 && p.ldx < (1L << 21);
   if (copies) {
-    constexpr int MF = sizeof(T) == 4 ? 2 : 4;
-    return pl.glu ? w4_tiles_launch<T, S, MF, true, FS>(p, st) : w4_tiles_launch<T, S, MF, false, FS>(p, st);
+    // (fp32 scales of groups of 64 beside 16-bit operands: two folds a group, the
+    // registers hold no more)
+    constexpr int MF = sizeof(T) == 4 ? 2 : 4, FT = FS == 2 && sizeof(S) > sizeof(T) ? 1 : FS;
+    W4Args q = p;
+    q.fold_shift = FT != FS;
+    return pl.glu ? w4_tiles_launch<T, S, MF, true, FT>(q, st) : w4_tiles_launch<T, S, MF, false, FT>(q, st);
   }
   if (p.M <= 16) return run(std::integral_constant<int, 1>{});
   if (p.M <= 32) return run(std::integral_constant<int, 2>{});
