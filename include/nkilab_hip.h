@@ -587,7 +587,8 @@ typedef struct {
 /*
  * nkl_cache_append with rotary a table (null: no rotation, then no q) and, for a
  * cache of 8 bits, rows of dtype `dtype` taken to codes (others: dtype is the
- * cache's, scales null).  Rows are rotated in 64 bits and rounded once.
+ * cache's, scales null).  Angles are of 64 bits; what becomes codes is rotated in 64
+ * bits, other rows in 32, and all rounded once.
  * 8 bits: a page whose first rows these are gets the smallest exponent with
  * which they stay within 448, s within 17 .. 246; one that holds rows before the
  * new ones its own or, if that is larger, theirs, and its rows before are brought

@@ -9,6 +9,8 @@
 // the new exponent: a shift that is exact but for codes that become subnormal.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.h"
 #include "rotary.h"
 
@@ -67,32 +69,65 @@ __device__ __forceinline__ float round_odd(double x) {
   return __uint_as_float(u);
 }
 
-// Value y of a row as the code under inv = 2^-e: nearest, ties to even; an
-// infinity is NaN, as NaN is (what exceeds the largest exponent saturates).
-__device__ __forceinline__ float code_value(double y, double inv) {
-  const double z = y * inv;
-  if (fabs(z) <= 448.0) return round_odd(z);
-  if (!(fabs(z) < INFINITY)) return NAN;
-  return z > 0 ? 448.f : -448.f;
+// What a code is rounded from: z, an infinity as NaN (the conversion's own
+// rule), and no more than 448.
+__device__ __forceinline__ float saturated(float z) {
+  const float a = fabsf(z);
+  return a > 448.f && a < INFINITY ? copysignf(448.f, z) : z;
 }
 
 template <int E>
-__device__ __forceinline__ void store_codes(unsigned char* p, const double (&y)[E], double inv) {
+__device__ __forceinline__ void store_codes(unsigned char* p, const float (&z)[E]) {
   if constexpr (E == 1) {
-    *p = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(code_value(y[0], inv), 0.f, 0, false) & 255);
+    *p = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(z[0], 0.f, 0, false) & 255);
   } else {
     unsigned w[E / 4];
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
-      int x = __builtin_amdgcn_cvt_pk_fp8_f32(code_value(y[4 * i], inv), code_value(y[4 * i + 1], inv), 0, false);
-      x = __builtin_amdgcn_cvt_pk_fp8_f32(code_value(y[4 * i + 2], inv), code_value(y[4 * i + 3], inv), x, true);
-      w[i] = (unsigned)x;
+      const int x = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i], z[4 * i + 1], 0, false);
+      w[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i + 2], z[4 * i + 3], x, true);
     }
     if constexpr (E == 4)
       *reinterpret_cast<unsigned*>(p) = w[0];
     else
       *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   }
+}
+
+// Values y as codes under exponent byte s: nearest, ties to even.  32 bits hold a
+// row's own values and their product with a power of two exactly.
+template <int E>
+__device__ __forceinline__ void store_row(unsigned char* p, const float (&y)[E], int s) {
+  // 2^(127 - s); below the smallest normal number for bytes that only others write
+  const float inv = __uint_as_float(s < 254 ? (unsigned)(254 - s) << 23 : 0x00400000u >> (s - 254));
+  float z[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) z[e] = y[e] * inv;
+  if (s == kScaleHi) {  // (below it nothing finite exceeds 448)
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = saturated(z[e]);
+  }
+  store_codes<E>(p, z);
+}
+
+// Rotated values come in 64 bits.  Rounding them to 32 first makes a difference
+// only where that lands on the middle of two codes, or where codes are
+// subnormal and their middles elsewhere.
+template <int E>
+__device__ __forceinline__ void store_row(unsigned char* p, const double (&y)[E], int s) {
+  const double inv = inv_scale(s);
+  float z[E];
+  bool odd = s == kScaleHi;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    z[e] = (float)(y[e] * inv);
+    odd |= (__float_as_uint(z[e]) & 0xfffffu) == 0x80000u || (fabsf(z[e]) < 0.015625f && z[e] != 0.f);
+  }
+  if (odd) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = saturated(round_odd(y[e] * inv));
+  }
+  store_codes<E>(p, z);
 }
 
 // 16 codes times 2^shift, shift <= 0.
@@ -112,41 +147,47 @@ __device__ __forceinline__ uint4 shift_codes(uint4 c, int shift) {
 }
 
 template <typename T, int E>
-__device__ __forceinline__ void load_wide(const T* p, double (&y)[E]) {
-  if constexpr (E == 1) {
-    y[0] = (double)to_f32(p[0]);
-  } else {
-    float x[E];
-    load16(p, x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = (double)x[e];
-  }
+__device__ __forceinline__ void load_row(const T* p, float (&y)[E]) {
+  if constexpr (E == 1)
+    y[0] = to_f32(p[0]);
+  else
+    load16(p, y);
 }
 
 template <typename T, int E>
-__device__ __forceinline__ void store_as(T* p, const double (&y)[E]) {
-  if constexpr (E == 1) {
-    *p = from_f32<T>(sizeof(T) == 4 ? (float)y[0] : round_odd(y[0]));
-  } else {
-    float x[E];
+__device__ __forceinline__ void store_as(T* p, const float (&y)[E]) {
+  if constexpr (E == 1)
+    *p = from_f32<T>(y[0]);
+  else
+    store_vec<E>(p, y);
+}
+
+// The largest finite magnitude of values.
+template <int E, typename V>
+__device__ __forceinline__ V top_of(const V (&y)[E]) {
+  V m = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = sizeof(T) == 4 ? (float)y[e] : round_odd(y[e]);
-    store_vec<E>(p, x);
+  for (int e = 0; e < E; ++e) m = fmax(m, fabs(y[e]));  // (NaN is no operand of a maximum)
+  if (m == (V)INFINITY) {
+    m = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmax(m, fabs(y[e]) < (V)INFINITY ? fabs(y[e]) : (V)0);
   }
+  return m;
 }
 
 // Workgroup (x, job): a page slot of a sequence -- the new rows that fall into one
 // page -- and some heads of K, V or q (q's rows in blocks of a page's size
-// instead).  The rows' angles go to LDS once for all its heads, in 64 bits, and
-// rows are rotated in 64 bits: a code is then the nearest one of the exact
-// rotation (in 32 bits one of a million lands on its neighbour), however its
-// row was batched.  Cheap beside the memory: a sine and cosine are 30
-// instructions, shared by the heads.  8 bits: a pass over the rows for the
-// largest magnitude of each head, then one that writes; the second reads what the
-// first brought to the caches.
-template <typename T, int E, bool Q8>
+// instead).  The rows' angles go to LDS once for all its heads.  K's rows for
+// codes are rotated in 64 bits: a code is then the nearest one of the exact
+// rotation (in 32 bits one of a million lands on its neighbour); everything else
+// in 32, with sines and cosines rounded once.
+// 8 bits: a pass over the rows for the largest magnitude of each head, then one
+// that writes, which reads what the first brought to the caches -- or holds it
+// in registers, where a thread has one piece (ONE: single tokens).
+template <typename T, int E, bool Q8, bool ONE>
 __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs p) {
-  extern __shared__ double2 cs[];  // [rb][pairs]
+  extern __shared__ double2 cs[];  // [rb][pairs] (float2 for what is rotated in 32 bits)
   constexpr int kHeads = 256;
   __shared__ int top[Q8 ? kHeads : 1], old[Q8 ? kHeads : 1];
   __shared__ int grown;
@@ -211,6 +252,7 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
   const bool codes = Q8 && !is_q;
   unsigned char* const cache = is_v ? c.v : c.k;
   const long c_page = is_v ? c.v_page : c.k_page, c_head = is_v ? c.v_head : c.k_head, c_row = is_v ? c.v_row : c.k_row;
+  float2* const cs32 = reinterpret_cast<float2*>(cs);
 
   if constexpr (Q8) {
     if (codes) {
@@ -219,7 +261,6 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
         old[h] = sc[(long)pid * sc_page + (long)(h0 + h) * sc_head];
       }
       if (tid == 0) grown = 0;
-      __syncthreads();
     }
   }
 
@@ -240,63 +281,171 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
       }
       double sn, co;
       sincos64((double)pos * p.t.freq[f], sn, co);
-      cs[x] = make_double2(p.t.magnitude * co, p.t.magnitude * sn);
+      sn *= p.t.magnitude;
+      co *= p.t.magnitude;
+      if (codes)
+        cs[x] = make_double2(co, sn);
+      else
+        cs32[x] = make_float2((float)co, (float)sn);
     }
     __syncthreads();
   };
-  // Calls fn(row, head, element, values) for the pieces of rows rs .. rs + rows - 1.
-  auto pieces = [&](int rs, int rows, auto&& fn) __attribute__((always_inline)) {
-    const int items = rows * heads_max * per;
-    for (int x = tid; x < items; x += 256) {
-      const int rh = (int)div32(dv_per, (unsigned)x), e = x - rh * per;
-      const int r = (int)div32(dv_h, (unsigned)rh), h = rh - r * heads_max;
-      if (h >= heads) continue;
-      const T* row = src + (long)(s.t0 + i0 + rs + r) * s_t + (long)(h0 + h) * s_h;
-      if (!rot || e >= p.per_rot) {
-        const int at = rot ? 2 * pairs + (e - p.per_rot) * E : e * E;
-        double y[E];
-        load_wide<T, E>(row + at, y);
-        fn(rs + r, h, at, y);
-      } else if (p.t.interleaved) {
-        constexpr int W = E > 1 ? E : 2;
-        double x2[W];
-        if constexpr (E > 1) {
-          load_wide<T, E>(row + e * W, x2);
-        } else {
-          x2[0] = (double)to_f32(row[2 * e]);
-          x2[1] = (double)to_f32(row[2 * e + 1]);
-        }
+  // Piece e of row r (of the rows whose angles LDS holds; its tensor's row) and
+  // head h: one or two runs of E elements, given to fn(element, values).
+  // Q8's rotated runs are of 64 bits.
+  auto piece = [&](int r, const T* row, int e, auto&& fn) __attribute__((always_inline)) {
+    if (!rot || e >= p.per_rot) {
+      const int at = rot ? 2 * pairs + (e - p.per_rot) * E : e * E;
+      float y[E];
+      load_row<T, E>(row + at, y);
+      fn(at, y);
+      return;
+    }
+    const bool il = p.t.interleaved;
+    // (interleaved runs: two elements of a pair side by side; E of them, or two)
+    constexpr int W = E > 1 ? E / 2 : 1;  // pairs of an interleaved piece
+    float x1[E], x2[E];
+    if (il) {
+      if constexpr (E > 1) {
+        float t[E];
+        load_row<T, E>(row + e * E, t);
 #pragma unroll
-        for (int k = 0; k < W / 2; ++k) {
-          const double2 w = cs[r * pairs + e * (W / 2) + k];
-          const double a = x2[2 * k], d = x2[2 * k + 1];
-          x2[2 * k] = a * w.x - d * w.y;
-          x2[2 * k + 1] = d * w.x + a * w.y;
-        }
+        for (int k = 0; k < W; ++k) x1[k] = t[2 * k], x2[k] = t[2 * k + 1];
+      } else {
+        x1[0] = to_f32(row[2 * e]), x2[0] = to_f32(row[2 * e + 1]);
+      }
+    } else {
+      load_row<T, E>(row + e * E, x1);
+      load_row<T, E>(row + e * E + pairs, x2);
+    }
+    auto rotated = [&](auto zero, auto* w) __attribute__((always_inline)) {
+      using V = decltype(zero);
+      if (il) {
         if constexpr (E > 1) {
-          fn(rs + r, h, e * W, x2);
+          V y[E];
+#pragma unroll
+          for (int k = 0; k < W; ++k) {
+            const V a = x1[k], d = x2[k];
+            y[2 * k] = a * w[e * W + k].x - d * w[e * W + k].y;
+            y[2 * k + 1] = d * w[e * W + k].x + a * w[e * W + k].y;
+          }
+          fn(e * E, y);
         } else {
-          const double a[1] = {x2[0]}, d[1] = {x2[1]};
-          fn(rs + r, h, 2 * e, a);
-          fn(rs + r, h, 2 * e + 1, d);
+          const V a = x1[0], d = x2[0];
+          const V y1[1] = {a * w[e].x - d * w[e].y}, y2[1] = {d * w[e].x + a * w[e].y};
+          fn(2 * e, y1);
+          fn(2 * e + 1, y2);
         }
       } else {
-        double a[E], d[E];
-        load_wide<T, E>(row + e * E, a);
-        load_wide<T, E>(row + e * E + pairs, d);
+        V y1[E], y2[E];
 #pragma unroll
         for (int k = 0; k < E; ++k) {
-          const double2 w = cs[r * pairs + e * E + k];
-          const double x1 = a[k], x2 = d[k];
-          a[k] = x1 * w.x - x2 * w.y;
-          d[k] = x2 * w.x + x1 * w.y;
+          const V a = x1[k], d = x2[k];
+          y1[k] = a * w[e * E + k].x - d * w[e * E + k].y;
+          y2[k] = d * w[e * E + k].x + a * w[e * E + k].y;
         }
-        fn(rs + r, h, e * E, a);
-        fn(rs + r, h, e * E + pairs, d);
+        fn(e * E, y1);
+        fn(e * E + pairs, y2);
+      }
+    };
+    if constexpr (Q8) {
+      if (codes) {
+        rotated(0.0, cs + r * pairs);
+        return;
+      }
+    }
+    rotated(0.f, cs32 + r * pairs);
+  };
+  auto row_of = [&](int r, int h) __attribute__((always_inline)) {
+    return src + (long)(s.t0 + i0 + r) * s_t + (long)(h0 + h) * s_h;
+  };
+  // Where row r's codes (or elements) of head h go.
+  auto place = [&](int r, int h) __attribute__((always_inline)) {
+    return (long)pid * c_page + (long)(h0 + h) * c_head + (long)(r0 + r) * c_row;
+  };
+  // The pages' exponents, behind a barrier with all magnitudes in; rows before the
+  // new ones follow where it rises.
+  auto settle = [&]() __attribute__((always_inline)) {
+    for (int h = tid; h < heads; h += 256) {
+      int t = top[h];
+      if (r0 > 0) {
+        t = max(t, old[h]);
+        if (t > old[h]) grown = 1;
+        top[h] = t;
+      }
+      sc[(long)pid * sc_page + (long)(h0 + h) * sc_head] = (unsigned char)t;
+    }
+    __syncthreads();
+    if (grown) {
+      const int each = r0 * (c.d / 16);  // 16-byte pieces of the rows before, a head
+      for (int h = 0; h < heads; ++h) {
+        const int shift = old[h] - top[h];
+        if (shift == 0) continue;
+        unsigned char* base = cache + (long)pid * c_page + (long)(h0 + h) * c_head;
+        for (int x = tid; x < each; x += 256) {
+          const int r = (int)div32(p.dv_pieces, (unsigned)x);
+          uint4* at = reinterpret_cast<uint4*>(base + (long)r * c_row + (x - r * (c.d / 16)) * 16);
+          *at = shift_codes(*at, shift);
+        }
       }
     }
   };
 
+  if constexpr (ONE) {
+    // cnt rows, heads and pieces: at most one to a thread.
+    const int rh = (int)div32(dv_per, (unsigned)tid), e = tid - rh * per;
+    const int r = (int)div32(dv_h, (unsigned)rh), h = rh - r * heads_max;
+    const bool have = r < cnt && h < heads;
+    if (rot)
+      angles(0, cnt);
+    else
+      __syncthreads();
+    const T* row = row_of(have ? r : 0, have ? h : 0);
+    if (codes) {
+      if constexpr (Q8) {
+        // (at most two runs a piece)
+        int at[2] = {0, 0}, n = 0;
+        double y[2][E];
+        piece(have ? r : 0, row, e, [&](int a, const auto& v) __attribute__((always_inline)) {
+#pragma unroll
+          for (int k = 0; k < E; ++k) (n == 0 ? y[0][k] : y[1][k]) = (double)v[k];
+          at[n == 0 ? 0 : 1] = a;
+          ++n;
+          if (have) atomicMax(&top[h], scale_byte((double)top_of<E>(v)));
+        });
+        __syncthreads();
+        settle();
+        if (have) {
+          const int sb = top[h];
+          unsigned char* dst = cache + place(r, h);
+          store_row<E>(dst + at[0], y[0], sb);
+          if (n > 1) store_row<E>(dst + at[1], y[1], sb);
+        }
+      }
+    } else if (have) {
+      piece(r, row, e, [&](int a, const auto& v) __attribute__((always_inline)) {
+        if constexpr (std::is_same<decltype(v), const float(&)[E]>::value) {
+          T* dst = is_q ? reinterpret_cast<T*>(p.qo) + (long)(s.t0 + i0 + r) * p.qo_t + (long)(h0 + h) * p.qo_h
+                        : reinterpret_cast<T*>(cache) + place(r, h);
+          store_as<T, E>(dst + a, v);
+        }
+      });
+    }
+    return;
+  }
+
+  // Calls fn(row of the block, head, piece) for this thread's pieces of a block
+  // of rows, head by head; done(head) behind each head's.
+  auto block = [&](int rows, auto&& fn, auto&& done) __attribute__((always_inline)) {
+    for (int h = 0; h < heads; ++h) {
+      for (int x = tid; x < rows * per; x += 256) {
+        const int r = (int)div32(dv_per, (unsigned)x);
+        fn(r, h, x - r * per);
+      }
+      done(h);
+    }
+  };
+  if (!rot) __syncthreads();
   const bool once = !rot || cnt <= p.rb;  // the angles stay for the second pass
   const int rb = rot ? p.rb : cnt;
   if constexpr (Q8) {
@@ -304,41 +453,29 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
       for (int rs = 0; rs < cnt; rs += rb) {
         const int rows = min(rb, cnt - rs);
         if (rot) angles(rs, rows);
-        pieces(rs, rows, [&](int, int h, int, const double (&y)[E]) __attribute__((always_inline)) {
-          double m = 0.0;
+        double md = 0.0;
+        float mf = 0.f;
+        block(
+            rows,
+            [&](int r, int h, int e) __attribute__((always_inline)) {
+              piece(r, row_of(rs + r, h), e, [&](int, const auto& v) __attribute__((always_inline)) {
+                if constexpr (std::is_same<decltype(v), const float(&)[E]>::value)
+                  mf = fmaxf(mf, top_of<E>(v));
+                else
+                  md = fmax(md, top_of<E>(v));
+              });
+            },
+            [&](int h) __attribute__((always_inline)) {
+              int t = scale_byte(fmax(md, (double)mf));
 #pragma unroll
-          for (int k = 0; k < E; ++k) {
-            const double a = fabs(y[k]);
-            m = fmax(m, a < INFINITY ? a : 0.0);
-          }
-          atomicMax(&top[h], scale_byte(m));
-        });
+              for (int o = 32; o >= 1; o >>= 1) t = max(t, __shfl_xor(t, o, kWave));
+              if ((tid & 63) == 0) atomicMax(&top[h], t);
+              md = 0.0;
+              mf = 0.f;
+            });
         __syncthreads();
       }
-      // The pages' exponents; rows before the new ones follow where it rises.
-      for (int h = tid; h < heads; h += 256) {
-        int t = top[h];
-        if (r0 > 0) {
-          t = max(t, old[h]);
-          if (t > old[h]) grown = 1;
-          top[h] = t;
-        }
-        sc[(long)pid * sc_page + (long)(h0 + h) * sc_head] = (unsigned char)t;
-      }
-      __syncthreads();
-      if (grown) {
-        const int each = r0 * (c.d / 16);  // 16-byte pieces of the rows before, a head
-        for (int h = 0; h < heads; ++h) {
-          const int shift = old[h] - top[h];
-          if (shift == 0) continue;
-          unsigned char* base = cache + (long)pid * c_page + (long)(h0 + h) * c_head;
-          for (int x = tid; x < each; x += 256) {
-            const int r = (int)div32(p.dv_pieces, (unsigned)x);
-            uint4* at = reinterpret_cast<uint4*>(base + (long)r * c_row + (x - r * (c.d / 16)) * 16);
-            *at = shift_codes(*at, shift);
-          }
-        }
-      }
+      settle();
     }
   }
   for (int rs = 0; rs < cnt; rs += rb) {
@@ -347,21 +484,24 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
       if (rs > 0 || codes) __syncthreads();  // (every piece has read the angles there are)
       angles(rs, rows);
     }
-    if (codes) {
-      pieces(rs, rows, [&](int r, int h, int at, const double (&y)[E]) __attribute__((always_inline)) {
-        unsigned char* dst = cache + (long)pid * c_page + (long)(h0 + h) * c_head + (long)(r0 + r) * c_row + at;
-        store_codes<E>(dst, y, inv_scale(top[Q8 ? h : 0]));
-      });
-    } else if (is_q) {
-      pieces(rs, rows, [&](int r, int h, int at, const double (&y)[E]) __attribute__((always_inline)) {
-        store_as<T, E>(reinterpret_cast<T*>(p.qo) + (long)(s.t0 + i0 + r) * p.qo_t + (long)(h0 + h) * p.qo_h + at, y);
-      });
-    } else if constexpr (!Q8) {
-      pieces(rs, rows, [&](int r, int h, int at, const double (&y)[E]) __attribute__((always_inline)) {
-        store_as<T, E>(reinterpret_cast<T*>(cache) + (long)pid * c_page + (long)(h0 + h) * c_head + (long)(r0 + r) * c_row + at,
-                       y);
-      });
-    }
+    block(
+        rows,
+        [&](int r, int h, int e) __attribute__((always_inline)) {
+          piece(r, row_of(rs + r, h), e, [&](int a, const auto& v) __attribute__((always_inline)) {
+            if constexpr (Q8) {
+              if (codes) {
+                store_row<E>(cache + place(rs + r, h) + a, v, top[h]);
+                return;
+              }
+            }
+            if constexpr (std::is_same<decltype(v), const float(&)[E]>::value) {
+              T* dst = is_q ? reinterpret_cast<T*>(p.qo) + (long)(s.t0 + i0 + rs + r) * p.qo_t + (long)(h0 + h) * p.qo_h
+                            : reinterpret_cast<T*>(cache) + place(rs + r, h);
+              store_as<T, E>(dst + a, v);
+            }
+          });
+        },
+        [](int) {});
   }
 }
 
@@ -379,14 +519,19 @@ int write_launch(const CacheArgs& c, WriteArgs p, hipStream_t st) {
   p.per_rot = pairs == 0 ? 0 : E == 1 ? pairs : p.t.interleaved ? 2 * pairs / E : pairs / E;
   p.per_rest = (c.d - 2 * pairs) / E;
   p.per_copy = c.d / E;
-  // Heads to a workgroup: some thousand pieces, four a thread.
+  // Heads to a workgroup: a piece to each thread where there are few rows, else
+  // as many heads as still leave four workgroups to a CU, to share the angles.
   const long rows = c.max_new < c.page_size ? c.max_new : c.page_size;
+  const int most = p.per_copy > p.per_rot + p.per_rest ? p.per_copy : p.per_rot + p.per_rest;
+  const bool one = rows * most <= 256;
   auto heads_of = [&](int heads, int per) {
-    long h = 1024 / (rows * per);
+    long h = one ? 256 / (rows * per) : 4;
+    if (!one)
+      while (h > 1 && gx * ((heads + h - 1) / h) < 4L * cu_count()) h /= 2;
     h = h < 1 ? 1 : h > 256 ? 256 : h;
     return (int)(h < heads ? h : heads);
   };
-  p.kv_heads = heads_of(c.kv_heads, p.per_copy);
+  p.kv_heads = heads_of(c.kv_heads, most);
   p.kv_jobs = (c.kv_heads + p.kv_heads - 1) / p.kv_heads;
   const int q_per = p.per_rot + (p.copy_rest ? p.per_rest : 0);
   p.q_heads = p.H ? heads_of(p.H, q_per) : 1;
@@ -405,7 +550,12 @@ int write_launch(const CacheArgs& c, WriteArgs p, hipStream_t st) {
   p.dv_qh = dv(p.q_heads);
   p.dv_pairs = dv(pairs);
   p.dv_pieces = dv(c.d / 16);
-  write_rows_kernel<T, E, Q8><<<dim3((unsigned)gx, (unsigned)gy), dim3(256), (size_t)p.rb * pairs * 16, st>>>(c, p);
+  const dim3 grid((unsigned)gx, (unsigned)gy);
+  const size_t lds = (size_t)p.rb * pairs * 16;
+  if (one)
+    write_rows_kernel<T, E, Q8, true><<<grid, dim3(256), lds, st>>>(c, p);
+  else
+    write_rows_kernel<T, E, Q8, false><<<grid, dim3(256), lds, st>>>(c, p);
   return check_launch(fn);
 }
 

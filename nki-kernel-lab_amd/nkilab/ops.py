@@ -1039,8 +1039,8 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     length and its depth.  Sequences of one call must not share a page that
     either writes.
 
-    rotary (in rope_base's place): any ``Rotary`` of the head, rows rotated in 64
-    bits and rounded once.
+    rotary (in rope_base's place): any ``Rotary`` of the head; angles in 64 bits,
+    rows rotated in fp32 (what becomes codes in 64 bits) and rounded once.
 
     A cache in 8 bits (float8_e4m3fn, d and strides multiples of 16) takes rows
     of any of the three dtypes, and k_scale and v_scale, uint8 [pages,

@@ -115,3 +115,14 @@ def rotate(x, pos, r):
         c, s = r.gain * np.cos(t), r.gain * np.sin(t)
         y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
     return y
+
+
+def rotate_bound(x, want, r, finfo):
+    """How far rows rotated in fp32 may be off: sine, cosine, their products and the sum are rounded by 2^-24 of at
+    most gain (|x1| + |x2|), three times over, and the result by half a step of its type."""
+    pair = np.zeros(x.shape)
+    half = r.dim // 2
+    a, b = (slice(0, r.dim, 2), slice(1, r.dim, 2)) if r.interleaved else (slice(0, half), slice(half, r.dim))
+    pair[..., a] = pair[..., b] = np.abs(x[..., a]) + np.abs(x[..., b])
+    inner = (3 * 2.0 ** -24 + 2.0 ** -30) * abs(r.gain) * pair
+    return inner + finfo.eps / 2 * (np.abs(want) + inner) + finfo.tiny * finfo.eps / 2

@@ -111,11 +111,10 @@ def test_append8(shape, dtype):
         kd = k.double().numpy()
         equal(c, before, kd if r is None else R8.rotate(kd, pos, r), v.double().numpy(), starts)
         if r is not None:
-            # rotated in 64 bits and rounded once: half a step (and 2^-40 for the 64-bit angles and products)
-            want = R8.rotate(q0.double().cpu().numpy(), pos, r)
-            fi = torch.finfo(DT[dtype])
+            x = q0.double().cpu().numpy()
+            want = R8.rotate(x, pos, r)
             err = np.abs(out.double().cpu().numpy() - want)
-            assert (err <= fi.eps / 2 * np.abs(want) + 2.0 ** -40 + fi.tiny * fi.eps / 2).all()
+            assert (err <= R8.rotate_bound(x, want, r, torch.finfo(DT[dtype]))).all()
 
 
 def test_append8_each_and_rope_base():
@@ -213,7 +212,7 @@ def test_append8_tree_missing_pages_and_rest():
 
 @pytest.mark.parametrize("dtype", DT)
 def test_append_rotary_into_other_caches(dtype):
-    """A table of frequencies over a cache that is not of 8 bits: rows rotated in 64 bits, rounded once."""
+    """A table of frequencies over a cache that is not of 8 bits."""
     from nkilab import ops
 
     g = torch.Generator().manual_seed(4)
@@ -235,14 +234,13 @@ def test_append_rotary_into_other_caches(dtype):
         ops.cache_append_into(k, v, kc, vc, table.int().cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
                               q_start=torch.tensor(starts, dtype=torch.int32).cuda(), max_q=40, q=q, q_out=q, rotary=r)
         pos = positions(lens, starts)
-        half = torch.finfo(DT[dtype]).eps / 2
-        for out, want in ((q, R8.rotate(x[:, :H * d].reshape(45, H, d), pos, r)),):
-            assert (np.abs(out.double().cpu().numpy() - want) <= half * np.abs(want) + 2.0 ** -26).all()
+        fi = torch.finfo(DT[dtype])
+        xq, xk = x[:, :H * d].reshape(45, H, d), x[:, H * d:(H + Hkv) * d].reshape(45, Hkv, d)
+        qr, kr = R8.rotate(xq, pos, r), R8.rotate(xk, pos, r)
+        assert (np.abs(q.double().cpu().numpy() - qr) <= R8.rotate_bound(xq, qr, r, fi)).all()
         seq = np.repeat(np.arange(3), news)
         pg, off = table.numpy()[seq, pos // page], pos % page
-        kr = R8.rotate(x[:, H * d:(H + Hkv) * d].reshape(45, Hkv, d), pos, r)
-        got = kc.double().cpu().numpy()[pg, :, off]
-        assert (np.abs(got - kr) <= half * np.abs(kr) + 2.0 ** -26).all()
+        assert (np.abs(kc.double().cpu().numpy()[pg, :, off] - kr) <= R8.rotate_bound(xk, kr, r, fi)).all()
         assert np.array_equal(vc.double().cpu().numpy()[pg, :, off], x[:, (H + Hkv) * d:].reshape(45, Hkv, d))
         assert int((kc != 0).any(dim=(1, 3)).sum()) <= 45  # (no other row was written)
 
