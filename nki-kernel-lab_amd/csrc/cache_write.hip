@@ -107,7 +107,7 @@ __device__ __forceinline__ void store_row(unsigned char* p, const float (&y)[E],
 #pragma unroll
     for (int e = 0; e < E; ++e) z[e] = saturated(z[e]);
   }
-  store_codes<E>(p, z);
+  store_codes(p, z);
 }
 
 // Rotated values come in 64 bits.  Rounding them to 32 first makes a difference
@@ -127,7 +127,7 @@ __device__ __forceinline__ void store_row(unsigned char* p, const double (&y)[E]
 #pragma unroll
     for (int e = 0; e < E; ++e) z[e] = saturated(round_odd(y[e] * inv));
   }
-  store_codes<E>(p, z);
+  store_codes(p, z);
 }
 
 // 16 codes times 2^shift, shift <= 0.
@@ -146,13 +146,28 @@ __device__ __forceinline__ uint4 shift_codes(uint4 c, int shift) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// E elements as loaded: 16 bytes in words, or one element.
 template <typename T, int E>
-__device__ __forceinline__ void load_row(const T* p, float (&y)[E]) {
-  if constexpr (E == 1)
-    y[0] = to_f32(p[0]);
-  else
-    load16(p, y);
-}
+struct Run {
+  typedef unsigned words __attribute__((ext_vector_type(4)));
+  words v = {0, 0, 0, 0};
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const words*>(p); }
+  __device__ __forceinline__ float at(int k) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(v[k]);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+      return k & 1 ? bf16hi(v[k / 2]) : bf16lo(v[k / 2]);
+    } else {
+      return (float)__builtin_bit_cast(f16x2, (unsigned)v[k / 2])[k & 1];
+    }
+  }
+};
+template <typename T>
+struct Run<T, 1> {
+  float v = 0.f;
+  __device__ __forceinline__ void load(const T* p) { v = to_f32(*p); }
+  __device__ __forceinline__ float at(int) const { return v; }
+};
 
 template <typename T, int E>
 __device__ __forceinline__ void store_as(T* p, const float (&y)[E]) {
@@ -183,10 +198,12 @@ __device__ __forceinline__ V top_of(const V (&y)[E]) {
 // rotation (in 32 bits one of a million lands on its neighbour); everything else
 // in 32, with sines and cosines rounded once.
 // 8 bits: a pass over the rows for the largest magnitude of each head, then one
-// that writes, which reads what the first brought to the caches -- or holds it
-// in registers, where a thread has one piece (ONE: single tokens).
-template <typename T, int E, bool Q8, bool ONE>
-__global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs p) {
+// that writes.  Pieces of 16 bytes are held in registers between them: one a
+// thread for all heads together (kOne: single tokens), or a head's at a time
+// (kHeld); pages too large for that are read again (kLoop).
+constexpr int kOne = 0, kHeld = 1, kLoop = 2, kHold = 4;
+template <typename T, int E, bool Q8, int MODE>
+__global__ __launch_bounds__(256, MODE == kHeld ? 3 : 1) void write_rows_kernel(CacheArgs c, WriteArgs p) {
   extern __shared__ double2 cs[];  // [rb][pairs] (float2 for what is rotated in 32 bits)
   constexpr int kHeads = 256;
   __shared__ int top[Q8 ? kHeads : 1], old[Q8 ? kHeads : 1];
@@ -290,62 +307,68 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
     }
     __syncthreads();
   };
-  // Piece e of row r (of the rows whose angles LDS holds; its tensor's row) and
-  // head h: one or two runs of E elements, given to fn(element, values).
-  // Q8's rotated runs are of 64 bits.
-  auto piece = [&](int r, const T* row, int e, auto&& fn) __attribute__((always_inline)) {
+  // Piece e of a row and head is one run of E elements, or two where it holds
+  // both halves of its pairs (or, an element a run, the two of a pair).
+  const bool il = p.t.interleaved;
+  struct Piece {
+    Run<T, E> a, b;
+  };
+  auto load = [&](const T* row, int e, Piece& x) __attribute__((always_inline)) {
     if (!rot || e >= p.per_rot) {
-      const int at = rot ? 2 * pairs + (e - p.per_rot) * E : e * E;
-      float y[E];
-      load_row<T, E>(row + at, y);
-      fn(at, y);
-      return;
-    }
-    const bool il = p.t.interleaved;
-    // (interleaved runs: two elements of a pair side by side; E of them, or two)
-    constexpr int W = E > 1 ? E / 2 : 1;  // pairs of an interleaved piece
-    float x1[E], x2[E];
-    if (il) {
+      x.a.load(row + (rot ? 2 * pairs + (e - p.per_rot) * E : e * E));
+    } else if (il) {
       if constexpr (E > 1) {
-        float t[E];
-        load_row<T, E>(row + e * E, t);
-#pragma unroll
-        for (int k = 0; k < W; ++k) x1[k] = t[2 * k], x2[k] = t[2 * k + 1];
+        x.a.load(row + e * E);
       } else {
-        x1[0] = to_f32(row[2 * e]), x2[0] = to_f32(row[2 * e + 1]);
+        x.a.load(row + 2 * e);
+        x.b.load(row + 2 * e + 1);
       }
     } else {
-      load_row<T, E>(row + e * E, x1);
-      load_row<T, E>(row + e * E + pairs, x2);
+      x.a.load(row + e * E);
+      x.b.load(row + e * E + pairs);
+    }
+  };
+  // Gives a piece's runs to fn(element, values), rotated by row r of the angles:
+  // in 64 bits if they become codes.
+  auto use = [&](int r, int e, const Piece& x, auto&& fn) __attribute__((always_inline)) {
+    if (!rot || e >= p.per_rot) {
+      float y[E];
+#pragma unroll
+      for (int k = 0; k < E; ++k) y[k] = x.a.at(k);
+      fn(rot ? 2 * pairs + (e - p.per_rot) * E : e * E, y);
+      return;
     }
     auto rotated = [&](auto zero, auto* w) __attribute__((always_inline)) {
       using V = decltype(zero);
-      if (il) {
-        if constexpr (E > 1) {
-          V y[E];
+      // (64 bits: four elements at a time, eight take too many registers)
+      constexpr int N = sizeof(V) == 8 && E > 4 ? 4 : E;
+      if (E > 1 && il) {
 #pragma unroll
-          for (int k = 0; k < W; ++k) {
-            const V a = x1[k], d = x2[k];
-            y[2 * k] = a * w[e * W + k].x - d * w[e * W + k].y;
-            y[2 * k + 1] = d * w[e * W + k].x + a * w[e * W + k].y;
+        for (int f = 0; f < E; f += N) {
+          V y[N];
+#pragma unroll
+          for (int k = 0; k < N / 2; ++k) {
+            const V a = x.a.at(f + 2 * k), d = x.a.at(f + 2 * k + 1);
+            const auto t = w[(e * E + f) / 2 + k];
+            y[2 * k] = a * t.x - d * t.y;
+            y[(2 * k + 1) % N] = d * t.x + a * t.y;
           }
-          fn(e * E, y);
-        } else {
-          const V a = x1[0], d = x2[0];
-          const V y1[1] = {a * w[e].x - d * w[e].y}, y2[1] = {d * w[e].x + a * w[e].y};
-          fn(2 * e, y1);
-          fn(2 * e + 1, y2);
+          fn(e * E + f, y);
         }
       } else {
-        V y1[E], y2[E];
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-          const V a = x1[k], d = x2[k];
-          y1[k] = a * w[e * E + k].x - d * w[e * E + k].y;
-          y2[k] = d * w[e * E + k].x + a * w[e * E + k].y;
+        for (int f = 0; f < E; f += N) {
+          V y1[N], y2[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const V a = x.a.at(f + k), d = x.b.at(f + k);
+            const auto t = w[e * E + f + k];
+            y1[k] = a * t.x - d * t.y;
+            y2[k] = d * t.x + a * t.y;
+          }
+          fn(il ? 2 * e : e * E + f, y1);
+          fn(il ? 2 * e + 1 : e * E + f + pairs, y2);
         }
-        fn(e * E, y1);
-        fn(e * E + pairs, y2);
       }
     };
     if constexpr (Q8) {
@@ -356,17 +379,29 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
     }
     rotated(0.f, cs32 + r * pairs);
   };
+  // Row i0 + r of a head, and where its codes (or elements) go.  (A product of
+  // 32-bit factors is one instruction.)
   auto row_of = [&](int r, int h) __attribute__((always_inline)) {
-    return src + (long)(s.t0 + i0 + r) * s_t + (long)(h0 + h) * s_h;
+    return src + ((long)(s.t0 + i0) * s_t + (long)(h0 + h) * s_h) + (unsigned long)(unsigned)r * (unsigned)s_t;
   };
-  // Where row r's codes (or elements) of head h go.
   auto place = [&](int r, int h) __attribute__((always_inline)) {
-    return (long)pid * c_page + (long)(h0 + h) * c_head + (long)(r0 + r) * c_row;
+    return ((long)pid * c_page + (long)(h0 + h) * c_head + (long)r0 * c_row) +
+           (long)((unsigned long)(unsigned)r * (unsigned)c_row);
+  };
+  auto q_place = [&](int r, int h) __attribute__((always_inline)) {
+    return reinterpret_cast<T*>(p.qo) + ((long)(s.t0 + i0) * p.qo_t + (long)(h0 + h) * p.qo_h) +
+           (unsigned long)(unsigned)r * (unsigned)p.qo_t;
+  };
+  // A run into q_out, or a cache that is not of 8 bits.
+  auto store_plain = [&](int r, int h, int at, const auto& v) __attribute__((always_inline)) {
+    if constexpr (std::is_same<decltype(v), const float(&)[E]>::value)
+      store_as<T, E>((is_q ? q_place(r, h) : reinterpret_cast<T*>(cache) + place(r, h)) + at, v);
   };
   // The pages' exponents, behind a barrier with all magnitudes in; rows before the
   // new ones follow where it rises.
-  auto settle = [&]() __attribute__((always_inline)) {
-    for (int h = tid; h < heads; h += 256) {
+  auto settle = [&](int from, int to) __attribute__((always_inline)) {
+    if constexpr (!Q8) return;
+    for (int h = from + tid; h < to; h += 256) {
       int t = top[h];
       if (r0 > 0) {
         t = max(t, old[h]);
@@ -378,7 +413,7 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
     __syncthreads();
     if (grown) {
       const int each = r0 * (c.d / 16);  // 16-byte pieces of the rows before, a head
-      for (int h = 0; h < heads; ++h) {
+      for (int h = from; h < to; ++h) {
         const int shift = old[h] - top[h];
         if (shift == 0) continue;
         unsigned char* base = cache + (long)pid * c_page + (long)(h0 + h) * c_head;
@@ -391,58 +426,108 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
     }
   };
 
-  if constexpr (ONE) {
+  if constexpr (MODE == kOne) {
     // cnt rows, heads and pieces: at most one to a thread.
     const int rh = (int)div32(dv_per, (unsigned)tid), e = tid - rh * per;
     const int r = (int)div32(dv_h, (unsigned)rh), h = rh - r * heads_max;
     const bool have = r < cnt && h < heads;
+    Piece x;
+    if (have) load(row_of(r, h), e, x);
     if (rot)
       angles(0, cnt);
     else
       __syncthreads();
-    const T* row = row_of(have ? r : 0, have ? h : 0);
     if (codes) {
       if constexpr (Q8) {
-        // (at most two runs a piece)
-        int at[2] = {0, 0}, n = 0;
-        double y[2][E];
-        piece(have ? r : 0, row, e, [&](int a, const auto& v) __attribute__((always_inline)) {
-#pragma unroll
-          for (int k = 0; k < E; ++k) (n == 0 ? y[0][k] : y[1][k]) = (double)v[k];
-          at[n == 0 ? 0 : 1] = a;
-          ++n;
-          if (have) atomicMax(&top[h], scale_byte((double)top_of<E>(v)));
-        });
+        if (have)
+          use(r, e, x, [&](int, const auto& v) __attribute__((always_inline)) {
+            atomicMax(&top[h], scale_byte((double)top_of(v)));
+          });
         __syncthreads();
-        settle();
-        if (have) {
-          const int sb = top[h];
-          unsigned char* dst = cache + place(r, h);
-          store_row<E>(dst + at[0], y[0], sb);
-          if (n > 1) store_row<E>(dst + at[1], y[1], sb);
-        }
+        settle(0, heads);
+        if (have)
+          use(r, e, x, [&](int at, const auto& v) __attribute__((always_inline)) {
+            store_row(cache + place(r, h) + at, v, top[h]);
+          });
       }
     } else if (have) {
-      piece(r, row, e, [&](int a, const auto& v) __attribute__((always_inline)) {
-        if constexpr (std::is_same<decltype(v), const float(&)[E]>::value) {
-          T* dst = is_q ? reinterpret_cast<T*>(p.qo) + (long)(s.t0 + i0 + r) * p.qo_t + (long)(h0 + h) * p.qo_h
-                        : reinterpret_cast<T*>(cache) + place(r, h);
-          store_as<T, E>(dst + a, v);
-        }
-      });
+      use(r, e, x, [&](int at, const auto& v) __attribute__((always_inline)) { store_plain(r, h, at, v); });
     }
     return;
   }
 
-  // Calls fn(row of the block, head, piece) for this thread's pieces of a block
-  // of rows, head by head; done(head) behind each head's.
-  auto block = [&](int rows, auto&& fn, auto&& done) __attribute__((always_inline)) {
+  // Largest magnitudes of a head's pieces, seen by this thread, to `top`.
+  double md = 0.0;
+  float mf = 0.f;
+  auto see = [&](int, const auto& v) __attribute__((always_inline)) {
+    if constexpr (std::is_same<decltype(v), const float(&)[E]>::value)
+      mf = fmaxf(mf, top_of(v));
+    else
+      md = fmax(md, top_of(v));
+  };
+  auto tell = [&](int h) __attribute__((always_inline)) {
+    int t = scale_byte(fmax(md, (double)mf));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) t = max(t, __shfl_xor(t, o, kWave));
+    if ((tid & 63) == 0) atomicMax(&top[Q8 ? h : 0], t);
+    md = 0.0;
+    mf = 0.f;
+  };
+
+  if constexpr (MODE == kHeld) {
+    // A head's pieces, at most kHold to a thread, stay in registers between the
+    // passes: its loads are all in flight at once.
+    const int n = cnt * per;
+    if (rot) angles(0, cnt);
+    if (!rot) __syncthreads();
     for (int h = 0; h < heads; ++h) {
-      for (int x = tid; x < rows * per; x += 256) {
-        const int r = (int)div32(dv_per, (unsigned)x);
-        fn(r, h, x - r * per);
+      Piece x[kHold];
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        const int i = tid + 256 * k;
+        if (i < n) {
+          const int r = (int)div32(dv_per, (unsigned)i);
+          load(row_of(r, h), i - r * per, x[k]);
+        }
       }
-      done(h);
+      if (codes) {
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) {
+          const int i = tid + 256 * k, r = (int)div32(dv_per, (unsigned)i);
+          if (i < n) use(r, i - r * per, x[k], see);
+          asm volatile("" : "+v"(md), "+v"(mf));  // (a piece at a time)
+        }
+        // (rotated anew in the second pass: kept, four pieces in 64 bits fill the registers)
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) asm volatile("" : "+v"(x[k].a.v), "+v"(x[k].b.v));
+        tell(h);
+        __syncthreads();
+        settle(h, h + 1);
+      }
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        const int i = tid + 256 * k, r = (int)div32(dv_per, (unsigned)i);
+        asm volatile("" : "+v"(x[k].a.v), "+v"(x[k].b.v)::"memory");
+        if (i >= n) continue;
+        use(r, i - r * per, x[k], [&](int at, const auto& v) __attribute__((always_inline)) {
+          if constexpr (Q8) {
+            if (codes) {
+              store_row(cache + place(r, h) + at, v, top[h]);
+              return;
+            }
+          }
+          store_plain(r, h, at, v);
+        });
+      }
+    }
+    return;
+  }
+
+  // Calls fn(row of the block, piece) for this thread's pieces of a block of rows.
+  auto block = [&](int rows, auto&& fn) __attribute__((always_inline)) {
+    for (int x = tid; x < rows * per; x += 256) {
+      const int r = (int)div32(dv_per, (unsigned)x);
+      fn(r, x - r * per);
     }
   };
   if (!rot) __syncthreads();
@@ -453,29 +538,17 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
       for (int rs = 0; rs < cnt; rs += rb) {
         const int rows = min(rb, cnt - rs);
         if (rot) angles(rs, rows);
-        double md = 0.0;
-        float mf = 0.f;
-        block(
-            rows,
-            [&](int r, int h, int e) __attribute__((always_inline)) {
-              piece(r, row_of(rs + r, h), e, [&](int, const auto& v) __attribute__((always_inline)) {
-                if constexpr (std::is_same<decltype(v), const float(&)[E]>::value)
-                  mf = fmaxf(mf, top_of<E>(v));
-                else
-                  md = fmax(md, top_of<E>(v));
-              });
-            },
-            [&](int h) __attribute__((always_inline)) {
-              int t = scale_byte(fmax(md, (double)mf));
-#pragma unroll
-              for (int o = 32; o >= 1; o >>= 1) t = max(t, __shfl_xor(t, o, kWave));
-              if ((tid & 63) == 0) atomicMax(&top[h], t);
-              md = 0.0;
-              mf = 0.f;
-            });
+        for (int h = 0; h < heads; ++h) {
+          block(rows, [&](int r, int e) __attribute__((always_inline)) {
+            Piece x;
+            load(row_of(rs + r, h), e, x);
+            use(r, e, x, see);
+          });
+          tell(h);
+        }
         __syncthreads();
       }
-      settle();
+      settle(0, heads);
     }
   }
   for (int rs = 0; rs < cnt; rs += rb) {
@@ -484,24 +557,20 @@ __global__ __launch_bounds__(256) void write_rows_kernel(CacheArgs c, WriteArgs 
       if (rs > 0 || codes) __syncthreads();  // (every piece has read the angles there are)
       angles(rs, rows);
     }
-    block(
-        rows,
-        [&](int r, int h, int e) __attribute__((always_inline)) {
-          piece(r, row_of(rs + r, h), e, [&](int a, const auto& v) __attribute__((always_inline)) {
-            if constexpr (Q8) {
-              if (codes) {
-                store_row<E>(cache + place(rs + r, h) + a, v, top[h]);
-                return;
-              }
+    for (int h = 0; h < heads; ++h)
+      block(rows, [&](int r, int e) __attribute__((always_inline)) {
+        Piece x;
+        load(row_of(rs + r, h), e, x);
+        use(r, e, x, [&](int at, const auto& v) __attribute__((always_inline)) {
+          if constexpr (Q8) {
+            if (codes) {
+              store_row(cache + place(rs + r, h) + at, v, top[h]);
+              return;
             }
-            if constexpr (std::is_same<decltype(v), const float(&)[E]>::value) {
-              T* dst = is_q ? reinterpret_cast<T*>(p.qo) + (long)(s.t0 + i0 + rs + r) * p.qo_t + (long)(h0 + h) * p.qo_h
-                            : reinterpret_cast<T*>(cache) + place(rs + r, h);
-              store_as<T, E>(dst + a, v);
-            }
-          });
-        },
-        [](int) {});
+          }
+          store_plain(rs + r, h, at, v);
+        });
+      });
   }
 }
 
@@ -527,7 +596,7 @@ int write_launch(const CacheArgs& c, WriteArgs p, hipStream_t st) {
   auto heads_of = [&](int heads, int per) {
     long h = one ? 256 / (rows * per) : 4;
     if (!one)
-      while (h > 1 && gx * ((heads + h - 1) / h) < 4L * cu_count()) h /= 2;
+      while (h > 1 && gx * ((heads + h - 1) / h) < 2L * cu_count()) h /= 2;
     h = h < 1 ? 1 : h > 256 ? 256 : h;
     return (int)(h < heads ? h : heads);
   };
@@ -536,7 +605,7 @@ int write_launch(const CacheArgs& c, WriteArgs p, hipStream_t st) {
   const int q_per = p.per_rot + (p.copy_rest ? p.per_rest : 0);
   p.q_heads = p.H ? heads_of(p.H, q_per) : 1;
   p.q_jobs = p.H ? (p.H + p.q_heads - 1) / p.q_heads : 0;
-  p.rb = pairs ? 2048 / pairs : 1;
+  p.rb = pairs ? 4096 / pairs : 1;  // (64 KB)
   if (p.rb > rows) p.rb = (int)rows;
   const long gy = 2L * p.kv_jobs + p.q_jobs;
   if (gx * 256 > kMaxGridThreads || gy > 65535 || gx * 256 * gy > kMaxGridThreads * 64 ||
@@ -553,9 +622,11 @@ int write_launch(const CacheArgs& c, WriteArgs p, hipStream_t st) {
   const dim3 grid((unsigned)gx, (unsigned)gy);
   const size_t lds = (size_t)p.rb * pairs * 16;
   if (one)
-    write_rows_kernel<T, E, Q8, true><<<grid, dim3(256), lds, st>>>(c, p);
+    write_rows_kernel<T, E, Q8, kOne><<<grid, dim3(256), lds, st>>>(c, p);
+  else if (rows * most <= 256 * kHold && (pairs == 0 || rows <= p.rb))
+    write_rows_kernel<T, E, Q8, kHeld><<<grid, dim3(256), lds, st>>>(c, p);
   else
-    write_rows_kernel<T, E, Q8, false><<<grid, dim3(256), lds, st>>>(c, p);
+    write_rows_kernel<T, E, Q8, kLoop><<<grid, dim3(256), lds, st>>>(c, p);
   return check_launch(fn);
 }
 
@@ -690,6 +761,8 @@ extern "C" int nkl_cache_write(const nkl_paged_cache* cache, const nkl_cache_sca
   if (c.batch == 0 || c.rows == 0 || c.max_new == 0) return NKL_OK;
   if (!c.table) return set_error(NKL_EINVAL, "%s: null page table", fn);
   if (!k || !v || (c.pages > 0 && (!c.k || !c.v))) return set_error(NKL_EINVAL, "%s: null pointer", fn);
+  if ((k_row | v_row | q_row | qo_row | c.k_row | c.v_row) >= 1L << 31)
+    return set_error(NKL_EINVAL, "%s: a row stride above 2^31 elements", fn);
   if (H && q == q_out && ((c.rows > 1 && q_row != qo_row) || (H > 1 && q_head != qo_head)))
     return set_error(NKL_EINVAL, "%s: q_out may be q with q's strides only", fn);
   p.nk = static_cast<const unsigned char*>(k);
