@@ -279,11 +279,15 @@ struct Lay {
   static constexpr int XO = NT > 1 ? NT * WPT * NDB * 4096 : 0;
   // Copied tiles: bytes of a tensor's, copies a wavefront (two copy K, two V),
   // stages.
-  static constexpr bool COPY = TP && WPT > 1 && NT == 1 && !C8;
+  // 8 bits: a wavefront's codes of a stage (REGION bytes, of its own), and two
+  // stages of tiles of T that they become.
+  static constexpr bool COPY = TP && WPT > 1 && NT == 1;
   static constexpr int ROWB = DP * (int)sizeof(T), TILEB = BN * ROWB;
-  static constexpr int NCP = TILEB / 2048;
+  static constexpr int REGION = BN / 2 * DP > 1024 ? BN / 2 * DP : 1024;
+  static constexpr int NCP = C8 ? REGION / 1024 : TILEB / 2048;
   static constexpr int CSTAGES = 4;
-  static constexpr int BYTES0 = COPY ? CSTAGES * 2 * TILEB : NT * TEAM * (int)sizeof(T);
+  static constexpr int CODES = C8 ? CSTAGES * WPT * REGION : 0;
+  static constexpr int BYTES0 = COPY ? CODES + (C8 ? 2 : CSTAGES) * 2 * TILEB : NT * TEAM * (int)sizeof(T);
   static constexpr int BYTES = BYTES0 > ML + XO ? BYTES0 : ML + XO;
   static_assert(BYTES <= 160 * 1024, "LDS");
 };
@@ -540,6 +544,7 @@ void paged_attn_kernel(PagedArgs p) {
     struct Lanes {
       unsigned lo, hi;
       int bytes, flags;
+      unsigned scale;  // 8 bits: the half's exponent byte
     } lt = {};
     int pid_next[2] = {-1, -1};
     auto tile_first = [&](int it) __attribute__((always_inline)) {
@@ -572,22 +577,28 @@ void paged_attn_kernel(PagedArgs p) {
       lt.lo = (unsigned)at;
       lt.hi = (unsigned)(at >> 32);
       lt.bytes = mine > 0 ? (mine - 1) * (int)row_b + row_bytes : 0;
+      if constexpr (C8) {
+        lt.scale = 127;
+        if (mine > 0) lt.scale = copies_v ? vsb[(long)pg * p.vs_page] : ksb[(long)pg * p.ks_page];
+        asm volatile("" : "+v"(lt.scale));  // (waited for here, not by every step)
+      }
       lt.flags = n[0] | (n[1] << 8) | ((unsigned)(x - f0) >= fn || n[0] + n[1] < BN ? kMasked : 0);
       load_pids(base + 64);
     };
     // Copies this wavefront's half of tile `it`'s K or V to LDS (lane l's 16 bytes
     // at the copy's place + 16 l; past the last tile nothing is read, and zeros
-    // are written); returns the tile's flags.
+    // are written); returns the tile's flags, and the half's exponent byte.
     unsigned lds0 = 0;
     int coff[L::NCP > 0 ? L::NCP : 1];
-    auto copy_tile = [&](int it) __attribute__((always_inline)) {
+    auto copy_tile = [&](int it, unsigned& scale) __attribute__((always_inline)) {
       if ((it & 63) == 0) fill_lanes(it);
       const int l = it & 63;
       auto lane_of = [&](unsigned x) __attribute__((always_inline)) { return (unsigned)__builtin_amdgcn_readlane(x, l); };
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           (void*)(((unsigned long)lane_of(lt.hi) << 32) | lane_of(lt.lo)), (short)0, (int)lane_of(lt.bytes),
           fsched::kBufferFlags);
-      const unsigned dst = lds0 + (it % L::CSTAGES) * 2 * L::TILEB + wq * L::NCP * 1024;
+      const unsigned dst = C8 ? lds0 + ((it % L::CSTAGES) * WPT + wq) * L::REGION
+                              : lds0 + (it % L::CSTAGES) * 2 * L::TILEB + wq * L::NCP * 1024;
 #pragma unroll
       for (int i = 0; i < L::NCP; ++i) {
         // (Through locals: written inline in the builtin's arguments they make
@@ -596,6 +607,7 @@ void paged_attn_kernel(PagedArgs p) {
         const unsigned at = dst + i * 1024;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_ptr(at), 16, off, 0, 0, 0);
       }
+      if constexpr (C8) scale = lane_of(lt.scale);
       return (int)lane_of(lt.flags);
     };
     // Non-temporal loads where no other workgroup reads the keys (reads of 1 GiB
@@ -895,10 +907,57 @@ void paged_attn_kernel(PagedArgs p) {
         const int row_b = (int)(copies_v ? p.v_row32 : p.k_row32);
 #pragma unroll
         for (int i = 0; i < L::NCP; ++i) {
-          const int r = i * (64 / CPR) + lane / CPR, ch = (lane % CPR) ^ swz<DP>(r);
-          coff[i] = ch * E < c.d ? r * row_b + 16 * ch : 0x40000000;
+          if constexpr (C8) {
+            const int at = i * 1024 + 16 * lane, col = at % DP;  // of the half's codes, row after row
+            coff[i] = at < BN / 2 * DP && col < c.d ? at / DP * row_b + col : 0x40000000;
+          } else {
+            const int r = i * (64 / CPR) + lane / CPR, ch = (lane % CPR) ^ swz<DP>(r);
+            coff[i] = ch * E < c.d ? r * row_b + 16 * ch : 0x40000000;
+          }
         }
       }
+      // The stage of tile `it` that fragments are read from.
+      auto stage_of = [&](int it) __attribute__((always_inline)) {
+        return C8 ? lds0 + L::CODES + (it & 1) * 2 * L::TILEB : lds0 + (it % L::CSTAGES) * 2 * L::TILEB;
+      };
+      // 8 bits: a lane takes the codes that it copied (they are there: its own
+      // wavefront's wait is enough) to values in the tile's stage; V's NaN leave a
+      // masked tile here (see lstore).
+      bf16x8 raw[L::NCP];
+      auto read_codes = [&](int it) __attribute__((always_inline)) {
+        const unsigned from = lds0 + ((it % L::CSTAGES) * WPT + wq) * L::REGION + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < L::NCP; ++i) raw[i] = lds_b128<0>(from + i * 1024);
+      };
+      auto convert = [&](int it, unsigned scale, bool masked) __attribute__((always_inline)) {
+        const unsigned to = stage_of(it) + (copies_v ? L::TILEB : 0);
+#pragma unroll
+        for (int i = 0; i < L::NCP; ++i) lds_wait_tie(raw[i]);
+#pragma unroll
+        for (int i = 0; i < L::NCP; ++i) {
+          const uint4 codes = __builtin_bit_cast(uint4, raw[i]);
+          unsigned v[8];
+          code_values<T>(codes.x, scale, v);
+          code_values<T>(codes.y, scale, v + 2);
+          code_values<T>(codes.z, scale, v + 4);
+          code_values<T>(codes.w, scale, v + 6);
+          if (masked && copies_v) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const unsigned odd = not_finite<T>(v[j]);
+              v[j] &= ~odd;
+              odd_v |= odd;
+            }
+          }
+          const int at = i * 1024 + 16 * lane, r = at / DP + BN / 2 * my_half, ch = at % DP / 8;
+          const unsigned dst = to + r * L::ROWB + ((ch ^ swz<DP>(r)) << 4);
+          const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+          if (at < BN / 2 * DP) {
+            asm volatile("ds_write_b128 %0, %1" ::"v"(dst), "v"(__builtin_bit_cast(bf16x8, lo)) : "memory");
+            asm volatile("ds_write_b128 %0, %1" ::"v"(dst ^ 16), "v"(__builtin_bit_cast(bf16x8, hi)) : "memory");
+          }
+        }
+      };
       // This lane's places in a stage: K row l32, chunk 2 f + h32 at
       // ka ^ 32 f; V rows r and r + 8 (then 16 further), d-block db at
       // va ^ 64 db.
@@ -920,20 +979,26 @@ void paged_attn_kernel(PagedArgs p) {
         for (int f = 0; f < L::NQ; ++f) lds_wait_tie(kf[f]);
       };
       load_pids(0);
-      int fl_cur = copy_tile(0), fl_nxt = copy_tile(1), fl_far = copy_tile(2);
+      unsigned sc_cur = 127, sc_nxt = 127, sc_far = 127;
+      int fl_cur = copy_tile(0, sc_cur), fl_nxt = copy_tile(1, sc_nxt), fl_far = copy_tile(2, sc_far);
       fsched::wait_vm<2 * L::NCP>();
+      if constexpr (C8) {
+        read_codes(0);
+        convert(0, sc_cur, fl_cur >= kMasked);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+      }
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
       __builtin_amdgcn_s_barrier();
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      read_kf(lds0);
+      read_kf(stage_of(0));
       tie_k();
 #pragma unroll 1
       for (int it = 0; it < nsteps; ++it) {
-        const unsigned st = lds0 + (it % L::CSTAGES) * 2 * L::TILEB;
+        const unsigned st = stage_of(it);
         const bool masked = fl_cur >= kMasked;
         floatx16 sc;
         qk(nullptr, sc);
-        if (masked) {
+        if (!C8 && masked) {
           // V's infinities and NaN leave a masked tile (see lstore): every
           // thread looks at its chunks.
 #pragma unroll
@@ -952,6 +1017,10 @@ void paged_attn_kernel(PagedArgs p) {
           }
           lds_barrier();
         }
+        if constexpr (C8) {  // the next tile's codes, converted while S is made
+          fsched::wait_vm<L::NCP>();  // (tile it + 2 may still be on its way)
+          read_codes(it + 1);
+        }
         shortx4 vr[NDB][4];  // (left as they are read until the wait: no copy of a register may precede it)
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
@@ -962,8 +1031,13 @@ void paged_attn_kernel(PagedArgs p) {
           vr[db][3] = lds_tr64<16 * L::ROWB>(b2);
         }
         __builtin_amdgcn_sched_barrier(0);
-        const int fl = copy_tile(it + 3);
+        unsigned sc_new = 127;
+        const int fl = copy_tile(it + 3, sc_new);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (C8) {
+          convert(it + 1, sc_nxt, fl_nxt >= kMasked);
+          sc_nxt = sc_far, sc_far = sc_new;
+        }
         softmax(sc, it, masked, fl_cur);
         bf16x8 pf[2];
         to_p(sc, pf);
@@ -977,11 +1051,14 @@ void paged_attn_kernel(PagedArgs p) {
             vf[db][k] = __builtin_bit_cast(
                 bf16x8, __builtin_shufflevector(vr[db][2 * k], vr[db][2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        fsched::wait_vm<2 * L::NCP>();  // tiles it + 2 and it + 3 may still be on their way
+        if constexpr (C8)
+          __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the converted tile is in LDS
+        else
+          fsched::wait_vm<2 * L::NCP>();  // tiles it + 2 and it + 3 may still be on their way
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_barrier();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        read_kf(lds0 + ((it + 1) % L::CSTAGES) * 2 * L::TILEB);
+        read_kf(stage_of(it + 1));
         __builtin_amdgcn_sched_barrier(0);
         mma_v(vf, pf, 0);
         __builtin_amdgcn_sched_barrier(0);
@@ -1435,7 +1512,7 @@ int paged_launch_d(PagedArgs& p, const Plan& pl, hipStream_t st) {
     // Where a CU has one workgroup at most, two teams of it share the keys
     // (16 x 2048 x 128 under a window of 512: 29 -> 26 us).
     constexpr int NT = El<T>::W32 ? 2 : 1;
-    if (!pl.split && pl.items <= cu_count()) {
+    if (!(C8 && !El<T>::W32) && !pl.split && pl.items <= cu_count()) {
       if (pl.dp == 32) return paged_launch<C8, T, 32, 4, 2, !El<T>::W32>(p, pl, st);
       if (pl.dp == 64) return paged_launch<C8, T, 64, 4, 2, !El<T>::W32>(p, pl, st);
       return paged_launch<C8, T, 128, 4, 2, !El<T>::W32>(p, pl, st);

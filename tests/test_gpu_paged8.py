@@ -68,6 +68,8 @@ SHAPES = [
     ([700, 10], [2, 9], 14, 2, 64, 8),              # pages of half a half tile
     ([260], [260], 4, 1, 96, 32),                   # a prompt
     ([50, 600], [20, 600], 2, 2, 32, 16),           # narrow heads, more than 32 rows
+    ([2300, 40], [70, 33], 4, 2, 64, 16),           # more key tiles than are looked up at a time
+    ([2200], [40], 2, 1, 128, 32),
 ]
 
 
