@@ -17,15 +17,17 @@ __device__ __forceinline__ void w4_fold(floatx4& acc, const floatx4& accg, float
 
 // Few rows (up to 16 MF of them a workgroup).  The wavefronts of a workgroup
 // take the chunks of 128 columns of the same NF weight tiles in turn, and join
-// their sums in LDS.  Weights go from memory to registers one chunk ahead of
-// use; the rows of x, which every workgroup reads, come from L2.  Bound by the
-// weights' bytes, or below some 10 MB of them by the latencies of a launch, a
-// load and the join.
+// their sums in LDS.  Weights go from memory to registers, U chunks at a time and
+// a batch ahead of use; the rows of x, which every workgroup reads, come from
+// L2, a batch's loads together.  Bound by the weights' bytes, or below some 10 MB of
+// them by the latencies of a launch, a load and the join.
 template <typename T, typename S, int MF, int NF, bool GLU, int FS>
-__global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p) {
+__global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
   constexpr int NS = W4Act<T>::NS, F = MF * NF, GC = 4 / FS;  // groups of a chunk
   constexpr bool H = W4Act<T>::H;
-  constexpr bool kAhead = MF * (int)sizeof(T) <= 2;  // x is loaded a chunk ahead too
+  // (fp32 and groups of 32 fill the registers sooner: batches of two took 12.3 us
+  // for 77 x 1001 x 1990 fp32, of one 9.7)
+  constexpr int U = MF > 1 || sizeof(T) == 4 || FS == 1 ? 1 : 4;
   extern __shared__ floatx4 red[];                   // [wavefront][mf][nf][lane]
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), KW = blockDim.x >> 6;
   const int l16 = lane & 15, lg = lane >> 4;
@@ -51,10 +53,17 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
     for (int nf = 0; nf < NF; ++nf) acc[mf][nf] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   auto load_w = [&](int c, u32x4 (&w)[NF]) __attribute__((always_inline)) {
+    if (c >= p.chunks) return;
 #pragma unroll
-    for (int nf = 0; nf < NF; ++nf) w[nf] = wt[nf][(long)min(c, p.chunks - 1) * 64];
+    for (int nf = 0; nf < NF; ++nf) w[nf] = wt[nf][(long)c * 64];
   };
-  auto load_x = [&](int c, W4Raw<T> (&x)[MF][4]) __attribute__((always_inline)) {
+  W4Raw<T> x[U][MF][4];
+  W4Scales<S> sc[U][NF][GC];
+  unsigned zc[U][NF][GC];
+  // Chunk c's x (zeros past K), scales and zeros.
+  auto load_x = [&](int c, W4Raw<T> (&x)[MF][4], W4Scales<S> (&sc)[NF][GC], unsigned (&zc)[NF][GC])
+      __attribute__((always_inline)) {
+    if (c >= p.chunks) return;
     const int left = p.K - 128 * c - 8 * lg;
     if (128 * (c + 1) <= p.K) {
 #pragma unroll
@@ -67,21 +76,6 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
 #pragma unroll
         for (int s = 0; s < 4; ++s) x[mf][s] = w4_load_x(xrow[mf] + 128 * c, 32 * s, left);
     }
-  };
-  u32x4 w[NF], wn[NF];
-  W4Raw<T> x[MF][4], xn[MF][4];
-  if (wid < p.chunks) {
-    load_w(wid, w);
-    if constexpr (kAhead) load_x(wid, x);
-  }
-  const bf16x8 ones = w4_ones<H>();
-  const W4Decode<H> decode;
-  const floatx4 zero4 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int c = wid; c < p.chunks; c += KW) {
-    if constexpr (!kAhead) load_x(c, x);
-    W4Scales<S> sc[NF][GC];
-    unsigned zc[NF][GC];
     const int g0 = FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)c) : c * GC;
 #pragma unroll
     for (int nf = 0; nf < NF; ++nf)
@@ -90,10 +84,12 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
         sc[nf][g] = *reinterpret_cast<const W4Scales<S>*>(st[nf] + (g0 + g) * 16);
         zc[nf][g] = zt[nf] ? *reinterpret_cast<const unsigned*>(zt[nf] + (g0 + g) * 16) : 0x08080808u;
       }
-    load_w(c + KW, wn);
-    if constexpr (kAhead) {
-      if (c + KW < p.chunks) load_x(c + KW, xn);
-    }
+  };
+  const bf16x8 ones = w4_ones<H>();
+  const W4Decode<H> decode;
+  const floatx4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  auto work = [&](const u32x4 (&w)[NF], const W4Raw<T> (&x)[MF][4], const W4Scales<S> (&sc)[NF][GC],
+                  const unsigned (&zc)[NF][GC]) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       bf16x8 wf[NF];
@@ -123,12 +119,24 @@ __global__ __launch_bounds__(MF == 1 ? 1024 : 512) void w4_rows_kernel(W4Args p)
         }
       }
     }
+  };
+  u32x4 w[U][NF], wn[U][NF];
 #pragma unroll
-    for (int nf = 0; nf < NF; ++nf) w[nf] = wn[nf];
-    if constexpr (kAhead) {
+  for (int u = 0; u < U; ++u) load_w(wid + u * KW, w[u]);
+#pragma unroll 1
+  for (int c = wid; c < p.chunks; c += U * KW) {
+    // (x first: a wait for it is then none for the weights behind it)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) x[0][s] = xn[0][s];
-    }
+    for (int u = 0; u < U; ++u) load_x(c + u * KW, x[u], sc[u], zc[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_w(c + (U + u) * KW, wn[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + u * KW < p.chunks) work(w[u], x[u], sc[u], zc[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int nf = 0; nf < NF; ++nf) w[u][nf] = wn[u][nf];
   }
   // ---- the wavefronts' sums joined
 #pragma unroll
@@ -192,14 +200,19 @@ __device__ __forceinline__ void w4_lds_wait(V& x) {
 // packed rows of W, each 16 MF by 64.  A chunk of 128 columns of x is copied to
 // LDS by the buffer unit while the one before it is worked on (rows of 256 bytes,
 // 16-byte piece c of row r at piece c ^ (r & 15): the 16 rows that a fragment
-// reads lie in banks of their own), and so are the eight tiles of W.  Bound by the matrix cores and the vector unit together: beside 16
-// MFMAs of 16 cycles and 4 of the row sums a step has 32 operations on codes,
-// and a group 128 on sums, of 4 cycles each.
-template <typename T, typename S, int MF, bool GLU, int FS>
+// reads lie in banks of their own), and so are the eight tiles of W.
+// Bound by the matrix cores and the vector unit together: beside 16 MFMAs of 16
+// cycles and 4 of the row sums a step has 32 operations on codes, and a group 128
+// on sums, of 4 cycles each.
+// Where those are too few to fill the card, the four wavefronts stand in one
+// column and share narrower tiles, 64 rows by two of W (100 x 4096 x 4096 bf16,
+// groups of 128: 24.5 us, and 55 with 32 workgroups of 128 x 128).
+template <typename T, typename S, int WM, int MF, int NF, bool GLU, int FS>
 __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks, int nblocks, int per_xcd) {
-  constexpr int NS = W4Act<T>::NS, NF = 4, GC = 4 / FS, EB = (int)sizeof(T);
-  constexpr int BM = 32 * MF, ROWB = 128 * EB, XSTAGE = BM * ROWB, CPL = XSTAGE / 4096;  // copies a wavefront
-  constexpr int STAGE = XSTAGE + 8 * 1024;                                               // x, then eight tiles of W
+  constexpr int NS = W4Act<T>::NS, GC = 4 / FS, EB = (int)sizeof(T);
+  constexpr int BM = 16 * WM * MF, ROWB = 128 * EB, XSTAGE = BM * ROWB, CPL = XSTAGE / 4096;  // copies a wavefront
+  constexpr int WT = 4 / WM * NF;              // tiles of W
+  constexpr int STAGE = XSTAGE + WT * 1024;    // x, then W
   constexpr int RPC = 1024 / ROWB, PPR = ROWB / 16;  // rows a copy, pieces a row
   constexpr int XR = EB / 2;  // reads a fragment
   constexpr bool H = W4Act<T>::H;
@@ -217,8 +230,8 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
     mb = 4 * strip + left - nb * wide;
   }
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l16 = lane & 15, lg = lane >> 4, wm = wid & 1, wn = wid >> 1;
-  const int m0 = mb * BM, t0 = nb * 8 + wn * NF;
+  const int l16 = lane & 15, lg = lane >> 4, wm = wid % WM, wn = wid / WM;
+  const int m0 = mb * BM, t0 = nb * WT + wn * NF;
 
   // ---- copies of x
   const int rows = min(BM, p.M - m0), ldb = (int)p.ldx * EB;
@@ -230,11 +243,13 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
                                                                         (int)(records - (long)c * ROWB), fsched::kBufferFlags);
     const unsigned dst = lds0 + (c & 1) * STAGE + wid * CPL * 1024;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // (tiles past the last: the last again)
-      const int t = min(nb * 8 + wid * 2 + i, p.tiles - 1);
+    for (int i = 0; i < (WT + 3) / 4; ++i) {  // (tiles past the last: the last again)
+      const int wt = wid + 4 * i;
+      if (WT % 4 && wt >= WT) break;
+      const int t = min(nb * WT + wt, p.tiles - 1);
       const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(
           (void*)(p.w + ((long)t * p.chunks + c) * 64), (short)0, 1024, fsched::kBufferFlags);
-      const unsigned at = lds0 + (c & 1) * STAGE + XSTAGE + (wid * 2 + i) * 1024;
+      const unsigned at = lds0 + (c & 1) * STAGE + XSTAGE + wt * 1024;
       const int off = lane * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ws, lds_ptr(at), 16, off, 0, 0, 0);
     }
@@ -290,7 +305,8 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
     // (here: left until later, sums of several groups would wait in registers)
 #pragma unroll
     for (int mf = 0; mf < MF; ++mf) asm volatile("" : "+v"(acc[mf][nf]));
-    if (nf < MF) xs[nf] = mine ? ax[nf][0] : xs[nf];
+#pragma unroll
+    for (int mf = nf; mf < MF; mf += NF) xs[mf] = mine ? ax[mf][0] : xs[mf];
   };
   copy(0);
   load_scales(0, sc[0]);
@@ -356,7 +372,9 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
           const bool first = s % FS == 0 && k == 0;
-          if (nf < MF) ax[nf] = mma16_16b<H>(ones, xf[nf][k], first ? zero4 : ax[nf]);
+          // (a tile's share of the row sums: fragments nf, nf + NF ..)
+#pragma unroll
+          for (int mf = nf; mf < MF; mf += NF) ax[mf] = mma16_16b<H>(ones, xf[mf][k], first ? zero4 : ax[mf]);
 #pragma unroll
           for (int mf = 0; mf < MF; ++mf) accg[mf][nf] = mma16_16b<H>(wf, xf[mf][k], first ? zero4 : accg[mf][nf]);
         }
@@ -365,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
         if (nf == 0 && s > 0 && s % FS == 0)
           fold(NF - 1, sc[(s - 1) / FS][NF - 1], lg == ((c * GC + (s - 1) / FS) & 3));
 #pragma unroll
-        for (int i = 0; i < (MF + 1) * NS; ++i) {
+        for (int i = 0; i < (MF + (MF + NF - 1) / NF) * NS; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA,
           __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // and vector operations behind it
         }
@@ -415,23 +433,26 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
 
 // ------------------------------------------------------------------ host --
 
-template <typename T, typename S, int MF, bool GLU, int FS>
+template <typename T, typename S, int WM, int MF, int NF, bool GLU, int FS>
 int w4_tiles_launch(const W4Args& p, hipStream_t st) {
-  const int mblocks = (p.M + 32 * MF - 1) / (32 * MF), nblocks = (p.tiles + 7) / 8;
+  constexpr int BM = 16 * WM * MF, WT = 4 / WM * NF;
+  const int mblocks = (p.M + BM - 1) / BM, nblocks = (p.tiles + WT - 1) / WT;
   const long items = (long)mblocks * nblocks, per_xcd = (items + 7) / 8;
   if (8 * per_xcd * 256 > kMaxGridThreads) return set_error(NKL_EINVAL, "nkl_gemm_w4: %ld tiles", items);
-  w4_tiles_kernel<T, S, MF, GLU, FS><<<dim3((unsigned)(8 * per_xcd)), dim3(256), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
+  w4_tiles_kernel<T, S, WM, MF, NF, GLU, FS><<<dim3((unsigned)(8 * per_xcd)), dim3(256), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
   return check_launch("nkl_gemm_w4");
 }
 
 template <typename T, typename S, int MF, int NF, bool GLU, int FS>
 int w4_rows_launch(const W4Args& p, hipStream_t st) {
   const int tx = (p.tiles + NF - 1) / NF, my = (p.M + 16 * MF - 1) / (16 * MF);
-  // Wavefronts to a workgroup: what brings 16 to each CU (8 of several rows'
-  // fragments), no more than there are chunks.
-  const long want = (MF == 1 ? 16L : 8L) * cu_count();
+  // Four wavefronts on K; eight where there is no more than a workgroup for each
+  // CU and a wavefront keeps two chunks (1 x 4096 x 11264 bf16: 10.9 us, 14.4 with
+  // four; 1 x 2048 x 2048 fp32 5.6 and 7.0; 352 workgroups, 16 x 11264 x 2048 fp16:
+  // 10.8 us with eight, 8.9 with four).
   int kw = 1;
-  while (kw < (MF == 1 ? 16 : 8) && kw < p.chunks && (kw < 4 || (long)tx * my * kw < want)) kw *= 2;
+  while (kw < 4 && kw < p.chunks) kw *= 2;
+  if (p.chunks >= 16 && (long)tx * my <= cu_count()) kw = 8;
   w4_rows_kernel<T, S, MF, NF, GLU, FS>
       <<<dim3((unsigned)tx, (unsigned)my), dim3(64 * kw), (size_t)kw * MF * NF * 1024, st>>>(p);
   return check_launch("nkl_gemm_w4");
@@ -447,9 +468,13 @@ int w4_launch_fold(const W4Args& p, const W4Plan& pl, hipStream_t st) {
     if (two) return w4_rows_launch<T, S, MF, 2, false, FS>(p, st);
     return w4_rows_launch<T, S, MF, 1, false, FS>(p, st);
   };
-  // Tiles through LDS where x's rows can be copied by 16 bytes and there are rows
-  // for more than two rounds of the other kernel's.
-  const bool copies = p.M > 64 && p.K % (16 / (int)sizeof(T)) == 0 && p.ldx % (16 / (int)sizeof(T)) == 0 &&
+  // Tiles through LDS where x's rows can be copied by 16 bytes and the narrow tiles
+  // (64 rows by two of W's) are workgroups for more than half the CUs: 64 x
+  // 8192 x 4096 bf16 24.6 us, the other kernel 35.0; 300 x 1001 x 1992 (160
+  // workgroups) 12.2 and 18.1; with 128 (128 x 2048 x 2048 fp32) 22.2 and 19.9,
+  // with 64 (64 x 2048 x 5632) 33.1 and 13.4.
+  const long narrow = (long)((p.M + 63) / 64) * ((p.tiles + 1) / 2);
+  const bool copies = p.M > 32 && 2 * narrow > cu_count() && p.K % (16 / (int)sizeof(T)) == 0 && p.ldx % (16 / (int)sizeof(T)) == 0 &&
                       (size_t)p.x % 16 == 0 && p.ldx < (1L << 21);
   if (copies) {
     // (fp32 scales of groups of 64 beside 16-bit operands: two folds a group, the
@@ -457,10 +482,18 @@ int w4_launch_fold(const W4Args& p, const W4Plan& pl, hipStream_t st) {
     constexpr int MF = sizeof(T) == 4 ? 2 : 4, FT = FS == 2 && sizeof(S) > sizeof(T) ? 1 : FS;
     W4Args q = p;
     q.fold_shift = FT != FS;
-    return pl.glu ? w4_tiles_launch<T, S, MF, true, FT>(q, st) : w4_tiles_launch<T, S, MF, false, FT>(q, st);
+    const long wide = (long)((p.M + 32 * MF - 1) / (32 * MF)) * ((p.tiles + 7) / 8);
+    if (wide >= cu_count())
+      return pl.glu ? w4_tiles_launch<T, S, 2, MF, 4, true, FT>(q, st) : w4_tiles_launch<T, S, 2, MF, 4, false, FT>(q, st);
+    return pl.glu ? w4_tiles_launch<T, S, 4, 1, 2, true, FT>(q, st) : w4_tiles_launch<T, S, 4, 1, 2, false, FT>(q, st);
   }
-  if (p.M <= 16) return run(std::integral_constant<int, 1>{});
-  if (p.M <= 32) return run(std::integral_constant<int, 2>{});
+  // As many rows a workgroup as leave one for each CU (up to 64: weights are then
+  // read from memory once).
+  const long tx = pl.glu || two ? (p.tiles + 1) / 2 : p.tiles;
+  int mf = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+  while (mf > 1 && tx * ((p.M + 16 * mf - 1) / (16 * mf)) < cu_count()) mf /= 2;
+  if (mf == 1) return run(std::integral_constant<int, 1>{});
+  if (mf == 2) return run(std::integral_constant<int, 2>{});
   return run(std::integral_constant<int, 4>{});
 }
 
