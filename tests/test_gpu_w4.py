@@ -177,3 +177,73 @@ def test_kinds_empty_streams_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ops.linear_w4(xg, w.w))
+
+
+# Enough of them for narrow tiles (one block of rows, and two) and for wide ones, with
+# more than four blocks of rows (M, N, K with edges inside every tile)
+TILES = [(40, 4200, 136), (70, 2117, 264), (530, 6603, 200)]
+
+
+@pytest.mark.parametrize("dtype,sdt", [(d, s) for d in DT for s in dict.fromkeys((d, "fp32"))])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_tiles_w4(M, N, K, dtype, sdt):
+    from nkilab import ops
+
+    g = torch.Generator().manual_seed(M + N + K)
+    x = torch.randn(M, K, generator=g).to(DT[dtype])
+    xd = x.double().numpy()
+    for i, group in enumerate((32, 64, 128, 256)):
+        w = Weight(N, K, group, zeros=i % 2 == 1, sdt=sdt, seed=i)
+        y = torch.full((M + 1, N), 7.0, dtype=DT[dtype], device="cuda")
+        ops.linear_w4_into(x.cuda(), w.w, y[:M])
+        check(y[:M], xd @ w.dense.T, sums_bound(xd, w), dtype)
+        assert (y[M] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("M,N,K", [(70, 1060, 264), (330, 3300, 136)])
+def test_swiglu_tiles_w4(M, N, K, dtype):
+    from nkilab import ops
+
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, K, generator=g).to(DT[dtype])
+    xd = x.double().numpy()
+    for group in (64, 128):
+        a, b = Weight(N, K, group, True, dtype, 1), Weight(N, K, group, True, dtype, 2)
+        gate, up = xd @ a.dense.T, xd @ b.dense.T
+        silu = gate / (1 + np.exp(-gate))
+        bound = 1.1 * sums_bound(xd, a) * (np.abs(up) + 1) + sums_bound(xd, b) * (np.abs(silu) + 1) + 2.0 ** -20 * np.abs(silu * up)
+        y = ops.linear_w4_swiglu_into(x.cuda(), ops.pair_w4(a.w, b.w), torch.empty(M, N, dtype=DT[dtype], device="cuda"))
+        check(y, silu * up, bound, dtype)
+
+
+def test_infinities_in_tiles():
+    """As test_rows_do_not_meet, where 16 rows of a tile are multiplied at once."""
+    from nkilab import ops
+
+    w = Weight(4200, 264, 128, True, "bf16", 5)
+    x = torch.randn(70, 264, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    want = ops.linear_w4(x, w.w)
+    x[1, 3], x[65, 263] = float("inf"), float("nan")
+    y = ops.linear_w4(x, w.w)
+    rest = [i for i in range(70) if i not in (1, 65)]
+    assert torch.equal(y[rest], want[rest]) and y[[1, 65]].isnan().all()
+
+
+def test_two_products_at_once():
+    """Two streams, one weight: nothing is shared between calls but what they read."""
+    from nkilab import ops
+
+    g = torch.Generator().manual_seed(3)
+    w = Weight(2117, 264, 64, True, "fp16", 2)
+    xs = [torch.randn(m, 264, generator=g).to(torch.float16).cuda() for m in (1, 70)]
+    want = [ops.linear_w4(x, w.w) for x in xs]
+    outs = [torch.empty_like(y) for y in want]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, x, y in zip(streams, xs, outs):
+            with torch.cuda.stream(s):
+                ops.linear_w4_into(x, w.w, y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
