@@ -126,3 +126,13 @@ def test_cache_has_scales():
     c = PagedCache(5, 2, 64, layers=3, page_size=16, dtype=torch.float8_e4m3fn, device="cpu")
     assert c.k_scale.shape == c.v_scale.shape == (3, 5, 2) and c.k_scale.dtype is torch.uint8
     assert PagedCache(5, 2, 64, device="cpu").k_scale is None
+
+
+def test_write_refuses_far_rows():
+    """Row strides that the kernels' 32-bit row offsets cannot hold."""
+    from nkilab import _lib, ops
+
+    r = ops.Rotary(64)._packed
+    for st, sq in (((1 << 31, 64, 256, 64), (256, 64, 256, 64)), ((256, 64, 1 << 31, 64), (256, 64, 256, 64)),
+                   ((256, 64, 256, 64), (1 << 31, 64, 256, 64)), ((256, 64, 256, 64), (256, 64, 1 << 31, 64))):
+        assert _lib.lib().nkl_cache_write(ctypes.byref(d8()), scales(), P, P, *st, P, P, 4, *sq, None, 0, r, 1, None) == -1

@@ -99,3 +99,19 @@ def test_abi_refusals():
     for bad in (dict(dt=3), dict(ds=2), dict(do=2), dict(dt=0, ds=1, do=0), dict(dt=0, ds=0, do=1)):
         assert call(**bad) == -2, bad
     assert call(M=0, x=None, y=None) == 0 and call(N=0, ldy=0, y=None) == 0
+
+
+def test_weight_refuses():
+    """A W4Weight put together by hand (from a file, say) is checked as the kernels rely on it."""
+    from nkilab import ops
+
+    w = ops.quantize_w4(torch.randn(20, 200), 64, zeros=True)
+    kw = dict(packed=w.packed, scales=w.scales, zeros=w.zeros, n=20, k=200, group=64)
+    assert ops.W4Weight(**kw).n == 20
+    for bad in (dict(packed=w.packed[:1]), dict(packed=w.packed.long()), dict(scales=w.scales[:, :2]), dict(zeros=w.zeros.int()),
+                dict(zeros=w.zeros[:1]), dict(n=33), dict(k=300), dict(group=32), dict(group=96), dict(paired=True),
+                dict(scales=w.scales.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises(ValueError):
+            ops.W4Weight(**{**kw, **bad})
+    with pytest.raises(TypeError):
+        ops.W4Weight(**{**kw, "scales": w.scales.double()})
