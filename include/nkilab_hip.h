@@ -14,7 +14,9 @@
  *   - dtype codes: NKL_F32 = 0 (float32), NKL_BF16 = 1 (bfloat16),
  *     NKL_F16 = 2 (float16: the 16-bit operand format with 11 significant
  *     bits, taken by the GEMMs, the RMSNorm output, the gate/up SwiGLU GEMM
- *     and the causal attention; see each entry point).
+ *     and the causal attention; see each entry point),
+ *     NKL_E4M3 = 3 (8-bit float, 4 exponent and 3 mantissa bits, no infinity:
+ *     a paged cache's rows only).
  *   - `stream` is a hipStream_t passed as void* (0 = the null stream).  Every
  *     call only enqueues work and returns; it is asynchronous with respect to
  *     the host.  State kept across calls: the per-thread error string; the

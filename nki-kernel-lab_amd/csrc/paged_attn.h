@@ -45,7 +45,11 @@
 //
 // 8 bits (C8): the cache holds e4m3 codes, and an exponent for each page and
 // head; codes become values of the query's type between VGPRs and LDS, two to an
-// instruction, and all else is as above.
+// instruction, and all else is as above.  Single tokens are bound by the codes'
+// bytes (64 over 200-16384 rows, 32/8 heads x 128 bf16: 185 + 10 us, the same from a
+// 16-bit cache 340); prompts by LDS, which the tiles pass twice, as codes and as
+// values (4 chunks over up to 8000 rows, 32/8 x 128 bf16, window 4096: 690-710 us,
+// from a 16-bit cache 573).
 //
 // Included by paged_attn.hip and, for caches of 8 bits, by paged_attn8.hip.
 #pragma once
