@@ -210,9 +210,11 @@ __device__ __forceinline__ void w4_lds_wait(V& x) {
 // 128: 0.90 PFLOP/s).
 // Where those are too few to fill the card, the four wavefronts stand in one
 // column and share narrower tiles, 64 rows by two of W (100 x 4096 x 4096 bf16,
-// groups of 128: 24.5 us, and 55 with 32 workgroups of 128 x 128).
-template <typename T, typename S, int WM, int MF, int NF, bool GLU, int FS>
-__global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks, int nblocks, int per_xcd) {
+// groups of 128: 19 us, and 55 with 32 workgroups of 128 x 128).
+// KG groups of four wavefronts take every KG-th chunk, with stages of their own,
+// and join their outputs in LDS: twice the copies on their way in a CU.
+template <typename T, typename S, int KG, int WM, int MF, int NF, bool GLU, int FS>
+__global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mblocks, int nblocks, int per_xcd) {
   constexpr int NS = W4Act<T>::NS, GC = 4 / FS, EB = (int)sizeof(T);
   constexpr int BM = 16 * WM * MF, ROWB = 128 * EB, XSTAGE = BM * ROWB, CPL = XSTAGE / 4096;  // copies a wavefront
   constexpr int WT = 4 / WM * NF;              // tiles of W
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
   constexpr int RPC = 1024 / ROWB, PPR = ROWB / 16;  // rows a copy, pieces a row
   constexpr int XR = EB / 2;  // reads a fragment
   constexpr bool H = W4Act<T>::H;
-  __shared__ __align__(1024) unsigned char smem[2 * STAGE];
+  __shared__ __align__(1024) unsigned char smem[2 * KG * STAGE];
   // Workgroups are dealt to the 8 XCDs in turn: each takes a stretch of the
   // items, four blocks of rows by all of W's and so on, whose weights and rows
   // its L2 holds.
@@ -233,7 +235,8 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
     nb = left / wide;
     mb = 4 * strip + left - nb * wide;
   }
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = KG > 1 ? wave >> 2 : 0, wid = KG > 1 ? wave & 3 : wave;
   const int l16 = lane & 15, lg = lane >> 4, wm = wid % WM, wn = wid / WM;
   const int m0 = mb * BM, t0 = nb * WT + wn * NF;
 
@@ -241,11 +244,11 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
   const int rows = min(BM, p.M - m0), ldb = (int)p.ldx * EB;
   const unsigned char* const xb = p.x + (long)m0 * p.ldx * EB;
   const long records = (long)(rows - 1) * ldb + (long)p.K * EB;
-  const unsigned lds0 = opaque_lds_addr(smem);
-  auto copy = [&](int c) __attribute__((always_inline)) {
+  const unsigned lds0 = opaque_lds_addr(smem) + kg * 2 * STAGE;
+  auto copy = [&](int c, int at_stage) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(xb + (long)c * ROWB), (short)0,
                                                                         (int)(records - (long)c * ROWB), fsched::kBufferFlags);
-    const unsigned dst = lds0 + (c & 1) * STAGE + wid * CPL * 1024;
+    const unsigned dst = lds0 + at_stage * STAGE + wid * CPL * 1024;
 #pragma unroll
     for (int i = 0; i < (WT + 3) / 4; ++i) {  // (tiles past the last: the last again)
       const int wt = wid + 4 * i;
@@ -253,7 +256,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
       const int t = min(nb * WT + wt, p.tiles - 1);
       const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(
           (void*)(p.w + ((long)t * p.chunks + c) * 64), (short)0, 1024, fsched::kBufferFlags);
-      const unsigned at = lds0 + (c & 1) * STAGE + XSTAGE + wt * 1024;
+      const unsigned at = lds0 + at_stage * STAGE + XSTAGE + wt * 1024;
       const int off = lane * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ws, lds_ptr(at), 16, off, 0, 0, 0);
     }
@@ -312,21 +315,26 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
 #pragma unroll
     for (int mf = nf; mf < MF; mf += NF) xs[mf] = mine ? ax[mf][0] : xs[mf];
   };
-  copy(0);
-  load_scales(0, sc[0]);
+  // (a group without a chunk: its sums stay zeros)
+  if (kg < p.chunks) copy(kg, 0);
+  load_scales(kg * GC, sc[0]);
+  // i: this group's chunks.
+  const int steps = (p.chunks + KG - 1) / KG;
 #pragma unroll 1
-  for (int c = 0; c < p.chunks; ++c) {
+  for (int i = 0; i < steps; ++i) {
+    const int c = i * KG + kg;
     // This wavefront's copies are done, then every wavefront's; and none reads
     // the other stage any more.
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    const bool more = c + 1 < p.chunks;
+    if (KG > 1 && c >= p.chunks) break;  // (the last step's barrier is behind)
+    const bool more = c + KG < p.chunks;
 #pragma unroll
-    for (int g = 1; g <= GC; ++g) load_scales(c * GC + g, sc[g]);
-    if (more) copy(c + 1);
-    const unsigned stage = lds0 + (c & 1) * STAGE;
+    for (int g = 1; g <= GC; ++g) load_scales(g < GC ? c * GC + g : (c + KG) * GC, sc[g]);
+    if (more) copy(c + KG, (i + 1) & 1);
+    const unsigned stage = lds0 + (i & 1) * STAGE;
     bf16x8 xr[2][MF][XR];
     auto read_x = [&](int s, bf16x8 (&x)[MF][XR]) __attribute__((always_inline)) {
 #pragma unroll
@@ -383,9 +391,9 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
           for (int mf = 0; mf < MF; ++mf) accg[mf][nf] = mma16_16b<H>(wf, xf[mf][k], first ? zero4 : accg[mf][nf]);
         }
         if (nf < NF - 1) wf = decode(w[s & 1][nf + 1]);
-        if (nf > 0 && ends) fold(nf - 1, sc[s / FS][nf - 1], lg == ((c * GC + s / FS) & 3));
+        if (nf > 0 && ends) fold(nf - 1, sc[s / FS][nf - 1], lg == ((i * GC + s / FS) & 3));
         if (nf == 0 && s > 0 && s % FS == 0)
-          fold(NF - 1, sc[(s - 1) / FS][NF - 1], lg == ((c * GC + (s - 1) / FS) & 3));
+          fold(NF - 1, sc[(s - 1) / FS][NF - 1], lg == ((i * GC + (s - 1) / FS) & 3));
 #pragma unroll
         for (int i = 0; i < (MF + (MF + NF - 1) / NF) * NS; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA,
@@ -398,13 +406,14 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
         wf = decode(w[(s + 1) & 1][0]);
       }
     });
-    fold(NF - 1, sc[3 / FS][NF - 1], lg == ((c * GC + 3 / FS) & 3));
+    fold(NF - 1, sc[3 / FS][NF - 1], lg == ((i * GC + 3 / FS) & 3));
 #pragma unroll
     for (int nf = 0; nf < NF; ++nf) sc[0][nf] = sc[GC][nf];
     // Four folds' row sums times -s (16 + z), in fp32 on the matrix unit.
-    const int folds = (c + 1) * GC;
+    const int folds = (i + 1) * GC;
     if ((folds & 3) == 0 || !more) {
-      const int f = ((folds - 1) & ~3) + lg;
+      const int own = ((folds - 1) & ~3) + lg;
+      const int f = KG > 1 ? (own / GC * KG + kg) * GC + own % GC : own;
       const unsigned g = min(FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)f) : f >> p.fold_shift, p.groups - 1);
 #pragma unroll
       for (int nf = 0; nf < NF; ++nf) {
@@ -416,6 +425,23 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
 #pragma unroll
       for (int mf = 0; mf < MF; ++mf) xs[mf] = 0.f;
     }
+  }
+  if constexpr (KG > 1) {  // ---- the groups' outputs joined, in the stages
+    static_assert(KG == 2 && 4 * MF * NF * 1024 <= 2 * KG * STAGE, "");
+    floatx4* const red = reinterpret_cast<floatx4*>(smem);
+    __syncthreads();  // (no wavefront reads a stage any more, and every copy into one was waited for)
+    if (kg) {
+#pragma unroll
+      for (int mf = 0; mf < MF; ++mf)
+#pragma unroll
+        for (int nf = 0; nf < NF; ++nf) red[((wid * MF + mf) * NF + nf) * 64 + lane] = acc[mf][nf];
+    }
+    __syncthreads();
+    if (kg) return;
+#pragma unroll
+    for (int mf = 0; mf < MF; ++mf)
+#pragma unroll
+      for (int nf = 0; nf < NF; ++nf) acc[mf][nf] += red[((wid * MF + mf) * NF + nf) * 64 + lane];
   }
   // ---- the outputs: four columns of a row a lane and fragment
   const bool whole = p.whole;
@@ -437,13 +463,14 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(W4Args p, int mblocks,
 
 // ------------------------------------------------------------------ host --
 
-template <typename T, typename S, int WM, int MF, int NF, bool GLU, int FS>
+template <typename T, typename S, int KG, int WM, int MF, int NF, bool GLU, int FS>
 int w4_tiles_launch(const W4Args& p, hipStream_t st) {
   constexpr int BM = 16 * WM * MF, WT = 4 / WM * NF;
   const int mblocks = (p.M + BM - 1) / BM, nblocks = (p.tiles + WT - 1) / WT;
   const long items = (long)mblocks * nblocks, per_xcd = (items + 7) / 8;
-  if (8 * per_xcd * 256 > kMaxGridThreads) return set_error(NKL_EINVAL, "nkl_gemm_w4: %ld tiles", items);
-  w4_tiles_kernel<T, S, WM, MF, NF, GLU, FS><<<dim3((unsigned)(8 * per_xcd)), dim3(256), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
+  if (8 * per_xcd * 256 * KG > kMaxGridThreads) return set_error(NKL_EINVAL, "nkl_gemm_w4: %ld tiles", items);
+  w4_tiles_kernel<T, S, KG, WM, MF, NF, GLU, FS>
+      <<<dim3((unsigned)(8 * per_xcd)), dim3(256 * KG), 0, st>>>(p, mblocks, nblocks, (int)per_xcd);
   return check_launch("nkl_gemm_w4");
 }
 
@@ -474,9 +501,9 @@ int w4_launch_fold(const W4Args& p, const W4Plan& pl, hipStream_t st) {
   };
   // Tiles through LDS where x's rows can be copied by 16 bytes and the narrow tiles
   // (64 rows by two of W's) are workgroups for more than half the CUs: 64 x
-  // 8192 x 4096 bf16 24.6 us, the other kernel 35.0; 300 x 1001 x 1992 (160
-  // workgroups) 12.2 and 18.1; with 128 (128 x 2048 x 2048 fp32) 22.2 and 19.9,
-  // with 64 (64 x 2048 x 5632) 33.1 and 13.4.
+  // 8192 x 4096 bf16 19.1 us, the other kernel 35.0; 300 x 1001 x 1992 (160
+  // workgroups) 10.4 and 18.1; with 128 (40 x 4096 x 4096 fp16, groups of 32) 27.0
+  // and 16.5, 128 x 2048 x 2048 bf16 10.7 and 11.0.
   const long narrow = (long)((p.M + 63) / 64) * ((p.tiles + 1) / 2);
   const bool copies = p.M > 32 && 2 * narrow > cu_count() && p.K % (16 / (int)sizeof(T)) == 0 && p.ldx % (16 / (int)sizeof(T)) == 0 &&
                       (size_t)p.x % 16 == 0 && p.ldx < (1L << 21);
@@ -487,9 +514,25 @@ int w4_launch_fold(const W4Args& p, const W4Plan& pl, hipStream_t st) {
     W4Args q = p;
     q.fold_shift = FT != FS;
     const long wide = (long)((p.M + 32 * MF - 1) / (32 * MF)) * ((p.tiles + 7) / 8);
-    if (wide >= cu_count())
-      return pl.glu ? w4_tiles_launch<T, S, 2, MF, 4, true, FT>(q, st) : w4_tiles_launch<T, S, 2, MF, 4, false, FT>(q, st);
-    return pl.glu ? w4_tiles_launch<T, S, 4, 1, 2, true, FT>(q, st) : w4_tiles_launch<T, S, 4, 1, 2, false, FT>(q, st);
+    const auto tiles = [&](auto kg, auto wm, auto mf, auto nf) {
+      constexpr int KG = decltype(kg)::value, WM = decltype(wm)::value, MB = decltype(mf)::value, NB = decltype(nf)::value;
+      return pl.glu ? w4_tiles_launch<T, S, KG, WM, MB, NB, true, FT>(q, st)
+                    : w4_tiles_launch<T, S, KG, WM, MB, NB, false, FT>(q, st);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> twice;
+    const integral_constant<int, 4> four;
+    const integral_constant<int, MF> rows;
+    // 128 x 128 (fp32: 64 x 128) for each CU, or half as wide (256 x 11264 x 2048
+    // bf16: 31.0 us, narrow 38.1; fp32 gains nothing), or narrow: up to two
+    // workgroups a CU with the chunks dealt to two groups (100 x 4096 x 4096 bf16:
+    // 19.0 us, one group 24.7; 704 workgroups, 100 x 11264 x 2048: 23.0 and 21.2).
+    if (wide >= cu_count()) return tiles(one, twice, rows, four);
+    if constexpr (sizeof(T) == 2)
+      if (2 * wide >= cu_count()) return tiles(one, twice, rows, twice);
+    if (narrow <= 2 * cu_count()) return tiles(twice, four, one, twice);
+    return tiles(one, four, one, twice);
   }
   // As many rows a workgroup as leave one for each CU (up to 64: weights are then
   // read from memory once).

@@ -179,9 +179,10 @@ def test_kinds_empty_streams_graphs():
         assert torch.equal(out, ops.linear_w4(xg, w.w))
 
 
-# Enough of them for narrow tiles (one block of rows, and two) and for wide ones, with
-# more than four blocks of rows (M, N, K with edges inside every tile)
-TILES = [(40, 4200, 136), (70, 2117, 264), (530, 6603, 200)]
+# Enough of them for narrow tiles in two groups (one block of rows, and two; one, two and
+# three chunks) and in one group, for those half as wide, and for wide ones with more than
+# four blocks of rows (M, N, K with edges inside every tile)
+TILES = [(40, 4200, 72), (40, 4200, 136), (70, 2117, 264), (70, 8300, 136), (200, 8300, 264), (530, 6603, 200)]
 
 
 @pytest.mark.parametrize("dtype,sdt", [(d, s) for d in DT for s in dict.fromkeys((d, "fp32"))])
@@ -201,7 +202,7 @@ def test_tiles_w4(M, N, K, dtype, sdt):
 
 
 @pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("M,N,K", [(70, 1060, 264), (330, 3300, 136)])
+@pytest.mark.parametrize("M,N,K", [(70, 1060, 264), (70, 4200, 264), (200, 4200, 136), (330, 3300, 136)])
 def test_swiglu_tiles_w4(M, N, K, dtype):
     from nkilab import ops
 
