@@ -597,7 +597,8 @@ typedef struct {
  * to it (rounded once where they become subnormal).  Codes are the nearest, ties
  * to even.  Infinities and NaN become NaN and do not count for the exponent; what
  * exceeds the largest exponent saturates.  Rows behind the new ones in their last
- * page hold nothing of meaning afterwards.
+ * page hold nothing of meaning afterwards.  Exponents that are written (here and by
+ * nkl_cache_accept8) are each page's, head's, layer's and tensor's own.
  */
 int nkl_cache_write(const nkl_paged_cache* cache, const nkl_cache_scales* scales,
                     const void* k, const void* v, long k_row, long k_head,

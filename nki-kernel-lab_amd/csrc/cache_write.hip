@@ -645,6 +645,14 @@ int scales_args(const char* fn, const CacheArgs& c, const nkl_cache_scales* s, S
   return NKL_OK;
 }
 
+// What is written to has exponents of its own for each page and head of K and V.
+int scales_apart(const char* fn, const CacheArgs& c, const Scales& s) {
+  if ((c.pages > 1 && (s.k_page == 0 || s.v_page == 0)) || (c.kv_heads > 1 && (s.k_head == 0 || s.v_head == 0)) ||
+      (c.pages > 0 && s.k == s.v))
+    return set_error(NKL_EINVAL, "%s: pages, heads, or K and V share scales", fn);
+  return NKL_OK;
+}
+
 // --------------------------------------------------------------- accept --
 
 struct Accept8Args {
@@ -767,6 +775,10 @@ extern "C" int nkl_cache_write(const nkl_paged_cache* cache, const nkl_cache_sca
   if (!k || !v || (c.pages > 0 && (!c.k || !c.v))) return set_error(NKL_EINVAL, "%s: null pointer", fn);
   if ((k_row | v_row | q_row | qo_row | c.k_row | c.v_row) >= 1L << 31)
     return set_error(NKL_EINVAL, "%s: a row stride above 2^31 elements", fn);
+  if (q8)
+    if (const int rc = scales_apart(fn, c, p.s)) return rc;
+  if (H && ((c.rows > 1 && qo_row == 0) || (H > 1 && qo_head == 0)))
+    return set_error(NKL_EINVAL, "%s: q_out's rows share memory (a stride of 0)", fn);
   if (H && q == q_out && ((c.rows > 1 && q_row != qo_row) || (H > 1 && q_head != qo_head)))
     return set_error(NKL_EINVAL, "%s: q_out may be q with q's strides only", fn);
   p.nk = static_cast<const unsigned char*>(k);
@@ -819,6 +831,9 @@ extern "C" int nkl_cache_accept8(const nkl_paged_cache* cache, const nkl_cache_s
   if ((size_t)new_lens < (size_t)(c.lens + c.batch) && (size_t)c.lens < (size_t)(new_lens + c.batch))
     return set_error(NKL_EINVAL, "%s: new_lens must lie apart from lens", fn);
   if (c.batch > 65535) return set_error(NKL_EINVAL, "%s: batch=%d above 65535", fn, c.batch);
+  if (const int rc = scales_apart(fn, c, p.s)) return rc;
+  if (layers > 1 && (k_scale_layer == 0 || v_scale_layer == 0))
+    return set_error(NKL_EINVAL, "%s: layers share scales", fn);
   p.paths = paths;
   p.path_row = path_row;
   p.path_cols = path_cols;

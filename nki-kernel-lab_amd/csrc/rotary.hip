@@ -203,6 +203,8 @@ extern "C" int nkl_rotary_apply(const nkl_rotary* rotary, const void* x, void* y
   if (!x || !y) return set_error(NKL_EINVAL, "%s: null pointer", fn);
   if (x == y && ((H > 1 && x_sh != y_sh) || (S > 1 && x_ss != y_ss)))
     return set_error(NKL_EINVAL, "%s: y may be x with x's strides only", fn);
+  if ((H > 1 && y_sh == 0) || (S > 1 && y_ss == 0))
+    return set_error(NKL_EINVAL, "%s: y's rows share memory (a stride of 0)", fn);
   p.x = x;
   p.y = y;
   p.x_sh = x_sh; p.x_ss = x_ss; p.y_sh = y_sh; p.y_ss = y_ss;

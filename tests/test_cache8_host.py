@@ -136,3 +136,26 @@ def test_write_refuses_far_rows():
     for st, sq in (((1 << 31, 64, 256, 64), (256, 64, 256, 64)), ((256, 64, 1 << 31, 64), (256, 64, 256, 64)),
                    ((256, 64, 256, 64), (1 << 31, 64, 256, 64)), ((256, 64, 256, 64), (256, 64, 1 << 31, 64))):
         assert _lib.lib().nkl_cache_write(ctypes.byref(d8()), scales(), P, P, *st, P, P, 4, *sq, None, 0, r, 1, None) == -1
+
+
+def test_writes_refuse_shared_scales():
+    """Exponents that pages, heads, layers, or K and V share; rows of q_out in one place."""
+    from nkilab import _lib, ops
+
+    L = _lib.lib()
+    r = ops.Rotary(64)._packed
+    apart = dict(v=P + 4096)
+
+    def write(s, so=(256, 64)):
+        return L.nkl_cache_write(ctypes.byref(d8()), s, P, P, 256, 64, 256, 64, P, P + 64, 4, 256, 64, *so, None, 0, r, 1, None)
+
+    for bad in (dict(v=P), dict(k_page=0), dict(v_page=0), dict(k_head=0), dict(v_head=0)):
+        s = scales(**{**apart, **bad})
+        assert write(s) == -1 and b"share scales" in L.nkl_last_error_string(), bad
+        assert L.nkl_cache_accept8(ctypes.byref(d8()), s, P, 4, 4, P + 256, 2, 16, 16, 16, 16, None) == -1, bad
+        assert b"share scales" in L.nkl_last_error_string()
+    for so in ((0, 64), (256, 0)):
+        assert write(scales(**apart), so) == -1 and b"share memory" in L.nkl_last_error_string()
+    for layers in ((0, 16), (16, 0)):
+        assert L.nkl_cache_accept8(ctypes.byref(d8()), scales(**apart), P, 4, 4, P + 256, 2, 16, 16, *layers, None) == -1
+        assert b"layers share" in L.nkl_last_error_string()

@@ -86,3 +86,13 @@ def test_rotary_into_refuses():
         ops.rotary_into(x, torch.zeros_like(x), r, positions=torch.zeros(3, dtype=torch.int32), pos0=1)
     with pytest.raises(ValueError, match="current device"):
         ops.rotary_into(x, torch.zeros_like(x), r)
+
+
+def test_rotary_refuses_shared_rows():
+    """An output whose rows lie in one place (an expanded tensor)."""
+    from nkilab import _lib, ops
+
+    L, P, r = _lib.lib(), 1 << 20, ops.Rotary(64)._packed
+    for st in ((0, 64), (192, 0)):
+        assert L.nkl_rotary_apply(r, P, P + (1 << 16), 2, 3, 64, 192, 64, *st, None, 0, 0, 0, 0, None) == -1
+        assert b"share memory" in L.nkl_last_error_string()
