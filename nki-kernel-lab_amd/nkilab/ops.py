@@ -325,8 +325,8 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
 
 def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype | None = None) -> W4Weight:
     """A weight [N, K] in 4 bits: each row's groups scaled so that their largest
-    values keep their places (with zeros: their least and largest), and rounded
-    to the nearest code.  Scales of scale_dtype (w's)."""
+    values keep their places (with zeros: the least and largest of them and 0), and
+    rounded to the nearest code.  Scales of scale_dtype (w's)."""
     fn = "quantize_w4"
     _w4_group(fn, group)
     if w.dim() != 2 or 0 in w.shape:
@@ -338,7 +338,9 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dt
     x = torch.nn.functional.pad(w.detach().float(), (0, G * group - K)).view(N, G, group)
     hi, lo = x.amax(dim=2).clamp(min=0), x.amin(dim=2).clamp(max=0)
     s = (hi - lo) / 15 if zeros else torch.maximum(hi / 7, lo / -8)
-    s = torch.where(s > 0, s, torch.ones_like(s)).to(sdt)
+    s = torch.where(s != 0, s, torch.ones_like(s)).to(sdt)
+    if not bool(torch.isfinite(s).all()):
+        raise ValueError(f"{fn}: w holds values that are not finite, or whose scale is none of {sdt}")
     sf = s.float().clamp(min=torch.finfo(sdt).tiny)  # (a scale that its type has none of holds zeros)
     z = (-lo / sf).round().clamp(0, 15) if zeros else torch.full_like(sf, 8.0)
     q = ((x / sf[:, :, None]).round() + z[:, :, None]).clamp(0, 15).to(torch.uint8)

@@ -115,3 +115,20 @@ def test_weight_refuses():
             ops.W4Weight(**{**kw, **bad})
     with pytest.raises(TypeError):
         ops.W4Weight(**{**kw, "scales": w.scales.double()})
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_refuses_what_has_no_scale(zeros):
+    """Infinities, NaN, and magnitudes whose scale leaves its type's range."""
+    from nkilab import ops
+
+    for x in (float("inf"), float("nan")):
+        w = torch.ones(4, 128)
+        w[2, 7] = x
+        with pytest.raises(ValueError, match="finite"):
+            ops.quantize_w4(w, zeros=zeros)
+    big = torch.full((1, 128), 2e6)
+    with pytest.raises(ValueError, match="finite"):
+        ops.quantize_w4(big, zeros=zeros, scale_dtype=torch.float16)
+    w = ops.quantize_w4(big, zeros=zeros, scale_dtype=torch.float32)
+    assert (w.scales[0, 0, 0] - (2e6 / 15 if zeros else 2e6 / 7)).abs() <= 2e6 * 2.0 ** -23
