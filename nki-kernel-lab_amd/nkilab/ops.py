@@ -337,11 +337,16 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dt
     G = -(-K // group)
     x = torch.nn.functional.pad(w.detach().float(), (0, G * group - K)).view(N, G, group)
     hi, lo = x.amax(dim=2).clamp(min=0), x.amin(dim=2).clamp(max=0)
-    s = (hi - lo) / 15 if zeros else torch.maximum(hi / 7, lo / -8)
-    s = torch.where(s != 0, s, torch.ones_like(s)).to(sdt)
+    need = (hi - lo) / 15 if zeros else torch.maximum(hi / 7, lo / -8)
+    s = torch.where(need != 0, need, torch.ones_like(need)).to(sdt)
     if not bool(torch.isfinite(s).all()):
         raise ValueError(f"{fn}: w holds values that are not finite, or whose scale is none of {sdt}")
-    sf = s.float().clamp(min=torch.finfo(sdt).tiny)  # (a scale that its type has none of holds zeros)
+    # Subnormal numbers are far apart, and what a scale rounded down to one leaves out is no
+    # rounding of the codes: the next larger one (whose bits are the next whole number).
+    bits = s.view(torch.int32 if sdt is torch.float32 else torch.int16)
+    wide = (hi.double() - lo.double()) / 15 if zeros else torch.maximum(hi.double() / 7, lo.double() / -8)
+    s = (bits + ((s < torch.finfo(sdt).smallest_normal) & (s.double() < wide)).to(bits.dtype)).view(sdt)
+    sf = s.float()
     z = (-lo / sf).round().clamp(0, 15) if zeros else torch.full_like(sf, 8.0)
     q = ((x / sf[:, :, None]).round() + z[:, :, None]).clamp(0, 15).to(torch.uint8)
     return pack_w4(q.view(N, G * group)[:, :K], s, z.to(torch.uint8) if zeros else None, group)
