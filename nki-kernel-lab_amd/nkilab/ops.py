@@ -344,8 +344,9 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dt
     # Subnormal numbers are far apart, and what a scale rounded down to one leaves out is no
     # rounding of the codes: the next larger one (whose bits are the next whole number).
     bits = s.view(torch.int32 if sdt is torch.float32 else torch.int16)
-    wide = (hi.double() - lo.double()) / 15 if zeros else torch.maximum(hi.double() / 7, lo.double() / -8)
-    s = (bits + ((s < torch.finfo(sdt).smallest_normal) & (s.double() < wide)).to(bits.dtype)).view(sdt)
+    top, low, sd = hi.double(), -lo.double(), s.double()
+    short = top + low > 15 * sd if zeros else (top > 7 * sd) | (low > 8 * sd)
+    s = (bits + (short & (s < torch.finfo(sdt).smallest_normal)).to(bits.dtype)).view(sdt)
     sf = s.float()
     z = (-lo / sf).round().clamp(0, 15) if zeros else torch.full_like(sf, 8.0)
     q = ((x / sf[:, :, None]).round() + z[:, :, None]).clamp(0, 15).to(torch.uint8)
