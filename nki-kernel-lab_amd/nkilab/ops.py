@@ -326,7 +326,7 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
 def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype | None = None) -> W4Weight:
     """A weight [N, K] in 4 bits: each row's groups scaled so that their largest
     values keep their places (with zeros: the least and largest of them and 0), and
-    rounded to the nearest code.  Scales of scale_dtype (w's)."""
+    rounded to the nearest code.  Scales of scale_dtype (w's); 0 for groups of zeros."""
     fn = "quantize_w4"
     _w4_group(fn, group)
     if w.dim() != 2 or 0 in w.shape:
@@ -338,7 +338,7 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dt
     x = torch.nn.functional.pad(w.detach().float(), (0, G * group - K)).view(N, G, group)
     hi, lo = x.amax(dim=2).clamp(min=0), x.amin(dim=2).clamp(max=0)
     need = (hi - lo) / 15 if zeros else torch.maximum(hi / 7, lo / -8)
-    s = torch.where(need != 0, need, torch.ones_like(need)).to(sdt)
+    s = need.to(sdt)
     if not bool(torch.isfinite(s).all()):
         raise ValueError(f"{fn}: w holds values that are not finite, or whose scale is none of {sdt}")
     # Subnormal numbers are far apart, and what a scale rounded down to one leaves out is no
@@ -347,7 +347,7 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dt
     top, low, sd = hi.double(), -lo.double(), s.double()
     short = top + low > 15 * sd if zeros else (top > 7 * sd) | (low > 8 * sd)
     s = (bits + (short & (s < torch.finfo(sdt).smallest_normal)).to(bits.dtype)).view(sdt)
-    sf = s.float()
+    sf = torch.where(s != 0, s, torch.ones_like(s)).float()  # (0: of zeros, whose products are then exactly 0)
     z = (-lo / sf).round().clamp(0, 15) if zeros else torch.full_like(sf, 8.0)
     q = ((x / sf[:, :, None]).round() + z[:, :, None]).clamp(0, 15).to(torch.uint8)
     return pack_w4(q.view(N, G * group)[:, :K], s, z.to(torch.uint8) if zeros else None, group)
