@@ -399,7 +399,9 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
 /*
  * y[M, N] = x[M, K] W^T (+ residual) for 4-bit weights, W[n, k] = s[n, g] (q[n, k]
  * - z[n, g]) with g = k / group (32, 64 or a multiple of 128 columns).  Sums in
- * fp32, weights never rounded, one rounding per output.
+ * fp32, weights never rounded, one rounding per output.  16-bit x: sums are of
+ * (16 + q) x, and off by some 2^-24 of those magnitudes (fp32 x: of (q - z) x);
+ * bf16 x beyond 2^116 may overflow in them.
  *
  * packed: tiles of 16 rows x 128 columns in the order [ceil(N / 16)][ceil(K / 128)],
  * 1 KB each: bytes 16 l + 4 s .. + 3 (l < 64, s < 4) are a little-endian word with

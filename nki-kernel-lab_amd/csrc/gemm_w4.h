@@ -10,14 +10,24 @@
 // low half's nibbles and 1, 3, 5, 7 the high half's: a shift and a mask give
 // the two codes of a register.
 //
-// A code becomes an operand without a conversion: as mantissa bits of 16 it is
-// 16 + q, exactly, in bf16 and in fp16 (where the sum below loses 3 of fp32's 24
-// bits at most), and the sum over a group is put right afterwards, in fp32:
+// 16-bit activations: a code becomes an operand without a conversion.  As mantissa
+// bits of 16 it is 16 + q, exactly, in bf16 and in fp16, and the sum over a group
+// is put right afterwards, in fp32:
 //   sum q x - z sum x = sum (16 + q) x - (16 + z) sum x,
-// with sum x from one more MFMA, whose A operand is ones.  Scales are applied to
-// the groups' fp32 sums: no weight is ever rounded.
+// with sum x from one more MFMA, whose A operand is ones.  Both sums round to 24
+// bits of their own magnitude, so the result is off by some 2^-24 of sum |16 + q||x|,
+// not of what is left of it: of codes within 1 of their zero (the worst there is;
+// sums of 264 to 4096) 1e-6 of the outputs' magnitude for activations of mean 0,
+// and up to 2e-5 where their mean is their spread or more.  Half a step of fp16 is
+// 5e-4, of bf16 4e-3.  And bf16 activations past 2^128 / (31 x 128) overflow in sums
+// whose difference might not.
+//
 // fp32 activations are taken apart into three bf16 numbers, which hold their 24
-// bits exactly, and multiplied three times.
+// bits exactly (down to 2^-110), and multiplied three times, by q - z, which bf16
+// holds exactly: nothing is left to put right (1e-7 throughout).  Making q - z of a code
+// takes twice the operations of 16 + q; tiles of many rows take 3-9% longer for it.
+//
+// Scales are applied to the groups' fp32 sums: no weight is ever rounded.
 #pragma once
 
 #include <type_traits>
@@ -47,16 +57,17 @@ struct W4Args {
   int whole;            // rows of y and of the residual begin on four elements' boundary
 };
 
-// MFMA operands made of activations of type T: NS bf16 or fp16 fragments.
+// MFMA operands made of activations of type T: NS bf16 or fp16 fragments, to be
+// multiplied by codes less their zeros (CEN) or by 16 + q.
 template <typename T>
 struct W4Act {
   static constexpr int NS = sizeof(T) == 4 ? 3 : 1;
-  static constexpr bool H = false;
+  static constexpr bool H = false, CEN = sizeof(T) == 4;
 };
 template <>
 struct W4Act<f16> {
   static constexpr int NS = 1;
-  static constexpr bool H = true;
+  static constexpr bool H = true, CEN = false;
 };
 
 template <bool H>
@@ -85,6 +96,23 @@ struct W4Decode {
     return __builtin_bit_cast(bf16x8, r);
   }
 };
+
+// Eight codes less their row's zero, in bf16: whole numbers within 15, exactly.
+// (As an e4m3 number a code is q 2^-9: its subnormal numbers and the first normal
+// ones are equally far apart.  One instruction converts two.)
+__device__ __forceinline__ bf16x8 w4_centred(unsigned w, float z) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const unsigned b0 = w & 0x0f0f0f0fu, b1 = (w >> 4) & 0x0f0f0f0fu;  // codes 0, 4, 1, 5; 2, 6, 3, 7
+  const f32x2 c04 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(b0, 512.f, false);
+  const f32x2 c15 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(b0, 512.f, true);
+  const f32x2 c26 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(b1, 512.f, false);
+  const f32x2 c37 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(b1, 512.f, true);
+  auto pair = [&](float lo, float hi) __attribute__((always_inline)) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi - z), __float_as_uint(lo - z), 0x07060302u);
+  };
+  const u32x4 r = {pair(c04[0], c15[0]), pair(c26[0], c37[0]), pair(c04[1], c15[1]), pair(c26[1], c37[1])};
+  return __builtin_bit_cast(bf16x8, r);
+}
 
 template <bool H>
 __device__ __forceinline__ bf16x8 w4_ones() {

@@ -26,7 +26,7 @@ __device__ __forceinline__ void w4_fold(floatx4& acc, const floatx4& accg, float
 template <typename T, typename S, int MF, int NF, bool GLU, int FS>
 __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
   constexpr int NS = W4Act<T>::NS, F = MF * NF, GC = 4 / FS;  // groups of a chunk
-  constexpr bool H = W4Act<T>::H;
+  constexpr bool H = W4Act<T>::H, CEN = W4Act<T>::CEN;
   // (fp32 and groups of 32 fill the registers sooner: batches of two took 12.3 us
   // for 77 x 1001 x 1990 fp32, of one 9.7)
   constexpr int U = MF > 1 || sizeof(T) == 4 || FS == 1 ? 1 : 4;
@@ -46,7 +46,8 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
     const int t = min(t0 + nf, p.tiles - 1);
     wt[nf] = p.w + (long)t * p.chunks * 64 + lane;
     st[nf] = reinterpret_cast<const S*>(p.scales) + (long)t * p.groups * 16 + 4 * lg;
-    zt[nf] = p.zeros ? p.zeros + (long)t * p.groups * 16 + 4 * lg : nullptr;
+    // (four rows' for the sums, the lane's own row's for its codes)
+    zt[nf] = p.zeros ? p.zeros + (long)t * p.groups * 16 + (CEN ? l16 : 4 * lg) : nullptr;
   }
   floatx4 acc[MF][NF], accg[MF][NF], ax[MF];
 #pragma unroll
@@ -54,15 +55,26 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
 #pragma unroll
     for (int nf = 0; nf < NF; ++nf) acc[mf][nf] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  auto load_w = [&](int c, u32x4 (&w)[NF]) __attribute__((always_inline)) {
+  auto first_group = [&](int c) __attribute__((always_inline)) {
+    return FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)c) : c * GC;
+  };
+  // Chunk c's codes, and what they are centred by.
+  auto load_w = [&](int c, u32x4 (&w)[NF], unsigned (&zc)[NF][GC]) __attribute__((always_inline)) {
     if (c >= p.chunks) return;
 #pragma unroll
     for (int nf = 0; nf < NF; ++nf) w[nf] = wt[nf][(long)c * 64];
+    if constexpr (CEN) {
+      const int g0 = first_group(c);
+#pragma unroll
+      for (int nf = 0; nf < NF; ++nf)
+#pragma unroll
+        for (int g = 0; g < GC; ++g) zc[nf][g] = zt[nf] ? zt[nf][(g0 + g) * 16] : 8u;
+    }
   };
   W4Raw<T> x[U][MF][4];
   W4Scales<S> sc[U][NF][GC];
-  unsigned zc[U][NF][GC];
-  // Chunk c's x (zeros past K), scales and zeros.
+  unsigned zc[U][NF][GC], zn[U][NF][GC];
+  // Chunk c's x (nothing past K), scales, and the zeros that sums are put right by.
   auto load_x = [&](int c, W4Raw<T> (&x)[MF][4], W4Scales<S> (&sc)[NF][GC], unsigned (&zc)[NF][GC])
       __attribute__((always_inline)) {
     if (c >= p.chunks) return;
@@ -78,13 +90,13 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) x[mf][s] = w4_load_x(xrow[mf] + 128 * c, 32 * s, left);
     }
-    const int g0 = FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)c) : c * GC;
+    const int g0 = first_group(c);
 #pragma unroll
     for (int nf = 0; nf < NF; ++nf)
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
         sc[nf][g] = *reinterpret_cast<const W4Scales<S>*>(st[nf] + (g0 + g) * 16);
-        zc[nf][g] = zt[nf] ? *reinterpret_cast<const unsigned*>(zt[nf] + (g0 + g) * 16) : 0x08080808u;
+        if constexpr (!CEN) zc[nf][g] = zt[nf] ? *reinterpret_cast<const unsigned*>(zt[nf] + (g0 + g) * 16) : 0x08080808u;
       }
   };
   const bf16x8 ones = w4_ones<H>();
@@ -96,7 +108,12 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
     for (int s = 0; s < 4; ++s) {
       bf16x8 wf[NF];
 #pragma unroll
-      for (int nf = 0; nf < NF; ++nf) wf[nf] = decode(w[nf][s]);
+      for (int nf = 0; nf < NF; ++nf) {
+        if constexpr (CEN)
+          wf[nf] = w4_centred(w[nf][s], (float)zc[nf][s / FS]);
+        else
+          wf[nf] = decode(w[nf][s]);
+      }
 #pragma unroll
       for (int mf = 0; mf < MF; ++mf) {
         bf16x8 xf[NS];
@@ -104,7 +121,7 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
           const bool first = s % FS == 0 && k == 0;
-          ax[mf] = mma16_16b<H>(ones, xf[k], first ? zero4 : ax[mf]);
+          if constexpr (!CEN) ax[mf] = mma16_16b<H>(ones, xf[k], first ? zero4 : ax[mf]);
 #pragma unroll
           for (int nf = 0; nf < NF; ++nf) accg[mf][nf] = mma16_16b<H>(wf[nf], xf[k], first ? zero4 : accg[mf][nf]);
         }
@@ -114,6 +131,13 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
         for (int nf = 0; nf < NF; ++nf) {
           float zz[4], sf[4];
           sc[nf][s / FS].get(sf);
+          if constexpr (CEN) {
+#pragma unroll
+            for (int mf = 0; mf < MF; ++mf)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[mf][nf][i] = fmaf(sf[i], accg[mf][nf][i], acc[mf][nf][i]);
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) zz[i] = 16.f + (float)((zc[nf][s / FS] >> (8 * i)) & 255u);
 #pragma unroll
@@ -124,21 +148,27 @@ __global__ __launch_bounds__(512) void w4_rows_kernel(W4Args p) {
   };
   u32x4 w[U][NF], wn[U][NF];
 #pragma unroll
-  for (int u = 0; u < U; ++u) load_w(wid + u * KW, w[u]);
+  for (int u = 0; u < U; ++u) load_w(wid + u * KW, w[u], zc[u]);
 #pragma unroll 1
   for (int c = wid; c < p.chunks; c += U * KW) {
     // (x first: a wait for it is then none for the weights behind it)
 #pragma unroll
     for (int u = 0; u < U; ++u) load_x(c + u * KW, x[u], sc[u], zc[u]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_w(c + (U + u) * KW, wn[u]);
+    for (int u = 0; u < U; ++u) load_w(c + (U + u) * KW, wn[u], zn[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (c + u * KW < p.chunks) work(w[u], x[u], sc[u], zc[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int nf = 0; nf < NF; ++nf) w[u][nf] = wn[u][nf];
+      for (int nf = 0; nf < NF; ++nf) {
+        w[u][nf] = wn[u][nf];
+        if constexpr (CEN) {
+#pragma unroll
+          for (int g = 0; g < GC; ++g) zc[u][nf][g] = zn[u][nf][g];
+        }
+      }
   }
   // ---- the wavefronts' sums joined
 #pragma unroll
@@ -221,7 +251,7 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
   constexpr int STAGE = XSTAGE + WT * 1024;    // x, then W
   constexpr int RPC = 1024 / ROWB, PPR = ROWB / 16;  // rows a copy, pieces a row
   constexpr int XR = EB / 2;  // reads a fragment
-  constexpr bool H = W4Act<T>::H;
+  constexpr bool H = W4Act<T>::H, CEN = W4Act<T>::CEN;
   __shared__ __align__(1024) unsigned char smem[2 * KG * STAGE];
   // Workgroups are dealt to the 8 XCDs in turn: each takes a stretch of the
   // items, four blocks of rows by all of W's and so on, whose weights and rows
@@ -290,16 +320,20 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
   // Scales of a chunk's groups, and of the next chunk's first one: loaded before
   // the copies of the next chunk, which a wait for them would else be one for.
   W4Scales<S> sc[GC + 1][NF];
+  // Zeros likewise, of the rows whose codes the lane has, where operands are centred.
+  unsigned zc[CEN ? GC + 1 : 1][NF];
   // Row sums of four folds, those of fold lg of them in this lane.
   float xs[MF];
 #pragma unroll
   for (int mf = 0; mf < MF; ++mf) xs[mf] = 0.f;
-  auto load_scales = [&](int f, W4Scales<S> (&to)[NF]) __attribute__((always_inline)) {
+  auto load_scales = [&](int f, int at) __attribute__((always_inline)) {
     const int g = min(FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)f) : f >> p.fold_shift, p.groups - 1);
     const unsigned mine = 4 * lg * (unsigned)sizeof(S);
 #pragma unroll
-    for (int nf = 0; nf < NF; ++nf)
-      to[nf] = *reinterpret_cast<const W4Scales<S>*>(p.scales + (size_t)(sbase[nf] + g) * (16 * sizeof(S)) + mine);
+    for (int nf = 0; nf < NF; ++nf) {
+      sc[at][nf] = *reinterpret_cast<const W4Scales<S>*>(p.scales + (size_t)(sbase[nf] + g) * (16 * sizeof(S)) + mine);
+      if constexpr (CEN) zc[at][nf] = p.zeros ? p.zeros[(size_t)(sbase[nf] + g) * 16 + l16] : 8u;
+    }
   };
   // A fold of tile nf: its fp32 sums, scaled, into the outputs; and its share of the row sums.
   auto fold = [&](int nf, const W4Scales<S>& sx, bool mine) __attribute__((always_inline)) {
@@ -312,12 +346,21 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
     // (here: left until later, sums of several groups would wait in registers)
 #pragma unroll
     for (int mf = 0; mf < MF; ++mf) asm volatile("" : "+v"(acc[mf][nf]));
+    if constexpr (!CEN) {
 #pragma unroll
-    for (int mf = nf; mf < MF; mf += NF) xs[mf] = mine ? ax[mf][0] : xs[mf];
+      for (int mf = nf; mf < MF; mf += NF) xs[mf] = mine ? ax[mf][0] : xs[mf];
+    }
+  };
+  // The operand of tile nf in a step whose group is g of its chunk.
+  auto operand = [&](unsigned w, int g, int nf) __attribute__((always_inline)) {
+    if constexpr (CEN)
+      return w4_centred(w, (float)zc[g][nf]);
+    else
+      return decode(w);
   };
   // (a group without a chunk: its sums stay zeros)
   if (kg < p.chunks) copy(kg, 0);
-  load_scales(kg * GC, sc[0]);
+  load_scales(kg * GC, 0);
   // i: this group's chunks.
   const int steps = (p.chunks + KG - 1) / KG;
 #pragma unroll 1
@@ -332,7 +375,7 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
     if (KG > 1 && c >= p.chunks) break;  // (the last step's barrier is behind)
     const bool more = c + KG < p.chunks;
 #pragma unroll
-    for (int g = 1; g <= GC; ++g) load_scales(g < GC ? c * GC + g : (c + KG) * GC, sc[g]);
+    for (int g = 1; g <= GC; ++g) load_scales(g < GC ? c * GC + g : (c + KG) * GC, g);
     if (more) copy(c + KG, (i + 1) & 1);
     const unsigned stage = lds0 + (i & 1) * STAGE;
     bf16x8 xr[2][MF][XR];
@@ -359,7 +402,7 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
     read_w(std::integral_constant<int, 0>{}, w[0]);
     read_x(0, xr[0]);
     wait_step(w[0], xr[0]);
-    bf16x8 wf = decode(w[0][0]);
+    bf16x8 wf = operand(w[0][0], 0, 0);
     // A step's MFMAs go out tile by tile, and between a tile's the vector unit
     // makes the next tile's operand and folds the one before.
     w4_static_for<0, 1, 4>([&](auto step) __attribute__((always_inline)) {
@@ -386,16 +429,16 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
           const bool first = s % FS == 0 && k == 0;
           // (a tile's share of the row sums: fragments nf, nf + NF ..)
 #pragma unroll
-          for (int mf = nf; mf < MF; mf += NF) ax[mf] = mma16_16b<H>(ones, xf[mf][k], first ? zero4 : ax[mf]);
+          for (int mf = nf; mf < MF && !CEN; mf += NF) ax[mf] = mma16_16b<H>(ones, xf[mf][k], first ? zero4 : ax[mf]);
 #pragma unroll
           for (int mf = 0; mf < MF; ++mf) accg[mf][nf] = mma16_16b<H>(wf, xf[mf][k], first ? zero4 : accg[mf][nf]);
         }
-        if (nf < NF - 1) wf = decode(w[s & 1][nf + 1]);
+        if (nf < NF - 1) wf = operand(w[s & 1][nf + 1], s / FS, nf + 1);
         if (nf > 0 && ends) fold(nf - 1, sc[s / FS][nf - 1], lg == ((i * GC + s / FS) & 3));
         if (nf == 0 && s > 0 && s % FS == 0)
           fold(NF - 1, sc[(s - 1) / FS][NF - 1], lg == ((i * GC + (s - 1) / FS) & 3));
 #pragma unroll
-        for (int i = 0; i < (MF + (MF + NF - 1) / NF) * NS; ++i) {
+        for (int i = 0; i < (MF + (CEN ? 0 : (MF + NF - 1) / NF)) * NS; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA,
           __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // and vector operations behind it
         }
@@ -403,15 +446,18 @@ __global__ __launch_bounds__(256 * KG, 2) void w4_tiles_kernel(W4Args p, int mbl
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (s < 3) {
         wait_step(w[(s + 1) & 1], xr[(s + 1) & 1]);
-        wf = decode(w[(s + 1) & 1][0]);
+        wf = operand(w[(s + 1) & 1][0], (s + 1) / FS, 0);
       }
     });
     fold(NF - 1, sc[3 / FS][NF - 1], lg == ((i * GC + 3 / FS) & 3));
 #pragma unroll
-    for (int nf = 0; nf < NF; ++nf) sc[0][nf] = sc[GC][nf];
+    for (int nf = 0; nf < NF; ++nf) {
+      sc[0][nf] = sc[GC][nf];
+      if constexpr (CEN) zc[0][nf] = zc[GC][nf];
+    }
     // Four folds' row sums times -s (16 + z), in fp32 on the matrix unit.
     const int folds = (i + 1) * GC;
-    if ((folds & 3) == 0 || !more) {
+    if (!CEN && ((folds & 3) == 0 || !more)) {
       const int own = ((folds - 1) & ~3) + lg;
       const int f = KG > 1 ? (own / GC * KG + kg) * GC + own % GC : own;
       const unsigned g = min(FS == 4 ? (int)fsched::div32(p.dv_gc, (unsigned)f) : f >> p.fold_shift, p.groups - 1);

@@ -413,8 +413,10 @@ def linear_w4_into(a: torch.Tensor, w: W4Weight, c: torch.Tensor, residual: torc
     """c = a @ w^T (+ residual) for a 4-bit weight; a [M, k] of any of the three
     dtypes, c [M, n] (which may be the residual) of a's or fp32, the weight's
     scales likewise.  The weight's values are not rounded: sums are of codes
-    times a in fp32, scaled group by group, and rounded once.  A row of a with
-    an infinity or NaN gives NaN."""
+    times a in fp32 (of 16-bit a: of 16 + code, put right by the sum of a, and as
+    exact as those magnitudes are), scaled group by group, and rounded once.  A
+    row of a with an infinity or NaN gives NaN, and one of bf16 that overflows
+    in 16 + code, beyond 2^116, may."""
     if w.paired:
         raise ValueError("linear_w4_into: a pair of weights; linear_w4_swiglu_into takes those")
     return _linear_w4("linear_w4_into", a, w, c, residual)
