@@ -1474,8 +1474,11 @@ int plan_paged(const char* fn, const CacheArgs& c, int elem, int cache_elem, int
     pl.min_tiles = 4;
   }
   // 8 bits, 128 rows a tile: a range is worth its part, 66 KB that the join reads
-  // again, from 12 key tiles on (8 trees of 24 nodes, 16 heads x 128 fp16, over
-  // 500-4000 rows: 38.6 us in all with 4 tiles, 34.1 with 12, 37.9 with 20).
+  // again, from 12 key tiles on, also where fewer would leave no CU idle (trees of
+  // 24 nodes, 16/4 heads x 128 fp16, pages of 16; us with 4, 8 and 12 tiles: 1 tree over
+  // 4000 rows 35.9, 30.6, 29.4, over 16000 80.6, 55.1, 46.6; 8 over 2000 rows 33.3, 34.9,
+  // 30.3, over 4000 38.8, 39.1, 41.0; 32 over 2000 49.4, 49.8, 49.7, over 16000 230, 225,
+  // 225.  8 over 500-4000: 38.6 with 4, 34.1 with 12, 37.9 with 20).
   if (cache_elem == 1 && elem != 4 && pl.wide) pl.min_tiles = 12;
   if (pl.split && pl.items * (key_tiles + pl.setup + pl.grid) >= 1L << 30) pl.split = false;
   // (32-bit byte offsets within a tile, and byte strides)
@@ -1518,12 +1521,15 @@ int paged_launch_d(PagedArgs& p, const Plan& pl, hipStream_t st) {
     // One team a workgroup lets two workgroups of a CU run out of step (their
     // LDS reads, MFMAs and exps overlap: 32 x 16384 x 128 1.35 -> 1.21 ms).
     // Where a CU has one workgroup at most, two teams of it share the keys
-    // (16 x 2048 x 128 under a window of 512: 29 -> 26 us).
+    // (16 x 2048 x 128 under a window of 512: 29 -> 26 us).  Codes of 8 bits are
+    // taken to 16 by the one team.
     constexpr int NT = El<T>::W32 ? 2 : 1;
-    if (!(C8 && !El<T>::W32) && !pl.split && pl.items <= cu_count()) {
-      if (pl.dp == 32) return paged_launch<C8, T, 32, 4, 2, !El<T>::W32>(p, pl, st);
-      if (pl.dp == 64) return paged_launch<C8, T, 64, 4, 2, !El<T>::W32>(p, pl, st);
-      return paged_launch<C8, T, 128, 4, 2, !El<T>::W32>(p, pl, st);
+    if constexpr (!C8 && !El<T>::W32) {
+      if (!pl.split && pl.items <= cu_count()) {
+        if (pl.dp == 32) return paged_launch<C8, T, 32, 4, 2, true>(p, pl, st);
+        if (pl.dp == 64) return paged_launch<C8, T, 64, 4, 2, true>(p, pl, st);
+        return paged_launch<C8, T, 128, 4, 2, true>(p, pl, st);
+      }
     }
     if (pl.dp == 32) return paged_launch<C8, T, 32, 4, NT>(p, pl, st);
     if (pl.dp == 64) return paged_launch<C8, T, 64, 4, NT>(p, pl, st);
