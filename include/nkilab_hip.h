@@ -416,7 +416,7 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
  *
  * x, y, residual: rows of elements together (ldx, ldy, ldr elements apart).  dt:
  * x's dtype; dt_scale, dt_out (y and residual): dt or NKL_F32.  y may be the
- * residual.  A row of x with an infinity or NaN gives NaN.  No workspace.
+ * residual, and shares no memory with x or otherwise with the residual.  A row of x with an infinity or NaN gives NaN.  No workspace.
  */
 int nkl_gemm_w4(const void* x, const void* packed, const void* scales,
                 const void* zeros, void* y, const void* residual, int M, int N,
@@ -441,7 +441,8 @@ typedef struct {
  * row s at positions[s] (int32, or int64 with positions64; null: pos0 + s),
  * positions within 2^31.  Elements past the 2 * pairs first of a head are
  * copied.  transposed: by -angle, which takes the gradient of y to x's.  y may be
- * x, with its strides.  Angles in 64 bits, products in fp32, one rounding per
+ * x, with its strides; else they share no memory (columns of the same rows do
+ * not).  Angles in 64 bits, products in fp32, one rounding per
  * output.  Does not depend on, or replace, nkl_rope's fp32 angles.
  */
 int nkl_rotary_apply(const nkl_rotary* rotary, const void* x, void* y, int H,
@@ -599,7 +600,8 @@ typedef struct {
  * to it (rounded once where they become subnormal).  Codes are the nearest, ties
  * to even.  Infinities and NaN become NaN and do not count for the exponent; what
  * exceeds the largest exponent saturates.  Rows behind the new ones in their last
- * page hold nothing of meaning afterwards.  Exponents that are written (here and by
+ * page hold nothing of meaning afterwards.  q_out may be q, with its strides, and
+ * shares no memory with k, v or otherwise with q.  Exponents that are written (here and by
  * nkl_cache_accept8) are each page's, head's, layer's and tensor's own.
  */
 int nkl_cache_write(const nkl_paged_cache* cache, const nkl_cache_scales* scales,

@@ -13,6 +13,7 @@
 
 #include "paged.h"
 #include "rotary.h"
+#include "rows.h"
 
 namespace nkl {
 
@@ -777,10 +778,19 @@ extern "C" int nkl_cache_write(const nkl_paged_cache* cache, const nkl_cache_sca
     return set_error(NKL_EINVAL, "%s: a row stride above 2^31 elements", fn);
   if (q8)
     if (const int rc = scales_apart(fn, c, p.s)) return rc;
-  if (H && ((c.rows > 1 && qo_row == 0) || (H > 1 && qo_head == 0)))
-    return set_error(NKL_EINVAL, "%s: q_out's rows share memory (a stride of 0)", fn);
-  if (H && q == q_out && ((c.rows > 1 && q_row != qo_row) || (H > 1 && q_head != qo_head)))
-    return set_error(NKL_EINVAL, "%s: q_out may be q with q's strides only", fn);
+  if (H) {
+    const long el = elem_bytes(dtype);
+    const auto rows = [&](const void* at, int heads, long row, long head) {
+      return Rows{(size_t)at, heads, c.rows, head * el, row * el, c.d * el};
+    };
+    const Rows out = rows(q_out, H, qo_row, qo_head);
+    if (rows_share(out)) return set_error(NKL_EINVAL, "%s: q_out's rows share memory", fn);
+    if (q == q_out && ((c.rows > 1 && q_row != qo_row) || (H > 1 && q_head != qo_head)))
+      return set_error(NKL_EINVAL, "%s: q_out may be q with q's strides only", fn);
+    if ((q != q_out && rows_meet(rows(q, H, q_row, q_head), out)) || rows_meet(rows(k, c.kv_heads, k_row, k_head), out) ||
+        rows_meet(rows(v, c.kv_heads, v_row, v_head), out))
+      return set_error(NKL_EINVAL, "%s: q_out and what is read share memory", fn);
+  }
   p.nk = static_cast<const unsigned char*>(k);
   p.nv = static_cast<const unsigned char*>(v);
   p.q = static_cast<const unsigned char*>(q);

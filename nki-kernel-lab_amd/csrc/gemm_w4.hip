@@ -1,6 +1,7 @@
 // Products with 4-bit weights: the entry point (gemm_w4.h has the layout and
 // the arithmetic, gemm_w4_kernels.h the kernels).
 #include "gemm_w4.h"
+#include "rows.h"
 
 using namespace nkl;
 
@@ -27,6 +28,13 @@ extern "C" int nkl_gemm_w4(const void* x, const void* packed, const void* scales
   if ((size_t)packed % 16 || (size_t)scales % 16 || (size_t)zeros % 16 || (size_t)x % el || (size_t)y % eo ||
       (size_t)residual % eo)
     return set_error(NKL_EINVAL, "%s: packed weights, scales and zeros on 16 bytes, tensors on their elements expected", fn);
+  // (a workgroup stores while others still read)
+  const Rows ry{(size_t)y, 1, M, 0, ldy * (long)eo, N * (long)eo};
+  if (rows_meet(Rows{(size_t)x, 1, M, 0, ldx * (long)el, K * (long)el}, ry))
+    return set_error(NKL_EINVAL, "%s: x and y share memory", fn);
+  if (residual && !(residual == y && (M == 1 || ldr == ldy)) &&
+      rows_meet(Rows{(size_t)residual, 1, M, 0, ldr * (long)eo, N * (long)eo}, ry))
+    return set_error(NKL_EINVAL, "%s: y and the residual share memory, and are not the same", fn);
   W4Args p{};
   p.x = static_cast<const unsigned char*>(x);
   p.w = static_cast<const u32x4*>(packed);

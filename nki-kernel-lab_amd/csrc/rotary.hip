@@ -14,7 +14,9 @@
 #include <math.h>
 
 #include "flash_sched.h"
+#include "paged.h"
 #include "rotary.h"
+#include "rows.h"
 
 namespace nkl {
 
@@ -203,8 +205,11 @@ extern "C" int nkl_rotary_apply(const nkl_rotary* rotary, const void* x, void* y
   if (!x || !y) return set_error(NKL_EINVAL, "%s: null pointer", fn);
   if (x == y && ((H > 1 && x_sh != y_sh) || (S > 1 && x_ss != y_ss)))
     return set_error(NKL_EINVAL, "%s: y may be x with x's strides only", fn);
-  if ((H > 1 && y_sh == 0) || (S > 1 && y_ss == 0))
-    return set_error(NKL_EINVAL, "%s: y's rows share memory (a stride of 0)", fn);
+  const long el = elem_bytes(dtype);
+  const Rows ry{(size_t)y, H, S, y_sh * el, y_ss * el, d * el};
+  if (rows_share(ry)) return set_error(NKL_EINVAL, "%s: y's rows share memory", fn);
+  if (x != y && rows_meet(Rows{(size_t)x, H, S, x_sh * el, x_ss * el, d * el}, ry))
+    return set_error(NKL_EINVAL, "%s: x and y share memory, and are not the same", fn);
   p.x = x;
   p.y = y;
   p.x_sh = x_sh; p.x_ss = x_ss; p.y_sh = y_sh; p.y_ss = y_ss;

@@ -411,8 +411,8 @@ def _linear_w4(fn: str, a: torch.Tensor, w: W4Weight, c: torch.Tensor, residual:
 
 def linear_w4_into(a: torch.Tensor, w: W4Weight, c: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
     """c = a @ w^T (+ residual) for a 4-bit weight; a [M, k] of any of the three
-    dtypes, c [M, n] (which may be the residual) of a's or fp32, the weight's
-    scales likewise.  The weight's values are not rounded: sums are of codes
+    dtypes, c [M, n] (which may be the residual, and not a) of a's or fp32, the
+    weight's scales likewise.  The weight's values are not rounded: sums are of codes
     times a in fp32 (of 16-bit a: of 16 + code, put right by the sum of a, and as
     exact as those magnitudes are), scaled group by group, and rounded once.  A
     row of a with an infinity or NaN gives NaN, and one of bf16 that overflows
@@ -537,7 +537,8 @@ def rotary_into(x: torch.Tensor, y: torch.Tensor, rotary: Rotary, positions: tor
                 grad: bool = False) -> torch.Tensor:
     """x [H, S, d] rotated into y (which may be x) as `rotary` says: row s by
     positions[s] (int32 or int64 [S], within 2^31) or pos0 + s.  Elements past
-    rotary.dim are copied.  Any strides along H and S; d contiguous.
+    rotary.dim are copied.  Any strides along H and S; d contiguous; y shares no
+    memory with x unless it is x.
     grad: the transposed map, which takes the gradient of y (as x) to x's."""
     fn = "rotary_into"
     if x.dim() != 3 or y.shape != x.shape or x.dtype != y.dtype:
