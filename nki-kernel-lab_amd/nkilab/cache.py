@@ -324,7 +324,8 @@ class PagedCache(PagePool):
 
     def accept(self, step: CacheStep, paths: list[list[int]]) -> None:
         """Keeps the accepted path of each sequence's rows of `step` (its latest),
-        strictly ascending nodes, and drops the others.  Once for a step."""
+        strictly ascending nodes, and drops the others.  Once for a step.  In 8 bits
+        paths of which rows move have at most 1024 nodes."""
         paths = [[int(i) for i in p] for p in paths]
         if len(paths) != len(step.seqs):
             raise ValueError(f"accept: {len(paths)} paths for {len(step.seqs)} sequences")
@@ -343,6 +344,9 @@ class PagedCache(PagePool):
                                  f"{c + len(path)}; release pages after a path is accepted")
         stay = [sum(i == node for i, node in enumerate(p)) for p in paths]  # (an ascending path's first: in place already)
         if any(m < len(p) for m, p in zip(stay, paths)):
+            width = max(len(p) for p in paths)
+            if self.k_scale is not None and width > ops.ACCEPT8_NODES:
+                raise ValueError(f"accept: a path of {width} nodes; at most {ops.ACCEPT8_NODES} in a cache of 8 bits")
             table = step.table
             # Pages of its own for the rows that move; those that they come from are only read.
             plan = self._plan(step.seqs, [c + m for c, m in zip(ctx, stay)], [c + len(p) for c, p in zip(ctx, paths)],
@@ -352,7 +356,6 @@ class PagedCache(PagePool):
                 self._copy(plan.copies)
                 rows = self._planned(plan)
                 table = self._tensor([rows[s] + [-1] * (table.shape[1] - len(rows[s])) for s in step.seqs])
-            width = max(len(p) for p in paths)
             ops.cache_accept(self.k, self.v, table, step.lens,
                              self._tensor([p + [-1] * (width - len(p)) for p in paths]), q_start=step.q_start,
                              k_scale=self.k_scale, v_scale=self.v_scale)

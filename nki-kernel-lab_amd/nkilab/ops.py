@@ -869,6 +869,7 @@ def attention(q, k, v, variant: str = "flash_pipelined", scale: float | None = N
 
 MAX_ROWS = 1 << 30  # rows a page table addresses at most, and new rows of a call
 E4M3 = torch.float8_e4m3fn  # codes of a cache in 8 bits
+ACCEPT8_NODES = 1024  # nodes of a path that is accepted in one
 
 
 def _cache_code(dt: torch.dtype) -> int:
