@@ -519,6 +519,8 @@ class Rotary:
 
                 first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), dim - 1)
                 kept = [1 - min(1.0, max(0.0, (i - first) / max(last - first, 0.001))) for i in range(dim // 2)]
+                if pair(low) < 0:  # (the first pair, too, turns less often)
+                    kept = [0.0] * (dim // 2)
                 magnitude = 0.1 * math.log(factor) + 1
             else:
                 kept = [min(1.0, max(0.0, (self.original * f / (2 * math.pi) - low) / (high - low))) for f in freq]
