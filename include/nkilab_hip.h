@@ -600,7 +600,9 @@ typedef struct {
  * to it (rounded once where they become subnormal).  Codes are the nearest, ties
  * to even.  Infinities and NaN become NaN and do not count for the exponent; what
  * exceeds the largest exponent saturates.  Rows behind the new ones in their last
- * page hold nothing of meaning afterwards.  q_out may be q, with its strides, and
+ * page hold nothing of meaning afterwards.  An exponent does not fall again: rows
+ * that are dropped later (drafts that are rejected, say) leave it, and the rows
+ * before them as they were rounded under it.  q_out may be q, with its strides, and
  * shares no memory with k, v or otherwise with q.  Exponents that are written (here and by
  * nkl_cache_accept8) are each page's, head's, layer's and tensor's own.
  */
@@ -627,7 +629,8 @@ int nkl_cache_accept8(const nkl_paged_cache* cache, const nkl_cache_scales* scal
  * (strides in its elements, on 16 bytes): scores and sums are of the codes'
  * values, taken to q's type -- exactly to bf16 and fp32 for exponent bytes 17 ..
  * 246, to fp16 rounded where they leave its range of normal numbers, at most
- * 65504 in magnitude.  The workspace's size depends on dtype too.
+ * 65504 in magnitude.  P is rounded to q's type, statistics and O are in fp32.
+ * The workspace's size depends on dtype too.
  */
 size_t nkl_paged_attention8_workspace_bytes(const nkl_paged_cache* cache, int H,
                                             int window, int sinks, int tree,

@@ -525,7 +525,7 @@ int w4_rows_launch(const W4Args& p, hipStream_t st) {
   const int tx = (p.tiles + NF - 1) / NF, my = (p.M + 16 * MF - 1) / (16 * MF);
   // Four wavefronts on K; eight where there is no more than a workgroup for each
   // CU and a wavefront keeps two chunks (1 x 4096 x 11264 bf16: 10.9 us, 14.4 with
-  // four; 1 x 2048 x 2048 fp32 5.6 and 7.0; 352 workgroups, 16 x 11264 x 2048 fp16:
+  // four; 352 workgroups, 16 x 11264 x 2048 fp16:
   // 10.8 us with eight, 8.9 with four).
   int kw = 1;
   while (kw < 4 && kw < p.chunks) kw *= 2;
@@ -546,10 +546,13 @@ int w4_launch_fold(const W4Args& p, const W4Plan& pl, hipStream_t st) {
     return w4_rows_launch<T, S, MF, 1, false, FS>(p, st);
   };
   // Tiles through LDS where x's rows can be copied by 16 bytes and the narrow tiles
-  // (64 rows by two of W's) are workgroups for more than half the CUs: 64 x
-  // 8192 x 4096 bf16 19.1 us, the other kernel 35.0; 300 x 1001 x 1992 (160
-  // workgroups) 10.4 and 18.1; with 128 (40 x 4096 x 4096 fp16, groups of 32) 27.0
-  // and 16.5, 128 x 2048 x 2048 bf16 10.7 and 11.0.
+  // (64 rows by two of W's) are workgroups for more than half the CUs.  Tiles and the
+  // other kernel, us, K = 1024 / 2048 / 4096, bf16 with groups of 32: 128 workgroups, 40 x
+  // 4096 8.6 / 15.0 / 27.3 and 6.5 / 9.5 / 16.0, 128 x 2048 8.6 / 14.1 / 26.1 and 7.5 /
+  // 11.8 / 20.5; 192, 64 x 6144 8.8 / 15.9 / 28.3 and 11.6 / 20.4 / 37.5; groups of 128:
+  // 6.5 / 10.4 / 18.0 and 6.2 / 8.7 / 14.6, 6.5 / 10.0 / 17.2 and 7.2 / 10.9 / 18.8; 6.7 /
+  // 11.2 / 19.0 and 10.8 / 18.9 / 34.9.  fp16 the same; fp32 gains from 128 on with
+  // groups of 32 (128 x 2048 x 4096 39.9 and 42.9, 40 x 4096 x 4096 39.7 and 35.9).
   const long narrow = (long)((p.M + 63) / 64) * ((p.tiles + 1) / 2);
   const bool copies = p.M > 32 && 2 * narrow > cu_count() && p.K % (16 / (int)sizeof(T)) == 0 && p.ldx % (16 / (int)sizeof(T)) == 0 &&
                       (size_t)p.x % 16 == 0 && p.ldx < (1L << 21);

@@ -47,9 +47,9 @@
 // head; codes become values of the query's type between VGPRs and LDS, two to an
 // instruction, and all else is as above.  Single tokens are bound by the codes'
 // bytes (64 over 200-16384 rows, 32/8 heads x 128 bf16: 185 + 10 us, the same from a
-// 16-bit cache 340); prompts by LDS, which the tiles pass twice, as codes and as
-// values (4 chunks over up to 8000 rows, 32/8 x 128 bf16, window 4096: 690-710 us,
-// from a 16-bit cache 573).
+// 16-bit cache 340); prompts by the conversion, whose codes and values both pass LDS
+// for every 128 rows (4 chunks over up to 8000 rows, 32/8 x 128 bf16, window 4096:
+// 690-710 us, from a 16-bit cache 573).
 //
 // Included by paged_attn.hip and, for caches of 8 bits, by paged_attn8.hip.
 #pragma once
@@ -845,6 +845,9 @@ void paged_attn_kernel(PagedArgs p) {
     };
     // P is rounded to the operands' type for the MFMA; the row sums are of the
     // unrounded values.
+    // P in the query's 16 bits, for the matrix unit (the row sum is of P as it was):
+    // an error about as large as the output's own rounding (4 chunks over up to 8000
+    // rows bf16: 2.3e-3 of the outputs' magnitude with it, 1.7e-3 without).
     auto to_p = [&](const floatx16& sc, bf16x8 (&pf)[2]) __attribute__((always_inline)) {
 #pragma unroll
       for (int u2 = 0; u2 < 2; ++u2)

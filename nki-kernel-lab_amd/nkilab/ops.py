@@ -468,15 +468,15 @@ class Rotary:
 
     scaling, for contexts `factor` times as long as the `original` one (in
     positions) that a model was trained for:
-      "linear"  every frequency divided by factor;
+      "linear"  every frequency divided by factor (position interpolation);
       "base"    the base times factor^(dim / (dim - 2)): the lowest frequency
-                divided by factor, the highest kept;
-      "parts"   the pairs that turn more than high_turns (32) times over the
+                divided by factor, the highest kept (the NTK-aware base);
+      "parts"   (YaRN's NTK-by-parts) the pairs that turn more than high_turns (32) times over the
                 original context kept, those that turn less than low_turns (1)
                 times divided by factor, a linear ramp over the pairs' numbers
                 between; the rotated elements times 0.1 ln(factor) + 1;
       "bands"   the same with the ramp over the turns themselves (high_turns
-                4), and no factor of the elements.
+                4), and no factor of the elements (Llama's longer contexts).
     magnitude replaces the factor of the rotated elements.
 
     An object is made once and kept: it holds its table of frequencies."""
@@ -1061,7 +1061,8 @@ def cache_append_into(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     kv_heads]: a value is its code times 2^(scale - 127), the scale its page's and
     head's.  A page gets the smallest scale with which its rows stay within
     448; where that rises with the new rows, the codes of the rows before
-    them follow (rounded again only where they become subnormal)."""
+    them follow (rounded again only where they become subnormal).  It does not
+    fall again when rows are dropped: a rejected draft can cost kept rows bits."""
     fn = "cache_append_into"
     ks = k.shape
     if len(ks) != 3 or ks != v.shape:
