@@ -416,7 +416,8 @@ int nkl_rope(const void* x, void* y, int H, int S, int d, long x_sh, long x_ss,
  *
  * x, y, residual: rows of elements together (ldx, ldy, ldr elements apart).  dt:
  * x's dtype; dt_scale, dt_out (y and residual): dt or NKL_F32.  y may be the
- * residual, and shares no memory with x or otherwise with the residual.  A row of x with an infinity or NaN gives NaN.  No workspace.
+ * residual, and shares no memory with x or otherwise with the residual.  A row of
+ * x with an infinity or NaN gives NaN.  No workspace.
  */
 int nkl_gemm_w4(const void* x, const void* packed, const void* scales,
                 const void* zeros, void* y, const void* residual, int M, int N,

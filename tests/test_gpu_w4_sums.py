@@ -98,3 +98,23 @@ def test_16_bit_sums(M, N, K, dtype, mean):
         # (random signs: the square root of the bound's K / 32 + 128 roundings a term)
         n = min(K, 128) + 3 + K / 32
         assert np.sqrt(((y - ref) ** 2).mean()) <= np.sqrt((bound ** 2).mean() / n)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("M,N,K", [(5, 40, 130), (20, 64, 264), (70, 2117, 264), (200, 8300, 264)])
+def test_rows_with_infinities(M, N, K, dtype):
+    """An infinity or NaN makes its row NaN, also where its codes are their zeros, and no other."""
+    from nkilab import ops
+
+    x = activations(M, K, 0.0, dtype, M).cuda()
+    for zeros, spread in ((True, 1), (False, 0)):
+        w = Close(N, K, 64, zeros, "fp32", 2, spread=spread)
+        want = ops.linear_w4(x, w.w)
+        odd = x.clone()
+        odd[1, K - 1], odd[2, 3], odd[4, 64] = float("-inf"), float("nan"), float("inf")
+        if dtype == "fp32":  # a NaN whose upper half is an infinity's
+            odd.view(torch.int32)[3, 5] = 0x7f800001
+        y = ops.linear_w4(odd, w.w)
+        bad = [1, 2, 4] + ([3] if dtype == "fp32" else [])
+        rest = [i for i in range(M) if i not in bad]
+        assert y[bad].isnan().all() and torch.equal(y[rest], want[rest])

@@ -45,3 +45,17 @@ def test_quantize_small_fp16_weight(std):
     # (a group's largest value is some 2.5 std: at 1e-5 its scale is 60 of the smallest subnormal number,
     # which rounded up is a step larger by a sixtieth at most; nearest codes' errors are a step's 0.29)
     assert rel(ops.quantize_w4(w, 64)) <= 1.05 * wide < 0.2
+
+
+def test_weights_of_any_strides():
+    """Codes, scales and zeros that are transposed or shared between rows, a transposed weight."""
+    from nkilab import ops
+
+    g = torch.Generator().manual_seed(4)
+    codes = torch.randint(0, 16, (128, 48), generator=g, dtype=torch.uint8)
+    scales, zeros = torch.rand(1, 2, generator=g).expand(48, 2), torch.full((1, 1), 3, dtype=torch.uint8).expand(48, 2)
+    w = ops.pack_w4(codes.t(), scales, zeros, 64)
+    assert torch.equal(ops.unpack_w4(w), (codes.t().float() - 3) * scales.repeat_interleave(64, 1))
+    m = torch.randn(128, 48, generator=g)
+    a, b = ops.quantize_w4(m.t(), 64), ops.quantize_w4(m.t().contiguous(), 64)
+    assert torch.equal(a.packed, b.packed) and torch.equal(a.scales, b.scales)
